@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define INB_ABI_VERSION 17
+#define INB_ABI_VERSION 18
 #define INB_MAX_C 3       /* cells (more need an ordered interference sum) */
 #define INB_MAX_S 32      /* RBGs per carrier */
 #define INB_MAX_P 32      /* HARQ processes */
@@ -402,6 +402,104 @@ typedef struct {
   uint8_t *delivered_any, *blocked_out, *los_out, *tag_delivered;   /* [E,R], [E,R], [E,R], [E] */
 } InbObsArgs;
 int inb_net_obs(const InbObsArgs *args, void *cuda_stream);
+
+/* ------------------------------------------------------------------------------------------------ policy operators
+ * What a policy computes between the observations (inb_net_obs) and the traffic requests it answers with.  No
+ * counterpart in the reference, whose policies are the simulator's user's.  Element types of `dtype`: */
+enum { INB_BF16 = 0, INB_F16 = 1, INB_F32 = 2 };
+#define INB_MAX_NORM_D 8192        /* columns of inb_block_norm_* */
+#define INB_CH_DROPOUT 0x44u        /* counter-RNG channel of inb_dropout */
+#define INB_MAX_SAMPLE_V (1 << 22)  /* logits of a row of inb_sample */
+#define INB_MAX_SAMPLE_N (1 << 27)  /* rows */
+
+/* Norms before and after a residual block, with its gate and residual scale, over N rows of D:
+ *   y = x + scale * gate * (post * h / rms(h)),  n = w * y / rms(y),  rms(v) = sqrt(mean(v^2) + eps).
+ * h NULL: y = x, only n is written.  post NULL: no norm of h.  gate: [N / gate_rows, D], gate g scaling the rows
+ * [g gate_rows, (g + 1) gate_rows); NULL: 1.  Rows of x, h, gy, gn are ldx, ldh, ldgy, ldgn elements apart; everything
+ * else is contiguous.  stats [N, 2] fp32 (1 / rms of h and of y): written by the forward call unless NULL, read by
+ * the backward call, which takes the gradients gy, gn of y and n (NULL: zero) and writes those of x, h, w, post and
+ * gate.  work: inb_block_norm_work() floats for the backward call's partial column sums (the call looks at the sizes,
+ * strides, pointer alignments and which of h, post and gate are given).
+ * -2: sizes out of range; -3: a required pointer is NULL; -4: gate_rows does not divide N; -5: work is too small. */
+typedef struct {
+  int32_t dtype, D;
+  int64_t N, ldx, ldh, gate_rows;
+  float scale, eps;
+  const void *x, *h, *w, *post, *gate;
+  void *y, *n;
+  float *stats;
+  int64_t ldgy, ldgn;
+  const void *gy, *gn;
+  void *gx, *gh, *gw, *gpost, *ggate;
+  float *work;
+  int64_t work_elems;
+} InbNormArgs;
+int inb_block_norm_fwd(const InbNormArgs *args, void *cuda_stream);
+int inb_block_norm_bwd(const InbNormArgs *args, void *cuda_stream);
+int inb_block_norm_work(const InbNormArgs *args, int64_t *elems);
+
+/* Gated feed-forward block over N rows: h = act(x wg^T) * (x wu^T), y = h wd^T; x [N, D], wg, wu [F, D], wd [D, F] of
+ * dtype bf16 or fp16, rows ld* elements apart; y, dx, dw* are contiguous.  Products accumulate in fp32; h, dg and du
+ * are rounded to dtype.  h [N, ldh] is written by the forward call; g, u [N, ldh] fp32 (both or neither) keep the
+ * projections for the backward call, which reads all three, takes dy [N, D], uses dg, du [N, ldh] as scratch and writes
+ * whichever of dx, (dwg, dwu), dwd are given.  ldh: a multiple of 8, at least F; h, g, u, dg, du, work: 16-byte aligned.
+ * work: inb_gated_ffn_work() bytes (for operands whose rows are not 16-byte aligned).  status: device word, set to 1 if a
+ * wait inside the kernel ran out (the outputs are then invalid), or NULL.
+ * -2: sizes, dtype or act out of range; -3: a required pointer is NULL or not aligned; -5: work is too small;
+ * -6: no tensor map could be made. */
+enum { INB_ACT_SILU = 0, INB_ACT_GELU = 1 };   /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
+#define INB_MAX_FFN (1 << 30)
+typedef struct {
+  int32_t dtype, act, D, F;
+  int64_t N, ldx, ldwg, ldwu, ldwd, ldh, lddy;
+  const void *x, *wg, *wu, *wd;
+  void *y, *h;
+  float *g, *u;
+  const void *dy;
+  void *dg, *du, *dx, *dwg, *dwu, *dwd, *work;
+  int64_t work_bytes;
+  int32_t *status;
+} InbFfnArgs;
+int inb_gated_ffn_fwd(const InbFfnArgs *args, void *cuda_stream);
+int inb_gated_ffn_bwd(const InbFfnArgs *args, void *cuda_stream);
+int inb_gated_ffn_work(const InbFfnArgs *args, int32_t backward, int64_t *bytes);
+
+/* Dropout of x [E, n] by the counter RNG: element i of env e is kept (and scaled by 65536 / (65536 - threshold)) where
+ * a 16-bit half of hash word i / 2 under the key (s0, env_id[e], episode[e], INB_CH_DROPOUT, ctr[e], stream) is >=
+ * threshold (low half: even i).  episode, ctr NULL: 0.  keys_out [E] (or NULL) receives the keys; with keys_in the
+ * keys are read instead of derived.  -2: sizes out of range; -3: a required pointer is NULL. */
+typedef struct {
+  int32_t dtype;
+  uint32_t threshold;           /* 0 .. 65536 */
+  int64_t E, n;
+  uint32_t s0, stream;
+  const int64_t *env_id, *episode, *ctr;
+  const uint32_t *keys_in;
+  uint32_t *keys_out;
+  const void *x;
+  void *y;
+} InbDropoutArgs;
+int inb_dropout(const InbDropoutArgs *args, void *cuda_stream);
+
+/* One token a row from logits [N, V] (rows ld apart) and uniforms u [N] in [0, 1): temperature (<= 0: the largest
+ * logit), then top-k (0: off), top-p (>= 1: off), min-p (0: off), each for all rows or (the *_row pointers) per row.
+ * mask (or NULL): bytes, rows ld_mask apart, 0 = not allowed.  NaN logits count as not allowed.  token -1 and logp
+ * -inf where nothing is allowed; otherwise logp is the token's log-probability among what the filters keep.
+ * -2: sizes out of range; -3: a required pointer is NULL. */
+typedef struct {
+  int32_t dtype, V;
+  int64_t N, ld, ld_mask;
+  const void *logits;
+  const uint8_t *mask;
+  const float *u;
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float *temperature_row, *top_p_row, *min_p_row;
+  const int32_t *top_k_row;
+  int64_t *token;
+  float *logp;
+} InbSampleArgs;
+int inb_sample(const InbSampleArgs *args, void *cuda_stream);
 
 /* ABI version of the loaded library (INB_ABI_VERSION).  No counterpart in the reference. */
 int inb_abi_version(void);

@@ -8,6 +8,7 @@ Public API (a drop-in for ``isaac_net.make_engine("L2", ...)`` on the uplink pat
     NRConfig, TrafficModel, Requests
     NetModule, IsaacNetCfg, TrafficRequest  (the Isaac-side module on the engine's radio, net_module.py)
     ShardedEngine, shard_invariant  (one batch split over several GPUs in one process, sharded.py)
+    policy_ops  (the operators of a policy over NetModule's observations: block_norm, counter_dropout, sample_logits)
 """
 import importlib as _importlib
 import importlib.abc as _abc
@@ -55,8 +56,11 @@ def __getattr__(name):
         return getattr(_importlib.import_module(__name__ + ".net_module"), name)
     if name in ("ShardedEngine", "shard_invariant"):
         return getattr(_importlib.import_module(__name__ + ".sharded"), name)
+    if name == "policy_ops":
+        return _importlib.import_module(__name__ + ".policy_ops")
     raise AttributeError(name)
 
 
 __all__ = ["make_engine", "NRConfig", "TrafficModel", "Requests", "NetModule", "IsaacNetCfg", "TrafficRequest",
-           "ShardedEngine", "shard_invariant"]
+           "ShardedEngine", "shard_invariant",
+           "policy_ops"]

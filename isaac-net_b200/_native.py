@@ -12,7 +12,7 @@ import os
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libisaac_net_b200_check.so" if os.environ.get("INB_CHECK") == "1"
                         else "libisaac_net_b200.so")
-ABI_VERSION = 17
+ABI_VERSION = 18
 MAX_ROWS = 128
 NCTR = 64
 BLK_REGIONS = 4        # INB_BLK_REGIONS
@@ -143,8 +143,46 @@ class InbObsArgs(ctypes.Structure):
                 + [(n, P) for n in OBS_IN + OBS_OUT])
 
 
+BF16, F16, F32 = 0, 1, 2          # INB_BF16, INB_F16, INB_F32
+MAX_NORM_D = 8192                # INB_MAX_NORM_D
+MAX_SAMPLE_V, MAX_SAMPLE_N = 1 << 22, 1 << 27
+MAX_DROPOUT_N = 0x1FFFFFFFF       # elements of one env
+
+
+class InbNormArgs(ctypes.Structure):
+    _fields_ = ([("dtype", i32), ("D", i32)] + [(n, i64) for n in ("N", "ldx", "ldh", "gate_rows")]
+                + [("scale", f32), ("eps", f32)]
+                + [(n, P) for n in ("x", "h", "w", "post", "gate", "y", "n", "stats")] + [("ldgy", i64), ("ldgn", i64)]
+                + [(n, P) for n in ("gy", "gn", "gx", "gh", "gw", "gpost", "ggate", "work")] + [("work_elems", i64)])
+
+
+ACTS = {"silu": 0, "gelu": 1}     # INB_ACT_SILU, INB_ACT_GELU
+MAX_FFN = 1 << 30
+
+
+class InbFfnArgs(ctypes.Structure):
+    _fields_ = ([(n, i32) for n in ("dtype", "act", "D", "F")]
+                + [(n, i64) for n in ("N", "ldx", "ldwg", "ldwu", "ldwd", "ldh", "lddy")]
+                + [(n, P) for n in ("x", "wg", "wu", "wd", "y", "h", "g", "u", "dy", "dg", "du", "dx", "dwg", "dwu",
+                                    "dwd", "work")] + [("work_bytes", i64), ("status", P)])
+
+
+class InbDropoutArgs(ctypes.Structure):
+    _fields_ = ([("dtype", i32), ("threshold", u32), ("E", i64), ("n", i64), ("s0", u32), ("stream", u32)]
+                + [(n, P) for n in ("env_id", "episode", "ctr", "keys_in", "keys_out", "x", "y")])
+
+
+class InbSampleArgs(ctypes.Structure):
+    _fields_ = ([("dtype", i32), ("V", i32), ("N", i64), ("ld", i64), ("ld_mask", i64)]
+                + [(n, P) for n in ("logits", "mask", "u")] + [(n, f32) for n in ("temperature", "top_p", "min_p")]
+                + [("top_k", i32)] + [(n, P) for n in ("temperature_row", "top_p_row", "min_p_row", "top_k_row", "token",
+                                                       "logp")])
+
+
+POLICY_EXPORTS = {"inb_block_norm_fwd": InbNormArgs, "inb_block_norm_bwd": InbNormArgs, "inb_dropout": InbDropoutArgs,
+                  "inb_sample": InbSampleArgs, "inb_gated_ffn_fwd": InbFfnArgs, "inb_gated_ffn_bwd": InbFfnArgs}    # int f(const Args *, void *stream)
 EXPORTS = ("inb_nr_step", "inb_nr_step_after", "inb_nr_step_noalloc", "inb_nr_reset", "inb_rng_draw", "inb_traffic_step",
-           "inb_store2", "inb_net_obs", "inb_abi_version")
+           "inb_store2", "inb_net_obs", "inb_abi_version", "inb_block_norm_work", "inb_gated_ffn_work", *POLICY_EXPORTS)
 NOALLOC_GAIN_MAX = 1 << 25
 _lib = None
 
@@ -178,6 +216,13 @@ def lib():
     L.inb_traffic_step.argtypes = [ctypes.POINTER(InbTrafficArgs), P]
     L.inb_net_obs.restype = ctypes.c_int
     L.inb_net_obs.argtypes = [ctypes.POINTER(InbObsArgs), P]
+    for name, args in POLICY_EXPORTS.items():
+        f = getattr(L, name)
+        f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(args), P]
+    L.inb_block_norm_work.restype = ctypes.c_int
+    L.inb_block_norm_work.argtypes = [ctypes.POINTER(InbNormArgs), ctypes.POINTER(i64)]
+    L.inb_gated_ffn_work.restype = ctypes.c_int
+    L.inb_gated_ffn_work.argtypes = [ctypes.POINTER(InbFfnArgs), i32, ctypes.POINTER(i64)]
     _lib = L
     return L
 

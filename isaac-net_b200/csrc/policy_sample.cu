@@ -1,0 +1,680 @@
+// sample_logits: one token a row from temperature, top-k, top-p, min-p and a given uniform, with its log-probability.
+//
+//   m = max l;  z_i = (l_i - m) / T;  w_i = exp(z_i);  q_i = floor(2^40 w_i)
+//   order: larger l first, ties by lower index
+//   top-k keeps the first k; top-p keeps an element while the mass before it is < p times the mass top-k left;
+//   min-p keeps w_i >= min_p;  token = first kept i by index with sum of q up to i > floor(u S), S = the kept mass
+//   logp = z - log(2^-40 S)
+//
+// The masses are integers, so a sum has one value whatever its order: no result depends on how a row is split over
+// lanes, warps or blocks, and the token is a function of the inputs alone.  2^-40 of the largest weight is the unit:
+// 2^20 elements together cannot be off by more than 2^-20 of the largest one, and 2^22 of them (the longest
+// row) do not overflow 64 bits.
+//
+// Rows of up to 128 logits take a warp each: the cut-offs are found by taking the largest remaining logit away until
+// the count or the mass is reached (one redux a step).  Longer rows take a block, or a cluster of 2 to 8 blocks when
+// there are fewer rows than SMs: the row stays in shared memory, a histogram over z finds the bin of the cut-off, and
+// histograms over the float's ordered bits narrow that bin to one value.  Either way the logits are read from memory
+// once, which is the floor; what bounds the kernel is the latency of its passes, not DRAM.
+#include <cooperative_groups.h>
+
+#include "policy_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace inb {
+namespace pol {
+
+constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;      // ordered bits of -inf
+constexpr float Z_SPAN = 28.f;                     // exp(-28) < 2^-40: below it the mass is 0
+constexpr float Q_ONE = 1099511627776.f;           // 2^40
+
+// order-preserving map of a float to unsigned
+__device__ __forceinline__ uint32_t key_of(float l) {
+  const uint32_t b = __float_as_uint(l);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// a logit as the operator sees it: masked and NaN entries are -inf, and -0 is +0
+__device__ __forceinline__ float clean(float l, bool ok) { return ok && l == l ? l + 0.f : -INFINITY; }
+
+struct RowParams {
+  float inv_t, top_p, min_p, u;
+  int k;               // 0: off
+};
+__device__ __forceinline__ RowParams row_params(const InbSampleArgs& a, int64_t row) {
+  RowParams p;
+  const float t = a.temperature_row ? a.temperature_row[row] : a.temperature;
+  p.top_p = a.top_p_row ? a.top_p_row[row] : a.top_p;
+  p.min_p = a.min_p_row ? a.min_p_row[row] : a.min_p;
+  p.k = a.top_k_row ? a.top_k_row[row] : a.top_k;
+  if (p.k < 0) p.k = 0;
+  if (!(t > 0.f)) {      // 0 (or below, or NaN): greedy
+    p.inv_t = 1.f;
+    p.k = 1;
+  } else {
+    p.inv_t = __fdiv_rn(1.f, t);
+  }
+  p.u = a.u[row];
+  return p;
+}
+__device__ __forceinline__ float z_of(float l, float m, float inv_t) {
+  return l == m ? 0.f : (l == -INFINITY ? -INFINITY : __fmul_rn(__fsub_rn(l, m), inv_t));
+}
+__device__ __forceinline__ long long q_of(float w) { return __float2ll_rz(__fmul_rn(w, Q_ONE)); }
+
+// how many of c equal masses q come before the mass thr is reached, `before` being what is above them (at least 1)
+__device__ __forceinline__ uint32_t ties_kept(long long before, long long q, uint32_t c, double thr) {
+  uint32_t lo = 1, hi = c;           // the first r in [1, c] with before + r q >= thr
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (__ll2double_rn(before + (long long)mid * q) >= thr)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+__device__ __forceinline__ double p_threshold(float p, long long total) {
+  const double t = __dmul_rn((double)p, __ll2double_rn(total));
+  return t > 1.0 ? t : 1.0;          // p <= 0 (or NaN) keeps the first element
+}
+__device__ __forceinline__ long long draw_at(float u, long long total) {
+  const double t = __dmul_rn((double)u, __ll2double_rn(total));
+  if (!(t > 0.0)) return 0;
+  const long long v = __double2ll_rz(t);
+  return v < total ? v : total - 1;
+}
+__device__ __forceinline__ float logp_of(float z, long long total) {
+  return (float)((double)z - log(__ll2double_rn(total) * (1.0 / 1099511627776.0)));
+}
+
+// ------------------------------------------------------------------------------------------------ a warp per row
+__device__ __forceinline__ long long warp_mass(uint32_t lo, uint32_t hi) {   // sums of the low 20 bits and of the rest
+  return (long long)__reduce_add_sync(M32_ALL, lo) + ((long long)__reduce_add_sync(M32_ALL, hi) << 20);
+}
+
+template <typename T, int EPL>
+__global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= a.N) return;
+  const T* lp = (const T*)a.logits + row * a.ld;
+  const uint8_t* mp = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  float l[EPL];
+  uint32_t key[EPL], top = 0;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int i = j * 32 + lane;
+    l[j] = -INFINITY;
+    if (i < a.V) l[j] = clean(to_f(lp[i]), mp == nullptr || mp[i] != 0);
+    key[j] = key_of(l[j]);
+    top = max(top, key[j]);
+  }
+  const RowParams p = row_params(a, row);
+  top = __reduce_max_sync(M32_ALL, top);
+  if (top <= KEY_NEG_INF) {
+    if (lane == 0) {
+      a.token[row] = -1;
+      a.logp[row] = -INFINITY;
+    }
+    return;
+  }
+  const float m = of_key(top);
+  float z[EPL], w[EPL];
+  long long q[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    z[j] = z_of(l[j], m, p.inv_t);
+    w[j] = expf(z[j]);
+    q[j] = l[j] == -INFINITY ? 0 : q_of(w[j]);
+  }
+  const uint32_t below = (1u << lane) - 1u;
+  if (p.k > 0 && p.k < a.V) {
+    uint32_t tau = M32_ALL, left = p.k;
+    while (true) {
+      uint32_t b = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && q[j] > 0 ? key[j] : 0u);
+      b = __reduce_max_sync(M32_ALL, b);
+      if (b == 0) break;                            // fewer than k with a mass: all stay
+      uint32_t c = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, key[j] == b));
+      tau = b;
+      if (c >= left) {
+        uint32_t rank = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          const uint32_t tie = __ballot_sync(M32_ALL, key[j] == tau);
+          if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= left)) q[j] = 0;
+          rank += __popc(tie);
+        }
+        break;
+      }
+      left -= c;
+    }
+  }
+  if (p.top_p < 1.f) {
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      lo += (uint32_t)q[j] & 0xFFFFFu;
+      hi += (uint32_t)(q[j] >> 20);
+    }
+    const double thr = p_threshold(p.top_p, warp_mass(lo, hi));
+    long long before = 0;
+    uint32_t tau = M32_ALL;
+    while (true) {
+      uint32_t b = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && q[j] > 0 ? key[j] : 0u);
+      b = __reduce_max_sync(M32_ALL, b);
+      if (b == 0) break;
+      uint32_t c = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, key[j] == b && q[j] > 0));
+      const long long qb = q_of(expf(z_of(of_key(b), m, p.inv_t)));
+      tau = b;
+      if (__ll2double_rn(before + (long long)c * qb) >= thr) {
+        const uint32_t r = ties_kept(before, qb, c, thr);
+        uint32_t rank = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          const uint32_t tie = __ballot_sync(M32_ALL, key[j] == tau && q[j] > 0);
+          if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= r)) q[j] = 0;
+          rank += __popc(tie);
+        }
+        break;
+      }
+      before += (long long)c * qb;
+    }
+  }
+  uint32_t lo = 0, hi = 0;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    if (w[j] < p.min_p && l[j] != m) q[j] = 0;      // the first element always stays
+    lo += (uint32_t)q[j] & 0xFFFFFu;
+    hi += (uint32_t)(q[j] >> 20);
+  }
+  const long long total = warp_mass(lo, hi);
+  long long at = draw_at(p.u, total);
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    long long run = q[j];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(M32_ALL, run, o);
+      if (lane >= o) run += v;
+    }
+    const uint32_t over = __ballot_sync(M32_ALL, run > at);
+    if (over != 0) {
+      if (lane == __ffs(over) - 1) {
+        a.token[row] = j * 32 + lane;
+        a.logp[row] = logp_of(z[j], total);
+      }
+      return;
+    }
+    at -= __shfl_sync(M32_ALL, run, 31);
+  }
+}
+
+// ------------------------------------------------------------------------------------- a block or cluster per row
+// What the blocks of a cluster exchange (read through distributed shared memory)
+struct Exchange {
+  uint32_t umax, umin;
+  long long mass;
+};
+
+template <int NT>
+struct BlockState {
+  uint32_t cnt[2][2 * NT];                 // histograms: [0] over z, kept; [1] of the refining levels
+  unsigned long long mass[2][2 * NT];
+  Exchange ex[2];                          // alternated, see all_reduce
+  uint32_t wu[32], wt[32];
+  long long wm[32];
+  uint32_t f_bin, f_cnt_above, f_count;
+  long long f_mass_above;
+};
+
+template <typename T, int NT, bool RES>
+struct Row {
+  const InbSampleArgs& a;
+  BlockState<NT>& s;
+  T* buf;
+  int64_t row;
+  int first, len;      // this block's slice
+  int ranks, rank;
+  float m, inv_t;
+  int par;
+
+  __device__ __forceinline__ float at(int i) const {
+    if (RES) return to_f(buf[i]);
+    return clean(to_f(((const T*)a.logits)[row * a.ld + first + i]),
+                 a.mask == nullptr || a.mask[row * a.ld_mask + first + i] != 0);
+  }
+  __device__ __forceinline__ void sync() {
+    if (ranks > 1)
+      cg::this_cluster().sync();
+    else
+      __syncthreads();
+  }
+  __device__ __forceinline__ BlockState<NT>* peer(int r) {
+    return ranks > 1 ? cg::this_cluster().map_shared_rank(&s, r) : &s;
+  }
+  // max, min and mass over the row; every thread gets them.  `ex` alternates between two slots, so the one
+  // barrier after the write also keeps a slot from being rewritten before every block has read it.
+  __device__ Exchange all_reduce(uint32_t umax, uint32_t umin, long long mass, bool with_mass) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    umax = __reduce_max_sync(M32_ALL, umax);
+    umin = __reduce_min_sync(M32_ALL, umin);
+    if (with_mass)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(M32_ALL, mass, o);
+    __syncthreads();
+    if (lane == 0) {
+      s.wu[wid] = umax;
+      s.wt[wid] = umin;
+      s.wm[wid] = mass;
+    }
+    __syncthreads();
+    par ^= 1;
+    if (threadIdx.x < 32) {
+      umax = lane < NT / 32 ? s.wu[lane] : 0u;
+      umin = lane < NT / 32 ? s.wt[lane] : M32_ALL;
+      mass = lane < NT / 32 ? s.wm[lane] : 0;
+      umax = __reduce_max_sync(M32_ALL, umax);
+      umin = __reduce_min_sync(M32_ALL, umin);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(M32_ALL, mass, o);
+      if (lane == 0) {
+        s.ex[par].umax = umax;
+        s.ex[par].umin = umin;
+        s.ex[par].mass = mass;
+      }
+    }
+    sync();
+    Exchange e = {0, M32_ALL, 0};
+    for (int r = 0; r < ranks; ++r) {
+      const Exchange& o = peer(r)->ex[par];
+      e.umax = max(e.umax, o.umax);
+      e.umin = min(e.umin, o.umin);
+      e.mass += o.mass;
+    }
+    return e;
+  }
+  // Over histogram h of the row (bin 0 = largest logits): the first bin at which the count (by_mass false) or the mass
+  // reaches the target, given what lies above the histogram.  False: no bin does.
+  __device__ bool cross(int h, bool by_mass, uint32_t k, double thr, uint32_t& cnt_above, long long& mass_above,
+                        uint32_t& bin, uint32_t& count) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, b = 2 * threadIdx.x;
+    __syncthreads();                          // the last call's result has been read
+    if (threadIdx.x == 0) s.f_bin = M32_ALL;
+    sync();                                   // every block's histogram is complete
+    uint32_t c[2] = {0, 0};
+    long long q[2] = {0, 0};
+    for (int r = 0; r < ranks; ++r) {
+      const BlockState<NT>* o = peer(r);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        c[i] += o->cnt[h][b + i];
+        q[i] += (long long)o->mass[h][b + i];
+      }
+    }
+    uint32_t ci = c[0] + c[1];
+    long long qi = q[0] + q[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t vc = __shfl_up_sync(M32_ALL, ci, o);
+      const long long vq = __shfl_up_sync(M32_ALL, qi, o);
+      if (lane >= o) {
+        ci += vc;
+        qi += vq;
+      }
+    }
+    if (lane == 31) {
+      s.wu[wid] = ci;
+      s.wm[wid] = qi;
+    }
+    __syncthreads();
+    uint32_t ca = cnt_above + ci - c[0] - c[1];
+    long long qa = mass_above + qi - q[0] - q[1];
+    for (int i = 0; i < wid; ++i) {
+      ca += s.wu[i];
+      qa += s.wm[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool was = by_mass ? __ll2double_rn(qa) >= thr : ca >= k;
+      const bool is = by_mass ? __ll2double_rn(qa + q[i]) >= thr : ca + c[i] >= k;
+      if (is && !was) {
+        s.f_bin = b + i;
+        s.f_cnt_above = ca;
+        s.f_mass_above = qa;
+        s.f_count = c[i];
+      }
+      ca += c[i];
+      qa += q[i];
+    }
+    sync();                                   // every block has read the histograms, and this one's result is there
+    bin = s.f_bin;
+    if (bin == M32_ALL) return false;
+    cnt_above = s.f_cnt_above;
+    mass_above = s.f_mass_above;
+    count = s.f_count;
+    return true;
+  }
+  __device__ __forceinline__ int z_bin(float z) const { return min(2 * NT - 1, (int)(-z * (2 * NT / Z_SPAN))); }
+
+  // The value tau at which the target is reached, how many hold it, and what lies above it.
+  __device__ bool find(bool by_mass, uint32_t k, double thr, uint32_t& tau, uint32_t& count, uint32_t& cnt_above,
+                       long long& mass_above) {
+    cnt_above = 0;
+    mass_above = 0;
+    uint32_t bin;
+    if (!cross(0, by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
+    uint32_t hi = 0, lo = M32_ALL;
+    for (int i = threadIdx.x; i < len; i += NT) {
+      const float l = at(i), z = z_of(l, m, inv_t);
+      if (z > -Z_SPAN && z_bin(z) == (int)bin && q_of(expf(z)) > 0) {
+        hi = max(hi, key_of(l));
+        lo = min(lo, key_of(l));
+      }
+    }
+    const Exchange e = all_reduce(hi, lo, 0, false);
+    hi = e.umax;
+    lo = e.umin;
+    while (hi != lo) {
+      const int bits = 32 - __clz(hi - lo), shift = max(0, bits - LOG_BINS);
+      __syncthreads();
+      for (int b = threadIdx.x; b < 2 * NT; b += NT) {
+        s.cnt[1][b] = 0;
+        s.mass[1][b] = 0;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < len; i += NT) {
+        const float l = at(i);
+        const uint32_t key = key_of(l);
+        if (key >= lo && key <= hi) {
+          const long long q = q_of(expf(z_of(l, m, inv_t)));
+          if (q > 0) {
+            const uint32_t b = (hi - key) >> shift;
+            atomicAdd(&s.cnt[1][b], 1u);
+            atomicAdd(&s.mass[1][b], (unsigned long long)q);
+          }
+        }
+      }
+      cross(1, by_mass, k, thr, cnt_above, mass_above, bin, count);   // the target lies within: a bin is found
+      hi = hi - (bin << shift);
+      const uint32_t span = (1u << shift) - 1u;
+      lo = hi - lo > span ? hi - span : lo;
+      if (shift == 0) lo = hi;
+    }
+    tau = hi;
+    return true;
+  }
+  static constexpr int LOG_BINS = NT == 128 ? 8 : 10;
+};
+
+template <typename T, int NT, bool RES>
+__global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int ranks, int slice) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  BlockState<NT>& s = *reinterpret_cast<BlockState<NT>*>(dyn);
+  constexpr int STATE = (sizeof(BlockState<NT>) + 15) / 16 * 16;
+  T* buf = reinterpret_cast<T*>(dyn + STATE);
+  const int64_t row = (int64_t)blockIdx.x / ranks;
+  const int rank = (int)(blockIdx.x % ranks);      // clusters are consecutive blocks: also the rank in the cluster
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  int first = rank * slice, len = a.V - first;
+  len = len < 0 ? 0 : (len > slice ? slice : len);
+  const RowParams p = row_params(a, row);
+  Row<T, NT, RES> R{a, s, buf, row, first, len, ranks, rank, 0.f, p.inv_t, 0};
+  const bool select_k = p.k > 0 && p.k < a.V, select_p = p.top_p < 1.f;
+
+  // the slice, and the row's largest logit
+  uint32_t top = 0;
+  if (RES) {
+    const T* lp = (const T*)a.logits + row * a.ld + first;
+    const uint8_t* mp = a.mask ? a.mask + row * a.ld_mask + first : nullptr;
+    constexpr int W = 16 / (int)sizeof(T);
+    int i0 = 0;
+    if (((uintptr_t)lp & 15) == 0 && ((uintptr_t)mp & (W - 1)) == 0) {
+      i0 = len / W * W;
+#pragma unroll 4
+      for (int i = threadIdx.x * W; i < i0; i += NT * W) {
+        Pack<T, W> v = ld<T, W>(lp + i);
+        Pack<uint8_t, W> ok;
+        if (mp) ok = ld<uint8_t, W>(mp + i);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float l = clean(to_f(v.v[e]), mp == nullptr || ok.v[e] != 0);
+          top = max(top, key_of(l));
+          v.v[e] = from_f<T>(l);
+        }
+        st<T, W>(buf + i, v);
+      }
+    }
+    for (int i = i0 + threadIdx.x; i < len; i += NT) {
+      const float l = clean(to_f(lp[i]), mp == nullptr || mp[i] != 0);
+      top = max(top, key_of(l));
+      buf[i] = from_f<T>(l);
+    }
+  } else {
+    for (int i = threadIdx.x; i < len; i += NT) top = max(top, key_of(R.at(i)));
+  }
+  if (select_k || select_p)
+    for (int b = threadIdx.x; b < 2 * NT; b += NT) {
+      s.cnt[0][b] = 0;
+      s.mass[0][b] = 0;
+    }
+  top = R.all_reduce(top, M32_ALL, 0, false).umax;
+  if (top <= KEY_NEG_INF) {
+    if (rank == 0 && threadIdx.x == 0) {
+      a.token[row] = -1;
+      a.logp[row] = -INFINITY;
+    }
+    R.sync();           // no block leaves while another may still read its shared memory
+    return;
+  }
+  const float m = of_key(top), inv_t = p.inv_t;
+  R.m = m;
+
+  // the cut-off (tau, kept): elements above tau stay, and the first `kept` of those equal to it
+  uint32_t tau = 0, kept = 0;
+  if (select_k || select_p) {
+    long long mass = 0;
+    for (int i = threadIdx.x; i < len; i += NT) {
+      const float z = z_of(R.at(i), m, inv_t);
+      if (z > -Z_SPAN) {
+        const long long q = q_of(expf(z));
+        if (q > 0) {
+          const int b = R.z_bin(z);
+          atomicAdd(&s.cnt[0][b], 1u);
+          atomicAdd(&s.mass[0][b], (unsigned long long)q);
+          mass += q;
+        }
+      }
+    }
+    long long total = 0;
+    if (!select_k) total = R.all_reduce(0, M32_ALL, mass, true).mass;
+    uint32_t count, above;
+    long long mass_above;
+    if (select_k) {
+      if (R.find(false, (uint32_t)p.k, 0.0, tau, count, above, mass_above)) {
+        kept = (uint32_t)p.k - above;
+        total = mass_above + (long long)kept * q_of(expf(z_of(of_key(tau), m, inv_t)));
+      } else {
+        total = R.all_reduce(0, M32_ALL, mass, true).mass;
+      }
+    }
+    if (select_p) {
+      const double thr = p_threshold(p.top_p, total);
+      uint32_t tp;
+      if (R.find(true, 0, thr, tp, count, above, mass_above)) {
+        tau = tp;
+        kept = ties_kept(mass_above, q_of(expf(z_of(of_key(tau), m, inv_t))), count, thr);
+      }
+    }
+  }
+
+  // the kept mass of each warp's run of the slice, by index
+  const int nw = NT / 32, seg = (len + nw * 32 - 1) / (nw * 32) * 32;
+  const int s0 = min(len, wid * seg), s1 = min(len, s0 + seg);
+  const float z_tau = z_of(of_key(tau), m, inv_t), w_tau = expf(z_tau);
+  const long long q_tau = tau == 0 || (w_tau < p.min_p && tau != top) ? 0 : q_of(w_tau);
+  long long mass = 0;
+  uint32_t ties = 0;
+  for (int i = s0 + lane; i < s1; i += 32) {
+    const float l = R.at(i);
+    const uint32_t key = key_of(l);
+    if (key == tau) {
+      ++ties;
+    } else if (key > tau) {
+      const float z = z_of(l, m, inv_t);
+      if (z > -Z_SPAN) {
+        const float w = expf(z);
+        if (!(w < p.min_p) || key == top) mass += q_of(w);
+      }
+    }
+  }
+  ties = __reduce_add_sync(M32_ALL, ties);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(M32_ALL, mass, o);
+  R.sync();
+  if (lane == 0) {
+    s.wt[wid] = ties;
+    s.wm[wid] = mass;
+  }
+  R.sync();
+  // every warp: the mass of the row, what comes before its own run, and the ties before it
+  long long total = 0, before = 0;
+  uint32_t seen = 0, my_seen = 0;
+  for (int r = 0; r < ranks; ++r) {
+    const BlockState<NT>* o = R.peer(r);
+    uint32_t t = lane < nw ? o->wt[lane] : 0u, ti = t;
+    long long v = lane < nw ? o->wm[lane] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t x = __shfl_up_sync(M32_ALL, ti, d);
+      if (lane >= d) ti += x;
+    }
+    const uint32_t tb = seen + ti - t;                                    // ties before warp `lane` of rank r
+    const uint32_t here = tb >= kept ? 0u : min(t, kept - tb);
+    v += (long long)here * q_tau;
+    long long vi = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long x = __shfl_up_sync(M32_ALL, vi, d);
+      if (lane >= d) vi += x;
+    }
+    if (r == rank) {
+      before = total + __shfl_sync(M32_ALL, vi - v, wid);
+      my_seen = __shfl_sync(M32_ALL, tb, wid);
+      mass = __shfl_sync(M32_ALL, v, wid);
+    }
+    total += __shfl_sync(M32_ALL, vi, 31);
+    seen += __shfl_sync(M32_ALL, ti, 31);
+  }
+  R.sync();             // no block leaves while another may still read its shared memory
+  const long long at = draw_at(p.u, total);
+  if (at < before || at >= before + mass) return;
+  long long run = before;
+  for (int i0 = s0; i0 < s1; i0 += 32) {
+    const int i = i0 + lane;
+    uint32_t key = 0;
+    float z = -INFINITY;
+    long long q = 0;
+    if (i < s1) {
+      const float l = R.at(i);
+      key = key_of(l);
+      z = z_of(l, m, inv_t);
+      if (key > tau && z > -Z_SPAN) {
+        const float w = expf(z);
+        if (!(w < p.min_p) || key == top) q = q_of(w);
+      }
+    }
+    const uint32_t tie = __ballot_sync(M32_ALL, i < s1 && key == tau);
+    if (i < s1 && key == tau && my_seen + __popc(tie & ((1u << lane) - 1u)) < kept) q = q_tau;
+    my_seen += __popc(tie);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long x = __shfl_up_sync(M32_ALL, q, d);
+      if (lane >= d) q += x;
+    }
+    const uint32_t over = __ballot_sync(M32_ALL, run + q > at);
+    if (over != 0) {
+      if (lane == __ffs(over) - 1) {
+        a.token[row] = first + i;
+        a.logp[row] = logp_of(z, total);
+      }
+      return;
+    }
+    run += __shfl_sync(M32_ALL, q, 31);
+  }
+}
+
+template <typename T, int NT, bool RES>
+static int block_launch(const InbSampleArgs& a, int ranks, int slice, cudaStream_t s) {
+  const size_t smem = (sizeof(BlockState<NT>) + 15) / 16 * 16 + (RES ? (size_t)slice * sizeof(T) : 0);
+  auto* k = sample_block_kernel<T, NT, RES>;
+  cudaError_t e;
+  if (smem > 48 * 1024) {
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return -100 - (int)e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.N * ranks));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = ranks;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, k, a, ranks, slice);
+  return e == cudaSuccess ? 0 : -100 - (int)e;
+}
+
+constexpr int SMEM_MOST = 227 * 1024;
+
+template <typename T>
+static int sample_type(const InbSampleArgs& a, cudaStream_t s) {
+  if (a.V <= 128) {
+    const unsigned grid = (unsigned)((a.N + 3) / 4);
+    if (a.V <= 32)
+      sample_warp_kernel<T, 1><<<grid, 128, 0, s>>>(a);
+    else if (a.V <= 64)
+      sample_warp_kernel<T, 2><<<grid, 128, 0, s>>>(a);
+    else
+      sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a);
+    return launch_status();
+  }
+  if (a.V <= 4096) return block_launch<T, 128, true>(a, 1, a.V, s);
+  // blocks of a row: enough to give every SM one while a slice keeps 4096 logits, and enough for the row to be resident
+  constexpr int CAP = (SMEM_MOST - (int)((sizeof(BlockState<512>) + 15) / 16 * 16)) / (int)sizeof(T) / 16 * 16;
+  int ranks = 1;
+  while (ranks < 8 && (a.N * ranks < sm_count() || (a.V + ranks - 1) / ranks > CAP) && a.V / (2 * ranks) >= 4096)
+    ranks *= 2;
+  const int slice = ((a.V + ranks - 1) / ranks + 15) / 16 * 16;
+  if (slice <= CAP) return block_launch<T, 512, true>(a, ranks, slice, s);
+  return block_launch<T, 512, false>(a, ranks, slice, s);
+}
+
+}  // namespace pol
+}  // namespace inb
+
+extern "C" int inb_sample(const InbSampleArgs* args, void* cuda_stream) {
+  if (args == nullptr) return -1;
+  const InbSampleArgs& a = *args;
+  if (a.dtype < 0 || a.dtype > 2 || a.N < 0 || a.N > INB_MAX_SAMPLE_N || a.V < 1 || a.V > INB_MAX_SAMPLE_V) return -2;
+  if (a.N == 0) return 0;
+  if (a.logits == nullptr || a.u == nullptr || a.token == nullptr || a.logp == nullptr) return -3;
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  if (a.dtype == INB_BF16) return inb::pol::sample_type<inb::pol::bf16>(a, s);
+  if (a.dtype == INB_F16) return inb::pol::sample_type<inb::pol::f16>(a, s);
+  return inb::pol::sample_type<float>(a, s);
+}
