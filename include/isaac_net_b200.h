@@ -408,6 +408,7 @@ int inb_net_obs(const InbObsArgs *args, void *cuda_stream);
  * counterpart in the reference, whose policies are the simulator's user's.  Element types of `dtype`: */
 enum { INB_BF16 = 0, INB_F16 = 1, INB_F32 = 2 };
 #define INB_MAX_NORM_D 8192        /* columns of inb_block_norm_* */
+#define INB_MAX_NORM_LD 0x3FFFFFFF  /* row strides, elements */
 #define INB_CH_DROPOUT 0x44u        /* counter-RNG channel of inb_dropout */
 #define INB_MAX_SAMPLE_V (1 << 22)  /* logits of a row of inb_sample */
 #define INB_MAX_SAMPLE_N (1 << 27)  /* rows */

@@ -145,6 +145,7 @@ class InbObsArgs(ctypes.Structure):
 
 BF16, F16, F32 = 0, 1, 2          # INB_BF16, INB_F16, INB_F32
 MAX_NORM_D = 8192                # INB_MAX_NORM_D
+MAX_NORM_LD = 0x3FFFFFFF          # INB_MAX_NORM_LD
 MAX_SAMPLE_V, MAX_SAMPLE_N = 1 << 22, 1 << 27
 MAX_DROPOUT_N = 0x1FFFFFFFF       # elements of one env
 

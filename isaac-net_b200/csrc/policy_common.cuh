@@ -40,6 +40,42 @@ __device__ __forceinline__ void st(T* p, const Pack<T, V>& v) {
   *reinterpret_cast<Pack<T, V>*>(p) = v;
 }
 
+// Two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// two elements to fp32 and back
+__device__ __forceinline__ float2 up2(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ float2 up2(bf16 a, bf16 b) { return __bfloat1622float2(__halves2bfloat162(a, b)); }
+__device__ __forceinline__ float2 up2(f16 a, f16 b) { return __half22float2(__halves2half2(a, b)); }
+__device__ __forceinline__ void down2(float2 v, float& a, float& b) {
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void down2(float2 v, bf16& a, bf16& b) {
+  const __nv_bfloat162 t = __float22bfloat162_rn(v);
+  a = t.x;
+  b = t.y;
+}
+__device__ __forceinline__ void down2(float2 v, f16& a, f16& b) {
+  const __half2 t = __float22half2_rn(v);
+  a = t.x;
+  b = t.y;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);

@@ -57,10 +57,11 @@ static NormPlan norm_plan(const InbNormArgs& a, bool bwd) {
   NormPlan p;
   p.V = norm_vec(a, bwd);
   const int esz = a.dtype == INB_F32 ? 4 : 2;
-  if (p.V * esz == 16)
-    p.IT = esz == 2 ? (a.D > 256 ? 2 : 1) : (a.D > 2048 ? 4 : 2);
-  else
-    p.IT = p.V == 2 ? 8 : 16;
+  // elements of a row in a thread: 16 in the forward pass (8 of a narrow row); 8 in the backward pass, whose column sums
+  // take the registers (16 spill: measured 664 us against 250 at N = 131072, D = 512), 16 of a row that 512 threads of 8
+  // do not cover
+  const int per = bwd ? (a.D > 4096 ? 16 : 8) : (a.D > 256 ? 16 : 8);
+  p.IT = per / p.V;
   const int lanes = (a.D + p.V * p.IT - 1) / (p.V * p.IT);
   p.tpr = (lanes + 31) / 32 * 32;
   p.groups = p.tpr >= 256 ? 1 : 256 / p.tpr;
@@ -81,250 +82,431 @@ __device__ __forceinline__ float row_sum(float v, int tpr, int group, int t, flo
   return s;
 }
 
-// MAXT: the largest block it is launched with, which sets the registers that a thread may hold a row in
-template <typename T, int V, int IT, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(InbNormArgs a, int tpr) {
-  __shared__ float red[8][64];
-  const int group = threadIdx.x / tpr, t = threadIdx.x % tpr, groups = blockDim.x / tpr;
-  const int D = a.D;
-  const float inv_d = 1.f / (float)D;
-  const T *w = (const T*)a.w, *post = (const T*)a.post;
-  Pack<T, V> wr[IT], pr[IT];
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int c = (i * tpr + t) * V;
-    if (c < D) {
-      wr[i] = ld<T, V>(w + c);
-      if (post) pr[i] = ld<T, V>(post + c);
-    }
+// Rows are cut into chunks that never cross a gate's rows: chunk c = rows [g R + k len, ...) of gate g = c / cpg.  All
+// counts are below 2^31.
+struct NormChunks {
+  uint32_t n;       // chunks
+  uint32_t rows;    // rows of one gate (N without a gate)
+  uint32_t len;     // rows of a chunk
+  uint32_t cpg;     // chunks of one gate
+};
+// Row strides in bytes, below 2^32: a row's address is one 32 x 32 -> 64-bit multiply-add
+struct NormStrides {
+  uint32_t x, h, gy, gn, d;      // d: of the contiguous tensors
+};
+__device__ __forceinline__ const char* row_at(const void* p, uint32_t row, uint32_t ld, int offset) {
+  return (const char*)p + ((uint64_t)row * ld + offset);
+}
+
+// A worker's walk over the rows of its chunks
+struct Cursor {
+  uint32_t c, gate, row, end;
+  bool first;      // row is the first of its chunk
+  __device__ __forceinline__ void start(const NormChunks& ch, uint32_t chunk) {
+    c = chunk;
+    first = true;
+    if (c >= ch.n) return;
+    gate = c / ch.cpg;
+    row = gate * ch.rows + (c - gate * ch.cpg) * ch.len;
+    end = min(row + ch.len, (gate + 1) * ch.rows);
   }
-  int par = 0;
-  const int64_t stride = (int64_t)gridDim.x * groups;
-  for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.N; row += stride) {
-    const T* xp = (const T*)a.x + row * a.ldx;
-    const T* hp = (const T*)a.h + row * a.ldh;
-    const T* gp = a.gate ? (const T*)a.gate + row / a.gate_rows * D : nullptr;
-    Pack<T, V> xr[IT], hr[IT], gr[IT];
+  __device__ __forceinline__ void next(const NormChunks& ch, uint32_t stride) {
+    first = false;
+    if (++row == end) start(ch, c + stride);
+  }
+};
+
+// Rows on their way: each thread copies its own part of the next rows of NT tensors (and 8 bytes of statistics) to its own
+// places of a ring of S rows in shared memory (cp.async) and reads only those back, so the ring needs no barrier and keeps
+// rows in flight that registers would have no room for.  S = 0: plain loads.
+template <typename T, int V, int IT, int MAXT, int NT, int WANT>
+struct Ring {
+  static constexpr int ROW = NT * IT * V * (int)sizeof(T) + 8;         // a thread's bytes of one row
+  static constexpr int MOST = 176 * 1024;
+  static constexpr int S = V * sizeof(T) < 4 ? 0 : (WANT * ROW * MAXT <= MOST ? WANT : (2 * ROW * MAXT <= MOST ? 2 : 0));
+  static constexpr int BLOCKS = S > 0 && S * ROW * MAXT <= 88 * 1024 ? 2 : 1;       // of them on an SM
+  static constexpr int ACCESS = V * (int)sizeof(T);
+  // access i of tensor k in slot `slot`, and the statistics: byte offsets from `mine()`, constant but for the slot
+  static __device__ __forceinline__ int place(int slot, int k, int i) { return slot * (ROW * MAXT) + (k * IT + i) * ACCESS * MAXT; }
+  static __device__ __forceinline__ unsigned char* mine(unsigned char* ring) { return ring + threadIdx.x * ACCESS; }
+  static __device__ __forceinline__ unsigned char* stat(unsigned char* ring, int slot) {
+    return ring + slot * (ROW * MAXT) + (ROW - 8) * MAXT + threadIdx.x * 8;
+  }
+  // zero the places: what is never copied (columns beyond D, absent tensors) reads as zero
+  static __device__ __forceinline__ void clear(unsigned char* ring) {
+#pragma unroll 1
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          Pack<T, V> z;
+#pragma unroll
+          for (int e = 0; e < V; ++e) z.v[e] = from_f<T>(0.f);
+          *reinterpret_cast<Pack<T, V>*>(mine(ring) + place(s, k, i)) = z;
+        }
+  }
+};
+template <typename T, int V, int IT, int MAXT>
+using FwdRing = Ring<T, V, IT, MAXT, 3, 3>;      // x, h, gate
+template <typename T, int V, int IT, int MAXT>
+using BwdRing = Ring<T, V, IT, MAXT, 5, 3>;      // x, h, gn, gy, gate
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  else if constexpr (BYTES == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A thread's part of a row: IT accesses of V elements, zero beyond D, as pairs of fp32 where it is worked on
+template <typename T, int V, int IT>
+struct Part {
+  static constexpr int N2 = V * IT / 2;
+  Pack<T, V> p[IT];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) p[i].v[e] = from_f<T>(0.f);
+  }
+  __device__ __forceinline__ void load(const T* row, int tpr, int t, int D) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int c = (i * tpr + t) * V;
-      if (c < D) {
-        xr[i] = ld<T, V>(xp + c);
-        if (a.h) hr[i] = ld<T, V>(hp + c);
-        if (gp) gr[i] = ld<T, V>(gp + c);
+      if (c < D) p[i] = ld<T, V>(row + c);
+    }
+  }
+  // to and from a ring: `row` is the tensor's row at this thread's first column
+  template <typename R>
+  static __device__ __forceinline__ void fetch(unsigned char* ring, int slot, int k, const char* row, int tpr, int t, int D) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      if ((i * tpr + t) * V < D)
+        copy_async<R::ACCESS>((uint32_t)__cvta_generic_to_shared(R::mine(ring) + R::place(slot, k, i)),
+                              row + i * tpr * R::ACCESS);
+  }
+  template <typename R>
+  __device__ __forceinline__ void read(unsigned char* ring, int slot, int k) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) p[i] = *reinterpret_cast<const Pack<T, V>*>(R::mine(ring) + R::place(slot, k, i));
+  }
+  __device__ __forceinline__ void store(T* row, int tpr, int t, int D) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int c = (i * tpr + t) * V;
+      if (c < D) st<T, V>(row + c, p[i]);
+    }
+  }
+  __device__ __forceinline__ float2 get(int j) const {
+    return V == 1 ? up2(p[2 * j].v[0], p[2 * j + 1].v[0]) : up2(p[2 * j / V].v[2 * j % V], p[2 * j / V].v[2 * j % V + 1]);
+  }
+  __device__ __forceinline__ void set(int j, float2 v) {
+    if constexpr (V == 1)
+      down2(v, p[2 * j].v[0], p[2 * j + 1].v[0]);
+    else
+      down2(v, p[2 * j / V].v[2 * j % V], p[2 * j / V].v[2 * j % V + 1]);
+  }
+  // the column of element 2 j (x) and of element 2 j + 1 (y)
+  static __device__ __forceinline__ int2 cols(int j, int tpr, int t) {
+    if (V == 1) return make_int2(2 * j * tpr + t, (2 * j + 1) * tpr + t);
+    const int c = (2 * j / V * tpr + t) * V + 2 * j % V;
+    return make_int2(c, c + 1);
+  }
+};
+
+// MAXT: the largest block it is launched with.
+template <typename T, int V, int IT, int MAXT>
+__global__ void __launch_bounds__(MAXT, FwdRing<T, V, IT, MAXT>::BLOCKS)
+norm_fwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks ch, const NormStrides ld) {
+  __shared__ float red[8][64];
+  extern __shared__ __align__(16) unsigned char ring[];
+  using P = Part<T, V, IT>;
+  using Rg = FwdRing<T, V, IT, MAXT>;
+  constexpr int S = Rg::S;
+  const int group = threadIdx.x / tpr, t = threadIdx.x % tpr, groups = blockDim.x / tpr;
+  const int D = a.D, col = t * V * (int)sizeof(T);
+  const float inv_d = 1.f / (float)D;
+  const bool has_h = a.h != nullptr, has_post = a.post != nullptr;
+  P w, post, x, h;
+  w.zero();
+  w.load((const T*)a.w, tpr, t, D);
+  post.zero();
+  if (has_post) post.load((const T*)a.post, tpr, t, D);
+  x.zero();
+  h.zero();
+  float2 coef[P::N2];                // scale * gate * post of the chunk
+  int par = 0;
+  const uint32_t stride = gridDim.x * groups;
+  Cursor at, ahead;
+  at.start(ch, blockIdx.x * groups + group);
+  ahead = at;
+  auto fetch = [&](int slot) {
+    if (ahead.c < ch.n) {
+      P::template fetch<Rg>(ring, slot, 0, row_at(a.x, ahead.row, ld.x, col), tpr, t, D);
+      if (has_h) P::template fetch<Rg>(ring, slot, 1, row_at(a.h, ahead.row, ld.h, col), tpr, t, D);
+      if (a.gate && ahead.first) P::template fetch<Rg>(ring, slot, 2, row_at(a.gate, ahead.gate, ld.d, col), tpr, t, D);
+      ahead.next(ch, stride);
+    }
+    copy_commit();
+  };
+  if constexpr (S > 0) {
+    Rg::clear(ring);
+    for (int i = 0; i < S - 1; ++i) fetch(i);
+  }
+  int slot = 0;
+  for (; at.c < ch.n; at.next(ch, stride)) {
+    P g;
+    g.zero();
+    if constexpr (S > 0) {
+      copy_wait<S - 2>();
+      x.template read<Rg>(ring, slot, 0);
+      if (has_h) h.template read<Rg>(ring, slot, 1);
+      if (a.gate && at.first) g.template read<Rg>(ring, slot, 2);
+      fetch(slot == 0 ? S - 1 : slot - 1);         // the place read in the last turn
+      slot = slot == S - 1 ? 0 : slot + 1;
+    } else {
+      x.load((const T*)row_at(a.x, at.row, ld.x, 0), tpr, t, D);
+      if (has_h) h.load((const T*)row_at(a.h, at.row, ld.h, 0), tpr, t, D);
+      if (a.gate && at.first) g.load((const T*)row_at(a.gate, at.gate, ld.d, 0), tpr, t, D);
+    }
+    if (at.first && has_h) {
+#pragma unroll
+      for (int j = 0; j < P::N2; ++j) {
+        coef[j] = both(a.scale);
+        if (has_post) coef[j] = mul2(coef[j], post.get(j));
+        if (a.gate) coef[j] = mul2(coef[j], g.get(j));
       }
     }
     float rh = 1.f;
-    if (post) {
-      float s = 0.f;
+    float2 s = both(0.f);
+    if (has_post) {
 #pragma unroll
-      for (int i = 0; i < IT; ++i)
-        if ((i * tpr + t) * V < D)
-#pragma unroll
-          for (int e = 0; e < V; ++e) s = fmaf(to_f(hr[i].v[e]), to_f(hr[i].v[e]), s);
-      rh = rsqrtf(row_sum(s, tpr, group, t, red[group], par) * inv_d + a.eps);
+      for (int j = 0; j < P::N2; ++j) s = fma2(h.get(j), h.get(j), s);
+      rh = rsqrtf(row_sum(s.x + s.y, tpr, group, t, red[group], par) * inv_d + a.eps);
     }
-    float y[IT][V], s = 0.f;
+    float2 y[P::N2];
+    s = both(0.f);
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int c = (i * tpr + t) * V;
-      if (c < D) {
-        Pack<T, V> o;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float v = to_f(xr[i].v[e]);
-          if (a.h) {
-            float p = to_f(hr[i].v[e]);
-            if (post) p = p * rh * to_f(pr[i].v[e]);
-            v += (gp ? a.scale * to_f(gr[i].v[e]) : a.scale) * p;
-          }
-          y[i][e] = v;
-          s = fmaf(v, v, s);
-          o.v[e] = from_f<T>(v);
-        }
-        if (a.y) st<T, V>((T*)a.y + row * D + c, o);
-      }
+    for (int j = 0; j < P::N2; ++j) {
+      y[j] = x.get(j);
+      if (has_h) y[j] = fma2(mul2(h.get(j), both(rh)), coef[j], y[j]);
+      s = fma2(y[j], y[j], s);
     }
-    const float ry = rsqrtf(row_sum(s, tpr, group, t, red[group], par) * inv_d + a.eps);
-    if (a.stats && t == 0) {
-      a.stats[2 * row] = rh;
-      a.stats[2 * row + 1] = ry;
-    }
+    if (has_h) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int c = (i * tpr + t) * V;
-      if (c < D) {
-        Pack<T, V> o;
-#pragma unroll
-        for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(y[i][e] * ry * to_f(wr[i].v[e]));
-        st<T, V>((T*)a.n + row * D + c, o);
-      }
+      for (int j = 0; j < P::N2; ++j) x.set(j, y[j]);
+      x.store((T*)row_at(a.y, at.row, ld.d, 0), tpr, t, D);
     }
+    const float ry = rsqrtf(row_sum(s.x + s.y, tpr, group, t, red[group], par) * inv_d + a.eps);
+    if (a.stats && t == 0) *reinterpret_cast<float2*>(a.stats + 2 * (int64_t)at.row) = make_float2(rh, ry);
+#pragma unroll
+    for (int j = 0; j < P::N2; ++j) x.set(j, mul2(mul2(y[j], both(ry)), w.get(j)));
+    x.store((T*)row_at(a.n, at.row, ld.d, 0), tpr, t, D);
   }
 }
 
-// Rows are cut into chunks that never cross a gate's rows: chunk c = rows [g R + k len, ...) of gate g = c / cpg.
-struct NormChunks {
-  int64_t n;       // chunks
-  int64_t rows;    // rows of one gate (N without a gate)
-  int64_t len;     // rows of a chunk
-  int cpg;         // chunks of one gate
-};
-
+// The row sums that gate's and post's gradients need differ only in factors that are fixed within a chunk:
+// e = sum over the chunk of t hh;  ggate = s post e, gpost = sum over the chunks of s gate e.  So the rows add to one
+// accumulator (and to gw's), and gpost's, touched once a chunk, lies in shared memory.
 template <typename T, int V, int IT, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(InbNormArgs a, int tpr, NormChunks ch) {
+__global__ void __launch_bounds__(MAXT, BwdRing<T, V, IT, MAXT>::BLOCKS)
+norm_bwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks ch, const NormStrides ld) {
   __shared__ float red[8][64];
-  extern __shared__ float comb[];
+  extern __shared__ __align__(16) unsigned char ring[];
+  using P = Part<T, V, IT>;
+  using Rg = BwdRing<T, V, IT, MAXT>;
+  constexpr int S = Rg::S;
   const int group = threadIdx.x / tpr, t = threadIdx.x % tpr, groups = blockDim.x / tpr;
-  const int D = a.D;
+  const int D = a.D, col = t * V * (int)sizeof(T);
+  float* sums = reinterpret_cast<float*>(ring + S * Rg::ROW * MAXT);   // [groups][D]
   const float inv_d = 1.f / (float)D;
-  const T *w = (const T*)a.w, *post = (const T*)a.post;
-  const bool has_h = a.h != nullptr;
-  Pack<T, V> wr[IT], pr[IT];
-  float aw[IT][V], ap[IT][V];
+  const bool has_h = a.h != nullptr, has_post = a.post != nullptr;
+  P w;
+  w.zero();
+  w.load((const T*)a.w, tpr, t, D);
+  float2 aw[P::N2], coef[P::N2], ae[P::N2];
+  float* mine = sums + group * D;
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int c = (i * tpr + t) * V;
-    if (c < D) {
-      wr[i] = ld<T, V>(w + c);
-      if (post) pr[i] = ld<T, V>(post + c);
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) aw[i][e] = ap[i][e] = 0.f;
+  for (int j = 0; j < P::N2; ++j) {
+    aw[j] = both(0.f);
+    const int2 c = P::cols(j, tpr, t);
+    if (c.x < D) mine[c.x] = 0.f;
+    if (c.y < D) mine[c.y] = 0.f;
   }
   int par = 0;
   float* part_gate = a.work + 2 * (int64_t)gridDim.x * D;
-  for (int64_t c0 = (int64_t)blockIdx.x * groups + group; c0 < ch.n; c0 += (int64_t)gridDim.x * groups) {
-    const int64_t gi = c0 / ch.cpg, k = c0 - gi * ch.cpg;
-    const int64_t r0 = gi * ch.rows + k * ch.len;
-    int64_t r1 = r0 + ch.len;
-    if (r1 > (gi + 1) * ch.rows) r1 = (gi + 1) * ch.rows;
-    Pack<T, V> gr[IT];
-    float ag[IT][V];
-#pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int c = (i * tpr + t) * V;
-      if (a.gate && c < D) gr[i] = ld<T, V>((const T*)a.gate + gi * D + c);
-#pragma unroll
-      for (int e = 0; e < V; ++e) ag[i][e] = 0.f;
+  const uint32_t stride = gridDim.x * groups;
+  Cursor at, ahead;
+  at.start(ch, blockIdx.x * groups + group);
+  ahead = at;
+  auto fetch = [&](int slot) {
+    if (ahead.c < ch.n) {
+      P::template fetch<Rg>(ring, slot, 0, row_at(a.x, ahead.row, ld.x, col), tpr, t, D);
+      if (has_h) P::template fetch<Rg>(ring, slot, 1, row_at(a.h, ahead.row, ld.h, col), tpr, t, D);
+      if (a.gn) P::template fetch<Rg>(ring, slot, 2, row_at(a.gn, ahead.row, ld.gn, col), tpr, t, D);
+      if (a.gy) P::template fetch<Rg>(ring, slot, 3, row_at(a.gy, ahead.row, ld.gy, col), tpr, t, D);
+      if (a.gate && ahead.first) P::template fetch<Rg>(ring, slot, 4, row_at(a.gate, ahead.gate, ld.d, col), tpr, t, D);
+      copy_async<8>((uint32_t)__cvta_generic_to_shared(Rg::stat(ring, slot)), row_at(a.stats, ahead.row, 8, 0));
+      ahead.next(ch, stride);
     }
-    for (int64_t row = r0; row < r1; ++row) {
-      Pack<T, V> xr[IT], hr[IT], yr[IT], nr[IT];
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int c = (i * tpr + t) * V;
-        if (c < D) {
-          xr[i] = ld<T, V>((const T*)a.x + row * a.ldx + c);
-          if (has_h) hr[i] = ld<T, V>((const T*)a.h + row * a.ldh + c);
-          if (a.gn) nr[i] = ld<T, V>((const T*)a.gn + row * a.ldgn + c);
-          if (a.gy) yr[i] = ld<T, V>((const T*)a.gy + row * a.ldgy + c);
-        }
+    copy_commit();
+  };
+  if constexpr (S > 0) {
+    Rg::clear(ring);
+    for (int i = 0; i < S - 1; ++i) fetch(i);
+  }
+  int slot = 0;
+  while (at.c < ch.n) {
+    const int here = slot;
+    // one tensor's part of this row; the passes below read it again rather than hold it, which would spill
+    auto take = [&](P& v, int k, const void* p, uint32_t stride) {
+      if constexpr (S > 0) {
+        asm volatile("" ::: "memory");
+        v.template read<Rg>(ring, here, k);
+      } else {
+        v.zero();
+        if (p != nullptr) v.load((const T*)row_at(p, at.row, stride, 0), tpr, t, D);
       }
-      const float rh = a.stats[2 * row], ry = a.stats[2 * row + 1];
-      float tt[IT][V];
-      // yh is recomputed from x and h, then replaced by t
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < IT; ++i)
-        if ((i * tpr + t) * V < D)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float v = to_f(xr[i].v[e]);
-            if (has_h) {
-              float p = to_f(hr[i].v[e]);
-              if (post) p = p * rh * to_f(pr[i].v[e]);
-              v += (a.gate ? a.scale * to_f(gr[i].v[e]) : a.scale) * p;
-            }
-            v *= ry;
-            tt[i][e] = v;
-            if (a.gn) {
-              const float gn = to_f(nr[i].v[e]);
-              aw[i][e] = fmaf(gn, v, aw[i][e]);
-              s = fmaf(gn * to_f(wr[i].v[e]), v, s);
-            }
-          }
-      const float c1 = a.gn ? row_sum(s, tpr, group, t, red[group], par) * inv_d : 0.f;
-      float s2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int c = (i * tpr + t) * V;
-        if (c < D) {
-          Pack<T, V> o;
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float q = a.gn ? to_f(nr[i].v[e]) * to_f(wr[i].v[e]) : 0.f;
-            float v = ry * (q - tt[i][e] * c1);
-            if (a.gy) v += to_f(yr[i].v[e]);
-            o.v[e] = from_f<T>(v);
-            if (has_h) {
-              const float hh = to_f(hr[i].v[e]) * rh;
-              const float p = post ? hh * to_f(pr[i].v[e]) : hh;
-              ag[i][e] = fmaf(v, p, ag[i][e]);
-              v *= a.gate ? a.scale * to_f(gr[i].v[e]) : a.scale;   // gp
-              if (post) {
-                ap[i][e] = fmaf(v, hh, ap[i][e]);
-                v *= to_f(pr[i].v[e]);
-                s2 = fmaf(v, hh, s2);
-              }
-              tt[i][e] = v;
-            }
-          }
-          st<T, V>((T*)a.gx + row * D + c, o);
-        }
+    };
+    float2 st;
+    if constexpr (S > 0) {
+      copy_wait<S - 2>();
+      st = *reinterpret_cast<const float2*>(Rg::stat(ring, slot));
+    } else {
+      st = *reinterpret_cast<const float2*>(row_at(a.stats, at.row, 8, 0));
+    }
+    if (at.first) {
+      P post, g;
+      post.zero();
+      if (has_post) post.load((const T*)a.post, tpr, t, D);
+      g.zero();
+      if (a.gate) {
+        if constexpr (S > 0)
+          g.template read<Rg>(ring, here, 4);
+        else
+          g.load((const T*)row_at(a.gate, at.gate, ld.d, 0), tpr, t, D);
       }
-      if (has_h) {
-        const float c2 = post ? row_sum(s2, tpr, group, t, red[group], par) * inv_d : 0.f;
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int c = (i * tpr + t) * V;
-          if (c < D) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              o.v[e] = from_f<T>(post ? rh * (tt[i][e] - to_f(hr[i].v[e]) * rh * c2) : tt[i][e]);
-            st<T, V>((T*)a.gh + row * D + c, o);
-          }
-        }
+      for (int j = 0; j < P::N2; ++j) {
+        ae[j] = both(0.f);
+        coef[j] = both(a.scale);
+        if (has_post) coef[j] = mul2(coef[j], post.get(j));
+        if (a.gate) coef[j] = mul2(coef[j], g.get(j));
       }
     }
-    if (a.ggate) {
+    if constexpr (S > 0) {
+      fetch(slot == 0 ? S - 1 : slot - 1);         // the place read in the last turn
+      slot = slot == S - 1 ? 0 : slot + 1;
+    }
+    const float rh = st.x, ry = st.y;
+    float2 v[P::N2], s = both(0.f);
+    {
+      P x, h, gn;                                  // v = yh
+      take(x, 0, a.x, ld.x);
+      take(h, 1, a.h, ld.h);
+      take(gn, 2, a.gn, ld.gn);
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int c = (i * tpr + t) * V;
-        if (c < D) {
-          if (ch.cpg == 1) {
-            Pack<T, V> o;
+      for (int j = 0; j < P::N2; ++j) {
+        v[j] = x.get(j);
+        if (has_h) v[j] = fma2(mul2(h.get(j), both(rh)), coef[j], v[j]);
+        v[j] = mul2(v[j], both(ry));
+        const float2 q = gn.get(j);
+        aw[j] = fma2(q, v[j], aw[j]);
+        s = fma2(mul2(q, w.get(j)), v[j], s);
+      }
+    }
+    const float c1 = row_sum(s.x + s.y, tpr, group, t, red[group], par) * inv_d;
+    s = both(0.f);
+    {
+      P gy, h, gn;                                 // v = t, then gp post
+      take(gn, 2, a.gn, ld.gn);
+      take(gy, 3, a.gy, ld.gy);
+      take(h, 1, a.h, ld.h);
 #pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = from_f<T>(a.scale * ag[i][e]);
-            st<T, V>((T*)a.ggate + gi * D + c, o);
-          } else {
+      for (int j = 0; j < P::N2; ++j) {
+        const float2 q = fma2(v[j], both(-c1), mul2(gn.get(j), w.get(j)));
+        v[j] = fma2(q, both(ry), gy.get(j));
+        gy.set(j, v[j]);
+        if (has_h) {
+          const float2 hh = mul2(h.get(j), both(rh));
+          ae[j] = fma2(v[j], hh, ae[j]);
+          v[j] = mul2(v[j], coef[j]);
+          s = fma2(v[j], hh, s);
+        }
+      }
+      gy.store((T*)row_at(a.gx, at.row, ld.d, 0), tpr, t, D);
+    }
+    if (has_h) {
+      const float c2 = has_post ? row_sum(s.x + s.y, tpr, group, t, red[group], par) * inv_d : 0.f;
+      P h;
+      take(h, 1, a.h, ld.h);
 #pragma unroll
-            for (int e = 0; e < V; ++e) part_gate[c0 * D + c + e] = a.scale * ag[i][e];
+      for (int j = 0; j < P::N2; ++j) {
+        if (has_post) v[j] = mul2(fma2(mul2(h.get(j), both(rh)), both(-c2), v[j]), both(rh));
+        h.set(j, v[j]);
+      }
+      h.store((T*)row_at(a.gh, at.row, ld.d, 0), tpr, t, D);
+    }
+    const uint32_t gate = at.gate, chunk = at.c;
+    const bool alone = at.first;
+    at.next(ch, stride);
+    if (at.first && (a.ggate || has_post)) {           // that was the chunk's last row
+      P post, g, x;
+      post.zero();
+      g.zero();
+      if (a.gate) {
+        bool loaded = false;
+        if constexpr (S > 0)
+          if (alone) {
+            g.template read<Rg>(ring, here, 4);
+            loaded = true;
+          }
+        if (!loaded) g.load((const T*)row_at(a.gate, gate, ld.d, 0), tpr, t, D);
+      }
+      if (has_post) post.load((const T*)a.post, tpr, t, D);
+#pragma unroll
+      for (int j = 0; j < P::N2; ++j) {
+        const int2 c = P::cols(j, tpr, t);
+        ae[j] = mul2(ae[j], both(a.scale));
+        const float2 add = a.gate ? mul2(ae[j], g.get(j)) : ae[j];
+        if (c.x < D) mine[c.x] += add.x;
+        if (c.y < D) mine[c.y] += add.y;
+        if (a.ggate) {
+          if (has_post) ae[j] = mul2(ae[j], post.get(j));
+          x.set(j, ae[j]);
+          if (ch.cpg > 1) {
+            if (c.x < D) part_gate[(int64_t)chunk * D + c.x] = ae[j].x;
+            if (c.y < D) part_gate[(int64_t)chunk * D + c.y] = ae[j].y;
           }
         }
       }
+      if (a.ggate && ch.cpg == 1) x.store((T*)a.ggate + (int64_t)gate * D, tpr, t, D);
     }
   }
-  // the block's column sums: group after group in order, then one partial row of each kind
-  for (int kind = 0; kind < (post ? 2 : 1); ++kind) {
-    for (int g = 0; g < groups; ++g) {
-      if (g == group) {
+  // the block's column sums, over its groups in order: gpost's lie in shared memory, then gw's take their place
+  float* out = a.work + (int64_t)blockIdx.x * 2 * D;
+  for (int kind = 1; kind >= 0; --kind) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < D; c += blockDim.x) {
+      float s = 0.f;
+      for (int g = 0; g < groups; ++g) s += sums[g * D + c];
+      out[kind * D + c] = s;
+    }
+    if (kind == 0) break;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int c = (i * tpr + t) * V;
-          if (c < D)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float v = kind ? ap[i][e] : aw[i][e];
-              const float sum = g == 0 ? v : comb[c + e] + v;
-              if (g == groups - 1)
-                a.work[((int64_t)blockIdx.x * 2 + kind) * D + c + e] = sum;
-              else
-                comb[c + e] = sum;
-            }
-        }
-      }
-      __syncthreads();
+    for (int j = 0; j < P::N2; ++j) {
+      const int2 c = P::cols(j, tpr, t);
+      if (c.x < D) mine[c.x] = aw[j].x;
+      if (c.y < D) mine[c.y] = aw[j].y;
     }
   }
 }
@@ -384,71 +566,81 @@ static int norm_blocks(const NormPlan& p, int64_t units, int per_sm) {
   return (int)(need < most ? need : most);
 }
 
-static NormChunks norm_chunks(const InbNormArgs& a, const NormPlan& p, int per_sm) {
+// per_sm: blocks that an SM holds (see Ring)
+static NormChunks norm_chunks(const InbNormArgs& a, const NormPlan& p, bool bwd, int per_sm) {
   NormChunks c;
-  const int64_t workers = (int64_t)sm_count() * per_sm * p.groups;
-  c.rows = a.gate != nullptr ? a.gate_rows : a.N;
-  const int64_t gates = a.N / c.rows;
+  // enough chunks for every worker; the forward pass, whose chunks leave no partial sums, takes four times as many so
+  // that the workers end together
+  const int64_t workers = (int64_t)sm_count() * per_sm * p.groups * (bwd ? 1 : 4);
+  const int64_t rows = a.gate != nullptr ? a.gate_rows : a.N, gates = a.N / rows;
   int64_t cpg = (workers + gates - 1) / gates;
-  if (cpg > c.rows) cpg = c.rows;
-  c.len = (c.rows + cpg - 1) / cpg;
-  c.cpg = (int)((c.rows + c.len - 1) / c.len);
-  c.n = gates * c.cpg;
+  if (cpg > rows) cpg = rows;
+  const int64_t len = (rows + cpg - 1) / cpg;
+  c.rows = (uint32_t)rows;
+  c.len = (uint32_t)len;
+  c.cpg = (uint32_t)((rows + len - 1) / len);
+  c.n = (uint32_t)(gates * c.cpg);
   return c;
 }
 
-static int norm_bwd_per_sm(const NormPlan& p) { return p.block > 512 ? 1 : 2; }
-
-static int64_t norm_work(const InbNormArgs& a) {
-  const NormPlan p = norm_plan(a, true);
-  const NormChunks ch = norm_chunks(a, p, norm_bwd_per_sm(p));
-  const int64_t blocks = norm_blocks(p, ch.n, norm_bwd_per_sm(p));
-  return (2 * blocks + (a.gate != nullptr && ch.cpg > 1 ? ch.n : 0)) * a.D;
-}
-
+// Runs the call, or (elems != NULL) says how many floats of work it needs
 template <typename T, int V, int IT, int MAXT>
-static void norm_launch(const InbNormArgs& a, const NormPlan& p, bool bwd, cudaStream_t s) {
+static int norm_launch(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_t* elems, cudaStream_t s) {
+  using F = FwdRing<T, V, IT, MAXT>;
+  using B = BwdRing<T, V, IT, MAXT>;
+  const int per_sm = bwd ? B::BLOCKS : F::BLOCKS;
+  const NormChunks ch = norm_chunks(a, p, bwd, per_sm);
+  const int blocks = norm_blocks(p, ch.n, per_sm);
+  if (bwd) {
+    const int64_t need = (2 * (int64_t)blocks + (a.gate != nullptr && ch.cpg > 1 ? ch.n : 0)) * a.D;
+    if (elems != nullptr) {
+      *elems = need;
+      return 0;
+    }
+    if (a.work_elems < need) return -5;
+  }
+  const int smem = bwd ? B::S * B::ROW * MAXT + p.groups * a.D * 4 : F::S * F::ROW * MAXT;
+  const uint32_t esz = sizeof(T);
+  const NormStrides ld = {(uint32_t)a.ldx * esz, (uint32_t)a.ldh * esz, (uint32_t)a.ldgy * esz, (uint32_t)a.ldgn * esz,
+                          (uint32_t)a.D * esz};
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(bwd ? (const void*)norm_bwd_kernel<T, V, IT, MAXT>
+                                                   : (const void*)norm_fwd_kernel<T, V, IT, MAXT>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return -100 - (int)e;
+  }
   if (!bwd) {
-    norm_fwd_kernel<T, V, IT, MAXT><<<norm_blocks(p, a.N, p.block > 512 ? 2 : 8), p.block, 0, s>>>(a, p.tpr);
-    return;
+    norm_fwd_kernel<T, V, IT, MAXT><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
+    return launch_status();
   }
-  const NormChunks ch = norm_chunks(a, p, norm_bwd_per_sm(p));
-  const int blocks = norm_blocks(p, ch.n, norm_bwd_per_sm(p));
-  const int smem = p.groups > 1 ? a.D * 4 : 0;
-  norm_bwd_kernel<T, V, IT, MAXT><<<blocks, p.block, smem, s>>>(a, p.tpr, ch);
-  const dim3 grid((a.D + 31) / 32, 2 + (a.gate != nullptr && ch.cpg > 1 ? (unsigned)(ch.n / ch.cpg) : 0));
+  norm_bwd_kernel<T, V, IT, MAXT><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
+  const dim3 grid((a.D + 31) / 32, 2 + (a.gate != nullptr && ch.cpg > 1 ? ch.n / ch.cpg : 0));
   norm_sum_kernel<T><<<grid, 1024, 0, s>>>(a, blocks, ch);
-}
-
-template <typename T, int V, int IT>
-static void norm_go(const InbNormArgs& a, const NormPlan& p, bool bwd, cudaStream_t s) {
-  if (p.block <= 256) norm_launch<T, V, IT, 256>(a, p, bwd, s);
-  else if constexpr (V * IT == 16) {     // narrow rows, of fewer elements a thread, never need more threads
-    norm_launch<T, V, IT, 512>(a, p, bwd, s);
-  }
-}
-
-template <typename T>
-static int norm_type(const InbNormArgs& a, bool bwd, cudaStream_t s) {
-  const NormPlan p = norm_plan(a, bwd);
-  constexpr int W = 16 / (int)sizeof(T);
-  if (p.V == W) {
-    if (p.IT == 1) norm_go<T, W, 1>(a, p, bwd, s);
-    else if (p.IT == 2) norm_go<T, W, 2>(a, p, bwd, s);
-    else if constexpr (sizeof(T) == 4) norm_go<T, W, 4>(a, p, bwd, s);
-  } else if (p.V == 2) {
-    if constexpr (sizeof(T) == 2) norm_go<T, 2, 8>(a, p, bwd, s);
-  } else {
-    norm_go<T, 1, 16>(a, p, bwd, s);
-  }
   return launch_status();
 }
 
-static int norm_run(const InbNormArgs& a, bool bwd, void* stream) {
+template <typename T, int V>
+static int norm_go(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_t* elems, cudaStream_t s) {
+  const bool wide = p.block > 256;
+  if (p.IT * V == 16)
+    return wide ? norm_launch<T, V, 16 / V, 512>(a, p, bwd, elems, s) : norm_launch<T, V, 16 / V, 256>(a, p, bwd, elems, s);
+  return wide ? norm_launch<T, V, 8 / V, 512>(a, p, bwd, elems, s) : norm_launch<T, V, 8 / V, 256>(a, p, bwd, elems, s);
+}
+
+template <typename T>
+static int norm_type(const InbNormArgs& a, bool bwd, int64_t* elems, cudaStream_t s) {
+  const NormPlan p = norm_plan(a, bwd);
+  if (p.V == 16 / (int)sizeof(T)) return norm_go<T, 16 / (int)sizeof(T)>(a, p, bwd, elems, s);
+  if constexpr (sizeof(T) == 2)
+    if (p.V == 2) return norm_go<T, 2>(a, p, bwd, elems, s);
+  return norm_go<T, 1>(a, p, bwd, elems, s);
+}
+
+static int norm_run(const InbNormArgs& a, bool bwd, int64_t* elems, void* stream) {
   cudaStream_t s = (cudaStream_t)stream;
-  if (a.dtype == INB_BF16) return norm_type<bf16>(a, bwd, s);
-  if (a.dtype == INB_F16) return norm_type<f16>(a, bwd, s);
-  return norm_type<float>(a, bwd, s);
+  if (a.dtype == INB_BF16) return norm_type<bf16>(a, bwd, elems, s);
+  if (a.dtype == INB_F16) return norm_type<f16>(a, bwd, elems, s);
+  return norm_type<float>(a, bwd, elems, s);
 }
 
 }  // namespace pol
@@ -457,7 +649,7 @@ static int norm_run(const InbNormArgs& a, bool bwd, void* stream) {
 extern "C" int inb_block_norm_fwd(const InbNormArgs* args, void* cuda_stream) {
   const int rc = inb::pol::norm_check(args, false);
   if (rc != 0 || args->N == 0) return rc;
-  return inb::pol::norm_run(*args, false, cuda_stream);
+  return inb::pol::norm_run(*args, false, nullptr, cuda_stream);
 }
 
 extern "C" int inb_block_norm_work(const InbNormArgs* args, int64_t* elems) {
@@ -465,13 +657,11 @@ extern "C" int inb_block_norm_work(const InbNormArgs* args, int64_t* elems) {
   *elems = 0;
   const int rc = inb::pol::norm_check(args, false, true);
   if (rc != 0 || args->N == 0) return rc;
-  *elems = inb::pol::norm_work(*args);
-  return 0;
+  return inb::pol::norm_run(*args, true, elems, nullptr);
 }
 
 extern "C" int inb_block_norm_bwd(const InbNormArgs* args, void* cuda_stream) {
   const int rc = inb::pol::norm_check(args, true);
   if (rc != 0 || args->N == 0) return rc;
-  if (args->work_elems < inb::pol::norm_work(*args)) return -5;
-  return inb::pol::norm_run(*args, true, cuda_stream);
+  return inb::pol::norm_run(*args, true, nullptr, cuda_stream);
 }

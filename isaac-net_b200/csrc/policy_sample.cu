@@ -27,6 +27,7 @@ namespace pol {
 
 constexpr uint32_t KEY_NEG_INF = 0x007FFFFFu;      // ordered bits of -inf
 constexpr float Z_SPAN = 28.f;                     // exp(-28) < 2^-40: below it the mass is 0
+constexpr float Z_SURE = 27.f;                     // exp(-27) > 2^-39: above it the mass is not 0
 constexpr float Q_ONE = 1099511627776.f;           // 2^40
 
 // order-preserving map of a float to unsigned
@@ -92,94 +93,72 @@ __device__ __forceinline__ float logp_of(float z, long long total) {
 }
 
 // ------------------------------------------------------------------------------------------------ a warp per row
-__device__ __forceinline__ long long warp_mass(uint32_t lo, uint32_t hi) {   // sums of the low 20 bits and of the rest
+// The sums of a row of up to 128 masses, from the masses' low 20 bits and the rest
+__device__ __forceinline__ long long warp_mass(uint32_t lo, uint32_t hi) {
   return (long long)__reduce_add_sync(M32_ALL, lo) + ((long long)__reduce_add_sync(M32_ALL, hi) << 20);
 }
 
-template <typename T, int EPL>
-__global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= a.N) return;
-  const T* lp = (const T*)a.logits + row * a.ld;
-  const uint8_t* mp = a.mask ? a.mask + row * a.ld_mask : nullptr;
-  float l[EPL];
-  uint32_t key[EPL], top = 0;
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int i = j * 32 + lane;
-    l[j] = -INFINITY;
-    if (i < a.V) l[j] = clean(to_f(lp[i]), mp == nullptr || mp[i] != 0);
-    key[j] = key_of(l[j]);
-    top = max(top, key[j]);
-  }
-  const RowParams p = row_params(a, row);
-  top = __reduce_max_sync(M32_ALL, top);
-  if (top <= KEY_NEG_INF) {
-    if (lane == 0) {
-      a.token[row] = -1;
-      a.logp[row] = -INFINITY;
-    }
-    return;
-  }
-  const float m = of_key(top);
-  float z[EPL], w[EPL];
+// One row: `key`, `z`, `q` of its elements, EPL a lane, element j * 32 + lane.  cut() zeroes the masses that a filter takes
+// away: by count (top-k) or by mass (top-p).  The largest remaining value is taken away until the target is reached; five
+// steps of bisection over z before that leave it a sixteenth of the range (0 .. -4, or -4 .. -28) to walk.
+template <int EPL>
+struct WarpRow {
+  uint32_t key[EPL];
+  float z[EPL];
   long long q[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    z[j] = z_of(l[j], m, p.inv_t);
-    w[j] = expf(z[j]);
-    q[j] = l[j] == -INFINITY ? 0 : q_of(w[j]);
-  }
-  const uint32_t below = (1u << lane) - 1u;
-  if (p.k > 0 && p.k < a.V) {
-    uint32_t tau = M32_ALL, left = p.k;
-    while (true) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && q[j] > 0 ? key[j] : 0u);
-      b = __reduce_max_sync(M32_ALL, b);
-      if (b == 0) break;                            // fewer than k with a mass: all stay
-      uint32_t c = 0;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, key[j] == b));
-      tau = b;
-      if (c >= left) {
-        uint32_t rank = 0;
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) {
-          const uint32_t tie = __ballot_sync(M32_ALL, key[j] == tau);
-          if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= left)) q[j] = 0;
-          rank += __popc(tie);
-        }
-        break;
-      }
-      left -= c;
-    }
-  }
-  if (p.top_p < 1.f) {
+
+  __device__ __forceinline__ long long mass_from(float least) const {
     uint32_t lo = 0, hi = 0;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      lo += (uint32_t)q[j] & 0xFFFFFu;
-      hi += (uint32_t)(q[j] >> 20);
-    }
-    const double thr = p_threshold(p.top_p, warp_mass(lo, hi));
+    for (int j = 0; j < EPL; ++j)
+      if (z[j] >= least) {
+        lo += (uint32_t)q[j] & 0xFFFFFu;
+        hi += (uint32_t)(q[j] >> 20);
+      }
+    return warp_mass(lo, hi);
+  }
+  __device__ __forceinline__ long long count_from(float least) const {
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, z[j] >= least && q[j] > 0));
+    return c;
+  }
+  template <bool MASS>
+  __device__ __forceinline__ void cut(long long target) {
+    // z >= up is above the target's value, z >= down holds it (or every element stays)
+    float up = 1.f, down = -Z_SPAN, mid = -4.f;
     long long before = 0;
+#pragma unroll 1
+    for (int i = 0; i < 5; ++i) {
+      const long long v = MASS ? mass_from(mid) : count_from(mid);
+      if (v >= target) {
+        down = mid;
+      } else {
+        up = mid;
+        before = v;
+      }
+      mid = 0.5f * (fminf(up, 0.f) + down);
+    }
     uint32_t tau = M32_ALL;
+#pragma unroll 1
     while (true) {
       uint32_t b = 0;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && q[j] > 0 ? key[j] : 0u);
+      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && z[j] < up && q[j] > 0 ? key[j] : 0u);
       b = __reduce_max_sync(M32_ALL, b);
-      if (b == 0) break;
+      if (b == 0) return;                    // the target is beyond what there is: all stay
       uint32_t c = 0;
+      long long qb = 1;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, key[j] == b && q[j] > 0));
-      const long long qb = q_of(expf(z_of(of_key(b), m, p.inv_t)));
+      for (int j = 0; j < EPL; ++j) {
+        const uint32_t tie = __ballot_sync(M32_ALL, key[j] == b && q[j] > 0);
+        if (MASS && tie != 0) qb = __shfl_sync(M32_ALL, q[j], __ffs(tie) - 1);
+        c += __popc(tie);
+      }
       tau = b;
-      if (__ll2double_rn(before + (long long)c * qb) >= thr) {
-        const uint32_t r = ties_kept(before, qb, c, thr);
+      if (before + (long long)c * qb >= target) {
+        const uint32_t r = c == 1 ? 1u : (uint32_t)((target - before + qb - 1) / qb);     // the first r of them
+        const uint32_t below = (1u << (threadIdx.x & 31)) - 1u;
         uint32_t rank = 0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
@@ -187,37 +166,100 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a) {
           if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= r)) q[j] = 0;
           rank += __popc(tie);
         }
-        break;
+        return;
       }
       before += (long long)c * qb;
     }
   }
-  uint32_t lo = 0, hi = 0;
+};
+
+// A warp takes `rows` consecutive rows: lane i holds the settings of row i and finishes it (the logarithm) with the others
+template <typename T, int EPL>
+__global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a, int rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * rows;
+  if (first >= a.N) return;
+  const int n = a.N - first < rows ? (int)(a.N - first) : rows;
+  RowParams mine = {1.f, 1.f, 0.f, 0.f, 0};
+  if (lane < n) mine = row_params(a, first + lane);
+  int my_token = -1;
+  float my_z = 0.f;
+  long long my_total = 0;
+  T next[EPL];
+  bool ok[EPL];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    if (w[j] < p.min_p && l[j] != m) q[j] = 0;      // the first element always stays
-    lo += (uint32_t)q[j] & 0xFFFFFu;
-    hi += (uint32_t)(q[j] >> 20);
-  }
-  const long long total = warp_mass(lo, hi);
-  long long at = draw_at(p.u, total);
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    long long run = q[j];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(M32_ALL, run, o);
-      if (lane >= o) run += v;
-    }
-    const uint32_t over = __ballot_sync(M32_ALL, run > at);
-    if (over != 0) {
-      if (lane == __ffs(over) - 1) {
-        a.token[row] = j * 32 + lane;
-        a.logp[row] = logp_of(z[j], total);
+    for (int j = 0; j < EPL; ++j) {
+      const int i = j * 32 + lane;
+      ok[j] = i < a.V;
+      if (ok[j]) {
+        next[j] = ((const T*)a.logits)[row * a.ld + i];
+        if (a.mask) ok[j] = a.mask[row * a.ld_mask + i] != 0;
       }
-      return;
     }
-    at -= __shfl_sync(M32_ALL, run, 31);
+  };
+  fetch(first);
+#pragma unroll 1
+  for (int r = 0; r < n; ++r) {
+    WarpRow<EPL> R;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      R.z[j] = clean(ok[j] ? to_f(next[j]) : 0.f, ok[j]);
+      R.key[j] = key_of(R.z[j]);
+      top = max(top, R.key[j]);
+    }
+    if (r + 1 < n) fetch(first + r + 1);
+    top = __reduce_max_sync(M32_ALL, top);
+    if (top <= KEY_NEG_INF) continue;
+    const float m = of_key(top), inv_t = __shfl_sync(M32_ALL, mine.inv_t, r);
+    const float top_p = __shfl_sync(M32_ALL, mine.top_p, r), min_p = __shfl_sync(M32_ALL, mine.min_p, r);
+    const int k = __shfl_sync(M32_ALL, mine.k, r);
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      R.z[j] = z_of(R.z[j], m, inv_t);
+      R.q[j] = q_of(expf(R.z[j]));              // exp(-inf) = 0
+    }
+    if (k > 0 && k < a.V) R.template cut<false>(k);
+    if (top_p < 1.f)      // every sum is exact in a double, so x >= threshold is x >= its ceiling in integers
+      R.template cut<true>(__double2ll_ru(p_threshold(top_p, R.mass_from(-Z_SPAN))));
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (min_p > 0.f && expf(R.z[j]) < min_p && R.key[j] != top) R.q[j] = 0;     // the first element always stays
+      lo += (uint32_t)R.q[j] & 0xFFFFFu;
+      hi += (uint32_t)(R.q[j] >> 20);
+    }
+    const long long total = warp_mass(lo, hi);
+    long long at = draw_at(__shfl_sync(M32_ALL, mine.u, r), total);
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (found) break;
+      long long run = R.q[j];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(M32_ALL, run, o);
+        if (lane >= o) run += v;
+      }
+      const uint32_t over = __ballot_sync(M32_ALL, run > at);
+      if (over != 0) {
+        const int src = __ffs(over) - 1;
+        const float zt = __shfl_sync(M32_ALL, R.z[j], src);
+        if (lane == r) {
+          my_token = j * 32 + src;
+          my_z = zt;
+          my_total = total;
+        }
+        found = true;
+      } else {
+        at -= __shfl_sync(M32_ALL, run, 31);
+      }
+    }
+  }
+  if (lane < n) {
+    a.token[first + lane] = my_token;
+    a.logp[first + lane] = my_token < 0 ? -INFINITY : logp_of(my_z, my_total);
   }
 }
 
@@ -230,17 +272,22 @@ struct Exchange {
 
 template <int NT>
 struct BlockState {
-  uint32_t cnt[2][2 * NT];                 // histograms: [0] over z, kept; [1] of the refining levels
-  unsigned long long mass[2][2 * NT];
+  static constexpr int BINS = 2 * NT, LIST = 4 * NT;
+  uint32_t cnt[BINS];                      // histogram: elements, and their mass where it is asked for
+  unsigned long long mass[BINS];
+  float lv[LIST];                          // the elements that can be kept, by index, where they are few
+  int li[LIST];
   Exchange ex[2];                          // alternated, see all_reduce
   uint32_t wu[32], wt[32];
   long long wm[32];
-  uint32_t f_bin, f_cnt_above, f_count;
+  uint32_t f_bin, f_cnt_above, f_count, f_key;
   long long f_mass_above;
 };
 
+// The row (or, once `list` is set, the list of its candidates in the first block) as the passes see it
 template <typename T, int NT, bool RES>
 struct Row {
+  static constexpr int BINS = 2 * NT, LIST = 4 * NT, LOG_BINS = NT == 128 ? 8 : 10;
   const InbSampleArgs& a;
   BlockState<NT>& s;
   T* buf;
@@ -248,13 +295,18 @@ struct Row {
   int first, len;      // this block's slice
   int ranks, rank;
   float m, inv_t;
+  bool list;
   int par;
 
   __device__ __forceinline__ float at(int i) const {
+    if (list) return s.lv[i];
     if (RES) return to_f(buf[i]);
     return clean(to_f(((const T*)a.logits)[row * a.ld + first + i]),
                  a.mask == nullptr || a.mask[row * a.ld_mask + first + i] != 0);
   }
+  __device__ __forceinline__ int index(int i) const { return list ? s.li[i] : first + i; }
+  __device__ __forceinline__ float z(float l) const { return z_of(l, m, inv_t); }
+  __device__ __forceinline__ int z_bin(float z) const { return min(BINS - 1, (int)(-z * (BINS / Z_SPAN))); }
   __device__ __forceinline__ void sync() {
     if (ranks > 1)
       cg::this_cluster().sync();
@@ -282,13 +334,13 @@ struct Row {
     __syncthreads();
     par ^= 1;
     if (threadIdx.x < 32) {
-      umax = lane < NT / 32 ? s.wu[lane] : 0u;
-      umin = lane < NT / 32 ? s.wt[lane] : M32_ALL;
-      mass = lane < NT / 32 ? s.wm[lane] : 0;
-      umax = __reduce_max_sync(M32_ALL, umax);
-      umin = __reduce_min_sync(M32_ALL, umin);
+      umax = __reduce_max_sync(M32_ALL, lane < NT / 32 ? s.wu[lane] : 0u);
+      umin = __reduce_min_sync(M32_ALL, lane < NT / 32 ? s.wt[lane] : M32_ALL);
+      if (with_mass) {
+        mass = lane < NT / 32 ? s.wm[lane] : 0;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(M32_ALL, mass, o);
+        for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(M32_ALL, mass, o);
+      }
       if (lane == 0) {
         s.ex[par].umax = umax;
         s.ex[par].umin = umin;
@@ -296,33 +348,66 @@ struct Row {
       }
     }
     sync();
-    Exchange e = {0, M32_ALL, 0};
-    for (int r = 0; r < ranks; ++r) {
-      const Exchange& o = peer(r)->ex[par];
-      e.umax = max(e.umax, o.umax);
-      e.umin = min(e.umin, o.umin);
-      e.mass += o.mass;
-    }
+    Exchange e = s.ex[par];
+    if (ranks > 1)
+      for (int r = 0; r < ranks; ++r)
+        if (r != rank) {
+          const Exchange& o = peer(r)->ex[par];
+          e.umax = max(e.umax, o.umax);
+          e.umin = min(e.umin, o.umin);
+          e.mass += o.mass;
+        }
     return e;
   }
-  // Over histogram h of the row (bin 0 = largest logits): the first bin at which the count (by_mass false) or the mass
+  __device__ void clear() {
+    __syncthreads();
+    for (int b = threadIdx.x; b < BINS; b += NT) {
+      s.cnt[b] = 0;
+      s.mass[b] = 0;
+    }
+    __syncthreads();
+  }
+  // Histogram over z of the elements that have a mass; with_mass: their masses too, whose sum (this thread's) it returns
+  __device__ long long fill(bool with_mass) {
+    clear();
+    long long sum = 0;
+    for (int i = threadIdx.x; i < len; i += NT) {
+      const float zi = z(at(i));
+      if (zi > -Z_SPAN) {
+        if (with_mass) {
+          const long long q = q_of(expf(zi));
+          if (q > 0) {
+            atomicAdd(&s.cnt[z_bin(zi)], 1u);
+            atomicAdd(&s.mass[z_bin(zi)], (unsigned long long)q);
+            sum += q;
+          }
+        } else if (zi > -Z_SURE || q_of(expf(zi)) > 0) {
+          atomicAdd(&s.cnt[z_bin(zi)], 1u);
+        }
+      }
+    }
+    return sum;
+  }
+  // Over the histogram of the row (bin 0 = largest logits): the first bin at which the count (by_mass false) or the mass
   // reaches the target, given what lies above the histogram.  False: no bin does.
-  __device__ bool cross(int h, bool by_mass, uint32_t k, double thr, uint32_t& cnt_above, long long& mass_above,
-                        uint32_t& bin, uint32_t& count) {
+  __device__ bool cross(bool by_mass, uint32_t k, double thr, uint32_t& cnt_above, long long& mass_above, uint32_t& bin,
+                        uint32_t& count) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, b = 2 * threadIdx.x;
     __syncthreads();                          // the last call's result has been read
     if (threadIdx.x == 0) s.f_bin = M32_ALL;
     sync();                                   // every block's histogram is complete
-    uint32_t c[2] = {0, 0};
-    long long q[2] = {0, 0};
-    for (int r = 0; r < ranks; ++r) {
-      const BlockState<NT>* o = peer(r);
+    uint32_t c[2] = {s.cnt[b], s.cnt[b + 1]};
+    long long q[2] = {(long long)s.mass[b], (long long)s.mass[b + 1]};
+    if (ranks > 1)
+      for (int r = 0; r < ranks; ++r)
+        if (r != rank) {
+          const BlockState<NT>* o = peer(r);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        c[i] += o->cnt[h][b + i];
-        q[i] += (long long)o->mass[h][b + i];
-      }
-    }
+          for (int i = 0; i < 2; ++i) {
+            c[i] += o->cnt[b + i];
+            q[i] += (long long)o->mass[b + i];
+          }
+        }
     uint32_t ci = c[0] + c[1];
     long long qi = q[0] + q[1];
 #pragma unroll
@@ -366,19 +451,91 @@ struct Row {
     count = s.f_count;
     return true;
   }
-  __device__ __forceinline__ int z_bin(float z) const { return min(2 * NT - 1, (int)(-z * (2 * NT / Z_SPAN))); }
-
-  // The value tau at which the target is reached, how many hold it, and what lies above it.
+  // The smallest key whose element lies in z bins 0 .. bin: z_bin falls with the key, so a warp finds it in seven rounds
+  // of 32 probes.
+  __device__ uint32_t bin_floor(uint32_t bin) {
+    if (threadIdx.x < 32) {
+      uint32_t lo = KEY_NEG_INF, hi = key_of(m);          // lo does not lie there, hi does
+      while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 31) / 32;
+        const uint64_t probe = (uint64_t)lo + (uint64_t)step * (threadIdx.x + 1);
+        bool in = true;
+        if (probe < hi) {
+          const float zi = z(of_key((uint32_t)probe));
+          in = zi > -Z_SPAN && z_bin(zi) <= (int)bin;
+        }
+        const int f = __ffs(__ballot_sync(M32_ALL, in));     // the last probe is at or above hi: one is in
+        const uint64_t up = (uint64_t)lo + (uint64_t)step * f;
+        lo = lo + step * (f - 1);
+        hi = up < hi ? (uint32_t)up : hi;
+      }
+      if (threadIdx.x == 0) s.f_key = hi;
+    }
+    __syncthreads();
+    return s.f_key;
+  }
+  // The run of the slice that a warp owns
+  __device__ __forceinline__ void run(int& s0, int& s1) const {
+    constexpr int nw = NT / 32;
+    const int seg = (len + nw * 32 - 1) / (nw * 32) * 32, wid = threadIdx.x >> 5;
+    s0 = min(len, wid * seg);
+    s1 = min(len, s0 + seg);
+  }
+  // Moves the elements from key `floor` up to the first block's list, by index.  0: they are more than the list holds and
+  // nothing was moved; 1: moved, and this is the first block; 2: moved, and this block is done.
+  __device__ int gather(uint32_t floor) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const float least = of_key(floor);
+    int s0, s1;
+    run(s0, s1);
+    uint32_t n = 0;
+    for (int i = s0 + lane; i < s1; i += 32) n += at(i) >= least;
+    n = __reduce_add_sync(M32_ALL, n);
+    if (lane == 0) s.wt[wid] = n;
+    sync();
+    uint32_t before = 0, total = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const BlockState<NT>* o = peer(r);
+      const uint32_t v = lane < NT / 32 ? o->wt[lane] : 0u;
+      total += __reduce_add_sync(M32_ALL, v);
+      before += __reduce_add_sync(M32_ALL, r < rank || (r == rank && lane < wid) ? v : 0u);
+    }
+    if (total > (uint32_t)LIST) {
+      sync();           // the counts have been read
+      return 0;
+    }
+    BlockState<NT>* to = peer(0);
+    if (n > 0)
+      for (int i0 = s0; i0 < s1; i0 += 32) {
+        const int i = i0 + lane;
+        const float l = i < s1 ? at(i) : -INFINITY;
+        const bool in = i < s1 && l >= least;
+        const uint32_t who = __ballot_sync(M32_ALL, in);
+        if (in) {
+          const uint32_t slot = before + __popc(who & ((1u << lane) - 1u));
+          to->lv[slot] = l;
+          to->li[slot] = first + i;
+        }
+        before += __popc(who);
+      }
+    sync();
+    if (rank != 0) return 2;
+    list = true;
+    len = (int)total;
+    ranks = 1;
+    return 1;
+  }
+  // With the histogram filled: the value tau at which the target is reached, how many hold it, and what lies above it.
   __device__ bool find(bool by_mass, uint32_t k, double thr, uint32_t& tau, uint32_t& count, uint32_t& cnt_above,
                        long long& mass_above) {
     cnt_above = 0;
     mass_above = 0;
     uint32_t bin;
-    if (!cross(0, by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
+    if (!cross(by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
     uint32_t hi = 0, lo = M32_ALL;
     for (int i = threadIdx.x; i < len; i += NT) {
-      const float l = at(i), z = z_of(l, m, inv_t);
-      if (z > -Z_SPAN && z_bin(z) == (int)bin && q_of(expf(z)) > 0) {
+      const float l = at(i), zi = z(l);
+      if (zi > -Z_SPAN && z_bin(zi) == (int)bin && q_of(expf(zi)) > 0) {
         hi = max(hi, key_of(l));
         lo = min(lo, key_of(l));
       }
@@ -388,34 +545,27 @@ struct Row {
     lo = e.umin;
     while (hi != lo) {
       const int bits = 32 - __clz(hi - lo), shift = max(0, bits - LOG_BINS);
-      __syncthreads();
-      for (int b = threadIdx.x; b < 2 * NT; b += NT) {
-        s.cnt[1][b] = 0;
-        s.mass[1][b] = 0;
-      }
-      __syncthreads();
+      clear();
       for (int i = threadIdx.x; i < len; i += NT) {
         const float l = at(i);
         const uint32_t key = key_of(l);
         if (key >= lo && key <= hi) {
-          const long long q = q_of(expf(z_of(l, m, inv_t)));
+          const long long q = q_of(expf(z(l)));
           if (q > 0) {
             const uint32_t b = (hi - key) >> shift;
-            atomicAdd(&s.cnt[1][b], 1u);
-            atomicAdd(&s.mass[1][b], (unsigned long long)q);
+            atomicAdd(&s.cnt[b], 1u);
+            atomicAdd(&s.mass[b], (unsigned long long)q);
           }
         }
       }
-      cross(1, by_mass, k, thr, cnt_above, mass_above, bin, count);   // the target lies within: a bin is found
+      cross(by_mass, k, thr, cnt_above, mass_above, bin, count);   // the target lies within: a bin is found
       hi = hi - (bin << shift);
       const uint32_t span = (1u << shift) - 1u;
       lo = hi - lo > span ? hi - span : lo;
-      if (shift == 0) lo = hi;
     }
     tau = hi;
     return true;
   }
-  static constexpr int LOG_BINS = NT == 128 ? 8 : 10;
 };
 
 template <typename T, int NT, bool RES>
@@ -425,12 +575,13 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   constexpr int STATE = (sizeof(BlockState<NT>) + 15) / 16 * 16;
   T* buf = reinterpret_cast<T*>(dyn + STATE);
   const int64_t row = (int64_t)blockIdx.x / ranks;
-  const int rank = (int)(blockIdx.x % ranks);      // clusters are consecutive blocks: also the rank in the cluster
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  int first = rank * slice, len = a.V - first;
+  const int own = (int)(blockIdx.x % ranks);       // clusters are consecutive blocks: also the rank in the cluster
+  const int first = own * slice;
+  int len = a.V - first;
   len = len < 0 ? 0 : (len > slice ? slice : len);
   const RowParams p = row_params(a, row);
-  Row<T, NT, RES> R{a, s, buf, row, first, len, ranks, rank, 0.f, p.inv_t, 0};
+  Row<T, NT, RES> R{a, s, buf, row, first, len, ranks, own, 0.f, p.inv_t, false, 0};
   const bool select_k = p.k > 0 && p.k < a.V, select_p = p.top_p < 1.f;
 
   // the slice, and the row's largest logit
@@ -440,6 +591,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     const uint8_t* mp = a.mask ? a.mask + row * a.ld_mask + first : nullptr;
     constexpr int W = 16 / (int)sizeof(T);
     int i0 = 0;
+    float best = -INFINITY;
     if (((uintptr_t)lp & 15) == 0 && ((uintptr_t)mp & (W - 1)) == 0) {
       i0 = len / W * W;
 #pragma unroll 4
@@ -450,7 +602,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           const float l = clean(to_f(v.v[e]), mp == nullptr || ok.v[e] != 0);
-          top = max(top, key_of(l));
+          best = fmaxf(best, l);
           v.v[e] = from_f<T>(l);
         }
         st<T, W>(buf + i, v);
@@ -458,71 +610,71 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     }
     for (int i = i0 + threadIdx.x; i < len; i += NT) {
       const float l = clean(to_f(lp[i]), mp == nullptr || mp[i] != 0);
-      top = max(top, key_of(l));
+      best = fmaxf(best, l);
       buf[i] = from_f<T>(l);
     }
+    top = key_of(best);
   } else {
     for (int i = threadIdx.x; i < len; i += NT) top = max(top, key_of(R.at(i)));
   }
-  if (select_k || select_p)
-    for (int b = threadIdx.x; b < 2 * NT; b += NT) {
-      s.cnt[0][b] = 0;
-      s.mass[0][b] = 0;
-    }
   top = R.all_reduce(top, M32_ALL, 0, false).umax;
   if (top <= KEY_NEG_INF) {
-    if (rank == 0 && threadIdx.x == 0) {
+    if (own == 0 && threadIdx.x == 0) {
       a.token[row] = -1;
       a.logp[row] = -INFINITY;
     }
     R.sync();           // no block leaves while another may still read its shared memory
     return;
   }
-  const float m = of_key(top), inv_t = p.inv_t;
+  const float m = of_key(top);
   R.m = m;
+  if (p.k == 1) {       // the first of the largest
+    uint32_t i1 = M32_ALL;
+    for (int i = threadIdx.x; i < R.len; i += NT)
+      if (R.at(i) == m) i1 = min(i1, (uint32_t)(first + i));
+    i1 = R.all_reduce(0, i1, 0, false).umin;
+    if (own == 0 && threadIdx.x == 0) {
+      a.token[row] = i1;
+      a.logp[row] = 0.f;
+    }
+    R.sync();
+    return;
+  }
 
   // the cut-off (tau, kept): elements above tau stay, and the first `kept` of those equal to it
   uint32_t tau = 0, kept = 0;
   if (select_k || select_p) {
-    long long mass = 0;
-    for (int i = threadIdx.x; i < len; i += NT) {
-      const float z = z_of(R.at(i), m, inv_t);
-      if (z > -Z_SPAN) {
-        const long long q = q_of(expf(z));
-        if (q > 0) {
-          const int b = R.z_bin(z);
-          atomicAdd(&s.cnt[0][b], 1u);
-          atomicAdd(&s.mass[0][b], (unsigned long long)q);
-          mass += q;
-        }
-      }
+    uint32_t count, above = 0, bin;
+    long long total = 0, mass_above = 0;
+    if (!select_k) total = R.all_reduce(0, M32_ALL, R.fill(true), true).mass;
+    else R.fill(false);
+    double thr = select_k ? 0.0 : p_threshold(p.top_p, total);
+    const bool found = R.cross(!select_k, (uint32_t)p.k, thr, above, mass_above, bin, count);
+    if (found && above + count <= (uint32_t)R.LIST && R.gather(R.bin_floor(bin)) == 2) return;
+    if (select_k || R.list) {
+      const long long sum = R.fill(true);
+      if (select_k) total = R.all_reduce(0, M32_ALL, sum, true).mass;     // stays if fewer than k have a mass
     }
-    long long total = 0;
-    if (!select_k) total = R.all_reduce(0, M32_ALL, mass, true).mass;
-    uint32_t count, above;
-    long long mass_above;
-    if (select_k) {
-      if (R.find(false, (uint32_t)p.k, 0.0, tau, count, above, mass_above)) {
-        kept = (uint32_t)p.k - above;
-        total = mass_above + (long long)kept * q_of(expf(z_of(of_key(tau), m, inv_t)));
-      } else {
-        total = R.all_reduce(0, M32_ALL, mass, true).mass;
-      }
+    if (select_k && R.find(false, (uint32_t)p.k, 0.0, tau, count, above, mass_above)) {
+      kept = (uint32_t)p.k - above;
+      total = mass_above + (long long)kept * q_of(expf(R.z(of_key(tau))));
+      if (select_p) R.fill(true);
     }
     if (select_p) {
-      const double thr = p_threshold(p.top_p, total);
+      if (select_k) thr = p_threshold(p.top_p, total);
       uint32_t tp;
       if (R.find(true, 0, thr, tp, count, above, mass_above)) {
         tau = tp;
-        kept = ties_kept(mass_above, q_of(expf(z_of(of_key(tau), m, inv_t))), count, thr);
+        kept = ties_kept(mass_above, q_of(expf(R.z(of_key(tau)))), count, thr);
       }
     }
   }
 
-  // the kept mass of each warp's run of the slice, by index
-  const int nw = NT / 32, seg = (len + nw * 32 - 1) / (nw * 32) * 32;
-  const int s0 = min(len, wid * seg), s1 = min(len, s0 + seg);
-  const float z_tau = z_of(of_key(tau), m, inv_t), w_tau = expf(z_tau);
+  // the kept mass of each warp's run, by index
+  constexpr int nw = NT / 32;
+  int s0, s1;
+  R.run(s0, s1);
+  const float w_tau = expf(R.z(of_key(tau)));
   const long long q_tau = tau == 0 || (w_tau < p.min_p && tau != top) ? 0 : q_of(w_tau);
   long long mass = 0;
   uint32_t ties = 0;
@@ -532,7 +684,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     if (key == tau) {
       ++ties;
     } else if (key > tau) {
-      const float z = z_of(l, m, inv_t);
+      const float z = R.z(l);
       if (z > -Z_SPAN) {
         const float w = expf(z);
         if (!(w < p.min_p) || key == top) mass += q_of(w);
@@ -551,7 +703,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   // every warp: the mass of the row, what comes before its own run, and the ties before it
   long long total = 0, before = 0;
   uint32_t seen = 0, my_seen = 0;
-  for (int r = 0; r < ranks; ++r) {
+  for (int r = 0; r < R.ranks; ++r) {
     const BlockState<NT>* o = R.peer(r);
     uint32_t t = lane < nw ? o->wt[lane] : 0u, ti = t;
     long long v = lane < nw ? o->wm[lane] : 0;
@@ -569,7 +721,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
       const long long x = __shfl_up_sync(M32_ALL, vi, d);
       if (lane >= d) vi += x;
     }
-    if (r == rank) {
+    if (r == R.rank) {
       before = total + __shfl_sync(M32_ALL, vi - v, wid);
       my_seen = __shfl_sync(M32_ALL, tb, wid);
       mass = __shfl_sync(M32_ALL, v, wid);
@@ -589,7 +741,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     if (i < s1) {
       const float l = R.at(i);
       key = key_of(l);
-      z = z_of(l, m, inv_t);
+      z = R.z(l);
       if (key > tau && z > -Z_SPAN) {
         const float w = expf(z);
         if (!(w < p.min_p) || key == top) q = q_of(w);
@@ -606,7 +758,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     const uint32_t over = __ballot_sync(M32_ALL, run + q > at);
     if (over != 0) {
       if (lane == __ffs(over) - 1) {
-        a.token[row] = first + i;
+        a.token[row] = R.index(i);
         a.logp[row] = logp_of(z, total);
       }
       return;
@@ -644,13 +796,16 @@ constexpr int SMEM_MOST = 227 * 1024;
 template <typename T>
 static int sample_type(const InbSampleArgs& a, cudaStream_t s) {
   if (a.V <= 128) {
-    const unsigned grid = (unsigned)((a.N + 3) / 4);
+    // a warp takes one row while the SMs' 64 warps are not all busy, and up to 8 then
+    int64_t rows = a.N / ((int64_t)sm_count() * 64);
+    rows = rows < 1 ? 1 : (rows > 8 ? 8 : rows);
+    const unsigned grid = (unsigned)((a.N + 4 * rows - 1) / (4 * rows));
     if (a.V <= 32)
-      sample_warp_kernel<T, 1><<<grid, 128, 0, s>>>(a);
+      sample_warp_kernel<T, 1><<<grid, 128, 0, s>>>(a, (int)rows);
     else if (a.V <= 64)
-      sample_warp_kernel<T, 2><<<grid, 128, 0, s>>>(a);
+      sample_warp_kernel<T, 2><<<grid, 128, 0, s>>>(a, (int)rows);
     else
-      sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a);
+      sample_warp_kernel<T, 4><<<grid, 128, 0, s>>>(a, (int)rows);
     return launch_status();
   }
   if (a.V <= 4096) return block_launch<T, 128, true>(a, 1, a.V, s);

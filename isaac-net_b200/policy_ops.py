@@ -21,30 +21,42 @@ from . import _native as nat
 from .engine import B200Unsupported
 
 _TYPES = {torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.float32: nat.F32}
+_TYPES_16 = {torch.bfloat16: nat.BF16, torch.float16: nat.F16}
 _M32 = 0xFFFFFFFF
 
 
 # ---------------------------------------------------------------------------------------------------- plumbing
-def _need(ok, msg, kind=ValueError):
-    if not ok:
-        raise kind(msg)
+# A serving call is a few microseconds of device time, so the checks on the way are plain comparisons; messages are only
+# put together once one fails.
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _tensor(t, name, like: Optional[torch.Tensor] = None, dtype=None):
-    """Checks one argument: a CUDA tensor, on `like`'s device and (dtype None: of its type, else of `dtype`)."""
-    _need(isinstance(t, torch.Tensor), f"{name} must be a tensor, got {type(t).__name__}", TypeError)
+def _fits(t, dev, dtype):
+    """Whether `t` is a tensor of `dtype` on CUDA device `dev` (an index)."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev
+
+
+def _refuse(t, name, like=None, dtype=None):
+    """Raises what is wrong with an argument that does not fit."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise B200Unsupported(f"{name} is on {t.device}: the policy operators run on CUDA tensors only")
     if like is not None:
-        _need(t.device == like.device, f"{name} is on {t.device}, the first tensor on {like.device}")
-        want = like.dtype if dtype is None else dtype
-        _need(t.dtype == want, f"{name} is {t.dtype}, expected {want}", TypeError)
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, the first tensor on {like.device}")
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype or like.dtype}")
+    raise B200Unsupported(f"{name} is {t.dtype}: not a type this operator takes")
 
 
-def _type(t, name, types=tuple(_TYPES)):
-    if t.dtype not in types:
-        raise B200Unsupported(f"{name} is {t.dtype}: supported are {', '.join(str(d) for d in types)}")
-    return _TYPES[t.dtype]
+def _first(t, name, types=_TYPES):
+    """Checks an operator's first tensor [..., D]; its type code and device index."""
+    code = types.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if code is None or not t.is_cuda:
+        _refuse(t, name)
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be [..., D] with D >= 1, got shape {tuple(t.shape)}")
+    return code, t.get_device()
 
 
 def _rows(t, d):
@@ -67,26 +79,46 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(fn, name, args, dev):
-    """Queue one launch on the current stream of `dev`."""
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+def _call(name, args, dev):
+    """Queue one call of the library on the current stream of device index `dev`."""
+    fn = getattr(_lib or _load(), name)
+    if _current_device() == dev:
+        rc = fn(ctypes.byref(args), _raw_stream(dev))
     else:
-        rc = fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
-    nat.check(rc, name)
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), _raw_stream(dev))
+    if rc != 0:
+        nat.check(rc, name)
+
+
+_lib = None
+
+
+def _load():
+    global _lib
+    _lib = nat.lib()
+    return _lib
 
 
 def _grad_on(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------------------------------- block_norm
+def _norm_rows(t, d):
+    r, ld = _rows(t, d)
+    return (r, ld) if ld <= nat.MAX_NORM_LD else (t.contiguous(), d)
+
+
 def _norm_args(x, w, h, post, gate, gate_rows, scale, eps):
     """The argument block of one call on [N, D] rows, and the tensors that it points into."""
     d = x.shape[-1]
-    xr, ldx = _rows(x, d)
-    hr, ldh = _rows(h, d) if h is not None else (None, 0)
+    xr, ldx = _norm_rows(x, d)
+    hr, ldh = _norm_rows(h, d) if h is not None else (None, 0)
     a = nat.InbNormArgs(_TYPES[x.dtype], d, x.numel() // d, ldx, ldh, gate_rows, scale, eps, xr.data_ptr(), _ptr(hr),
                         w.data_ptr(), _ptr(post), _ptr(gate))
     return a, (xr, hr, w, post, gate)
@@ -94,11 +126,11 @@ def _norm_args(x, w, h, post, gate, gate_rows, scale, eps):
 
 def _norm_forward(x, w, h, post, gate, gate_rows, scale, eps, stats):
     a, keep = _norm_args(x, w, h, post, gate, gate_rows, scale, eps)
-    n = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if h is not None else None
+    n = x.new_empty(x.shape)
+    y = x.new_empty(x.shape) if h is not None else None
     a.y, a.n, a.stats = _ptr(y), n.data_ptr(), _ptr(stats)
     if x.numel():
-        _call(nat.lib().inb_block_norm_fwd, "inb_block_norm_fwd", a, x.device)
+        _call("inb_block_norm_fwd", a, x.get_device())
     return y, n
 
 
@@ -126,32 +158,32 @@ class _BlockNorm(torch.autograd.Function):
                     t.zero_()
             return (*outs, None, None, None)
         a, keep = _norm_args(x, w, h, post, gate, *ctx.settings)
-        yr, a.ldgy = _rows(gy, d) if gy is not None else (None, 0)
-        nr, a.ldgn = _rows(gn, d) if gn is not None else (None, 0)
+        yr, a.ldgy = _norm_rows(gy, d) if gy is not None else (None, 0)
+        nr, a.ldgn = _norm_rows(gn, d) if gn is not None else (None, 0)
         a.gy, a.gn, a.stats = _ptr(yr), _ptr(nr), stats.data_ptr()
         a.gx, a.gw, a.gh, a.gpost, a.ggate = gx.data_ptr(), gw.data_ptr(), _ptr(gh), _ptr(gpost), _ptr(ggate)
-        L = nat.lib()
         size = nat.i64()
-        nat.check(L.inb_block_norm_work(ctypes.byref(a), ctypes.byref(size)), "inb_block_norm_work")
+        nat.check(nat.lib().inb_block_norm_work(ctypes.byref(a), ctypes.byref(size)), "inb_block_norm_work")
         work = torch.empty(size.value, device=x.device)
         a.work, a.work_elems = work.data_ptr(), size.value
-        _call(L.inb_block_norm_bwd, "inb_block_norm_bwd", a, x.device)
+        _call("inb_block_norm_bwd", a, x.get_device())
         return (*outs, None, None, None)
 
 
 def _gate_rows(gate, x):
     """How many consecutive rows of x [..., D] one gate of `gate` [g..., D] scales: gate's leading dims equal x's up to
     some axis and are 1 from there on (missing leading dims count as 1)."""
-    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
-    msg = (f"gate of shape {tuple(gate.shape)} does not fit x of shape {tuple(x.shape)}: [..., D] with x's leading sizes, "
-           "then ones")
-    _need(len(shape) == x.dim() and shape[-1] == x.shape[-1], msg)
-    rows, axis = 1, x.dim() - 2
-    while axis >= 0 and shape[axis] == 1:
-        rows *= x.shape[axis]
-        axis -= 1
-    _need(shape[:axis + 1] == tuple(x.shape[:axis + 1]), msg)
-    return rows
+    full = tuple(x.shape)
+    shape = (1,) * (len(full) - gate.dim()) + tuple(gate.shape)
+    rows, axis = 1, len(full) - 2
+    if len(shape) == len(full) and shape[-1] == full[-1]:
+        while axis >= 0 and shape[axis] == 1:
+            rows *= full[axis]
+            axis -= 1
+        if shape[:axis + 1] == full[:axis + 1]:
+            return rows
+    raise ValueError(f"gate of shape {tuple(gate.shape)} does not fit x of shape {full}: [..., D] with x's leading sizes, "
+                     "then ones")
 
 
 def block_norm(x, weight, h=None, *, post_weight=None, gate=None, scale=1.0, eps=1e-6):
@@ -163,30 +195,37 @@ def block_norm(x, weight, h=None, *, post_weight=None, gate=None, scale=1.0, eps
     (h is added as it is), gate [..., D] or None: leading sizes those of x, then ones ([D]: one gate; [E, 1, D]: one per
     env; [E, R, D]: one per robot).  Returns (y, n); without h just n, the pre-norm of x.  Differentiable in every
     tensor.  D up to 8192."""
-    _tensor(x, "x")
-    _type(x, "x")
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, f"x must be [..., D], got shape {tuple(x.shape)}")
-    d = x.shape[-1]
+    dev = _first(x, "x")[1]
+    d, dt = x.shape[-1], x.dtype
     if d > nat.MAX_NORM_D:
         raise B200Unsupported(f"block_norm: D = {d} is above {nat.MAX_NORM_D}")
     if x.numel() // d > 0x7FFFFFFF:
         raise B200Unsupported("block_norm: more than 2^31 - 1 rows")
-    for t, name in ((weight, "weight"), (post_weight, "post_weight")):
-        if t is not None or name == "weight":
-            _tensor(t, name, x)
-            _need(t.shape == (d,), f"{name} must have shape ({d},), got {tuple(t.shape)}")
+    if not _fits(weight, dev, dt):
+        _refuse(weight, "weight", x)
+    if weight.shape != (d,):
+        raise ValueError(f"weight must have shape ({d},), got {tuple(weight.shape)}")
     rows = 0
     if h is None:
-        _need(post_weight is None and gate is None, "post_weight and gate need h")
+        if post_weight is not None or gate is not None:
+            raise ValueError("post_weight and gate need h")
     else:
-        _tensor(h, "h", x)
-        _need(h.shape == x.shape, f"h of shape {tuple(h.shape)} does not match x of shape {tuple(x.shape)}")
+        if not _fits(h, dev, dt):
+            _refuse(h, "h", x)
+        if h.shape != x.shape:
+            raise ValueError(f"h of shape {tuple(h.shape)} does not match x of shape {tuple(x.shape)}")
+        if post_weight is not None:
+            if not _fits(post_weight, dev, dt):
+                _refuse(post_weight, "post_weight", x)
+            if post_weight.shape != (d,):
+                raise ValueError(f"post_weight must have shape ({d},), got {tuple(post_weight.shape)}")
+            post_weight = post_weight.contiguous()
         if gate is not None:
-            _tensor(gate, "gate", x)
+            if not _fits(gate, dev, dt):
+                _refuse(gate, "gate", x)
             rows = _gate_rows(gate, x)
+            gate = gate.contiguous()
     weight = weight.contiguous()
-    post_weight = post_weight.contiguous() if post_weight is not None else None
-    gate = gate.contiguous() if gate is not None else None
     scale, eps = float(scale), float(eps)
     if _grad_on(x, weight, h, post_weight, gate):
         return _BlockNorm.apply(x, weight, h, post_weight, gate, rows, scale, eps)
@@ -201,15 +240,15 @@ _status = {}
 def status(device="cuda"):
     """The device status word of the operators' kernels on `device` (0 = no wait inside a kernel ever ran out); reading it
     synchronizes."""
-    w = _status.get(torch.device(device, torch.cuda.current_device()).index if torch.device(device).index is None
-                    else torch.device(device).index)
+    i = torch.device(device).index
+    w = _status.get(torch.cuda.current_device() if i is None else i)
     return 0 if w is None else int(w.item())
 
 
 def _status_word(dev):
-    w = _status.get(dev.index)
+    w = _status.get(dev)
     if w is None:
-        w = _status[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
+        w = _status[dev] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
     return w
 
 
@@ -219,7 +258,7 @@ def _ffn_args(x, wg, wu, wd, act, h, g, u):
     (xr, ldx), (gr, ldg), (ur, ldu), (dr, ldd) = _rows(x, d), _rows(wg, d), _rows(wu, d), _rows(wd, f)
     a = nat.InbFfnArgs(_TYPES[x.dtype], act, d, f, x.numel() // d, ldx, ldg, ldu, ldd, h.shape[-1], 0, xr.data_ptr(),
                        gr.data_ptr(), ur.data_ptr(), dr.data_ptr(), None, h.data_ptr(), _ptr(g), _ptr(u))
-    a.status = _status_word(x.device).data_ptr()
+    a.status = _status_word(x.get_device()).data_ptr()
     return a, (xr, gr, ur, dr)
 
 
@@ -236,14 +275,13 @@ def _ffn_work(a, backward, dev):
 def _ffn_forward(x, wg, wu, wd, act, keep):
     """(y, h, g, u): g, u None unless `keep`."""
     n, ldh = x.numel() // x.shape[-1], (wg.shape[0] + 7) // 8 * 8
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(n, ldh, dtype=x.dtype, device=x.device)
+    y, h = x.new_empty(x.shape), x.new_empty(n, ldh)
     g, u = (torch.empty(n, ldh, device=x.device) if keep else None for _ in range(2))
     if n:
         a, held = _ffn_args(x, wg, wu, wd, act, h, g, u)
         a.y = y.data_ptr()
         work = _ffn_work(a, 0, x.device)
-        _call(nat.lib().inb_gated_ffn_fwd, "inb_gated_ffn_fwd", a, x.device)
+        _call("inb_gated_ffn_fwd", a, x.get_device())
     return y, h, g, u
 
 
@@ -274,7 +312,7 @@ class _GatedFfn(torch.autograd.Function):
             dg, du = torch.empty_like(h), torch.empty_like(h)
             a.dg, a.du = dg.data_ptr(), du.data_ptr()
         work = _ffn_work(a, 1, x.device)
-        _call(nat.lib().inb_gated_ffn_bwd, "inb_gated_ffn_bwd", a, x.device)
+        _call("inb_gated_ffn_bwd", a, x.get_device())
         return dx, dwg if need[1] else None, dwu if need[2] else None, dwd, None
 
 
@@ -286,18 +324,17 @@ def gated_ffn(x, w_gate, w_up, w_down, *, act="silu"):
     the two projections are rounded to the inputs' type.  Differentiable in every tensor: a call that autograd records
     keeps the projections, 10 bytes for each of the N x F hidden elements.  Rows of x and of the weights may be strided;
     where they are not 16-byte aligned a padded copy is made in the call."""
-    _tensor(x, "x")
-    _type(x, "x", (torch.bfloat16, torch.float16))
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, f"x must be [..., D], got shape {tuple(x.shape)}")
-    _need(act in nat.ACTS, f"act must be one of {tuple(nat.ACTS)}, got {act!r}")
-    d = x.shape[-1]
+    dev = _first(x, "x", _TYPES_16)[1]
+    if act not in nat.ACTS:
+        raise ValueError(f"act must be one of {tuple(nat.ACTS)}, got {act!r}")
+    d, dt = x.shape[-1], x.dtype
     for t, name in ((w_gate, "w_gate"), (w_up, "w_up"), (w_down, "w_down")):
-        _tensor(t, name, x)
-        _need(t.dim() == 2, f"{name} must be a matrix, got shape {tuple(t.shape)}")
-    f = w_gate.shape[0]
-    _need(f >= 1 and w_gate.shape == (f, d) and w_up.shape == (f, d) and w_down.shape == (d, f),
-          f"w_gate and w_up must be [F, {d}] and w_down [{d}, F], got {tuple(w_gate.shape)}, {tuple(w_up.shape)}, "
-          f"{tuple(w_down.shape)}")
+        if not _fits(t, dev, dt):
+            _refuse(t, name, x)
+    f = w_gate.shape[0] if w_gate.dim() == 2 else 0
+    if f < 1 or w_gate.shape != (f, d) or w_up.shape != (f, d) or w_down.shape != (d, f):
+        raise ValueError(f"w_gate and w_up must be [F, {d}] and w_down [{d}, F], got {tuple(w_gate.shape)}, "
+                         f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
     if max(d, f, x.numel() // d) > nat.MAX_FFN:
         raise B200Unsupported(f"gated_ffn: sizes above {nat.MAX_FFN}")
     if _grad_on(x, w_gate, w_up, w_down):
@@ -313,7 +350,7 @@ def _dropout_run(x, threshold, s0, stream, env_id, episode, ctr, keys_in, keys_o
     if x.numel():
         a = nat.InbDropoutArgs(_TYPES[x.dtype], threshold, e, x.numel() // e, s0, stream, _ptr(env_id), _ptr(episode),
                                _ptr(ctr), _ptr(keys_in), _ptr(keys_out), x.data_ptr(), y.data_ptr())
-        _call(nat.lib().inb_dropout, "inb_dropout", a, x.device)
+        _call("inb_dropout", a, x.get_device())
     return y
 
 
@@ -341,20 +378,28 @@ def counter_dropout(x, p, s0, env_id, episode=None, ctr=None, *, stream=0):
     the layers of one step apart.  The draw follows the global env id: shards of a batch drop what the whole batch
     drops.  A backward call uses the keys of its forward call, whatever has become of the counters since.  With
     inference, do not call it."""
-    _tensor(x, "x")
-    _type(x, "x")
-    _need(x.dim() >= 1, "x must be [E, ...]")
-    _need(0.0 <= p <= 1.0, f"p must be in [0, 1], got {p}")
-    _need(0 <= int(s0) <= _M32 and 0 <= int(stream) <= _M32, "s0 and stream are 32-bit words")
-    e = x.shape[0]
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES or not x.is_cuda:
+        _refuse(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must be [E, ...]")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if not (0 <= s0 <= _M32 and 0 <= stream <= _M32):
+        raise ValueError("s0 and stream are 32-bit words")
+    e, dev = x.shape[0], x.get_device()
     for t, name in ((env_id, "env_id"), (episode, "episode"), (ctr, "ctr")):
-        if t is not None or name == "env_id":
-            _tensor(t, name, x, torch.int64)
-            _need(t.shape == (e,), f"{name} must have shape ({e},), got {tuple(t.shape)}")
+        if t is None and name != "env_id":
+            continue
+        if not _fits(t, dev, torch.int64):
+            _refuse(t, name, x, torch.int64)
+        if t.shape != (e,):
+            raise ValueError(f"{name} must have shape ({e},), got {tuple(t.shape)}")
     n = x.numel() // e if e else 0
     if n > nat.MAX_DROPOUT_N or e * max(1, -(-n // 4096)) > 0x7FFFFFFF:
         raise B200Unsupported(f"counter_dropout: {e} envs of {n} elements are more than one call can draw")
-    env_id, episode, ctr = (None if t is None else t.contiguous() for t in (env_id, episode, ctr))
+    env_id = env_id.contiguous()
+    episode = None if episode is None else episode.contiguous()
+    ctr = None if ctr is None else ctr.contiguous()
     threshold = round(p * 65536)
     if _grad_on(x):
         return _Dropout.apply(x, threshold, int(s0), int(stream), env_id, episode, ctr)
@@ -375,50 +420,47 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
 
     The masses are summed in fixed point (2^-40 of the largest), so the token does not depend on how the sum is split;
     weights below 2^-40 of the largest are never drawn."""
-    _tensor(logits, "logits")
-    _type(logits, "logits")
-    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, f"logits must be [..., V], got shape {tuple(logits.shape)}")
+    code, dev = _first(logits, "logits")
     v, lead = logits.shape[-1], logits.shape[:-1]
     n = logits.numel() // v
     if v > nat.MAX_SAMPLE_V or n > nat.MAX_SAMPLE_N:
         raise B200Unsupported(f"sample_logits: {n} rows of {v}: at most {nat.MAX_SAMPLE_N} rows of {nat.MAX_SAMPLE_V}")
-    _tensor(u, "u", logits, torch.float32)
-    _need(u.shape == lead, f"u must have shape {tuple(lead)}, got {tuple(u.shape)}")
-    logits = logits.detach()
+    if not _fits(u, dev, torch.float32):
+        _refuse(u, "u", logits, torch.float32)
+    if u.shape != lead:
+        raise ValueError(f"u must have shape {tuple(lead)}, got {tuple(u.shape)}")
     lr, ld = _rows(logits, v)
-    keep, scalars, rows = [lr], [], []
-    for value, name, dt in ((temperature, "temperature", torch.float32), (top_p, "top_p", torch.float32),
-                            (min_p, "min_p", torch.float32), (top_k, "top_k", torch.int32)):
+    keep, scalars, rows = [], [], []
+    for value, name in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (top_k, "top_k")):
         if isinstance(value, torch.Tensor):
-            _tensor(value, name, logits, dt)
-            _need(value.shape == lead, f"{name} must be a number or have shape {tuple(lead)}, got {tuple(value.shape)}")
+            dt = torch.int32 if name == "top_k" else torch.float32
+            if not _fits(value, dev, dt):
+                _refuse(value, name, logits, dt)
+            if value.shape != lead:
+                raise ValueError(f"{name} must be a number or have shape {tuple(lead)}, got {tuple(value.shape)}")
             value = value.contiguous()
             keep.append(value)
             scalars.append(0)
             rows.append(value.data_ptr())
         else:
+            if not value >= 0 or (name == "min_p" and value > 1.0) or (name == "top_k" and int(value) != value):
+                raise ValueError(f"{name} = {value} is out of range")
             rows.append(None)
-            scalars.append(value)
-            if name == "top_k":
-                _need(0 <= int(value) == value, f"top_k must be a whole number >= 0, got {value}")
-                scalars[-1] = min(int(value), 0x7FFFFFFF)
-            else:
-                _need(value >= 0.0 and (name != "min_p" or value <= 1.0), f"{name} = {value} is out of range")
+            scalars.append(min(int(value), 0x7FFFFFFF) if name == "top_k" else value)
     mr, ldm = None, 0
     if mask is not None:
-        _tensor(mask, "mask", logits, torch.bool)
-        _need(mask.shape == logits.shape or mask.shape == (v,),
-              f"mask must have shape {tuple(logits.shape)} or ({v},), got {tuple(mask.shape)}")
+        if not _fits(mask, dev, torch.bool):
+            _refuse(mask, "mask", logits, torch.bool)
+        if mask.shape != logits.shape and mask.shape != (v,):
+            raise ValueError(f"mask must have shape {tuple(logits.shape)} or ({v},), got {tuple(mask.shape)}")
         mr, ldm = (mask.contiguous(), 0) if mask.dim() == 1 and logits.dim() > 1 else _rows(mask, v)
-        keep.append(mr)
     u = u.contiguous()
-    token = torch.empty(lead, dtype=torch.int64, device=logits.device)
-    logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    token, logp = u.new_empty(lead, dtype=torch.int64), u.new_empty(lead)
     if n:
-        a = nat.InbSampleArgs(_TYPES[logits.dtype], v, n, ld, ldm, lr.data_ptr(), _ptr(mr), u.data_ptr(), scalars[0],
+        a = nat.InbSampleArgs(code, v, n, ld, ldm, lr.data_ptr(), _ptr(mr), u.data_ptr(), scalars[0],
                               scalars[1], scalars[2], scalars[3], rows[0], rows[1], rows[2], rows[3], token.data_ptr(),
                               logp.data_ptr())
-        _call(nat.lib().inb_sample, "inb_sample", a, logits.device)
+        _call("inb_sample", a, dev)
     return token, logp
 
 
