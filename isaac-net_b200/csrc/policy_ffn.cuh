@@ -1,0 +1,471 @@
+// gated_ffn: the gated feed-forward block and its gradients, six products on the tensor cores (policy_gemm.cuh).
+//
+//   forward   g = x Wg^T, u = x Wu^T, h = act(g) * u     one product over [Wg | Wu], activation and product in its epilogue
+//             y = h Wd^T
+//   backward  dh = dy Wd, dg = dh u act'(g), du = dh act(g)     one product, both gradients in its epilogue
+//             dx = dg Wg + du Wu                                one product over k = 2 F
+//             dWg = dg^T x, dWu = du^T x                        one product over m = 2 F
+//             dWd = dy^T h
+//
+// A tile of the first product holds 128 columns of g and the same 128 of u, so act(g) * u needs no exchange.  g and u are
+// kept for the backward pass in fp32: rounding them to the operand type would put two more roundings into dg and du (the
+// weights' gradients then are 1.4 times as far from the exact ones), and reading them costs 16 bytes an element of h
+// against the 18 D operations the step does for it.  h, dg and du are rounded to the operand type because the next
+// product multiplies them.
+#pragma once
+#include "policy_gemm.cuh"
+
+namespace inb {
+namespace pol {
+
+__device__ __forceinline__ float act_of(float g, int act) {
+  if (act == INB_ACT_SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
+  return g * (0.5f * (1.f + erff(g * 0.70710678f)));
+}
+// act(g) and its derivative
+__device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
+  if (act == INB_ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    a = g * s;
+    da = s * (1.f + g * (1.f - s));
+  } else {
+    const float c = 0.5f * (1.f + erff(g * 0.70710678f));
+    a = g * c;
+    da = c + g * __expf(-0.5f * g * g) * 0.39894228f;
+  }
+}
+template <int N>
+__device__ __forceinline__ void buffers_free(const EpiCtx& c) {      // all but this warp's last N sent tiles have left
+  if (c.lane == 0) store_wait<N>();
+  __syncwarp();
+}
+
+// C, or (tiles from m_split on) a second C, rounded
+template <typename T, int CG>
+struct EpiStore {
+  T *c0, *c1;
+  int M, N, m_split;
+  bool tma;
+  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap* o1) const {
+    const bool second = c.tm >= m_split;
+    const int r0 = (second ? c.tm - m_split : c.tm) * Gemm<CG>::TM + (c.row & ~31), n0 = c.tn * BN;
+#pragma unroll 1
+    for (int b = 0; b < BN / 64 && n0 + b * 64 < N; ++b) {
+      if (tma) buffers_free<EPI_BUFS - 1>(c);
+#pragma unroll
+      for (int q = 0; q < 64; q += 16) {
+        float v[16];
+        tmem_ld16(c.tmem + b * 64 + q, v);
+        tmem_ld_wait();
+        stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, q, v);
+      }
+      send_stage<T>(tma ? (second ? o1 : o0) : nullptr, second ? c1 : c0, N, M, N, r0, n0 + b * 64, c, b);
+    }
+  }
+};
+
+// One part of k of a tile, fp32: [item][column group][row][4]
+template <int CG>
+struct EpiPartial {
+  float* part;
+  __device__ void operator()(const EpiCtx& c, const CUtensorMap*, const CUtensorMap*) const {
+    float* p = part + ((int64_t)c.item * (BN / 4) * Gemm<CG>::TM + c.row) * 4;
+#pragma unroll 2
+    for (int q = 0; q < BN; q += 16) {
+      float v[16];
+      tmem_ld16(c.tmem + q, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(p + (int64_t)(q / 4 + i) * Gemm<CG>::TM * 4) =
+            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+  }
+};
+// Adds the parts of every tile in order.  Block: (tile, 16 columns); thread: row.
+template <typename T, int CG>
+__global__ void __launch_bounds__(Gemm<CG>::TM) sum_parts_kernel(const float* part, const GemmShape g, T* c0, T* c1, int M, int N,
+                                                                 bool vec) {
+  constexpr int TM = Gemm<CG>::TM;
+  const int tiles = g.tiles_m * g.tiles_n;
+  int tm, tn;
+  tile_at(g, blockIdx.x, tm, tn);
+  const bool second = tm >= g.m_split;
+  const int r = (second ? tm - g.m_split : tm) * TM + threadIdx.x, col = tn * BN + blockIdx.y * 16;
+  if (r >= M || col >= N) return;
+  float4 s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < g.splits; ++k) {
+    const float* p = part + (((int64_t)k * tiles + blockIdx.x) * (BN / 4) + blockIdx.y * 4) * TM * 4 + threadIdx.x * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i * TM * 4);
+      s[i].x += v.x;
+      s[i].y += v.y;
+      s[i].z += v.z;
+      s[i].w += v.w;
+    }
+  }
+  T* d = (second ? c1 : c0) + (int64_t)r * N + col;
+  const float* f = &s[0].x;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    if (vec && col + i + 8 <= N) {
+      Pack<T, 8> o;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) down2(make_float2(f[i + e], f[i + e + 1]), o.v[e], o.v[e + 1]);
+      st<T, 8>(d + i, o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + i + e < N) d[i + e] = from_f<T>(f[i + e]);
+    }
+  }
+}
+
+// h = act(g) u of 128 columns; g and u kept in blocked fp32 (NULL: not kept)
+template <typename T, int CG>
+struct EpiGate {
+  float *g, *u;
+  int M, F, act, groups;
+  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap*) const {
+    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * (BN / 2);
+#pragma unroll 1
+    for (int b = 0; b < 2 && n0 + b * 64 < F; ++b) {
+      buffers_free<1>(c);
+#pragma unroll
+      for (int q = 0; q < 64; q += 16) {
+        float vg[16], vu[16];
+        tmem_ld16(c.tmem + b * 64 + q, vg);
+        tmem_ld16(c.tmem + BN / 2 + b * 64 + q, vu);
+        tmem_ld_wait();
+        if (g != nullptr && r < M) {
+          const int cg = (n0 + b * 64 + q) >> 2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (cg + i < groups) {
+              const int64_t at = blocked(r, cg + i, groups);
+              *reinterpret_cast<float4*>(g + at) = make_float4(vg[4 * i], vg[4 * i + 1], vg[4 * i + 2], vg[4 * i + 3]);
+              *reinterpret_cast<float4*>(u + at) = make_float4(vu[4 * i], vu[4 * i + 1], vu[4 * i + 2], vu[4 * i + 3]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) vg[i] = act_of(vg[i], act) * vu[i];
+        stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, q, vg);
+      }
+      send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, b);
+    }
+  }
+};
+
+// dg = dh u act'(g), du = dh act(g)
+template <typename T, int CG>
+struct EpiDh {
+  const float *g, *u;
+  int M, F, act, groups;
+  __device__ __forceinline__ void fetch(float4 (&pg)[4], float4 (&pu)[4], int r, int col) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pg[i] = pu[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < M && (col >> 2) + i < groups) {
+        const int64_t at = blocked(r, (col >> 2) + i, groups);
+        pg[i] = *reinterpret_cast<const float4*>(g + at);
+        pu[i] = *reinterpret_cast<const float4*>(u + at);
+      }
+    }
+  }
+  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap* o1) const {
+    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * BN;
+    float4 ng[4], nu[4];              // the next 16 columns, on their way while these are worked on
+    fetch(ng, nu, r, n0);
+#pragma unroll 1
+    for (int b = 0; b < BN / 64 && n0 + b * 64 < F; ++b) {
+      const int buf = 2 * (b & 1);
+      buffers_free<2>(c);
+#pragma unroll
+      for (int q = 0; q < 64; q += 16) {
+        float v[16], fg[16], fu[16];
+        tmem_ld16(c.tmem + b * 64 + q, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fg[4 * i] = ng[i].x, fg[4 * i + 1] = ng[i].y, fg[4 * i + 2] = ng[i].z, fg[4 * i + 3] = ng[i].w;
+          fu[4 * i] = nu[i].x, fu[4 * i + 1] = nu[i].y, fu[4 * i + 2] = nu[i].z, fu[4 * i + 3] = nu[i].w;
+        }
+        if (b * 64 + q + 16 < BN) fetch(ng, nu, r, n0 + b * 64 + q + 16);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, da;
+          act_both(fg[i], act, a, da);
+          fg[i] = v[i] * fu[i] * da;
+          fu[i] = v[i] * a;
+        }
+        stage16<T>(c.stage_ptr + buf * EPI_BUF, c.lane, q, fg);
+        stage16<T>(c.stage_ptr + (buf + 1) * EPI_BUF, c.lane, q, fu);
+      }
+      send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, buf);
+      send_stage<T>(o1, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, buf + 1);
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------- operands
+// Rows that TMA cannot address (a base or a row stride off 16 bytes) are copied once to padded rows.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const T* src, T* dst, int64_t rows, int cols, int64_t ls, int64_t ldst) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const T* s = src + r * ls;
+    T* d = dst + r * ldst;
+    for (int c = (blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += gridDim.x * 256 * 8) {
+      Pack<T, 8> v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = c + e < cols ? s[c + e] : from_f<T>(0.f);
+      st<T, 8>(d + c, v);
+    }
+  }
+}
+
+struct Operand {
+  const void* p;
+  int64_t rows, ld;
+  int cols;
+};
+inline int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+inline int cdiv(int64_t a, int b) { return (int)((a + b - 1) / b); }
+inline bool addressable(Operand& o) {
+  if (o.rows == 1) o.ld = pad8(o.cols);
+  return ((uintptr_t)o.p & 15) == 0 && o.ld % 8 == 0;
+}
+inline int64_t packed_bytes(Operand o) {
+  return addressable(o) ? 0 : (o.rows * pad8(o.cols) * 2 + 255) / 256 * 256;
+}
+template <typename T>
+void pack(Operand& o, char*& work, cudaStream_t s) {
+  const int64_t b = packed_bytes(o);
+  addressable(o);
+  if (b == 0) return;
+  const dim3 grid(cdiv(o.cols, 2048), (unsigned)(o.rows < 65535 ? o.rows : 65535));
+  pack_kernel<T><<<grid, 256, 0, s>>>((const T*)o.p, (T*)work, o.rows, o.cols, o.ld, pad8(o.cols));
+  o.p = work;
+  o.ld = pad8(o.cols);
+  work += b;
+}
+
+// ------------------------------------------------------------------------------------------------- plans
+// How a product of M (or twice M: `twin`) x N over kb slices is cut: blocks a tile and parts of k.
+struct Plan {
+  int cg, splits;
+  int64_t part_floats;
+};
+// An estimate of a plan's time in us: waves of tiles, each its slices (256 cycles of the tensor cores) and a fill and
+// drain; single blocks run their products slower than pairs; parts are written and read once.
+inline double plan_time(int64_t M, int N, int kb, bool twin, int cg, int splits, int bn) {
+  const int64_t tiles = (int64_t)cdiv(M, BM * cg) * (twin ? 2 : 1) * cdiv(N, bn);
+  const int64_t waves = (tiles * splits * cg + sm_count() - 1) / sm_count();
+  double t = waves * (cdiv(kb, splits) * 0.14 * (cg == 1 ? 1.2 : 1.0) + 1.5);
+  if (splits > 1) t += 3.0 + (double)tiles * splits * BM * cg * BN * 8 / 5e6;
+  return t;
+}
+inline Plan plan(int64_t M, int N, int kb, bool twin, bool may_split, int bn) {
+  Plan best = {1, 1, 0};
+  double least = 1e30;
+  for (int cg = 1; cg <= 2; ++cg)
+    for (int s = 1; s <= (may_split ? 16 : 1); ++s) {
+      if (s > 1 && kb / s < 4) break;
+      const int64_t parts = s == 1 ? 0 : (int64_t)cdiv(M, BM * cg) * (twin ? 2 : 1) * cdiv(N, bn) * s * BM * cg * BN;
+      if (parts > (64 << 20)) break;
+      const double t = plan_time(M, N, kb, twin, cg, s, bn);
+      if (t < least) {
+        least = t;
+        best = {cg, s, parts};
+      }
+    }
+  return best;
+}
+
+template <typename T, int MAJOR>
+bool map_of(CUtensorMap* m, const Operand& o) {
+  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, MAJOR == MAJOR_K ? 128 : 64);
+}
+template <typename T>
+bool out_map(CUtensorMap* m, const Operand& o) {
+  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, 32);
+}
+
+struct GemmMaps {
+  CUtensorMap a0, a1, b0, b1, o0, o1;
+};
+
+template <typename T, int CG, int AMAJ, int BMAJ, typename Epi>
+int gemm_launch(const GemmMaps& m, GemmShape g, const Epi& epi, int* status, cudaStream_t s) {
+  auto* k = gemm_kernel<T, CG, AMAJ, BMAJ, Epi>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Gemm<CG>::SMEM);
+  if (e != cudaSuccess) return -100 - (int)e;
+  const int64_t items = (int64_t)g.tiles_m * g.tiles_n * g.splits, most = sm_count() / CG;
+  if (items > 0x3FFFFFFF) return -2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items < most ? items : most) * CG);
+  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.dynamicSmemBytes = Gemm<CG>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = CG;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, k, m.a0, m.a1, m.b0, m.b1, m.o0, m.o1, g, epi, status);
+  return e == cudaSuccess ? 0 : -100 - (int)e;
+}
+
+// Makes the current device's context current to this thread: the driver call that makes tensor maps needs it, and a fresh
+// thread (autograd's) has none before a runtime call like this one, which a graph capture allows
+template <typename T>
+bool bind_context() {
+  return cudaFuncSetAttribute(pack_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 0) == cudaSuccess;
+}
+
+template <typename T, int AMAJ, int BMAJ>
+bool operand_maps(GemmMaps& m, const Operand& a0, const Operand& a1, const Operand& b0, const Operand& b1) {
+  if (!map_of<T, AMAJ>(&m.a0, a0) || !map_of<T, BMAJ>(&m.b0, b0)) return false;
+  m.a1 = m.a0;
+  m.b1 = m.b0;
+  return (a1.p == a0.p || map_of<T, AMAJ>(&m.a1, a1)) && (b1.p == b0.p || map_of<T, BMAJ>(&m.b1, b1));
+}
+
+// A product whose result is stored: C (and, twin, a second C under it, from a1)
+template <typename T, int CG, int AMAJ, int BMAJ>
+int product_cg(const GemmMaps& m, int64_t M, int N, int kb0, int kb1, bool twin, const Plan& pl, void* c0, void* c1, bool tma,
+               float* part, int* status, cudaStream_t s) {
+  const int tm = cdiv(M, BM * CG), kb = kb0 + kb1, kbs = cdiv(kb, pl.splits);
+  GemmShape g = {twin ? 2 * tm : tm, cdiv(N, BN), kb0, kb1, tm, 0, 16 / CG, cdiv(kb, kbs), kbs};
+  if (g.splits == 1)
+    return gemm_launch<T, CG, AMAJ, BMAJ>(m, g, EpiStore<T, CG>{(T*)c0, (T*)c1, (int)M, N, tm, tma}, status, s);
+  const int rc = gemm_launch<T, CG, AMAJ, BMAJ>(m, g, EpiPartial<CG>{part}, status, s);
+  if (rc != 0) return rc;
+  const bool vec = (((uintptr_t)c0 | (uintptr_t)(c1 ? c1 : c0) | (uintptr_t)N * 2) & 15) == 0;
+  sum_parts_kernel<T, CG><<<dim3(g.tiles_m * g.tiles_n, BN / 16), BM * CG, 0, s>>>(part, g, (T*)c0, (T*)c1, (int)M, N, vec);
+  return launch_status();
+}
+template <typename T, int AMAJ, int BMAJ>
+int product(const Operand& a0, const Operand& a1, const Operand& b0, const Operand& b1, int64_t M, int N, int64_t k, bool two_k,
+            bool twin, void* c0, void* c1, float* part, int* status, cudaStream_t s) {
+  GemmMaps m;
+  if (!operand_maps<T, AMAJ, BMAJ>(m, a0, a1, b0, b1)) return -6;
+  Operand o0 = {c0, M, N, N}, o1 = {c1 ? c1 : c0, M, N, N};
+  const bool tma = addressable(o0) && addressable(o1) && out_map<T>(&m.o0, o0) && out_map<T>(&m.o1, o1);
+  if (!tma) m.o0 = m.o1 = m.a0;
+  const int kb = cdiv(k, BK);
+  const Plan pl = plan(M, N, two_k ? 2 * kb : kb, twin, true, BN);
+  if (pl.cg == 1)
+    return product_cg<T, 1, AMAJ, BMAJ>(m, M, N, kb, two_k ? kb : 0, twin, pl, c0, c1, tma, part, status, s);
+  return product_cg<T, 2, AMAJ, BMAJ>(m, M, N, kb, two_k ? kb : 0, twin, pl, c0, c1, tma, part, status, s);
+}
+
+struct FfnOperands {
+  Operand x, wg, wu, wd, dy, h, dg, du;
+};
+inline FfnOperands operands(const InbFfnArgs& a) {
+  FfnOperands o;
+  o.x = {a.x, a.N, a.ldx, a.D};
+  o.wg = {a.wg, a.F, a.ldwg, a.D};
+  o.wu = {a.wu, a.F, a.ldwu, a.D};
+  o.wd = {a.wd, a.D, a.ldwd, a.F};
+  o.dy = {a.dy, a.N, a.lddy, a.D};
+  o.h = {a.h, a.N, a.ldh, a.F};
+  o.dg = {a.dg, a.N, a.ldh, a.F};
+  o.du = {a.du, a.N, a.ldh, a.F};
+  return o;
+}
+inline int64_t pack_bytes(const InbFfnArgs& a, bool bwd) {
+  const FfnOperands o = operands(a);
+  return packed_bytes(o.x) + packed_bytes(o.wg) + packed_bytes(o.wu) + packed_bytes(o.wd) + (bwd ? packed_bytes(o.dy) : 0);
+}
+// packed operands, then the largest product's parts
+inline int64_t ffn_work(const InbFfnArgs& a, bool bwd) {
+  int64_t parts = 0;
+  auto need = [&](int64_t M, int N, int64_t k, bool two_k, bool twin) {
+    const int64_t p = plan(M, N, (two_k ? 2 : 1) * cdiv(k, BK), twin, true, BN).part_floats;
+    parts = p > parts ? p : parts;
+  };
+  if (!bwd) {
+    need(a.N, a.D, a.F, false, false);
+  } else {
+    need(a.N, a.D, a.F, true, false);
+    need(a.F, a.D, a.N, false, true);
+    need(a.D, a.F, a.N, false, false);
+  }
+  return pack_bytes(a, bwd) + parts * 4;
+}
+
+template <typename T>
+int ffn_forward(const InbFfnArgs& a, cudaStream_t s) {
+  if (!bind_context<T>()) return -6;
+  FfnOperands o = operands(a);
+  char* w = (char*)a.work;
+  pack<T>(o.x, w, s);
+  pack<T>(o.wg, w, s);
+  pack<T>(o.wu, w, s);
+  pack<T>(o.wd, w, s);
+  const int kb = cdiv(a.D, BK), groups = (int)(a.ldh / 4);
+  GemmMaps m;
+  if (!operand_maps<T, MAJOR_K, MAJOR_K>(m, o.x, o.x, o.wg, o.wu) || !out_map<T>(&m.o0, o.h)) return -6;
+  m.o1 = m.o0;
+  const Plan pl = plan(a.N, a.F, kb, false, false, BN / 2);
+  const int tm = cdiv(a.N, BM * pl.cg);
+  const GemmShape g = {tm, cdiv(a.F, BN / 2), kb, 0, tm, 1, 16 / pl.cg, 1, kb};
+  int rc;
+  if (pl.cg == 1)
+    rc = gemm_launch<T, 1, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, 1>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+  else
+    rc = gemm_launch<T, 2, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, 2>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+  if (rc != 0) return rc;
+  return product<T, MAJOR_K, MAJOR_K>(o.h, o.h, o.wd, o.wd, a.N, a.D, a.F, false, false, a.y, nullptr, (float*)w, a.status, s);
+}
+
+template <typename T>
+int ffn_backward(const InbFfnArgs& a, cudaStream_t s) {
+  if (!bind_context<T>()) return -6;
+  FfnOperands o = operands(a);
+  char* w = (char*)a.work;
+  pack<T>(o.x, w, s);
+  pack<T>(o.wg, w, s);
+  pack<T>(o.wu, w, s);
+  pack<T>(o.wd, w, s);
+  pack<T>(o.dy, w, s);
+  float* part = (float*)w;
+  int rc = 0;
+  if (a.dx != nullptr || a.dwg != nullptr) {
+    const int kb = cdiv(a.D, BK), groups = (int)(a.ldh / 4);
+    GemmMaps m;
+    if (!operand_maps<T, MAJOR_K, MAJOR_MN>(m, o.dy, o.dy, o.wd, o.wd) || !out_map<T>(&m.o0, o.dg) ||
+        !out_map<T>(&m.o1, o.du))
+      return -6;
+    const Plan pl = plan(a.N, a.F, kb, false, false, BN);
+    const int tm = cdiv(a.N, BM * pl.cg);
+    const GemmShape g = {tm, cdiv(a.F, BN), kb, 0, tm, 0, 16 / pl.cg, 1, kb};
+    if (pl.cg == 1)
+      rc = gemm_launch<T, 1, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, 1>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+    else
+      rc = gemm_launch<T, 2, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, 2>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+    if (rc != 0) return rc;
+  }
+  if (a.dx != nullptr) {
+    rc = product<T, MAJOR_K, MAJOR_MN>(o.dg, o.du, o.wg, o.wu, a.N, a.D, a.F, true, false, a.dx, nullptr, part, a.status, s);
+    if (rc != 0) return rc;
+  }
+  if (a.dwg != nullptr) {
+    rc = product<T, MAJOR_MN, MAJOR_MN>(o.dg, o.du, o.x, o.x, a.F, a.D, a.N, false, true, a.dwg, a.dwu, part, a.status, s);
+    if (rc != 0) return rc;
+  }
+  if (a.dwd != nullptr)
+    rc = product<T, MAJOR_MN, MAJOR_MN>(o.dy, o.dy, o.h, o.h, a.D, a.F, a.N, false, false, a.dwd, nullptr, part, a.status, s);
+  return rc;
+}
+
+int ffn_bf16(const InbFfnArgs& a, bool bwd, cudaStream_t s);
+int ffn_f16(const InbFfnArgs& a, bool bwd, cudaStream_t s);
+
+}  // namespace pol
+}  // namespace inb

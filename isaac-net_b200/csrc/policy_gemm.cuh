@@ -3,11 +3,14 @@
 //
 //   C[m, n] = sum over k of A[m, k] B[n, k],  16-bit operands, fp32 accumulation
 //
-// One persistent block per SM walks the tiles of C (BM x BN = 128 x 256).  Warp 0 fills a ring of STAGES x (A, B) slices of
-// 64 k with TMA, warp 1 issues the matrix instructions, four more warps read finished accumulators out and run the
-// epilogue.  Tensor memory holds two accumulators of 256 columns, so the epilogue of one tile runs under the products of
-// the next.  Each operand is read as it lies in memory, k or m / n contiguous: the 128-byte swizzle of the shared tiles
-// and the descriptor's major bits cover both, so no operand is ever transposed by a pass of its own.
+// Persistent blocks walk the tiles of C, 128 CG x 256: one block a tile (CG = 1), or a cluster of two whose SMs work on it
+// together (CG = 2: each holds half of A's rows and half of B's, so a slice of B crosses L2 once for both).  Warp 0 fills a
+// ring of slices of 64 k with TMA, warp 1 of the first block issues the matrix instructions, four more warps read finished
+// accumulators out and run the epilogue.  Tensor memory holds two accumulators of 256 columns, so the epilogue of one tile
+// runs under the products of the next.  Each operand is read as it lies in memory, k or m / n contiguous: the 128-byte
+// swizzle of the shared tiles and the descriptor's major bits cover both, so no operand is ever transposed by a pass of its
+// own.  Where a product has fewer tiles than the GPU has SMs, its k is split and the parts are added by a second launch in
+// a fixed order.
 //
 // Every wait has a time limit (WAIT_NS).  A wait that runs out sets the device status word and ends the block: its copies
 // in flight are waited for, its tensor memory is freed, its results are not to be used.
@@ -19,13 +22,18 @@
 namespace inb {
 namespace pol {
 
-constexpr int BM = 128, BN = 256, BK = 64;
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int BM = 128, BN = 256, BK = 64;             // of one block: rows of A; columns of C; k of a slice
 constexpr int GEMM_THREADS = 192;                      // TMA, MMA, 4 x epilogue
-constexpr int GEMM_SMEM = STAGES * (A_BYTES + B_BYTES) + 1024 + 256;
+constexpr int EPI_BUF = 4096, EPI_BUFS = 4;            // an epilogue warp's staging: 32 rows x 128 bytes, and how many
 constexpr unsigned long long WAIT_NS = 2000000000ull;  // far above any tile's time
 constexpr int MAJOR_K = 0, MAJOR_MN = 1;
+template <int CG>
+struct Gemm {
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = CG == 1 ? 3 : 5;
+  static constexpr int TM = BM * CG;
+  static constexpr int EPI = STAGES * STAGE, BARS = EPI + 4 * EPI_BUFS * EPI_BUF, SMEM = BARS + 256 + 1024;
+};
 
 // ------------------------------------------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -55,7 +63,7 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 // Waits for a phase; false when the limit ran out or another role gave up (`stop`, in shared memory).
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* stop) {
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* stop) {
   const unsigned long long t0 = now_ns();
   while (true) {
     for (int i = 0; i < 64; ++i)
@@ -71,11 +79,55 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   if (mbar_try(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, stop);
 }
+// CG = 2: the barrier may be the other block's
+template <int CG>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void store_wait() {       // all but the last N groups have been read out of shared memory
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+template <int CG>
+__device__ __forceinline__ void group_sync() {       // the blocks of one tile
+  if constexpr (CG == 1) {
+    __syncthreads();
+  } else {
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
 }
 // Shared-memory matrix descriptor of a 128-byte-swizzled tile.  K-major: rows of 128 bytes (64 k), groups of 8 rows 1024
 // bytes apart.  MN-major: chunks of 64 m or n x 64 k, 8192 bytes apart; within a chunk groups of 8 k 1024 bytes apart.
@@ -95,26 +147,60 @@ __host__ __device__ constexpr uint32_t mma_desc(int m, int n) {
          ((IsBf16<T>::value ? 1u : 0u) << 10) | ((uint32_t)AMAJ << 15) | ((uint32_t)BMAJ << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
 }
+// Arrives at the barrier once the matrix instructions issued so far are done; CG = 2: at both blocks' (same offset)
+template <int CG>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+// 16 columns of a warp's 32 rows: thread = row
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-      "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -130,6 +216,7 @@ struct GemmShape {
   int m_split;        // first m tile that reads a1 (tiles_m: none)
   int dual;
   int band;           // m tiles that are walked together, see tile_at
+  int splits, kbs;    // parts of k, and slices of one
 };
 
 // Tile order: bands of `band` m tiles, all n tiles within a band: the blocks that run at one time share their operands
@@ -142,143 +229,222 @@ __device__ __forceinline__ void tile_at(const GemmShape& g, int i, int& m, int& 
 }
 
 // The operand tile of 64 k at (row0, k0) into dst: one box of `rows` rows k-major, or boxes of 64 rows MN-major
-template <int MAJOR>
+template <int MAJOR, int CG>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int row0, int k0, int rows, uint32_t bar) {
   if (MAJOR == MAJOR_K) {
-    for (int r = 0; r < rows; r += 128) tma_2d(dst + r * 128, map, k0, row0 + r, bar);
+    for (int r = 0; r < rows; r += 128) tma_2d<CG>(dst + r * 128, map, k0, row0 + r, bar);
   } else {
-    for (int r = 0; r < rows; r += 64) tma_2d(dst + r * 128, map, row0 + r, k0, bar);
+    for (int r = 0; r < rows; r += 64) tma_2d<CG>(dst + r * 128, map, row0 + r, k0, bar);
   }
 }
 
-// Epi: struct with  __device__ void operator()(int tile_m, int tile_n, int row, uint32_t tmem) const, called by every
-// thread of the four epilogue warps with its row (0..127) of the tile and the address of that row's warp's accumulator.
-template <typename T, int AMAJ, int BMAJ, typename Epi>
+// What an epilogue warp gets for one tile: its row (thread = row) and where it lies
+struct EpiCtx {
+  int tm, tn, split, item;   // tile, part of k, and the running number of both
+  int row;                   // of the tile: 0 .. 128 CG - 1
+  int lane;
+  uint32_t tmem;             // this warp's rows of the accumulator
+  uint32_t stage;            // shared address of EPI_BUFS x EPI_BUF bytes of this warp's own
+  unsigned char* stage_ptr;
+};
+
+// Epi: struct with  void operator()(const EpiCtx&, const CUtensorMap* o0, const CUtensorMap* o1) const, called by the four
+// epilogue warps for every tile.
+template <typename T, int CG, int AMAJ, int BMAJ, typename Epi>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
-            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1, const GemmShape g,
-            const Epi epi, int* status) {
+            const __grid_constant__ CUtensorMap b0, const __grid_constant__ CUtensorMap b1,
+            const __grid_constant__ CUtensorMap o0, const __grid_constant__ CUtensorMap o1, const GemmShape g, const Epi epi,
+            int* status) {
+  using G = Gemm<CG>;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t bars = base + STAGES * (A_BYTES + B_BYTES);
-  const uint32_t full = bars, empty = bars + 8 * STAGES, tfull = bars + 16 * STAGES, tempty = tfull + 16,
+  const uint32_t full = base + G::BARS, empty = full + 8 * G::STAGES, tfull = empty + 8 * G::STAGES, tempty = tfull + 16,
                  drain = tempty + 16;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int stop;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < G::STAGES; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + 8 * i, 1);
-      mbar_init(tempty + 8 * i, 4);
+      mbar_init(tempty + 8 * i, 4 * CG);
     }
     mbar_init(drain, 1);
     stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    tmem_alloc<CG>(smem_u32(&tmem_slot));
     tc_before();
   }
-  __syncthreads();
+  group_sync<CG>();
   tc_after();
   const uint32_t tmem = tmem_slot;
-  const int tiles = g.tiles_m * g.tiles_n, kb = g.kb0 + g.kb1;
-  const int bn = g.dual ? BN / 2 : BN;
+  const int tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits, kb = g.kb0 + g.kb1;
+  const int bn = g.dual ? BN / 2 : BN, first = blockIdx.x / CG, stride = gridDim.x / CG;
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int t = first; ok && t < items; t += stride) {
         int tm, tn;
-        tile_at(g, t, tm, tn);
+        const int split = t / tiles;
+        tile_at(g, t - split * tiles, tm, tn);
         const bool second = tm >= g.m_split;
-        const int m0 = (second ? tm - g.m_split : tm) * BM, n0 = tn * bn;
-        for (int k = 0; k < kb; ++k, ++it) {
-          const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait(empty + 8 * s, (it / STAGES - 1) & 1, &stop)) {
+        const int m0 = (second ? tm - g.m_split : tm) * G::TM + (int)rank * BM, n0 = tn * bn;
+        const int k1 = min(kb, (split + 1) * g.kbs);
+        for (int k = split * g.kbs; k < k1; ++k, ++it) {
+          const int s = it % G::STAGES;
+          if (it >= G::STAGES && !mbar_wait(empty + 8 * s, (it / G::STAGES - 1) & 1, &stop)) {
             ok = false;
             break;
           }
           const bool seg = k >= g.kb0;
           const int k0 = (seg ? k - g.kb0 : k) * BK;
-          const uint32_t sa = base + s * (A_BYTES + B_BYTES), sb = sa + A_BYTES, bar = full + 8 * s;
-          mbar_expect(bar, A_BYTES + B_BYTES);
-          load_tile<AMAJ>(sa, seg || second ? &a1 : &a0, m0, k0, BM, bar);
-          if (g.dual) {
-            load_tile<BMAJ>(sb, &b0, n0, k0, BN / 2, bar);
-            load_tile<BMAJ>(sb + B_BYTES / 2, &b1, n0, k0, BN / 2, bar);
+          const uint32_t sa = base + s * G::STAGE, sb = sa + G::A_BYTES;
+          uint32_t bar = full + 8 * s;
+          if (rank == 0) mbar_expect(bar, G::STAGE * CG);      // both blocks' bytes count on the first one's barrier
+          if (CG == 2) bar = map_rank(bar, 0);
+          load_tile<AMAJ, CG>(sa, seg || second ? &a1 : &a0, m0, k0, BM, bar);
+          if (CG == 2) {
+            if (g.dual)
+              load_tile<BMAJ, CG>(sb, rank ? &b1 : &b0, n0, k0, BN / 2, bar);
+            else
+              load_tile<BMAJ, CG>(sb, seg ? &b1 : &b0, n0 + (int)rank * (BN / 2), k0, BN / 2, bar);
+          } else if (g.dual) {
+            load_tile<BMAJ, CG>(sb, &b0, n0, k0, BN / 2, bar);
+            load_tile<BMAJ, CG>(sb + G::B_BYTES / 2, &b1, n0, k0, BN / 2, bar);
           } else {
-            load_tile<BMAJ>(sb, seg ? &b1 : &b0, n0, k0, BN, bar);
+            load_tile<BMAJ, CG>(sb, seg ? &b1 : &b0, n0, k0, BN, bar);
           }
         }
       }
-      if (stop) {       // the copies in flight still write this block's shared memory: wait for them, within a limit
+      if (stop && rank == 0) {   // the copies in flight still write shared memory: wait for them, within a limit
         volatile int never = 0;
-        for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-          mbar_wait_slow(full + 8 * (i % STAGES), (i / STAGES) & 1, &never);
+        for (uint32_t i = it > G::STAGES ? it - G::STAGES : 0; i < it; ++i)
+          mbar_wait_slow(full + 8 * (i % G::STAGES), (i / G::STAGES) & 1, &never);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = mma_desc<T, AMAJ, BMAJ>(BM, BN);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = mma_desc<T, AMAJ, BMAJ>(G::TM, BN);
       uint32_t it = 0, n = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++n) {
+      for (int t = first; ok && t < items; t += stride, ++n) {
         const uint32_t acc = n & 1, d = tmem + acc * BN;
+        const int k1 = min(kb, (t / tiles + 1) * g.kbs);
         if (n >= 2 && !mbar_wait(tempty + 8 * acc, ((n >> 1) - 1) & 1, &stop)) break;
         tc_after();
-        for (int k = 0; k < kb; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(full + 8 * s, (it / STAGES) & 1, &stop)) {
+        uint32_t more = 0;
+        for (int k = t / tiles * g.kbs; k < k1; ++k, ++it) {
+          const int s = it % G::STAGES;
+          if (!mbar_wait(full + 8 * s, (it / G::STAGES) & 1, &stop)) {
             ok = false;
             break;
           }
           tc_after();
-          const uint32_t sa = base + s * (A_BYTES + B_BYTES);
-          const uint64_t da = smem_desc<AMAJ>(sa), db = smem_desc<BMAJ>(sa + A_BYTES);
+          const uint32_t sa = base + s * G::STAGE;
+          const uint64_t da = smem_desc<AMAJ>(sa), db = smem_desc<BMAJ>(sa + G::A_BYTES);
 #pragma unroll
-          for (int j = 0; j < BK / 16; ++j)
-            mma_f16(d, da + j * desc_step<AMAJ>(), db + j * desc_step<BMAJ>(), idesc, (k | j) != 0);
-          mma_commit(empty + 8 * s);
+          for (int j = 0; j < BK / 16; ++j) {
+            mma_f16<CG>(d, da + j * desc_step<AMAJ>(), db + j * desc_step<BMAJ>(), idesc, more);
+            more = 1;
+          }
+          mma_commit<CG>(empty + 8 * s);
         }
-        if (ok) mma_commit(tfull + 8 * acc);
+        if (ok) mma_commit<CG>(tfull + 8 * acc);
       }
       if (stop) {
         volatile int never = 0;
-        mma_commit(drain);
+        mma_commit<CG>(drain);
         mbar_wait_slow(drain, 0, &never);
       }
     }
   } else {
     const int quarter = warp & 3;            // the tensor-memory lanes that this warp can read
+    EpiCtx c;
+    c.lane = lane;
+    c.row = (int)rank * BM + quarter * 32 + lane;
+    c.stage = base + G::EPI + (warp - 2) * EPI_BUFS * EPI_BUF;
+    c.stage_ptr = raw + (c.stage - smem_u32(raw));
     uint32_t n = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-      int tm, tn;
-      tile_at(g, t, tm, tn);
+    for (int t = first; t < items; t += stride, ++n) {
+      c.item = t;
+      c.split = t / tiles;
+      tile_at(g, t - c.split * tiles, c.tm, c.tn);
       const uint32_t acc = n & 1;
       const bool ok = mbar_wait(tfull + 8 * acc, (n >> 1) & 1, &stop);
       if (!__all_sync(M32_ALL, ok)) break;
       tc_after();
-      epi(tm, tn, quarter * 32 + lane, tmem + acc * BN + ((uint32_t)(quarter * 32) << 16));
+      c.tmem = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      epi(c, &o0, &o1);
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty + 8 * acc);
+      if (lane == 0) {
+        if (CG == 1)
+          mbar_arrive(tempty + 8 * acc);
+        else
+          mbar_arrive_at(map_rank(tempty + 8 * acc, 0));
+      }
     }
+    if (lane == 0) store_wait<0>();
   }
   __syncwarp();
-  __syncthreads();
+  group_sync<CG>();
   if (warp == 1) {
     tc_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    tmem_free<CG>(tmem);
   }
   if (threadIdx.x == 0 && stop && status != nullptr) atomicExch(status, 1);
+}
+
+// ------------------------------------------------------------------------------------------------- epilogue helpers
+// 16 values of this thread's row into its warp's staging tile of 32 rows x 64 columns (the layout of a 128-byte-swizzled
+// TMA box): columns q, q + 16
+template <typename T>
+__device__ __forceinline__ void stage16(unsigned char* buf, int lane, int q, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    Pack<T, 8> o;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) down2(make_float2(v[8 * i + e], v[8 * i + e + 1]), o.v[e], o.v[e + 1]);
+    st<T, 8>(reinterpret_cast<T*>(buf + lane * 128 + (((q >> 3) + i) ^ (lane & 7)) * 16), o);
+  }
+}
+// Sends a staged tile to rows [r0, r0 + 32) x columns [c0, c0 + 64) of a matrix of M rows x N columns: by TMA, which clips at
+// its edges, or (rows that TMA cannot address: `p`, `ld`) by the warp itself, row after row
+template <typename T>
+__device__ __forceinline__ void send_stage(const CUtensorMap* map, T* p, int64_t ld, int M, int N, int r0, int c0,
+                                           const EpiCtx& c, int b) {
+  if (map != nullptr) {
+    proxy_fence();
+    __syncwarp();
+    if (c.lane == 0) {
+      if (r0 < M) tma_store_2d(map, c0, r0, c.stage + b * EPI_BUF);
+      store_commit();
+    }
+    return;
+  }
+  __syncwarp();
+  const int rows = min(32, M - r0), col = 2 * c.lane;
+  for (int r = 0; r < rows; ++r) {
+    const T* s = reinterpret_cast<const T*>(c.stage_ptr + b * EPI_BUF + r * 128 + (((col >> 3) ^ (r & 7)) * 16)) + (col & 7);
+    T* d = p + (int64_t)(r0 + r) * ld + c0 + col;
+    if (c0 + col < N) d[0] = s[0];
+    if (c0 + col + 1 < N) d[1] = s[1];
+  }
+  __syncwarp();
+}
+// Blocked fp32 matrices that only these kernels read: 128-row blocks, in them groups of 4 columns, in them the rows: a
+// warp's 32 rows of one group are 512 consecutive bytes.  The place of column group `cg` of row r, groups groups a row:
+__device__ __forceinline__ int64_t blocked(int r, int cg, int groups) {
+  return (((int64_t)(r >> 7) * groups + cg) * 128 + (r & 127)) * 4;
 }
 
 // ------------------------------------------------------------------------------------------------- host side

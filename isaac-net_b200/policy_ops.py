@@ -276,7 +276,7 @@ def _ffn_forward(x, wg, wu, wd, act, keep):
     """(y, h, g, u): g, u None unless `keep`."""
     n, ldh = x.numel() // x.shape[-1], (wg.shape[0] + 7) // 8 * 8
     y, h = x.new_empty(x.shape), x.new_empty(n, ldh)
-    g, u = (torch.empty(n, ldh, device=x.device) if keep else None for _ in range(2))
+    g, u = (torch.empty(-(-n // 128) * 128, ldh, device=x.device) if keep else None for _ in range(2))
     if n:
         a, held = _ffn_args(x, wg, wu, wd, act, h, g, u)
         a.y = y.data_ptr()
