@@ -18,13 +18,15 @@
 namespace inb {
 namespace pol {
 
-__device__ __forceinline__ float act_of(float g, int act) {
-  if (act == INB_ACT_SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
+template <int ACT>
+__device__ __forceinline__ float act_of(float g) {
+  if (ACT == INB_ACT_SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
   return g * (0.5f * (1.f + erff(g * 0.70710678f)));
 }
 // act(g) and its derivative
-__device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
-  if (act == INB_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& a, float& da) {
+  if (ACT == INB_ACT_SILU) {
     const float s = __fdividef(1.f, 1.f + __expf(-g));
     a = g * s;
     da = s * (1.f + g * (1.f - s));
@@ -40,26 +42,32 @@ __device__ __forceinline__ void buffers_free(const EpiCtx& c) {      // all but 
   __syncwarp();
 }
 
+struct NoState {};
+
 // C, or (tiles from m_split on) a second C, rounded
 template <typename T, int CG>
 struct EpiStore {
+  using State = NoState;
   T *c0, *c1;
   int M, N, m_split;
   bool tma;
-  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap* o1) const {
+  __device__ void begin(const EpiCtx&, State&) const {}
+  __device__ void operator()(const EpiCtx& c, State&, const CUtensorMap* o0, const CUtensorMap* o1) const {
+    constexpr int COLS = BN / EPI_COLS;
     const bool second = c.tm >= m_split;
-    const int r0 = (second ? c.tm - m_split : c.tm) * Gemm<CG>::TM + (c.row & ~31), n0 = c.tn * BN;
-#pragma unroll 1
-    for (int b = 0; b < BN / 64 && n0 + b * 64 < N; ++b) {
-      if (tma) buffers_free<EPI_BUFS - 1>(c);
+    const int r0 = (second ? c.tm - m_split : c.tm) * Gemm<CG>::TM + (c.row & ~31), n0 = c.tn * BN + c.part * COLS;
+    const uint32_t acc = c.tmem + c.part * COLS;
 #pragma unroll
-      for (int q = 0; q < 64; q += 16) {
-        float v[16];
-        tmem_ld16(c.tmem + b * 64 + q, v);
-        tmem_ld_wait();
-        stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, q, v);
-      }
-      send_stage<T>(tma ? (second ? o1 : o0) : nullptr, second ? c1 : c0, N, M, N, r0, n0 + b * 64, c, b);
+    for (int b = 0; b < COLS / 32; ++b) {
+      if (n0 + b * 32 >= N) break;
+      float v[2][16];
+      tmem_ld16(acc + b * 32, v[0]);
+      tmem_ld16(acc + b * 32 + 16, v[1]);
+      if (tma) buffers_free<EPI_BUFS - 1>(c);
+      tmem_ld_wait();
+      stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, 0, v[0]);
+      stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, 16, v[1]);
+      send_stage<T>(tma ? (second ? o1 : o0) : nullptr, second ? c1 : c0, N, M, N, r0, n0 + b * 32, c, b);
     }
   }
 };
@@ -67,13 +75,16 @@ struct EpiStore {
 // One part of k of a tile, fp32: [item][column group][row][4]
 template <int CG>
 struct EpiPartial {
+  using State = NoState;
   float* part;
-  __device__ void operator()(const EpiCtx& c, const CUtensorMap*, const CUtensorMap*) const {
-    float* p = part + ((int64_t)c.item * (BN / 4) * Gemm<CG>::TM + c.row) * 4;
-#pragma unroll 2
-    for (int q = 0; q < BN; q += 16) {
+  __device__ void begin(const EpiCtx&, State&) const {}
+  __device__ void operator()(const EpiCtx& c, State&, const CUtensorMap*, const CUtensorMap*) const {
+    constexpr int COLS = BN / EPI_COLS;
+    float* p = part + (((int64_t)c.item * (BN / 4) + c.part * (COLS / 4)) * Gemm<CG>::TM + c.row) * 4;
+#pragma unroll
+    for (int q = 0; q < COLS; q += 16) {
       float v[16];
-      tmem_ld16(c.tmem + q, v);
+      tmem_ld16(c.tmem + c.part * COLS + q, v);
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -124,88 +135,102 @@ __global__ void __launch_bounds__(Gemm<CG>::TM) sum_parts_kernel(const float* pa
   }
 }
 
-// h = act(g) u of 128 columns; g and u kept in blocked fp32 (NULL: not kept)
-template <typename T, int CG>
+// h = act(g) u of 128 columns, 32 a warp; g and u kept in blocked fp32 (NULL: not kept)
+template <typename T, int CG, int ACT>
 struct EpiGate {
+  using State = NoState;
   float *g, *u;
-  int M, F, act, groups;
-  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap*) const {
-    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * (BN / 2);
-#pragma unroll 1
-    for (int b = 0; b < 2 && n0 + b * 64 < F; ++b) {
-      buffers_free<1>(c);
+  int M, F, groups;
+  __device__ void begin(const EpiCtx&, State&) const {}
+  __device__ void operator()(const EpiCtx& c, State&, const CUtensorMap* o0, const CUtensorMap*) const {
+    constexpr int COLS = BN / 2 / EPI_COLS;
+    static_assert(COLS == 32, "one staged tile a warp");
+    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * (BN / 2) + c.part * COLS;
+    if (n0 >= F) return;
+    const int buf = c.tn & 1;
+    float vg[2][16], vu[2][16];
 #pragma unroll
-      for (int q = 0; q < 64; q += 16) {
-        float vg[16], vu[16];
-        tmem_ld16(c.tmem + b * 64 + q, vg);
-        tmem_ld16(c.tmem + BN / 2 + b * 64 + q, vu);
-        tmem_ld_wait();
-        if (g != nullptr && r < M) {
-          const int cg = (n0 + b * 64 + q) >> 2;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (cg + i < groups) {
-              const int64_t at = blocked(r, cg + i, groups);
-              *reinterpret_cast<float4*>(g + at) = make_float4(vg[4 * i], vg[4 * i + 1], vg[4 * i + 2], vg[4 * i + 3]);
-              *reinterpret_cast<float4*>(u + at) = make_float4(vu[4 * i], vu[4 * i + 1], vu[4 * i + 2], vu[4 * i + 3]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) vg[i] = act_of(vg[i], act) * vu[i];
-        stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, q, vg);
-      }
-      send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, b);
+    for (int q = 0; q < 2; ++q) {
+      tmem_ld16(c.tmem + c.part * COLS + 16 * q, vg[q]);
+      tmem_ld16(c.tmem + BN / 2 + c.part * COLS + 16 * q, vu[q]);
     }
+    buffers_free<0>(c);
+    tmem_ld_wait();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (g != nullptr && r < M) {
+        const int cg = (n0 >> 2) + 4 * q;
+        const int64_t at = blocked(r, cg, groups);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (cg + i < groups) {
+            *reinterpret_cast<float4*>(g + at + i * 512) =
+                make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]);
+            *reinterpret_cast<float4*>(u + at + i * 512) =
+                make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) vg[q][i] = act_of<ACT>(vg[q][i]) * vu[q][i];
+      stage16<T>(c.stage_ptr + buf * EPI_BUF, c.lane, 16 * q, vg[q]);
+    }
+    send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0, c, buf);
   }
 };
 
-// dg = dh u act'(g), du = dh act(g)
-template <typename T, int CG>
+// dg = dh u act'(g), du = dh act(g) of 256 columns, 64 a warp
+template <typename T, int CG, int ACT>
 struct EpiDh {
+  struct State {
+    float4 g[4], u[4];              // the next 16 columns, on their way while these are worked on
+  };
   const float *g, *u;
-  int M, F, act, groups;
-  __device__ __forceinline__ void fetch(float4 (&pg)[4], float4 (&pu)[4], int r, int col) const {
+  int M, F, groups;
+  __device__ __forceinline__ void fetch(State& s, int r, int col) const {
+    const int64_t at = blocked(r, col >> 2, groups);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      pg[i] = pu[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      s.g[i] = s.u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < M && (col >> 2) + i < groups) {
-        const int64_t at = blocked(r, (col >> 2) + i, groups);
-        pg[i] = *reinterpret_cast<const float4*>(g + at);
-        pu[i] = *reinterpret_cast<const float4*>(u + at);
+        s.g[i] = *reinterpret_cast<const float4*>(g + at + i * 512);
+        s.u[i] = *reinterpret_cast<const float4*>(u + at + i * 512);
       }
     }
   }
-  __device__ void operator()(const EpiCtx& c, const CUtensorMap* o0, const CUtensorMap* o1) const {
-    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * BN;
-    float4 ng[4], nu[4];              // the next 16 columns, on their way while these are worked on
-    fetch(ng, nu, r, n0);
-#pragma unroll 1
-    for (int b = 0; b < BN / 64 && n0 + b * 64 < F; ++b) {
-      const int buf = 2 * (b & 1);
-      buffers_free<2>(c);
+  __device__ void begin(const EpiCtx& c, State& s) const {
+    fetch(s, c.tm * Gemm<CG>::TM + c.row, c.tn * BN + c.part * (BN / EPI_COLS));
+  }
+  __device__ void operator()(const EpiCtx& c, State& s, const CUtensorMap* o0, const CUtensorMap* o1) const {
+    constexpr int COLS = BN / EPI_COLS;
+    const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * BN + c.part * COLS;
+    const uint32_t acc = c.tmem + c.part * COLS;
 #pragma unroll
-      for (int q = 0; q < 64; q += 16) {
+    for (int b = 0; b < COLS / 32; ++b) {
+      if (n0 + b * 32 >= F) break;
+#pragma unroll
+      for (int q = 0; q < 32; q += 16) {
         float v[16], fg[16], fu[16];
-        tmem_ld16(c.tmem + b * 64 + q, v);
+        tmem_ld16(acc + b * 32 + q, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          fg[4 * i] = ng[i].x, fg[4 * i + 1] = ng[i].y, fg[4 * i + 2] = ng[i].z, fg[4 * i + 3] = ng[i].w;
-          fu[4 * i] = nu[i].x, fu[4 * i + 1] = nu[i].y, fu[4 * i + 2] = nu[i].z, fu[4 * i + 3] = nu[i].w;
+          fg[4 * i] = s.g[i].x, fg[4 * i + 1] = s.g[i].y, fg[4 * i + 2] = s.g[i].z, fg[4 * i + 3] = s.g[i].w;
+          fu[4 * i] = s.u[i].x, fu[4 * i + 1] = s.u[i].y, fu[4 * i + 2] = s.u[i].z, fu[4 * i + 3] = s.u[i].w;
         }
-        if (b * 64 + q + 16 < BN) fetch(ng, nu, r, n0 + b * 64 + q + 16);
+        if (b * 32 + q + 16 < COLS) fetch(s, r, n0 + b * 32 + q + 16);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float a, da;
-          act_both(fg[i], act, a, da);
+          act_both<ACT>(fg[i], a, da);
           fg[i] = v[i] * fu[i] * da;
           fu[i] = v[i] * a;
         }
-        stage16<T>(c.stage_ptr + buf * EPI_BUF, c.lane, q, fg);
-        stage16<T>(c.stage_ptr + (buf + 1) * EPI_BUF, c.lane, q, fu);
+        if (q == 0) buffers_free<0>(c);
+        stage16<T>(c.stage_ptr, c.lane, q, fg);
+        stage16<T>(c.stage_ptr + EPI_BUF, c.lane, q, fu);
       }
-      send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, buf);
-      send_stage<T>(o1, (T*)nullptr, 0, M, F, r0, n0 + b * 64, c, buf + 1);
+      send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0 + b * 32, c, 0);
+      send_stage<T>(o1, (T*)nullptr, 0, M, F, r0, n0 + b * 32, c, 1);
     }
   }
 };
@@ -286,11 +311,11 @@ inline Plan plan(int64_t M, int N, int kb, bool twin, bool may_split, int bn) {
 
 template <typename T, int MAJOR>
 bool map_of(CUtensorMap* m, const Operand& o) {
-  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, MAJOR == MAJOR_K ? 128 : 64);
+  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, 64, MAJOR == MAJOR_K ? 128 : 64);
 }
 template <typename T>
 bool out_map(CUtensorMap* m, const Operand& o) {
-  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, 32);
+  return make_map<T>(m, o.p, o.rows, o.cols, o.ld, 32, 32);
 }
 
 struct GemmMaps {
@@ -399,6 +424,20 @@ inline int64_t ffn_work(const InbFfnArgs& a, bool bwd) {
   return pack_bytes(a, bwd) + parts * 4;
 }
 
+// The two products with an activation in their epilogue
+template <typename T, int CG, int ACT>
+int gate_product(const GemmMaps& m, const InbFfnArgs& a, int kb, cudaStream_t s) {
+  const int tm = cdiv(a.N, BM * CG);
+  const GemmShape g = {tm, cdiv(a.F, BN / 2), kb, 0, tm, 1, 16 / CG, 1, kb};
+  return gemm_launch<T, CG, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, CG, ACT>{a.g, a.u, (int)a.N, a.F, (int)(a.ldh / 4)}, a.status, s);
+}
+template <typename T, int CG, int ACT>
+int dh_product(const GemmMaps& m, const InbFfnArgs& a, int kb, cudaStream_t s) {
+  const int tm = cdiv(a.N, BM * CG);
+  const GemmShape g = {tm, cdiv(a.F, BN), kb, 0, tm, 0, 16 / CG, 1, kb};
+  return gemm_launch<T, CG, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, CG, ACT>{a.g, a.u, (int)a.N, a.F, (int)(a.ldh / 4)}, a.status, s);
+}
+
 template <typename T>
 int ffn_forward(const InbFfnArgs& a, cudaStream_t s) {
   if (!bind_context<T>()) return -6;
@@ -408,18 +447,16 @@ int ffn_forward(const InbFfnArgs& a, cudaStream_t s) {
   pack<T>(o.wg, w, s);
   pack<T>(o.wu, w, s);
   pack<T>(o.wd, w, s);
-  const int kb = cdiv(a.D, BK), groups = (int)(a.ldh / 4);
+  const int kb = cdiv(a.D, BK);
   GemmMaps m;
   if (!operand_maps<T, MAJOR_K, MAJOR_K>(m, o.x, o.x, o.wg, o.wu) || !out_map<T>(&m.o0, o.h)) return -6;
   m.o1 = m.o0;
-  const Plan pl = plan(a.N, a.F, kb, false, false, BN / 2);
-  const int tm = cdiv(a.N, BM * pl.cg);
-  const GemmShape g = {tm, cdiv(a.F, BN / 2), kb, 0, tm, 1, 16 / pl.cg, 1, kb};
+  const int cg = plan(a.N, a.F, kb, false, false, BN / 2).cg;
   int rc;
-  if (pl.cg == 1)
-    rc = gemm_launch<T, 1, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, 1>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+  if (a.act == INB_ACT_SILU)
+    rc = cg == 1 ? gate_product<T, 1, INB_ACT_SILU>(m, a, kb, s) : gate_product<T, 2, INB_ACT_SILU>(m, a, kb, s);
   else
-    rc = gemm_launch<T, 2, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, 2>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+    rc = cg == 1 ? gate_product<T, 1, INB_ACT_GELU>(m, a, kb, s) : gate_product<T, 2, INB_ACT_GELU>(m, a, kb, s);
   if (rc != 0) return rc;
   return product<T, MAJOR_K, MAJOR_K>(o.h, o.h, o.wd, o.wd, a.N, a.D, a.F, false, false, a.y, nullptr, (float*)w, a.status, s);
 }
@@ -437,18 +474,16 @@ int ffn_backward(const InbFfnArgs& a, cudaStream_t s) {
   float* part = (float*)w;
   int rc = 0;
   if (a.dx != nullptr || a.dwg != nullptr) {
-    const int kb = cdiv(a.D, BK), groups = (int)(a.ldh / 4);
+    const int kb = cdiv(a.D, BK);
     GemmMaps m;
     if (!operand_maps<T, MAJOR_K, MAJOR_MN>(m, o.dy, o.dy, o.wd, o.wd) || !out_map<T>(&m.o0, o.dg) ||
         !out_map<T>(&m.o1, o.du))
       return -6;
-    const Plan pl = plan(a.N, a.F, kb, false, false, BN);
-    const int tm = cdiv(a.N, BM * pl.cg);
-    const GemmShape g = {tm, cdiv(a.F, BN), kb, 0, tm, 0, 16 / pl.cg, 1, kb};
-    if (pl.cg == 1)
-      rc = gemm_launch<T, 1, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, 1>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+    const int cg = plan(a.N, a.F, kb, false, false, BN).cg;
+    if (a.act == INB_ACT_SILU)
+      rc = cg == 1 ? dh_product<T, 1, INB_ACT_SILU>(m, a, kb, s) : dh_product<T, 2, INB_ACT_SILU>(m, a, kb, s);
     else
-      rc = gemm_launch<T, 2, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, 2>{a.g, a.u, (int)a.N, a.F, a.act, groups}, a.status, s);
+      rc = cg == 1 ? dh_product<T, 1, INB_ACT_GELU>(m, a, kb, s) : dh_product<T, 2, INB_ACT_GELU>(m, a, kb, s);
     if (rc != 0) return rc;
   }
   if (a.dx != nullptr) {

@@ -5,8 +5,9 @@
 //
 // Persistent blocks walk the tiles of C, 128 CG x 256: one block a tile (CG = 1), or a cluster of two whose SMs work on it
 // together (CG = 2: each holds half of A's rows and half of B's, so a slice of B crosses L2 once for both).  Warp 0 fills a
-// ring of slices of 64 k with TMA, warp 1 of the first block issues the matrix instructions, four more warps read finished
-// accumulators out and run the epilogue.  Tensor memory holds two accumulators of 256 columns, so the epilogue of one tile
+// ring of slices of 64 k with TMA, warp 1 of the first block issues the matrix instructions, sixteen more warps read
+// finished accumulators out and run the epilogue (four to a scheduler: one alone waits on its own instructions most of the
+// time, and a product over few slices is bound by its epilogue).  Tensor memory holds two accumulators of 256 columns, so the epilogue of one tile
 // runs under the products of the next.  Each operand is read as it lies in memory, k or m / n contiguous: the 128-byte
 // swizzle of the shared tiles and the descriptor's major bits cover both, so no operand is ever transposed by a pass of its
 // own.  Where a product has fewer tiles than the GPU has SMs, its k is split and the parts are added by a second launch in
@@ -23,8 +24,9 @@ namespace inb {
 namespace pol {
 
 constexpr int BM = 128, BN = 256, BK = 64;             // of one block: rows of A; columns of C; k of a slice
-constexpr int GEMM_THREADS = 192;                      // TMA, MMA, 4 x epilogue
-constexpr int EPI_BUF = 4096, EPI_BUFS = 4;            // an epilogue warp's staging: 32 rows x 128 bytes, and how many
+constexpr int EPI_WARPS = 16, EPI_COLS = EPI_WARPS / 4; // four warps to each of four column ranges
+constexpr int GEMM_THREADS = 64 + 32 * EPI_WARPS;      // TMA, MMA, epilogue
+constexpr int EPI_BUF = 2048, EPI_BUFS = 2;            // an epilogue warp's staging: 32 rows x 64 bytes, and how many
 constexpr unsigned long long WAIT_NS = 2000000000ull;  // far above any tile's time
 constexpr int MAJOR_K = 0, MAJOR_MN = 1;
 template <int CG>
@@ -32,7 +34,7 @@ struct Gemm {
   static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = CG == 1 ? 3 : 5;
   static constexpr int TM = BM * CG;
-  static constexpr int EPI = STAGES * STAGE, BARS = EPI + 4 * EPI_BUFS * EPI_BUF, SMEM = BARS + 256 + 1024;
+  static constexpr int EPI = STAGES * STAGE, BARS = EPI + EPI_WARPS * EPI_BUFS * EPI_BUF, SMEM = BARS + 256 + 1024;
 };
 
 // ------------------------------------------------------------------------------------------------- instructions
@@ -242,14 +244,16 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 struct EpiCtx {
   int tm, tn, split, item;   // tile, part of k, and the running number of both
   int row;                   // of the tile: 0 .. 128 CG - 1
+  int part;                  // which of the EPI_COLS column ranges is this warp's
   int lane;
   uint32_t tmem;             // this warp's rows of the accumulator
   uint32_t stage;            // shared address of EPI_BUFS x EPI_BUF bytes of this warp's own
   unsigned char* stage_ptr;
 };
 
-// Epi: struct with  void operator()(const EpiCtx&, const CUtensorMap* o0, const CUtensorMap* o1) const, called by the four
-// epilogue warps for every tile.
+// Epi: struct with  void begin(const EpiCtx&, State&) const  (before the accumulator is complete: what can be fetched early) and
+// void operator()(const EpiCtx&, State&, const CUtensorMap* o0, const CUtensorMap* o1) const, called by the epilogue warps
+// for every tile.
 template <typename T, int CG, int AMAJ, int BMAJ, typename Epi>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUtensorMap a1,
@@ -272,7 +276,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUte
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + 8 * i, 1);
-      mbar_init(tempty + 8 * i, 4 * CG);
+      mbar_init(tempty + 8 * i, EPI_WARPS * CG);
     }
     mbar_init(drain, 1);
     stop = 0;
@@ -371,6 +375,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUte
     EpiCtx c;
     c.lane = lane;
     c.row = (int)rank * BM + quarter * 32 + lane;
+    c.part = (warp - 2) >> 2;
     c.stage = base + G::EPI + (warp - 2) * EPI_BUFS * EPI_BUF;
     c.stage_ptr = raw + (c.stage - smem_u32(raw));
     uint32_t n = 0;
@@ -379,11 +384,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUte
       c.split = t / tiles;
       tile_at(g, t - c.split * tiles, c.tm, c.tn);
       const uint32_t acc = n & 1;
+      typename Epi::State state;
+      epi.begin(c, state);
       const bool ok = mbar_wait(tfull + 8 * acc, (n >> 1) & 1, &stop);
       if (!__all_sync(M32_ALL, ok)) break;
       tc_after();
       c.tmem = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-      epi(c, &o0, &o1);
+      epi(c, state, &o0, &o1);
       tc_before();
       __syncwarp();
       if (lane == 0) {
@@ -405,8 +412,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap a0, const __grid_constant__ CUte
 }
 
 // ------------------------------------------------------------------------------------------------- epilogue helpers
-// 16 values of this thread's row into its warp's staging tile of 32 rows x 64 columns (the layout of a 128-byte-swizzled
-// TMA box): columns q, q + 16
+// 16 values of this thread's row into its warp's staging tile of 32 rows x 32 columns (the layout of a 64-byte-swizzled TMA
+// box): columns q, q + 16
 template <typename T>
 __device__ __forceinline__ void stage16(unsigned char* buf, int lane, int q, const float (&v)[16]) {
 #pragma unroll
@@ -414,11 +421,11 @@ __device__ __forceinline__ void stage16(unsigned char* buf, int lane, int q, con
     Pack<T, 8> o;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) down2(make_float2(v[8 * i + e], v[8 * i + e + 1]), o.v[e], o.v[e + 1]);
-    st<T, 8>(reinterpret_cast<T*>(buf + lane * 128 + (((q >> 3) + i) ^ (lane & 7)) * 16), o);
+    st<T, 8>(reinterpret_cast<T*>(buf + lane * 64 + (((q >> 3) + i) ^ ((lane >> 1) & 3)) * 16), o);
   }
 }
-// Sends a staged tile to rows [r0, r0 + 32) x columns [c0, c0 + 64) of a matrix of M rows x N columns: by TMA, which clips at
-// its edges, or (rows that TMA cannot address: `p`, `ld`) by the warp itself, row after row
+// Sends a staged tile to rows [r0, r0 + 32) x columns [c0, c0 + 32) of a matrix of M rows x N columns: by TMA, which clips at
+// its edges, or (rows that TMA cannot address: `p`, `ld`) by the warp itself, two rows at a time
 template <typename T>
 __device__ __forceinline__ void send_stage(const CUtensorMap* map, T* p, int64_t ld, int M, int N, int r0, int c0,
                                            const EpiCtx& c, int b) {
@@ -432,9 +439,9 @@ __device__ __forceinline__ void send_stage(const CUtensorMap* map, T* p, int64_t
     return;
   }
   __syncwarp();
-  const int rows = min(32, M - r0), col = 2 * c.lane;
-  for (int r = 0; r < rows; ++r) {
-    const T* s = reinterpret_cast<const T*>(c.stage_ptr + b * EPI_BUF + r * 128 + (((col >> 3) ^ (r & 7)) * 16)) + (col & 7);
+  const int rows = min(32, M - r0), col = 2 * (c.lane & 15);
+  for (int r = c.lane >> 4; r < rows; r += 2) {
+    const T* s = reinterpret_cast<const T*>(c.stage_ptr + b * EPI_BUF + r * 64 + (((col >> 3) ^ ((r >> 1) & 3)) * 16)) + (col & 7);
     T* d = p + (int64_t)(r0 + r) * ld + c0 + col;
     if (c0 + col < N) d[0] = s[0];
     if (c0 + col + 1 < N) d[1] = s[1];
@@ -461,19 +468,21 @@ inline EncodeTiled encode_tiled() {
   return fn;
 }
 
-// A row-major [rows, cols] matrix of 16-bit elements, rows `ld` elements apart, as an operand whose k runs along the columns
-// (MAJOR_K, box 64 columns x `box_rows` rows) or along the rows (MAJOR_MN, box 64 x 64).  Needs ld % 8 == 0 and a 16-byte
-// aligned base; what lies outside the matrix reads as zero.
+// A row-major [rows, cols] matrix of 16-bit elements, rows `ld` elements apart, in boxes of `box_cols` x `box_rows`: as an
+// operand whose k runs along the columns (MAJOR_K, 64 x 128) or along the rows (MAJOR_MN, 64 x 64), or as an epilogue's
+// output (32 x 32).  The swizzle spans a box's row.  Needs ld % 8 == 0 and a 16-byte aligned base; what lies outside the
+// matrix reads as zero and is not written.
 template <typename T>
-static bool make_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+static bool make_map(CUtensorMap* m, const void* p, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
   EncodeTiled f = encode_tiled();
   return f != nullptr &&
          f(m, IsBf16<T>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p),
-           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace pol
