@@ -441,7 +441,8 @@ int inb_block_norm_work(const InbNormArgs *args, int64_t *elems);
 
 /* Gated feed-forward block over N rows: h = act(x wg^T) * (x wu^T), y = h wd^T; x [N, D], wg, wu [F, D], wd [D, F] of
  * dtype bf16 or fp16, rows ld* elements apart; y, dx, dw* are contiguous.  Products accumulate in fp32; h, dg and du
- * are rounded to dtype.  h [N, ldh] is written by the forward call; g, u (both or neither; N rounded up to 128, times
+ * are rounded to dtype.  h [N, ldh] is written by the forward call ([2, N, ldh] for up to INB_FFN_ROWS rows without
+ * g and u, where h is kept to twice dtype's precision); g, u (both or neither; N rounded up to 128, times
  * ldh, fp32, in an order of the kernels' own) keep the projections for the backward call, which reads all three, takes
  * dy [N, D], uses dg, du [N, ldh] as scratch and writes whichever of dx, (dwg, dwu), dwd are given.  ldh: a multiple of
  * 8, at least F; h, g, u, dg, du, work: 16-byte aligned.  work: inb_gated_ffn_work() bytes, for operands whose rows are
@@ -451,6 +452,7 @@ int inb_block_norm_work(const InbNormArgs *args, int64_t *elems);
  * -6: no tensor map could be made. */
 enum { INB_ACT_SILU = 0, INB_ACT_GELU = 1 };   /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
 #define INB_MAX_FFN (1 << 30)
+#define INB_FFN_ROWS 32       /* rows up to which a call without g and u streams the weights past the rows */
 typedef struct {
   int32_t dtype, act, D, F;
   int64_t N, ldx, ldwg, ldwu, ldwd, ldh, lddy;

@@ -159,6 +159,7 @@ class InbNormArgs(ctypes.Structure):
 
 ACTS = {"silu": 0, "gelu": 1}     # INB_ACT_SILU, INB_ACT_GELU
 MAX_FFN = 1 << 30
+FFN_ROWS = 32                     # INB_FFN_ROWS
 
 
 class InbFfnArgs(ctypes.Structure):

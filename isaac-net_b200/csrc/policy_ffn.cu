@@ -19,6 +19,7 @@ static int ffn_check(const InbFfnArgs* p, bool bwd, bool sizes_only) {
               ((a.dx != nullptr || a.dwg != nullptr) &&
                (a.dg == nullptr || a.du == nullptr || (((uintptr_t)a.dg | (uintptr_t)a.du) & 15) != 0))))
     return -3;
+  if (few_rows(a, bwd)) return 0;
   if (a.work_bytes < ffn_work(a, bwd) || (a.work_bytes > 0 && ((uintptr_t)a.work & 15) != 0)) return -5;
   return 0;
 }
@@ -26,6 +27,7 @@ static int ffn_check(const InbFfnArgs* p, bool bwd, bool sizes_only) {
 static int ffn_run(const InbFfnArgs* args, bool bwd, void* stream) {
   const int rc = ffn_check(args, bwd, false);
   if (rc != 0 || args->N == 0) return rc;
+  if (few_rows(*args, bwd)) return ffn_rows_any(*args, (cudaStream_t)stream);
   return (args->dtype == INB_BF16 ? ffn_bf16 : ffn_f16)(*args, bwd, (cudaStream_t)stream);
 }
 
@@ -45,6 +47,6 @@ extern "C" int inb_gated_ffn_work(const InbFfnArgs* args, int32_t backward, int6
   *bytes = 0;
   const int rc = inb::pol::ffn_check(args, backward != 0, true);
   if (rc != 0 || args->N == 0) return rc;
-  *bytes = inb::pol::ffn_work(*args, backward != 0);
+  if (!inb::pol::few_rows(*args, backward != 0)) *bytes = inb::pol::ffn_work(*args, backward != 0);
   return 0;
 }

@@ -501,6 +501,9 @@ int ffn_backward(const InbFfnArgs& a, cudaStream_t s) {
 
 int ffn_bf16(const InbFfnArgs& a, bool bwd, cudaStream_t s);
 int ffn_f16(const InbFfnArgs& a, bool bwd, cudaStream_t s);
+int ffn_rows_any(const InbFfnArgs& a, cudaStream_t s);
+// Whether a call is one of few rows that keeps nothing for a backward pass (policy_ffn_rows.cu)
+inline bool few_rows(const InbFfnArgs& a, bool bwd) { return !bwd && a.g == nullptr && a.N <= INB_FFN_ROWS; }
 
 }  // namespace pol
 }  // namespace inb

@@ -275,12 +275,13 @@ def _ffn_work(a, backward, dev):
 def _ffn_forward(x, wg, wu, wd, act, keep):
     """(y, h, g, u): g, u None unless `keep`."""
     n, ldh = x.numel() // x.shape[-1], (wg.shape[0] + 7) // 8 * 8
-    y, h = x.new_empty(x.shape), x.new_empty(n, ldh)
+    few = not keep and n <= nat.FFN_ROWS
+    y, h = x.new_empty(x.shape), x.new_empty(2 * n if few else n, ldh)
     g, u = (torch.empty(-(-n // 128) * 128, ldh, device=x.device) if keep else None for _ in range(2))
     if n:
         a, held = _ffn_args(x, wg, wu, wd, act, h, g, u)
         a.y = y.data_ptr()
-        work = _ffn_work(a, 0, x.device)
+        work = None if few else _ffn_work(a, 0, x.device)
         _call("inb_gated_ffn_fwd", a, x.get_device())
     return y, h, g, u
 

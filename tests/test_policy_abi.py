@@ -23,7 +23,7 @@ def test_policy_struct_layouts_match_the_header(tmp_path):
         lines.append(f'  printf("{cname} %zu\\n", sizeof({cname}));')
         lines += [f'  printf("{cname}.{f} %zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
     consts = ("INB_BF16", "INB_F16", "INB_F32", "INB_MAX_NORM_D", "INB_MAX_SAMPLE_V", "INB_MAX_SAMPLE_N", "INB_MAX_FFN",
-              "INB_ACT_SILU", "INB_ACT_GELU")
+              "INB_FFN_ROWS", "INB_MAX_NORM_LD", "INB_ACT_SILU", "INB_ACT_GELU")
     lines += [f'  printf("{c} %d\\n", (int){c});' for c in consts] + ["  return 0;", "}"]
     c, exe = tmp_path / "layout.c", tmp_path / "layout"
     c.write_text("\n".join(lines))
@@ -35,7 +35,7 @@ def test_policy_struct_layouts_match_the_header(tmp_path):
         for f, _ in cls._fields_:
             assert int(got[f"{cname}.{f}"]) == getattr(cls, f).offset, f"{cname}.{f}"
     want = (nat.BF16, nat.F16, nat.F32, nat.MAX_NORM_D, nat.MAX_SAMPLE_V, nat.MAX_SAMPLE_N, nat.MAX_FFN,
-            nat.ACTS["silu"], nat.ACTS["gelu"])
+            nat.FFN_ROWS, nat.MAX_NORM_LD, nat.ACTS["silu"], nat.ACTS["gelu"])
     assert [int(got[k]) for k in consts] == list(want)
 
 
@@ -66,7 +66,7 @@ def test_refused_calls_return_their_status():
     f = lambda **kw: nat.InbFfnArgs(**{**dict(dtype=nat.BF16, D=8, F=8, N=4, ldx=8, ldwg=8, ldwu=8, ldwd=8, ldh=8, x=256,
                                               wg=256, wu=256, wd=256, y=256, h=256), **kw})
     for kw, rc in [(dict(dtype=nat.F32), -2), (dict(act=2), -2), (dict(ldh=9), -2), (dict(ldh=0), -2), (dict(F=0), -2),
-                   (dict(x=None), -3), (dict(h=264), -3), (dict(g=256), -3), (dict(ldx=9), -5), (dict(N=0), 0)]:
+                   (dict(x=None), -3), (dict(h=264), -3), (dict(g=256), -3), (dict(N=40, ldx=9), -5), (dict(N=0), 0)]:
         assert L.inb_gated_ffn_fwd(r(f(**kw)), None) == rc, kw
     assert L.inb_gated_ffn_bwd(r(f()), None) == -3
 
@@ -74,9 +74,11 @@ def test_refused_calls_return_their_status():
 def test_work_sizes():
     L = nat.lib()
     size = nat.i64()
-    a = nat.InbFfnArgs(dtype=nat.BF16, D=9, F=8, N=4, ldx=9, ldwg=16, ldwu=9, ldwd=8, ldh=8, x=256, wg=256, wu=256, wd=258)
+    a = nat.InbFfnArgs(dtype=nat.BF16, D=9, F=8, N=40, ldx=9, ldwg=16, ldwu=9, ldwd=8, ldh=8, x=256, wg=256, wu=256, wd=258)
     assert L.inb_gated_ffn_work(ctypes.byref(a), 0, ctypes.byref(size)) == 0
-    assert size.value == 256 + 256 + 256              # x, wu (rows of 9) and wd (base off 16 bytes), each padded
+    assert size.value == 1280 + 256 + 256             # x, wu (rows of 9) and wd (base off 16 bytes), each padded
+    a.N = 4                                           # few rows: the weights are read as they are
+    assert L.inb_gated_ffn_work(ctypes.byref(a), 0, ctypes.byref(size)) == 0 and size.value == 0
     assert L.inb_gated_ffn_work(ctypes.byref(a), 0, None) == -1
 
 
