@@ -18,12 +18,35 @@ namespace pol {
 
 constexpr int DROP_THREADS = 256;
 constexpr int DROP_SPAN = 16;     // elements of one thread
+constexpr int DROP_TILE = DROP_THREADS * DROP_SPAN;
 
-// One block per tile of one env: tile = DROP_THREADS * DROP_SPAN elements of its n.
+// One block per tile of one env's row.  Bound by instruction issue: a word takes 17 operations to hash and 10 to apply to
+// its two elements.  184.5 M bf16 elements take 136 us, their bytes 113 at the measured copy rate.  Tried and slower: several tiles a block with the
+// next one loaded ahead (7 us more), shifts as multiplies on the idle pipe (3 us more).
 template <typename T, int V>
 __global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(InbDropoutArgs a, uint32_t tiles, float scale) {
-  const uint64_t unit = blockIdx.x;
-  const uint32_t e = (uint32_t)(unit / tiles), tile = (uint32_t)(unit % tiles);
+  const uint32_t e = blockIdx.x / tiles, tile = blockIdx.x - e * tiles;
+  const int64_t n = a.n;
+  const T* x = (const T*)a.x + (int64_t)e * n;
+  T* y = (T*)a.y + (int64_t)e * n;
+  constexpr int W = V < 2 ? 2 : V;           // elements of one step: whole words
+  const int64_t start = (int64_t)tile * DROP_TILE + threadIdx.x * W;
+  // the elements are on their way before the key, which takes a few dependent loads of its own
+  T in[DROP_SPAN];
+#pragma unroll
+  for (int i = 0; i < DROP_SPAN / W; ++i) {
+    const int64_t c = start + i * DROP_THREADS * W;
+    if (V >= 2) {
+      if (c < n) {
+        const Pack<T, W> p = ld<T, W>(x + c);
+#pragma unroll
+        for (int k = 0; k < W; ++k) in[i * W + k] = p.v[k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) in[i * W + k] = c + k < n ? x[c + k] : from_f<T>(0.f);
+    }
+  }
   __shared__ uint32_t key;
   if (threadIdx.x == 0) {
     uint32_t k;
@@ -37,39 +60,20 @@ __global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(InbDropoutArgs a,
     key = k;
   }
   __syncthreads();
-  const uint32_t base = key, thr = a.threshold;
-  const int64_t n = a.n;
-  const T* x = (const T*)a.x + (int64_t)e * n;
-  T* y = (T*)a.y + (int64_t)e * n;
-  constexpr int W = V < 2 ? 2 : V;           // elements of one step: whole words
-  const int64_t start = (int64_t)tile * (DROP_THREADS * DROP_SPAN) + threadIdx.x * W;
-  T in[DROP_SPAN];
+  // a half is compared with the threshold in the upper half of a word, without being taken out; 65536 does not fit there
+  const uint32_t base = key, thr = a.threshold << 16;
+  const bool none = a.threshold > 65535u;
 #pragma unroll
   for (int i = 0; i < DROP_SPAN / W; ++i) {
-    const int64_t c = start + (int64_t)i * DROP_THREADS * W;
-    if (V >= 2) {
-      if (c < n) {
-        const Pack<T, W> p = ld<T, W>(x + c);
-#pragma unroll
-        for (int k = 0; k < W; ++k) in[i * W + k] = p.v[k];
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-        if (c + k < n) in[i * W + k] = x[c + k];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < DROP_SPAN / W; ++i) {
-    const int64_t c = start + (int64_t)i * DROP_THREADS * W;
+    const int64_t c = start + i * DROP_THREADS * W;
     if (c >= n) break;
     Pack<T, W> o;
+    const uint32_t word = base + (uint32_t)(c >> 1) * GOLD;      // c is even
 #pragma unroll
     for (int k = 0; k < W; k += 2) {
-      const uint32_t w = elem(base, (uint32_t)((c + k) >> 1));
-      const float lo = to_f(in[i * W + k]) * scale, hi = to_f(in[i * W + k + 1]) * scale;
-      o.v[k] = from_f<T>((w & 0xFFFFu) >= thr ? lo : 0.f);
-      o.v[k + 1] = from_f<T>((w >> 16) >= thr ? hi : 0.f);
+      const uint32_t w = mix32(mix32(word + (uint32_t)(k / 2) * GOLD) ^ base);      // elem(base, c / 2 + k / 2)
+      const float2 v = mul2(up2(in[i * W + k], in[i * W + k + 1]), both(scale));
+      down2(make_float2(w << 16 >= thr && !none ? v.x : 0.f, w >= thr && !none ? v.y : 0.f), o.v[k], o.v[k + 1]);
     }
     if (V >= 2) {
       st<T, W>(y + c, o);
@@ -83,8 +87,7 @@ __global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(InbDropoutArgs a,
 
 template <typename T>
 static int dropout_go(const InbDropoutArgs& a, cudaStream_t s) {
-  const uint64_t tiles = ((uint64_t)a.n + DROP_THREADS * DROP_SPAN - 1) / (DROP_THREADS * DROP_SPAN);
-  const uint64_t grid = tiles * (uint64_t)a.E;
+  const uint64_t tiles = ((uint64_t)a.n + DROP_TILE - 1) / DROP_TILE, grid = tiles * (uint64_t)a.E;
   if (grid > 0x7FFFFFFFull) return -2;
   const float scale = a.threshold < 65536u ? 65536.f / (float)(65536u - a.threshold) : 0.f;
   constexpr int W = 16 / (int)sizeof(T);
