@@ -93,77 +93,99 @@ __device__ __forceinline__ float logp_of(float z, long long total) {
 }
 
 // ------------------------------------------------------------------------------------------------ a warp per row
-// The sums of a row of up to 128 masses, from the masses' low 20 bits and the rest
-__device__ __forceinline__ long long warp_mass(uint32_t lo, uint32_t hi) {
-  return (long long)__reduce_add_sync(M32_ALL, lo) + ((long long)__reduce_add_sync(M32_ALL, hi) << 20);
+// Masses of up to 128 elements as two words, q = hi 2^20 + lo with lo < 2^20: either sum fits 32 bits, so a warp adds them
+// with one redux each
+__device__ __forceinline__ long long mass_of(uint32_t hi, uint32_t lo) { return ((long long)hi << 20) + lo; }
+__device__ __forceinline__ long long warp_mass(uint32_t hi, uint32_t lo) {
+  return mass_of(__reduce_add_sync(M32_ALL, hi), __reduce_add_sync(M32_ALL, lo));
 }
 
-// One row: `key`, `z`, `q` of its elements, EPL a lane, element j * 32 + lane.  cut() zeroes the masses that a filter takes
-// away: by count (top-k) or by mass (top-p).  The largest remaining value is taken away until the target is reached; five
-// steps of bisection over z before that leave it a sixteenth of the range (0 .. -4, or -4 .. -28) to walk.
+// One row: keys, exponents z and masses of its elements, EPL a lane, element j * 32 + lane.  cut() zeroes the masses that a
+// filter takes away: by count (top-k) or by mass (top-p).  Bisection over z, on the high words alone, narrows the range that
+// holds the cut-off; then the largest remaining value is taken away until the target is reached.
 template <int EPL>
 struct WarpRow {
-  uint32_t key[EPL];
+  uint32_t key[EPL], hi[EPL], lo[EPL];
   float z[EPL];
-  long long q[EPL];
 
-  __device__ __forceinline__ long long mass_from(float least) const {
-    uint32_t lo = 0, hi = 0;
+  __device__ __forceinline__ bool has(int j) const { return (hi[j] | lo[j]) != 0; }
+  __device__ __forceinline__ void mass_from(float least, uint32_t& h, uint32_t& l) const {
+    h = l = 0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j)
       if (z[j] >= least) {
-        lo += (uint32_t)q[j] & 0xFFFFFu;
-        hi += (uint32_t)(q[j] >> 20);
+        h += hi[j];
+        l += lo[j];
       }
-    return warp_mass(lo, hi);
   }
-  __device__ __forceinline__ long long count_from(float least) const {
+  __device__ __forceinline__ uint32_t count_from(float least) const {
     uint32_t c = 0;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, z[j] >= least && q[j] > 0));
+    for (int j = 0; j < EPL; ++j) c += __popc(__ballot_sync(M32_ALL, z[j] >= least && has(j)));
     return c;
   }
   template <bool MASS>
   __device__ __forceinline__ void cut(long long target) {
-    // z >= up is above the target's value, z >= down holds it (or every element stays)
+    // z >= up lies above the target's value; z >= down holds it, or every element stays
     float up = 1.f, down = -Z_SPAN, mid = -4.f;
-    long long before = 0;
+    const uint32_t want = (uint32_t)(MASS ? target >> 20 : target);
 #pragma unroll 1
     for (int i = 0; i < 5; ++i) {
-      const long long v = MASS ? mass_from(mid) : count_from(mid);
-      if (v >= target) {
-        down = mid;
+      bool reached;
+      if (MASS) {
+        uint32_t h = 0;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) h += z[j] >= mid ? hi[j] : 0u;
+        h = __reduce_add_sync(M32_ALL, h);       // the low words add less than 32 EPL to it
+        reached = h > want;
+        if (!reached && h + 32 * EPL >= want) break;      // the high words cannot tell
       } else {
-        up = mid;
-        before = v;
+        reached = count_from(mid) >= want;
       }
+      if (reached)
+        down = mid;
+      else
+        up = mid;
       mid = 0.5f * (fminf(up, 0.f) + down);
+    }
+    long long before = 0;
+    if (up < 1.f) {
+      if (MASS) {
+        uint32_t h, l;
+        mass_from(up, h, l);
+        before = warp_mass(h, l);
+      } else {
+        before = count_from(up);
+      }
     }
     uint32_t tau = M32_ALL;
 #pragma unroll 1
     while (true) {
       uint32_t b = 0;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && z[j] < up && q[j] > 0 ? key[j] : 0u);
+      for (int j = 0; j < EPL; ++j) b = max(b, key[j] < tau && z[j] < up && has(j) ? key[j] : 0u);
       b = __reduce_max_sync(M32_ALL, b);
       if (b == 0) return;                    // the target is beyond what there is: all stay
-      uint32_t c = 0;
-      long long qb = 1;
+      uint32_t c = 0, qh = 0, ql = 1;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
-        const uint32_t tie = __ballot_sync(M32_ALL, key[j] == b && q[j] > 0);
-        if (MASS && tie != 0) qb = __shfl_sync(M32_ALL, q[j], __ffs(tie) - 1);
+        const uint32_t tie = __ballot_sync(M32_ALL, key[j] == b && has(j));
+        if (MASS && tie != 0) {
+          qh = __shfl_sync(M32_ALL, hi[j], __ffs(tie) - 1);
+          ql = __shfl_sync(M32_ALL, lo[j], __ffs(tie) - 1);
+        }
         c += __popc(tie);
       }
       tau = b;
+      const long long qb = mass_of(qh, ql);
       if (before + (long long)c * qb >= target) {
         const uint32_t r = c == 1 ? 1u : (uint32_t)((target - before + qb - 1) / qb);     // the first r of them
         const uint32_t below = (1u << (threadIdx.x & 31)) - 1u;
         uint32_t rank = 0;
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
-          const uint32_t tie = __ballot_sync(M32_ALL, key[j] == tau && q[j] > 0);
-          if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= r)) q[j] = 0;
+          const uint32_t tie = __ballot_sync(M32_ALL, key[j] == tau && has(j));
+          if (key[j] < tau || (key[j] == tau && rank + __popc(tie & below) >= r)) hi[j] = lo[j] = 0;
           rank += __popc(tie);
         }
         return;
@@ -185,63 +207,75 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a, int r
   int my_token = -1;
   float my_z = 0.f;
   long long my_total = 0;
+  const T* lp = (const T*)a.logits + first * a.ld + lane;
+  const uint8_t* mp = a.mask ? a.mask + first * a.ld_mask + lane : nullptr;
   T next[EPL];
-  bool ok[EPL];
-  auto fetch = [&](int64_t row) {
+  uint8_t ok[EPL];
+  auto fetch = [&]() {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      const int i = j * 32 + lane;
-      ok[j] = i < a.V;
+      ok[j] = j * 32 + lane < a.V;
       if (ok[j]) {
-        next[j] = ((const T*)a.logits)[row * a.ld + i];
-        if (a.mask) ok[j] = a.mask[row * a.ld_mask + i] != 0;
+        next[j] = lp[j * 32];
+        if (mp) ok[j] = mp[j * 32];
       }
     }
+    lp += a.ld;
+    if (mp) mp += a.ld_mask;
   };
-  fetch(first);
+  fetch();
 #pragma unroll 1
   for (int r = 0; r < n; ++r) {
     WarpRow<EPL> R;
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      R.z[j] = clean(ok[j] ? to_f(next[j]) : 0.f, ok[j]);
+      R.z[j] = clean(ok[j] ? to_f(next[j]) : 0.f, ok[j] != 0);
       R.key[j] = key_of(R.z[j]);
       top = max(top, R.key[j]);
     }
-    if (r + 1 < n) fetch(first + r + 1);
+    if (r + 1 < n) fetch();
     top = __reduce_max_sync(M32_ALL, top);
     if (top <= KEY_NEG_INF) continue;
     const float m = of_key(top), inv_t = __shfl_sync(M32_ALL, mine.inv_t, r);
     const float top_p = __shfl_sync(M32_ALL, mine.top_p, r), min_p = __shfl_sync(M32_ALL, mine.min_p, r);
     const int k = __shfl_sync(M32_ALL, mine.k, r);
-    uint32_t lo = 0, hi = 0;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       R.z[j] = z_of(R.z[j], m, inv_t);
-      R.q[j] = q_of(expf(R.z[j]));              // exp(-inf) = 0
+      // floor(2^40 w) in two words: w 2^20 and what its whole part leaves are exact
+      const float w = __fmul_rn(expf(R.z[j]), 1048576.f);              // exp(-inf) = 0
+      R.hi[j] = __float2uint_rz(w);
+      R.lo[j] = __float2uint_rz(__fmul_rn(__fsub_rn(w, __uint2float_rn(R.hi[j])), 1048576.f));
     }
+    uint32_t h, l;
     if (k > 0 && k < a.V) R.template cut<false>(k);
-    if (top_p < 1.f)      // every sum is exact in a double, so x >= threshold is x >= its ceiling in integers
-      R.template cut<true>(__double2ll_ru(p_threshold(top_p, R.mass_from(-Z_SPAN))));
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (min_p > 0.f && expf(R.z[j]) < min_p && R.key[j] != top) R.q[j] = 0;     // the first element always stays
-      lo += (uint32_t)R.q[j] & 0xFFFFFu;
-      hi += (uint32_t)(R.q[j] >> 20);
+    if (top_p < 1.f) {    // every sum is exact in a double, so x >= threshold is x >= its ceiling in integers
+      R.mass_from(-Z_SPAN, h, l);
+      R.template cut<true>(__double2ll_ru(p_threshold(top_p, warp_mass(h, l))));
     }
-    const long long total = warp_mass(lo, hi);
+    if (min_p > 0.f)
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (expf(R.z[j]) < min_p && R.key[j] != top) R.hi[j] = R.lo[j] = 0;     // the first element always stays
+    R.mass_from(-Z_SPAN, h, l);
+    const long long total = warp_mass(h, l);
     long long at = draw_at(__shfl_sync(M32_ALL, mine.u, r), total);
     bool found = false;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       if (found) break;
-      long long run = R.q[j];
+      h = R.hi[j];
+      l = R.lo[j];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(M32_ALL, run, o);
-        if (lane >= o) run += v;
+        const uint32_t vh = __shfl_up_sync(M32_ALL, h, o), vl = __shfl_up_sync(M32_ALL, l, o);
+        if (lane >= o) {
+          h += vh;
+          l += vl;
+        }
       }
+      const long long run = mass_of(h, l);
       const uint32_t over = __ballot_sync(M32_ALL, run > at);
       if (over != 0) {
         const int src = __ffs(over) - 1;
