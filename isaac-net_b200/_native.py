@@ -12,6 +12,7 @@ import os
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libisaac_net_b200_check.so" if os.environ.get("INB_CHECK") == "1"
                         else "libisaac_net_b200.so")
+TORCH_LIB = "isaac_net_b200_torch.so"       # policy_ops on torch tensors (csrc/policy_torch.cpp)
 ABI_VERSION = 18
 MAX_ROWS = 128
 NCTR = 64

@@ -4,7 +4,8 @@
 
 Each .cu file under csrc/ is compiled to an object in parallel (-gencode arch=compute_100a,code=sm_100a, -O3,
 -lineinfo, IEEE division / square root, no fast math), then linked into _lib/libisaac_net_b200.so.  The library is
-rebuilt only when a source or header is newer than it.
+rebuilt only when a source or header is newer than it.  build_torch() compiles csrc/policy_torch.cpp, the policy operators'
+entry points on torch tensors, into _lib/isaac_net_b200_torch.so with the C++ compiler against the installed torch.
 """
 from __future__ import annotations
 
@@ -76,6 +77,34 @@ def build(force=False, verbose=False, extra_flags=(), check=False):
     for o in objs:
         os.remove(o)
     return lib
+
+
+TORCH_SRC = os.path.join(CSRC, "policy_torch.cpp")
+TORCH_LIB = os.path.join(OUT_DIR, "isaac_net_b200_torch.so")
+
+
+def build_torch(force=False):
+    """Compile and link the torch extension of the policy operators; returns its path."""
+    deps = [TORCH_SRC, os.path.join(INCLUDE, "isaac_net_b200.h")]
+    if not force and os.path.exists(TORCH_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in deps):
+        return TORCH_LIB
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension as ext
+    os.makedirs(OUT_DIR, exist_ok=True)
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    inc = [INCLUDE, *ext.include_paths(), sysconfig.get_paths()["include"], cuda]
+    tmp = TORCH_LIB + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-DTORCH_EXTENSION_NAME=isaac_net_b200_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{i}" for i in inc), TORCH_SRC, "-o", tmp, f"-L{lib}", f"-Wl,-rpath,{lib}", "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {TORCH_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 if __name__ == "__main__":
