@@ -13,6 +13,9 @@
 // against the 18 D operations the step does for it.  h, dg and du are rounded to the operand type because the next
 // product multiplies them.
 #pragma once
+#include <algorithm>
+#include <initializer_list>
+
 #include "policy_gemm.cuh"
 
 namespace inb {
@@ -93,44 +96,48 @@ struct EpiPartial {
     }
   }
 };
-// Adds the parts of every tile in order.  Block: (tile, 16 columns); thread: row.
+// Adds the parts of every tile in order.  A block takes 32 rows x 64 columns of a tile: it reads with a row to a lane, as
+// the parts lie, and writes with two columns to a lane, as the result does.
 template <typename T, int CG>
-__global__ void __launch_bounds__(Gemm<CG>::TM) sum_parts_kernel(const float* part, const GemmShape g, T* c0, T* c1, int M, int N,
-                                                                 bool vec) {
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, const GemmShape g, T* c0, T* c1, int M, int N,
+                                                        bool pairs) {
+  __shared__ float sm[32][65];
   constexpr int TM = Gemm<CG>::TM;
-  const int tiles = g.tiles_m * g.tiles_n;
+  const int tiles = g.tiles_m * g.tiles_n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int tm, tn;
   tile_at(g, blockIdx.x, tm, tn);
   const bool second = tm >= g.m_split;
-  const int r = (second ? tm - g.m_split : tm) * TM + threadIdx.x, col = tn * BN + blockIdx.y * 16;
-  if (r >= M || col >= N) return;
-  float4 s[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int r0 = (second ? tm - g.m_split : tm) * TM + blockIdx.z * 32, n0 = tn * BN + blockIdx.y * 64;
+  if (r0 >= M || n0 >= N) return;
+  float4 s[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int k = 0; k < g.splits; ++k) {
-    const float* p = part + (((int64_t)k * tiles + blockIdx.x) * (BN / 4) + blockIdx.y * 4) * TM * 4 + threadIdx.x * 4;
+    const float* p = part + ((((int64_t)k * tiles + blockIdx.x) * (BN / 4) + blockIdx.y * 16 + warp * 2) * TM +
+                             blockIdx.z * 32 + lane) * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const float4 v = *reinterpret_cast<const float4*>(p + i * TM * 4);
-      s[i].x += v.x;
-      s[i].y += v.y;
-      s[i].z += v.z;
-      s[i].w += v.w;
+      s[i].x += v.x, s[i].y += v.y, s[i].z += v.z, s[i].w += v.w;
     }
   }
-  T* d = (second ? c1 : c0) + (int64_t)r * N + col;
-  const float* f = &s[0].x;
 #pragma unroll
-  for (int i = 0; i < 16; i += 8) {
-    if (vec && col + i + 8 <= N) {
-      Pack<T, 8> o;
+  for (int i = 0; i < 2; ++i) {
+    float* d = &sm[lane][warp * 8 + i * 4];
+    d[0] = s[i].x, d[1] = s[i].y, d[2] = s[i].z, d[3] = s[i].w;
+  }
+  __syncthreads();
+  const int col = n0 + 2 * lane;
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) down2(make_float2(f[i + e], f[i + e + 1]), o.v[e], o.v[e + 1]);
-      st<T, 8>(d + i, o);
+  for (int i = 0; i < 4; ++i) {
+    const int r = warp * 4 + i;
+    if (r0 + r >= M || col >= N) continue;
+    T* d = (second ? c1 : c0) + (int64_t)(r0 + r) * N + col;
+    Pack<T, 2> o;
+    down2(make_float2(sm[r][2 * lane], sm[r][2 * lane + 1]), o.v[0], o.v[1]);
+    if (pairs) {
+      st<T, 2>(d, o);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + i + e < N) d[i + e] = from_f<T>(f[i + e]);
+      d[0] = o.v[0];
+      if (col + 1 < N) d[1] = o.v[1];
     }
   }
 }
@@ -164,10 +171,11 @@ struct EpiGate {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (cg + i < groups) {
-            *reinterpret_cast<float4*>(g + at + i * 512) =
-                make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]);
-            *reinterpret_cast<float4*>(u + at + i * 512) =
-                make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]);
+            // streamed past the cache: read once, in the backward pass
+            __stcs(reinterpret_cast<float4*>(g + at + i * 512),
+                   make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]));
+            __stcs(reinterpret_cast<float4*>(u + at + i * 512),
+                   make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]));
           }
       }
 #pragma unroll
@@ -192,8 +200,8 @@ struct EpiDh {
     for (int i = 0; i < 4; ++i) {
       s.g[i] = s.u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < M && (col >> 2) + i < groups) {
-        s.g[i] = *reinterpret_cast<const float4*>(g + at + i * 512);
-        s.u[i] = *reinterpret_cast<const float4*>(u + at + i * 512);
+        s.g[i] = __ldcs(reinterpret_cast<const float4*>(g + at + i * 512));
+        s.u[i] = __ldcs(reinterpret_cast<const float4*>(u + at + i * 512));
       }
     }
   }
@@ -236,18 +244,35 @@ struct EpiDh {
 };
 
 // ------------------------------------------------------------------------------------------------- operands
-// Rows that TMA cannot address (a base or a row stride off 16 bytes) are copied once to padded rows.
+// Rows that TMA cannot address (a base or a row stride off 16 bytes) are copied once to padded rows, all of a call's in one
+// launch: blockIdx.z is the matrix.
+struct PackJobs {
+  const void* src[5];
+  void* dst[5];
+  int64_t rows[5], ls[5];
+  int cols[5];
+  int n;
+};
+inline int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+// A thread makes 8 elements of a row from the aligned words that hold them (rows start on any element: every other one of
+// an odd stride half a word late).  Each word read holds at least one element of the row.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* src, T* dst, int64_t rows, int cols, int64_t ls, int64_t ldst) {
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const T* s = src + r * ls;
-    T* d = dst + r * ldst;
-    for (int c = (blockIdx.x * 256 + threadIdx.x) * 8; c < cols; c += gridDim.x * 256 * 8) {
-      Pack<T, 8> v;
+__global__ void __launch_bounds__(256) pack_kernel(const PackJobs j) {
+  const int m = blockIdx.z, cols = j.cols[m];
+  const uint32_t per_row = (cols + 7) / 8;
+  const int64_t all = j.rows[m] * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row;
+    const int c = (int)(i - r * per_row) * 8, n = min(8, cols - c);
+    const uintptr_t at = (uintptr_t)((const uint16_t*)j.src[m] + r * j.ls[m] + c);
+    const uint32_t* w = (const uint32_t*)(at & ~(uintptr_t)3);
+    const int shift = at & 2 ? 16 : 0, words = (n * 2 + (shift ? 2 : 0) + 3) / 4;
+    uint32_t v[5], o[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v.v[e] = c + e < cols ? s[c + e] : from_f<T>(0.f);
-      st<T, 8>(d + c, v);
-    }
+    for (int k = 0; k < 5; ++k) v[k] = k < words ? w[k] : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = __funnelshift_r(v[k], v[k + 1], shift);
+    reinterpret_cast<uint4*>((uint16_t*)j.dst[m] + r * per_row * 8)[c / 8] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -256,7 +281,6 @@ struct Operand {
   int64_t rows, ld;
   int cols;
 };
-inline int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 inline int cdiv(int64_t a, int b) { return (int)((a + b - 1) / b); }
 inline bool addressable(Operand& o) {
   if (o.rows == 1) o.ld = pad8(o.cols);
@@ -266,15 +290,23 @@ inline int64_t packed_bytes(Operand o) {
   return addressable(o) ? 0 : (o.rows * pad8(o.cols) * 2 + 255) / 256 * 256;
 }
 template <typename T>
-void pack(Operand& o, char*& work, cudaStream_t s) {
-  const int64_t b = packed_bytes(o);
-  addressable(o);
-  if (b == 0) return;
-  const dim3 grid(cdiv(o.cols, 2048), (unsigned)(o.rows < 65535 ? o.rows : 65535));
-  pack_kernel<T><<<grid, 256, 0, s>>>((const T*)o.p, (T*)work, o.rows, o.cols, o.ld, pad8(o.cols));
-  o.p = work;
-  o.ld = pad8(o.cols);
-  work += b;
+void pack(std::initializer_list<Operand*> os, char*& work, cudaStream_t s) {
+  PackJobs j = {};
+  int64_t most = 0;
+  for (Operand* o : os) {
+    const int64_t b = packed_bytes(*o);
+    addressable(*o);
+    if (b == 0) continue;
+    j.src[j.n] = o->p, j.dst[j.n] = work, j.rows[j.n] = o->rows, j.cols[j.n] = o->cols, j.ls[j.n] = o->ld;
+    ++j.n;
+    most = std::max(most, o->rows * (pad8(o->cols) / 8));
+    o->p = work;
+    o->ld = pad8(o->cols);
+    work += b;
+  }
+  if (j.n == 0) return;
+  const unsigned blocks = (unsigned)std::min<int64_t>((most + 255) / 256, (int64_t)sm_count() * 8);
+  pack_kernel<T><<<dim3(blocks, 1, j.n), 256, 0, s>>>(j);
 }
 
 // ------------------------------------------------------------------------------------------------- plans
@@ -283,12 +315,12 @@ struct Plan {
   int cg, splits;
   int64_t part_floats;
 };
-// An estimate of a plan's time in us: waves of tiles, each its slices (256 cycles of the tensor cores) and a fill and
+// An estimate of a plan's time in us: waves of tiles, each its slices (512 cycles of the tensor cores) and a fill and
 // drain; single blocks run their products slower than pairs; parts are written and read once.
 inline double plan_time(int64_t M, int N, int kb, bool twin, int cg, int splits, int bn) {
   const int64_t tiles = (int64_t)cdiv(M, BM * cg) * (twin ? 2 : 1) * cdiv(N, bn);
   const int64_t waves = (tiles * splits * cg + sm_count() - 1) / sm_count();
-  double t = waves * (cdiv(kb, splits) * 0.14 * (cg == 1 ? 1.2 : 1.0) + 1.5);
+  double t = waves * (cdiv(kb, splits) * 0.3 * (cg == 1 ? 1.2 : 1.0) + 2.0);
   if (splits > 1) t += 3.0 + (double)tiles * splits * BM * cg * BN * 8 / 5e6;
   return t;
 }
@@ -369,8 +401,9 @@ int product_cg(const GemmMaps& m, int64_t M, int N, int kb0, int kb1, bool twin,
     return gemm_launch<T, CG, AMAJ, BMAJ>(m, g, EpiStore<T, CG>{(T*)c0, (T*)c1, (int)M, N, tm, tma}, status, s);
   const int rc = gemm_launch<T, CG, AMAJ, BMAJ>(m, g, EpiPartial<CG>{part}, status, s);
   if (rc != 0) return rc;
-  const bool vec = (((uintptr_t)c0 | (uintptr_t)(c1 ? c1 : c0) | (uintptr_t)N * 2) & 15) == 0;
-  sum_parts_kernel<T, CG><<<dim3(g.tiles_m * g.tiles_n, BN / 16), BM * CG, 0, s>>>(part, g, (T*)c0, (T*)c1, (int)M, N, vec);
+  const bool pairs = (((uintptr_t)c0 | (uintptr_t)(c1 ? c1 : c0) | (uintptr_t)N * 2) & 3) == 0;
+  sum_parts_kernel<T, CG><<<dim3(g.tiles_m * g.tiles_n, BN / 64, BM * CG / 32), 256, 0, s>>>(part, g, (T*)c0, (T*)c1, (int)M,
+                                                                                           N, pairs);
   return launch_status();
 }
 template <typename T, int AMAJ, int BMAJ>
@@ -443,10 +476,7 @@ int ffn_forward(const InbFfnArgs& a, cudaStream_t s) {
   if (!bind_context<T>()) return -6;
   FfnOperands o = operands(a);
   char* w = (char*)a.work;
-  pack<T>(o.x, w, s);
-  pack<T>(o.wg, w, s);
-  pack<T>(o.wu, w, s);
-  pack<T>(o.wd, w, s);
+  pack<T>({&o.x, &o.wg, &o.wu, &o.wd}, w, s);
   const int kb = cdiv(a.D, BK);
   GemmMaps m;
   if (!operand_maps<T, MAJOR_K, MAJOR_K>(m, o.x, o.x, o.wg, o.wu) || !out_map<T>(&m.o0, o.h)) return -6;
@@ -466,11 +496,7 @@ int ffn_backward(const InbFfnArgs& a, cudaStream_t s) {
   if (!bind_context<T>()) return -6;
   FfnOperands o = operands(a);
   char* w = (char*)a.work;
-  pack<T>(o.x, w, s);
-  pack<T>(o.wg, w, s);
-  pack<T>(o.wu, w, s);
-  pack<T>(o.wd, w, s);
-  pack<T>(o.dy, w, s);
+  pack<T>({&o.x, &o.wg, &o.wu, &o.wd, &o.dy}, w, s);
   float* part = (float*)w;
   int rc = 0;
   if (a.dx != nullptr || a.dwg != nullptr) {
