@@ -165,24 +165,28 @@ struct EpiGate {
     tmem_ld_wait();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      if (g != nullptr && r < M) {
-        const int cg = (n0 >> 2) + 4 * q;
-        const int64_t at = blocked(r, cg, groups);
+      float vh[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (cg + i < groups) {
-            // streamed past the cache: read once, in the backward pass
-            __stcs(reinterpret_cast<float4*>(g + at + i * 512),
-                   make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]));
-            __stcs(reinterpret_cast<float4*>(u + at + i * 512),
-                   make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]));
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) vg[q][i] = act_of<ACT>(vg[q][i]) * vu[q][i];
-      stage16<T>(c.stage_ptr + buf * EPI_BUF, c.lane, 16 * q, vg[q]);
+      for (int i = 0; i < 16; ++i) vh[i] = act_of<ACT>(vg[q][i]) * vu[q][i];
+      stage16<T>(c.stage_ptr + buf * EPI_BUF, c.lane, 16 * q, vh);
     }
     send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0, c, buf);
+    if (g == nullptr || r >= M) return;
+    // after the staged tile has gone: its fence would wait for these stores.  Streamed past the cache: they are read once,
+    // in the backward pass.
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int cg = (n0 >> 2) + 4 * q;
+      const int64_t at = blocked(r, cg, groups);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (cg + i < groups) {
+          __stcs(reinterpret_cast<float4*>(g + at + i * 512),
+                 make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]));
+          __stcs(reinterpret_cast<float4*>(u + at + i * 512),
+                 make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]));
+        }
+    }
   }
 };
 
