@@ -4,6 +4,7 @@
     y    = gated_ffn(x, w_gate, w_up, w_down, act=)           the block itself: act(x Wg^T) * (x Wu^T), times Wd^T
     y    = counter_dropout(x, p, s0, env_id, episode, ctr)    dropout keyed by global env id, mask never stored
     token, logp = sample_logits(logits, u, ...)               temperature, top-k, top-p, min-p from given uniforms
+    u    = uniforms(s0, n, env_id, episode, ctr)              such uniforms from the engine's counter RNG
 
 The first three are differentiable (torch.autograd, once).  As everywhere in this package there is no CPU path and no
 fallback: tensors live on one CUDA device, unsupported settings raise B200Unsupported, wrong shapes ValueError and wrong
@@ -101,6 +102,30 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     return _sample_logits(logits, u, temperature, top_k, top_p, min_p, mask)
 
 
+CH_SAMPLE = 0x53       # counter-RNG channel of uniforms()
+
+
+def uniforms(s0, n, env_id, episode=None, ctr=None, *, stream=0):
+    """[E, n] fp32 uniforms in [0, 1) of the engine's counter RNG (inb_rng_draw), keyed like counter_dropout's draws by
+    (s0, env_id[e], episode[e], ctr[e], stream): the given random numbers of sample_logits."""
+    ids = [t for t in (env_id, episode, ctr) if t is not None]
+    for t in ids:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int64 and t.shape == env_id.shape):
+            raise ValueError("env_id, episode and ctr must be int64 CUDA tensors of one shape [E]")
+    e = env_id.shape[0]
+    if n < 0 or e * n > 0x7FFFFFFF:
+        raise B200Unsupported(f"uniforms: {e} x {n} draws are more than one call makes")
+    episode = torch.zeros_like(env_id) if episode is None else episode
+    env_id, episode, ctr = (t if t is None else t.contiguous() for t in (env_id, episode, ctr))
+    out = torch.empty(e, n, device=env_id.device)
+    with torch.cuda.device(env_id.device):
+        rc = nat.lib().inb_rng_draw(e, n, s0, CH_SAMPLE, stream, env_id.data_ptr(), episode.data_ptr(),
+                                    None if ctr is None else ctr.data_ptr(), 0, out.data_ptr(),
+                                    torch.cuda.current_stream().cuda_stream)
+    nat.check(rc, "inb_rng_draw")
+    return out
+
+
 def status(device="cuda"):
     """The device status word of the operators' kernels on `device` (0 = no wait inside a kernel ever ran out); reading it
     synchronizes."""
@@ -108,4 +133,4 @@ def status(device="cuda"):
     return _ext.status(torch.cuda.current_device() if i is None else i)
 
 
-__all__ = ["block_norm", "gated_ffn", "counter_dropout", "sample_logits", "status"]
+__all__ = ["block_norm", "gated_ffn", "counter_dropout", "sample_logits", "uniforms", "status"]
