@@ -193,6 +193,65 @@ struct WarpRow {
       before += (long long)c * qb;
     }
   }
+  // z holds the logits: makes z and the masses
+  __device__ __forceinline__ void weigh(float m, float inv_t) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      z[j] = z_of(z[j], m, inv_t);
+      // floor(2^40 w) in two words: w 2^20 and what its whole part leaves are exact
+      const float w = __fmul_rn(expf(z[j]), 1048576.f);              // exp(-inf) = 0
+      hi[j] = __float2uint_rz(w);
+      lo[j] = __float2uint_rz(__fmul_rn(__fsub_rn(w, __uint2float_rn(hi[j])), 1048576.f));
+    }
+  }
+  // top-k (0: off), top-p (thr: the mass to reach, 0: that share of what top-k left) and min-p, in that order
+  __device__ __forceinline__ void filter(int k, float top_p, double thr, float min_p, uint32_t top) {
+    if (k > 0) cut<false>(k);
+    if (top_p < 1.f) {    // every sum is exact in a double, so x >= threshold is x >= its ceiling in integers
+      if (thr == 0.0) {
+        uint32_t h, l;
+        mass_from(-Z_SPAN, h, l);
+        thr = p_threshold(top_p, warp_mass(h, l));
+      }
+      cut<true>(__double2ll_ru(thr));
+    }
+    if (min_p > 0.f)
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (expf(z[j]) < min_p && key[j] != top) hi[j] = lo[j] = 0;     // the first element always stays
+  }
+  // the element drawn, its z, and the kept mass
+  __device__ __forceinline__ int draw(float u, float& z_out, long long& total) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t h, l;
+    mass_from(-Z_SPAN, h, l);
+    total = warp_mass(h, l);
+    long long at = draw_at(u, total);
+    int token = -1;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (token >= 0) break;
+      h = hi[j];
+      l = lo[j];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t vh = __shfl_up_sync(M32_ALL, h, o), vl = __shfl_up_sync(M32_ALL, l, o);
+        if (lane >= o) {
+          h += vh;
+          l += vl;
+        }
+      }
+      const long long run = mass_of(h, l);
+      const uint32_t over = __ballot_sync(M32_ALL, run > at);
+      if (over != 0) {
+        token = j * 32 + __ffs(over) - 1;
+        z_out = __shfl_sync(M32_ALL, z[j], __ffs(over) - 1);
+      } else {
+        at -= __shfl_sync(M32_ALL, run, 31);
+      }
+    }
+    return token;
+  }
 };
 
 // A warp takes `rows` consecutive rows: lane i holds the settings of row i and finishes it (the logarithm) with the others
@@ -237,58 +296,16 @@ __global__ void __launch_bounds__(128) sample_warp_kernel(InbSampleArgs a, int r
     if (r + 1 < n) fetch();
     top = __reduce_max_sync(M32_ALL, top);
     if (top <= KEY_NEG_INF) continue;
-    const float m = of_key(top), inv_t = __shfl_sync(M32_ALL, mine.inv_t, r);
-    const float top_p = __shfl_sync(M32_ALL, mine.top_p, r), min_p = __shfl_sync(M32_ALL, mine.min_p, r);
     const int k = __shfl_sync(M32_ALL, mine.k, r);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      R.z[j] = z_of(R.z[j], m, inv_t);
-      // floor(2^40 w) in two words: w 2^20 and what its whole part leaves are exact
-      const float w = __fmul_rn(expf(R.z[j]), 1048576.f);              // exp(-inf) = 0
-      R.hi[j] = __float2uint_rz(w);
-      R.lo[j] = __float2uint_rz(__fmul_rn(__fsub_rn(w, __uint2float_rn(R.hi[j])), 1048576.f));
-    }
-    uint32_t h, l;
-    if (k > 0 && k < a.V) R.template cut<false>(k);
-    if (top_p < 1.f) {    // every sum is exact in a double, so x >= threshold is x >= its ceiling in integers
-      R.mass_from(-Z_SPAN, h, l);
-      R.template cut<true>(__double2ll_ru(p_threshold(top_p, warp_mass(h, l))));
-    }
-    if (min_p > 0.f)
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (expf(R.z[j]) < min_p && R.key[j] != top) R.hi[j] = R.lo[j] = 0;     // the first element always stays
-    R.mass_from(-Z_SPAN, h, l);
-    const long long total = warp_mass(h, l);
-    long long at = draw_at(__shfl_sync(M32_ALL, mine.u, r), total);
-    bool found = false;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (found) break;
-      h = R.hi[j];
-      l = R.lo[j];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t vh = __shfl_up_sync(M32_ALL, h, o), vl = __shfl_up_sync(M32_ALL, l, o);
-        if (lane >= o) {
-          h += vh;
-          l += vl;
-        }
-      }
-      const long long run = mass_of(h, l);
-      const uint32_t over = __ballot_sync(M32_ALL, run > at);
-      if (over != 0) {
-        const int src = __ffs(over) - 1;
-        const float zt = __shfl_sync(M32_ALL, R.z[j], src);
-        if (lane == r) {
-          my_token = j * 32 + src;
-          my_z = zt;
-          my_total = total;
-        }
-        found = true;
-      } else {
-        at -= __shfl_sync(M32_ALL, run, 31);
-      }
+    R.weigh(of_key(top), __shfl_sync(M32_ALL, mine.inv_t, r));
+    R.filter(k < a.V ? k : 0, __shfl_sync(M32_ALL, mine.top_p, r), 0.0, __shfl_sync(M32_ALL, mine.min_p, r), top);
+    float z;
+    long long total;
+    const int token = R.draw(__shfl_sync(M32_ALL, mine.u, r), z, total);
+    if (lane == r) {
+      my_token = token;
+      my_z = z;
+      my_total = total;
     }
   }
   if (lane < n) {
@@ -318,10 +335,65 @@ struct BlockState {
   long long f_mass_above;
 };
 
+// Which of a vector's elements are at least `least`, one bit each
+template <int W>
+__device__ __forceinline__ uint32_t ge_bits(const Pack<float, W>& v, float least) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int e = 0; e < W; ++e) b |= (uint32_t)(v.v[e] >= least) << e;
+  return b;
+}
+template <int W>
+__device__ __forceinline__ uint32_t ge_bits(const Pack<bf16, W>& v, float least) {
+  const __nv_bfloat162 t = __bfloat162bfloat162(__float2bfloat16_ru(least));      // l >= least is l >= the next bf16 up
+  uint32_t b = 0;
+#pragma unroll
+  for (int e = 0; e < W; e += 2) {
+    const uint32_t m = __hge2_mask(__halves2bfloat162(v.v[e], v.v[e + 1]), t);
+    b |= (m & (1u << e)) | ((m >> 16) & (2u << e));
+  }
+  return b;
+}
+template <int W>
+__device__ __forceinline__ uint32_t ge_bits(const Pack<f16, W>& v, float least) {
+  const __half2 t = __half2half2(__float2half_ru(least));
+  uint32_t b = 0;
+#pragma unroll
+  for (int e = 0; e < W; e += 2) {
+    const uint32_t m = __hge2_mask(__halves2half2(v.v[e], v.v[e + 1]), t);
+    b |= (m & (1u << e)) | ((m >> 16) & (2u << e));
+  }
+  return b;
+}
+// The larger of each element, a number before a NaN
+template <int W>
+__device__ __forceinline__ void keep_max(Pack<float, W>& a, const Pack<float, W>& v) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) a.v[e] = fmaxf(a.v[e], v.v[e]);
+}
+template <int W>
+__device__ __forceinline__ void keep_max(Pack<bf16, W>& a, const Pack<bf16, W>& v) {
+#pragma unroll
+  for (int e = 0; e < W; e += 2) {
+    const __nv_bfloat162 m = __hmax2(__halves2bfloat162(a.v[e], a.v[e + 1]), __halves2bfloat162(v.v[e], v.v[e + 1]));
+    a.v[e] = m.x;
+    a.v[e + 1] = m.y;
+  }
+}
+template <int W>
+__device__ __forceinline__ void keep_max(Pack<f16, W>& a, const Pack<f16, W>& v) {
+#pragma unroll
+  for (int e = 0; e < W; e += 2) {
+    const __half2 m = __hmax2(__halves2half2(a.v[e], a.v[e + 1]), __halves2half2(v.v[e], v.v[e + 1]));
+    a.v[e] = m.x;
+    a.v[e + 1] = m.y;
+  }
+}
+
 // The row (or, once `list` is set, the list of its candidates in the first block) as the passes see it
 template <typename T, int NT, bool RES>
 struct Row {
-  static constexpr int BINS = 2 * NT, LIST = 4 * NT, LOG_BINS = NT == 128 ? 8 : 10;
+  static constexpr int BINS = 2 * NT, LIST = 4 * NT, LOG_BINS = NT == 128 ? 8 : 10, W = 16 / (int)sizeof(T);
   const InbSampleArgs& a;
   BlockState<NT>& s;
   T* buf;
@@ -334,7 +406,7 @@ struct Row {
 
   __device__ __forceinline__ float at(int i) const {
     if (list) return s.lv[i];
-    if (RES) return to_f(buf[i]);
+    if (RES) return to_f(buf[i]) + 0.f;      // -0 counts as +0; a NaN stays one and compares as out of every range
     return clean(to_f(((const T*)a.logits)[row * a.ld + first + i]),
                  a.mask == nullptr || a.mask[row * a.ld_mask + first + i] != 0);
   }
@@ -400,6 +472,12 @@ struct Row {
       s.mass[b] = 0;
     }
     __syncthreads();
+  }
+  // Histogram over z of each thread's largest logit: the k-th of them is at most the k-th of the row
+  __device__ void fill_best(float best) {
+    clear();
+    const float zi = z(best);
+    if (zi > -Z_SPAN && q_of(expf(zi)) > 0) atomicAdd(&s.cnt[z_bin(zi)], 1u);
   }
   // Histogram over z of the elements that have a mass; with_mass: their masses too, whose sum (this thread's) it returns
   __device__ long long fill(bool with_mass) {
@@ -508,22 +586,30 @@ struct Row {
     __syncthreads();
     return s.f_key;
   }
-  // The run of the slice that a warp owns
+  // The run of the slice that a warp owns: whole accesses of 32 lanes
   __device__ __forceinline__ void run(int& s0, int& s1) const {
-    constexpr int nw = NT / 32;
-    const int seg = (len + nw * 32 - 1) / (nw * 32) * 32, wid = threadIdx.x >> 5;
+    constexpr int nw = NT / 32, unit = RES ? 32 * W : 32;
+    const int seg = (len + nw * unit - 1) / (nw * unit) * unit, wid = threadIdx.x >> 5;
     s0 = min(len, wid * seg);
     s1 = min(len, s0 + seg);
+  }
+  // Which of the W (RES) or 1 elements from i on are at least `least`, one bit each
+  __device__ __forceinline__ uint32_t at_least(int i, int end, float least) const {
+    if (!RES) return i < end && at(i) >= least;
+    if (i >= end) return 0;
+    const Pack<T, W> v = ld<T, W>(buf + i);           // what lies beyond the slice is -inf
+    return ge_bits(v, least);
   }
   // Moves the elements from key `floor` up to the first block's list, by index.  0: they are more than the list holds and
   // nothing was moved; 1: moved, and this is the first block; 2: moved, and this block is done.
   __device__ int gather(uint32_t floor) {
+    constexpr int STEP = RES ? W : 1;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const float least = of_key(floor);
     int s0, s1;
     run(s0, s1);
     uint32_t n = 0;
-    for (int i = s0 + lane; i < s1; i += 32) n += at(i) >= least;
+    for (int i = s0 + lane * STEP; i < s1; i += 32 * STEP) n += __popc(at_least(i, s1, least));
     n = __reduce_add_sync(M32_ALL, n);
     if (lane == 0) s.wt[wid] = n;
     sync();
@@ -540,17 +626,25 @@ struct Row {
     }
     BlockState<NT>* to = peer(0);
     if (n > 0)
-      for (int i0 = s0; i0 < s1; i0 += 32) {
-        const int i = i0 + lane;
-        const float l = i < s1 ? at(i) : -INFINITY;
-        const bool in = i < s1 && l >= least;
-        const uint32_t who = __ballot_sync(M32_ALL, in);
-        if (in) {
-          const uint32_t slot = before + __popc(who & ((1u << lane) - 1u));
-          to->lv[slot] = l;
-          to->li[slot] = first + i;
+      for (int i0 = s0; i0 < s1; i0 += 32 * STEP) {
+        const int i = i0 + lane * STEP;
+        uint32_t bits = at_least(i, s1, least);
+        if (__ballot_sync(M32_ALL, bits != 0) == 0) continue;
+        const uint32_t c = __popc(bits);
+        uint32_t slot = c;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const uint32_t v = __shfl_up_sync(M32_ALL, slot, d);
+          if (lane >= d) slot += v;
         }
-        before += __popc(who);
+        const uint32_t all = __shfl_sync(M32_ALL, slot, 31);
+        slot += before - c;
+        for (; bits != 0; bits &= bits - 1, ++slot) {
+          const int e = i + __ffs(bits) - 1;
+          to->lv[slot] = at(e);
+          to->li[slot] = first + e;
+        }
+        before += all;
       }
     sync();
     if (rank != 0) return 2;
@@ -619,39 +713,44 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   const bool select_k = p.k > 0 && p.k < a.V, select_p = p.top_p < 1.f;
 
   // the slice, and the row's largest logit
-  uint32_t top = 0;
+  float best = -INFINITY;      // of this thread's elements
   if (RES) {
     const T* lp = (const T*)a.logits + row * a.ld + first;
     const uint8_t* mp = a.mask ? a.mask + row * a.ld_mask + first : nullptr;
     constexpr int W = 16 / (int)sizeof(T);
+    const T none = from_f<T>(-INFINITY);
     int i0 = 0;
-    float best = -INFINITY;
     if (((uintptr_t)lp & 15) == 0 && ((uintptr_t)mp & (W - 1)) == 0) {
       i0 = len / W * W;
+      Pack<T, W> most;
+#pragma unroll
+      for (int e = 0; e < W; ++e) most.v[e] = none;
 #pragma unroll 4
       for (int i = threadIdx.x * W; i < i0; i += NT * W) {
         Pack<T, W> v = ld<T, W>(lp + i);
-        Pack<uint8_t, W> ok;
-        if (mp) ok = ld<uint8_t, W>(mp + i);
+        if (mp) {
+          const Pack<uint8_t, W> ok = ld<uint8_t, W>(mp + i);
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float l = clean(to_f(v.v[e]), mp == nullptr || ok.v[e] != 0);
-          best = fmaxf(best, l);
-          v.v[e] = from_f<T>(l);
+          for (int e = 0; e < W; ++e)
+            if (ok.v[e] == 0) v.v[e] = none;
         }
+        keep_max(most, v);
         st<T, W>(buf + i, v);
       }
+#pragma unroll
+      for (int e = 0; e < W; ++e) best = fmaxf(best, to_f(most.v[e]));
     }
-    for (int i = i0 + threadIdx.x; i < len; i += NT) {
-      const float l = clean(to_f(lp[i]), mp == nullptr || mp[i] != 0);
-      best = fmaxf(best, l);
-      buf[i] = from_f<T>(l);
+    // the rest, and -inf up to a whole access
+    for (int i = i0 + threadIdx.x; i < (len + W - 1) / W * W; i += NT) {
+      const T l = i < len && (mp == nullptr || mp[i] != 0) ? lp[i] : none;
+      best = fmaxf(best, to_f(l));
+      buf[i] = l;
     }
-    top = key_of(best);
+    best += 0.f;
   } else {
-    for (int i = threadIdx.x; i < len; i += NT) top = max(top, key_of(R.at(i)));
+    for (int i = threadIdx.x; i < len; i += NT) best = fmaxf(best, R.at(i));
   }
-  top = R.all_reduce(top, M32_ALL, 0, false).umax;
+  const uint32_t top = R.all_reduce(key_of(best), M32_ALL, 0, false).umax;
   if (top <= KEY_NEG_INF) {
     if (own == 0 && threadIdx.x == 0) {
       a.token[row] = -1;
@@ -680,11 +779,46 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   if (select_k || select_p) {
     uint32_t count, above = 0, bin;
     long long total = 0, mass_above = 0;
-    if (!select_k) total = R.all_reduce(0, M32_ALL, R.fill(true), true).mass;
-    else R.fill(false);
-    double thr = select_k ? 0.0 : p_threshold(p.top_p, total);
-    const bool found = R.cross(!select_k, (uint32_t)p.k, thr, above, mass_above, bin, count);
-    if (found && above + count <= (uint32_t)R.LIST && R.gather(R.bin_floor(bin)) == 2) return;
+    double thr = 0.0;
+    if (select_k) {
+      // the k-th of the threads' largest bounds the k-th of the row from below: what lies above it is few enough, or else
+      // the k-th bin of every element is looked for
+      R.fill_best(best);
+      int done = R.cross(false, (uint32_t)p.k, 0.0, above, mass_above, bin, count) ? R.gather(R.bin_floor(bin)) : 0;
+      if (done == 0) {
+        above = 0;
+        R.fill(false);
+        if (R.cross(false, (uint32_t)p.k, 0.0, above, mass_above, bin, count) && above + count <= (uint32_t)R.LIST)
+          done = R.gather(R.bin_floor(bin));
+      }
+      if (done == 2) return;
+    } else {
+      total = R.all_reduce(0, M32_ALL, R.fill(true), true).mass;
+      thr = p_threshold(p.top_p, total);
+      if (R.cross(true, 0, thr, above, mass_above, bin, count) && above + count <= (uint32_t)R.LIST &&
+          R.gather(R.bin_floor(bin)) == 2)
+        return;
+    }
+    if (R.list && R.len <= 128) {        // few enough for one warp
+      if (wid > 0) return;
+      WarpRow<4> w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = j * 32 + lane;
+        w.z[j] = i < R.len ? s.lv[i] : -INFINITY;
+        w.key[j] = key_of(w.z[j]);
+      }
+      w.weigh(m, p.inv_t);
+      w.filter(select_k ? p.k : 0, p.top_p, thr, p.min_p, top);
+      float z;
+      long long kept_mass;
+      const int i = w.draw(p.u, z, kept_mass);
+      if (lane == 0) {
+        a.token[row] = s.li[i];
+        a.logp[row] = logp_of(z, kept_mass);
+      }
+      return;
+    }
     if (select_k || R.list) {
       const long long sum = R.fill(true);
       if (select_k) total = R.all_reduce(0, M32_ALL, sum, true).mass;     // stays if fewer than k have a mass
