@@ -172,8 +172,7 @@ struct EpiGate {
     }
     send_stage<T>(o0, (T*)nullptr, 0, M, F, r0, n0, c, buf);
     if (g == nullptr || r >= M) return;
-    // after the staged tile has gone: its fence would wait for these stores.  Streamed past the cache: they are read once,
-    // in the backward pass.
+    // after the staged tile has gone: its fence would wait for these stores.
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int cg = (n0 >> 2) + 4 * q;
@@ -181,10 +180,10 @@ struct EpiGate {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (cg + i < groups) {
-          __stcs(reinterpret_cast<float4*>(g + at + i * 512),
-                 make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]));
-          __stcs(reinterpret_cast<float4*>(u + at + i * 512),
-                 make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]));
+          *reinterpret_cast<float4*>(g + at + i * 512) =
+              make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]);
+          *reinterpret_cast<float4*>(u + at + i * 512) =
+              make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]);
         }
     }
   }
@@ -204,8 +203,8 @@ struct EpiDh {
     for (int i = 0; i < 4; ++i) {
       s.g[i] = s.u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < M && (col >> 2) + i < groups) {
-        s.g[i] = __ldcs(reinterpret_cast<const float4*>(g + at + i * 512));
-        s.u[i] = __ldcs(reinterpret_cast<const float4*>(u + at + i * 512));
+        s.g[i] = *reinterpret_cast<const float4*>(g + at + i * 512);
+        s.u[i] = *reinterpret_cast<const float4*>(u + at + i * 512);
       }
     }
   }

@@ -15,6 +15,8 @@
 // equal inputs give equal bits.
 //
 // Both directions are bound by DRAM: 4 (forward) and 6 (backward) row passes of N x D elements.
+#include <algorithm>
+
 #include "policy_common.cuh"
 
 namespace inb {
@@ -56,11 +58,9 @@ static int norm_vec(const InbNormArgs& a, bool bwd) {
 static NormPlan norm_plan(const InbNormArgs& a, bool bwd) {
   NormPlan p;
   p.V = norm_vec(a, bwd);
-  const int esz = a.dtype == INB_F32 ? 4 : 2;
-  // elements of a row in a thread: 16 in the forward pass (8 of a narrow row); 8 in the backward pass, whose column sums
-  // take the registers (16 spill: measured 664 us against 250 at N = 131072, D = 512), 16 of a row that 512 threads of 8
-  // do not cover
-  const int per = bwd ? (a.D > 4096 ? 16 : 8) : (a.D > 256 ? 16 : 8);
+  // elements of a row in a thread: 16, or 8 of a narrow row.  (The backward pass on N = 131072, D = 512 takes 175 us with 16,
+  // of which one block of 256 threads fits an SM, and 210 with 8 and two blocks: a row's fixed work counts for more.)
+  const int per = a.D > 256 ? 16 : 8;
   p.IT = per / p.V;
   const int lanes = (a.D + p.V * p.IT - 1) / (p.V * p.IT);
   p.tpr = (lanes + 31) / 32 * 32;
@@ -570,11 +570,10 @@ static int norm_blocks(const NormPlan& p, int64_t units, int per_sm) {
 static NormChunks norm_chunks(const InbNormArgs& a, const NormPlan& p, bool bwd, int per_sm) {
   NormChunks c;
   // enough chunks for every worker; the forward pass, whose chunks leave no partial sums, takes four times as many so
-  // that the workers end together
+  // that the workers end together (in the backward pass the partial rows cost what that gains)
   const int64_t workers = (int64_t)sm_count() * per_sm * p.groups * (bwd ? 1 : 4);
   const int64_t rows = a.gate != nullptr ? a.gate_rows : a.N, gates = a.N / rows;
-  int64_t cpg = (workers + gates - 1) / gates;
-  if (cpg > rows) cpg = rows;
+  const int64_t cpg = std::min(rows, (workers + gates - 1) / gates);
   const int64_t len = (rows + cpg - 1) / cpg;
   c.rows = (uint32_t)rows;
   c.len = (uint32_t)len;
