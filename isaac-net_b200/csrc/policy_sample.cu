@@ -99,16 +99,22 @@ struct Group {
   static __device__ __forceinline__ int lane() { return threadIdx.x & (GW - 1); }
   static __device__ __forceinline__ uint32_t below() { return (1u << lane()) - 1u; }
   static __device__ __forceinline__ uint32_t max_of(uint32_t v) {
-    if (GW == 32) return __reduce_max_sync(M32_ALL, v);
+    if constexpr (GW == 32) {
+      return __reduce_max_sync(M32_ALL, v);
+    } else {
 #pragma unroll
-    for (int o = GW / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(M32_ALL, v, o));
-    return v;
+      for (int o = GW / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(M32_ALL, v, o));
+      return v;
+    }
   }
   static __device__ __forceinline__ uint32_t sum_of(uint32_t v) {
-    if (GW == 32) return __reduce_add_sync(M32_ALL, v);
+    if constexpr (GW == 32) {
+      return __reduce_add_sync(M32_ALL, v);
+    } else {
 #pragma unroll
-    for (int o = GW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(M32_ALL, v, o);
-    return v;
+      for (int o = GW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(M32_ALL, v, o);
+      return v;
+    }
   }
   static __device__ __forceinline__ uint32_t ballot(bool p) {
     const uint32_t b = __ballot_sync(M32_ALL, p);
@@ -430,6 +436,13 @@ __device__ __forceinline__ void keep_max(Pack<f16, W>& a, const Pack<f16, W>& v)
   }
 }
 
+// A 64-bit sum in shared memory by 32-bit atomics, which it has natively: low word, then high word with the carry
+__device__ __forceinline__ void add_mass(unsigned long long& sum, long long q) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&sum);
+  const uint32_t ql = (uint32_t)q, old = atomicAdd(w, ql), qh = (uint32_t)(q >> 32) + (old + ql < old ? 1u : 0u);
+  if (qh != 0) atomicAdd(w + 1, qh);
+}
+
 // The row (or, once `list` is set, the list of its candidates in the first block) as the passes see it
 template <typename T, int NT, bool RES>
 struct Row {
@@ -530,7 +543,7 @@ struct Row {
           const long long q = q_of(expf(zi));
           if (q > 0) {
             atomicAdd(&s.cnt[z_bin(zi)], 1u);
-            atomicAdd(&s.mass[z_bin(zi)], (unsigned long long)q);
+            add_mass(s.mass[z_bin(zi)], q);
             sum += q;
           }
         } else if (zi > -Z_SURE || q_of(expf(zi)) > 0) {
@@ -700,17 +713,24 @@ struct Row {
     mass_above = 0;
     uint32_t bin;
     if (!cross(by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
-    uint32_t hi = 0, lo = M32_ALL;
-    for (int i = threadIdx.x; i < len; i += NT) {
-      const float l = at(i), zi = z(l);
-      if (zi > -Z_SPAN && z_bin(zi) == (int)bin && q_of(expf(zi)) > 0) {
-        hi = max(hi, key_of(l));
-        lo = min(lo, key_of(l));
+    // the keys of that bin: what its elements span (a short pass over a list), or all that fall there
+    uint32_t lo = M32_ALL, hi = 0;
+    if (list) {
+      for (int i = threadIdx.x; i < len; i += NT) {
+        const float l = at(i), zi = z(l);
+        if (zi > -Z_SPAN && z_bin(zi) == (int)bin && q_of(expf(zi)) > 0) {
+          hi = max(hi, key_of(l));
+          lo = min(lo, key_of(l));
+        }
       }
+      const Exchange e = all_reduce(hi, lo, 0, false);
+      hi = e.umax;
+      lo = e.umin;
+    } else {
+      lo = bin_floor(bin);
+      __syncthreads();                        // f_key has been read
+      hi = bin > 0 ? bin_floor(bin - 1) - 1 : key_of(m);
     }
-    const Exchange e = all_reduce(hi, lo, 0, false);
-    hi = e.umax;
-    lo = e.umin;
     while (hi != lo) {
       const int bits = 32 - __clz(hi - lo), shift = max(0, bits - LOG_BINS);
       clear();
@@ -722,7 +742,7 @@ struct Row {
           if (q > 0) {
             const uint32_t b = (hi - key) >> shift;
             atomicAdd(&s.cnt[b], 1u);
-            atomicAdd(&s.mass[b], (unsigned long long)q);
+            add_mass(s.mass[b], q);
           }
         }
       }
