@@ -95,6 +95,22 @@ inline int sm_count() {
   return n[d];
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory on the current device: one call of the runtime for a kernel, device
+// and thread (so that a thread's first call also makes the device's context current to it, see policy_ffn.cuh).  KEY: a type
+// of the kernel's own.
+template <typename KEY>
+inline cudaError_t allow_smem(const void* kernel, int bytes) {
+  static thread_local uint64_t done = 0;
+  int d = 0;
+  const cudaError_t e = cudaGetDevice(&d);
+  if (e != cudaSuccess || (d < 64 && (done >> d & 1))) return e;
+  const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (r == cudaSuccess && d < 64) done |= 1ull << d;
+  return r;
+}
+template <auto K>
+struct KernelKey {};
+
 inline int launch_status() {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -100 - (int)e;

@@ -360,7 +360,7 @@ struct GemmMaps {
 template <typename T, int CG, int AMAJ, int BMAJ, typename Epi>
 int gemm_launch(const GemmMaps& m, GemmShape g, const Epi& epi, int* status, cudaStream_t s) {
   auto* k = gemm_kernel<T, CG, AMAJ, BMAJ, Epi>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Gemm<CG>::SMEM);
+  cudaError_t e = allow_smem<KernelKey<gemm_kernel<T, CG, AMAJ, BMAJ, Epi>>>((const void*)k, Gemm<CG>::SMEM);
   if (e != cudaSuccess) return -100 - (int)e;
   const int64_t items = (int64_t)g.tiles_m * g.tiles_n * g.splits, most = sm_count() / CG;
   if (items > 0x3FFFFFFF) return -2;
@@ -383,7 +383,7 @@ int gemm_launch(const GemmMaps& m, GemmShape g, const Epi& epi, int* status, cud
 // thread (autograd's) has none before a runtime call like this one, which a graph capture allows
 template <typename T>
 bool bind_context() {
-  return cudaFuncSetAttribute(pack_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 0) == cudaSuccess;
+  return allow_smem<KernelKey<pack_kernel<T>>>((const void*)pack_kernel<T>, 0) == cudaSuccess;
 }
 
 template <typename T, int AMAJ, int BMAJ>

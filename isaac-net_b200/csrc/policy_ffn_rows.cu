@@ -226,7 +226,7 @@ static int rows_launch(const RowsArgs& a, cudaStream_t s) {
   // blocks of one k: enough for two to an SM while a warp keeps the steps of a ring
   int ranks = 1;
   while (ranks < 8 && blocks * ranks < 2 * sm_count() && a.K / (2 * ranks * ROWS_WARPS) >= ROWS_K * Rg::S) ranks *= 2;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<KernelKey<ffn_rows_kernel<T, NT, VEC, GATE, ACT>>>((const void*)k, smem);
   if (e != cudaSuccess) return -100 - (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * ranks));

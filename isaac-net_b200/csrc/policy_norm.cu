@@ -603,9 +603,12 @@ static int norm_launch(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_
   const NormStrides ld = {(uint32_t)a.ldx * esz, (uint32_t)a.ldh * esz, (uint32_t)a.ldgy * esz, (uint32_t)a.ldgn * esz,
                           (uint32_t)a.D * esz};
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(bwd ? (const void*)norm_bwd_kernel<T, V, IT, MAXT>
-                                                   : (const void*)norm_fwd_kernel<T, V, IT, MAXT>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the most that any D asks of the kernel: a block has 16 elements of a row to a thread at most
+    const cudaError_t e =
+        bwd ? allow_smem<KernelKey<norm_bwd_kernel<T, V, IT, MAXT>>>((const void*)norm_bwd_kernel<T, V, IT, MAXT>,
+                                                                     B::S * B::ROW * MAXT + MAXT * 16 * 4)
+            : allow_smem<KernelKey<norm_fwd_kernel<T, V, IT, MAXT>>>((const void*)norm_fwd_kernel<T, V, IT, MAXT>,
+                                                                     F::S * F::ROW * MAXT);
     if (e != cudaSuccess) return -100 - (int)e;
   }
   if (!bwd) {

@@ -995,13 +995,15 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   }
 }
 
+constexpr int SMEM_MOST = 227 * 1024;
+
 template <typename T, int NT, bool RES>
 static int block_launch(const InbSampleArgs& a, int ranks, int slice, cudaStream_t s) {
   const size_t smem = (sizeof(BlockState<NT>) + 15) / 16 * 16 + (RES ? (size_t)slice * sizeof(T) : 0);
   auto* k = sample_block_kernel<T, NT, RES>;
   cudaError_t e;
   if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    e = allow_smem<KernelKey<sample_block_kernel<T, NT, RES>>>((const void*)k, SMEM_MOST);
     if (e != cudaSuccess) return -100 - (int)e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1018,8 +1020,6 @@ static int block_launch(const InbSampleArgs& a, int ranks, int slice, cudaStream
   e = cudaLaunchKernelEx(&cfg, k, a, ranks, slice);
   return e == cudaSuccess ? 0 : -100 - (int)e;
 }
-
-constexpr int SMEM_MOST = 227 * 1024;
 
 template <typename T>
 static int sample_type(const InbSampleArgs& a, cudaStream_t s) {
