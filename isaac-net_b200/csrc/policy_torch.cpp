@@ -474,7 +474,8 @@ struct Setting {
       rows = rows.contiguous();
       return;
     }
-    const double d = v.cast<double>();
+    const double d = PyFloat_AsDouble(v.ptr());
+    if (d == -1.0 && PyErr_Occurred()) throw py::error_already_set();      // a TypeError
     const bool whole = std::is_integral<V>::value;
     VALUE_CHECK(d >= 0 && (!whole || d == std::floor(d)), name, " = ", d, " is out of range");
     value = whole ? (V)std::min(d, 2147483647.0) : (V)d;
