@@ -8,7 +8,8 @@ Public API (a drop-in for ``isaac_net.make_engine("L2", ...)`` on the uplink pat
     NRConfig, TrafficModel, Requests
     NetModule, IsaacNetCfg, TrafficRequest  (the Isaac-side module on the engine's radio, net_module.py)
     ShardedEngine, shard_invariant  (one batch split over several GPUs in one process, sharded.py)
-    policy_ops  (the operators of a policy over NetModule's observations: block_norm, counter_dropout, sample_logits)
+    policy_ops  (the operators of a policy over NetModule's observations: block_norm, gated_ffn, counter_dropout,
+                 sample_logits, uniforms)
 """
 import importlib as _importlib
 import importlib.abc as _abc
@@ -62,5 +63,4 @@ def __getattr__(name):
 
 
 __all__ = ["make_engine", "NRConfig", "TrafficModel", "Requests", "NetModule", "IsaacNetCfg", "TrafficRequest",
-           "ShardedEngine", "shard_invariant",
-           "policy_ops"]
+           "ShardedEngine", "shard_invariant", "policy_ops"]
