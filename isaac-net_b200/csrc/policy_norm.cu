@@ -24,6 +24,7 @@ namespace pol {
 
 struct NormPlan {
   int V, IT;          // elements of one access, accesses of one thread
+  bool mis;           // 16-bit elements that may start on half a word: accesses of 8 of them, by words (see Part)
   int tpr;            // threads of a row (multiple of 32)
   int block, groups;  // threads of a block, rows in flight in it
 };
@@ -58,6 +59,8 @@ static int norm_vec(const InbNormArgs& a, bool bwd) {
 static NormPlan norm_plan(const InbNormArgs& a, bool bwd) {
   NormPlan p;
   p.V = norm_vec(a, bwd);
+  p.mis = p.V == 1 && a.dtype != INB_F32;
+  if (p.mis) p.V = 8;
   // elements of a row in a thread: 16, or 8 of a narrow row.  (The backward pass on N = 131072, D = 512 takes 175 us with 16,
   // of which one block of 256 threads fits an SM, and 210 with 8 and two blocks: a row's fixed work counts for more.)
   const int per = a.D > 256 ? 16 : 8;
@@ -119,15 +122,19 @@ struct Cursor {
 // Rows on their way: each thread copies its own part of the next rows of NT tensors (and 8 bytes of statistics) to its own
 // places of a ring of S rows in shared memory (cp.async) and reads only those back, so the ring needs no barrier and keeps
 // rows in flight that registers would have no room for.  S = 0: plain loads.
-template <typename T, int V, int IT, int MAXT, int NT, int WANT>
+template <typename T, int V, int IT, int MAXT, int NT, int WANT, bool MIS>
 struct Ring {
-  static constexpr int ROW = NT * IT * V * (int)sizeof(T) + 8;         // a thread's bytes of one row
+  static constexpr int WORDS = 5;                                      // MIS: the words that 8 elements may touch
+  static constexpr int ROW = NT * IT * (MIS ? 4 * WORDS : V * (int)sizeof(T)) + 8;     // a thread's bytes of one row
   static constexpr int MOST = 176 * 1024;
   static constexpr int S = V * sizeof(T) < 4 ? 0 : (WANT * ROW * MAXT <= MOST ? WANT : (2 * ROW * MAXT <= MOST ? 2 : 0));
   static constexpr int BLOCKS = S > 0 && S * ROW * MAXT <= 88 * 1024 ? 2 : 1;       // of them on an SM
-  static constexpr int ACCESS = V * (int)sizeof(T);
-  // access i of tensor k in slot `slot`, and the statistics: byte offsets from `mine()`, constant but for the slot
-  static __device__ __forceinline__ int place(int slot, int k, int i) { return slot * (ROW * MAXT) + (k * IT + i) * ACCESS * MAXT; }
+  static constexpr int ACCESS = MIS ? 4 : V * (int)sizeof(T), PER = MIS ? WORDS : 1;    // bytes and number of a copy's pieces
+  // access i (and its word w) of tensor k in slot `slot`, and the statistics: byte offsets from `mine()`, constant but for
+  // the slot
+  static __device__ __forceinline__ int place(int slot, int k, int i, int w = 0) {
+    return slot * (ROW * MAXT) + ((k * IT + i) * PER + w) * ACCESS * MAXT;
+  }
   static __device__ __forceinline__ unsigned char* mine(unsigned char* ring) { return ring + threadIdx.x * ACCESS; }
   static __device__ __forceinline__ unsigned char* stat(unsigned char* ring, int slot) {
     return ring + slot * (ROW * MAXT) + (ROW - 8) * MAXT + threadIdx.x * 8;
@@ -139,18 +146,21 @@ struct Ring {
 #pragma unroll
       for (int k = 0; k < NT; ++k)
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          Pack<T, V> z;
+        for (int i = 0; i < IT; ++i)
 #pragma unroll
-          for (int e = 0; e < V; ++e) z.v[e] = from_f<T>(0.f);
-          *reinterpret_cast<Pack<T, V>*>(mine(ring) + place(s, k, i)) = z;
-        }
+          for (int w = 0; w < PER; ++w)
+#pragma unroll
+            for (int b = 0; b < ACCESS; b += ACCESS < 4 ? 2 : 4)
+              if constexpr (ACCESS < 4)
+                *reinterpret_cast<uint16_t*>(mine(ring) + place(s, k, i, w) + b) = 0;
+              else
+                *reinterpret_cast<uint32_t*>(mine(ring) + place(s, k, i, w) + b) = 0;
   }
 };
-template <typename T, int V, int IT, int MAXT>
-using FwdRing = Ring<T, V, IT, MAXT, 3, 3>;      // x, h, gate
-template <typename T, int V, int IT, int MAXT>
-using BwdRing = Ring<T, V, IT, MAXT, 5, 3>;      // x, h, gn, gy, gate
+template <typename T, int V, int IT, int MAXT, bool MIS>
+using FwdRing = Ring<T, V, IT, MAXT, 3, 3, MIS>;      // x, h, gate
+template <typename T, int V, int IT, int MAXT, bool MIS>
+using BwdRing = Ring<T, V, IT, MAXT, 5, 3, MIS>;      // x, h, gn, gy, gate
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if constexpr (BYTES == 16)
@@ -166,8 +176,11 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A thread's part of a row: IT accesses of V elements, zero beyond D, as pairs of fp32 where it is worked on
-template <typename T, int V, int IT>
+// A thread's part of a row: IT accesses of V elements, zero beyond D, as pairs of fp32 where it is worked on.
+// MIS: rows of 16-bit elements that start anywhere.  An access of 8 elements is copied as the four or five aligned words that
+// hold them (each holds at least one of the row's elements) and shifted into place when it is read; it is stored as words
+// but for its ends.  (Element by element and without the ring, rows of odd length ran at a seventh of the aligned rate.)
+template <typename T, int V, int IT, bool MIS>
 struct Part {
   static constexpr int N2 = V * IT / 2;
   Pack<T, V> p[IT];
@@ -181,7 +194,13 @@ struct Part {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int c = (i * tpr + t) * V;
-      if (c < D) p[i] = ld<T, V>(row + c);
+      if (MIS) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e < D) p[i].v[e] = row[c + e];
+      } else if (c < D) {
+        p[i] = ld<T, V>(row + c);
+      }
     }
   }
   // to and from a ring: `row` is the tensor's row at this thread's first column
@@ -189,20 +208,65 @@ struct Part {
   static __device__ __forceinline__ void fetch(unsigned char* ring, int slot, int k, const char* row, int tpr, int t, int D) {
 #pragma unroll
     for (int i = 0; i < IT; ++i)
-      if ((i * tpr + t) * V < D)
-        copy_async<R::ACCESS>((uint32_t)__cvta_generic_to_shared(R::mine(ring) + R::place(slot, k, i)),
-                              row + i * tpr * R::ACCESS);
+      if ((i * tpr + t) * V < D) {
+        const char* at = row + i * tpr * V * (int)sizeof(T);
+        if constexpr (MIS) {
+          const int half = (int)((uintptr_t)at & 2), words = (half + 2 * min(V, D - (i * tpr + t) * V) + 3) >> 2;
+#pragma unroll
+          for (int w = 0; w < R::WORDS; ++w)
+            if (w < words)
+              copy_async<4>((uint32_t)__cvta_generic_to_shared(R::mine(ring) + R::place(slot, k, i, w)), at - half + 4 * w);
+        } else {
+          copy_async<R::ACCESS>((uint32_t)__cvta_generic_to_shared(R::mine(ring) + R::place(slot, k, i)), at);
+        }
+      }
   }
   template <typename R>
-  __device__ __forceinline__ void read(unsigned char* ring, int slot, int k) {
+  __device__ __forceinline__ void read(unsigned char* ring, int slot, int k, const char* row, int tpr, int t, int D) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) p[i] = *reinterpret_cast<const Pack<T, V>*>(R::mine(ring) + R::place(slot, k, i));
+    for (int i = 0; i < IT; ++i) {
+      if constexpr (MIS) {
+        const int shift = (int)((uintptr_t)row & 2) * 8, left = D - (i * tpr + t) * V;
+        uint32_t v[R::WORDS];
+#pragma unroll
+        for (int w = 0; w < R::WORDS; ++w) v[w] = *reinterpret_cast<const uint32_t*>(R::mine(ring) + R::place(slot, k, i, w));
+        uint32_t* o = reinterpret_cast<uint32_t*>(&p[i]);
+#pragma unroll
+        for (int w = 0; w < V / 2; ++w) {
+          o[w] = __funnelshift_r(v[w], v[w + 1], shift);
+          // what lies beyond D in the last words, or was left there by a row that started on the other half
+          if (2 * w + 1 >= left) o[w] = 2 * w < left ? o[w] & 0xFFFFu : 0u;
+        }
+      } else {
+        p[i] = *reinterpret_cast<const Pack<T, V>*>(R::mine(ring) + R::place(slot, k, i));
+      }
+    }
   }
   __device__ __forceinline__ void store(T* row, int tpr, int t, int D) const {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int c = (i * tpr + t) * V;
-      if (c < D) st<T, V>(row + c, p[i]);
+      if constexpr (MIS) {
+        T* d = row + c;
+        if (c + V <= D) {
+          const bool half = ((uintptr_t)d & 2) != 0;
+          if (half) d[0] = p[i].v[0];
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            if (!half)
+              st<T, 2>(d + e, Pack<T, 2>{p[i].v[e], p[i].v[e + 1]});
+            else if (e + 2 < V)
+              st<T, 2>(d + e + 1, Pack<T, 2>{p[i].v[e + 1], p[i].v[e + 2]});
+          }
+          if (half) d[V - 1] = p[i].v[V - 1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < D) d[e] = p[i].v[e];
+        }
+      } else if (c < D) {
+        st<T, V>(row + c, p[i]);
+      }
     }
   }
   __device__ __forceinline__ float2 get(int j) const {
@@ -223,13 +287,13 @@ struct Part {
 };
 
 // MAXT: the largest block it is launched with.
-template <typename T, int V, int IT, int MAXT>
-__global__ void __launch_bounds__(MAXT, FwdRing<T, V, IT, MAXT>::BLOCKS)
+template <typename T, int V, int IT, int MAXT, bool MIS>
+__global__ void __launch_bounds__(MAXT, FwdRing<T, V, IT, MAXT, MIS>::BLOCKS)
 norm_fwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks ch, const NormStrides ld) {
   __shared__ float red[8][64];
   extern __shared__ __align__(16) unsigned char ring[];
-  using P = Part<T, V, IT>;
-  using Rg = FwdRing<T, V, IT, MAXT>;
+  using P = Part<T, V, IT, MIS>;
+  using Rg = FwdRing<T, V, IT, MAXT, MIS>;
   constexpr int S = Rg::S;
   const int group = threadIdx.x / tpr, t = threadIdx.x % tpr, groups = blockDim.x / tpr;
   const int D = a.D, col = t * V * (int)sizeof(T);
@@ -267,9 +331,9 @@ norm_fwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
     g.zero();
     if constexpr (S > 0) {
       copy_wait<S - 2>();
-      x.template read<Rg>(ring, slot, 0);
-      if (has_h) h.template read<Rg>(ring, slot, 1);
-      if (a.gate && at.first) g.template read<Rg>(ring, slot, 2);
+      x.template read<Rg>(ring, slot, 0, row_at(a.x, at.row, ld.x, col), tpr, t, D);
+      if (has_h) h.template read<Rg>(ring, slot, 1, row_at(a.h, at.row, ld.h, col), tpr, t, D);
+      if (a.gate && at.first) g.template read<Rg>(ring, slot, 2, row_at(a.gate, at.gate, ld.d, col), tpr, t, D);
       fetch(slot == 0 ? S - 1 : slot - 1);         // the place read in the last turn
       slot = slot == S - 1 ? 0 : slot + 1;
     } else {
@@ -316,13 +380,13 @@ norm_fwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
 // The row sums that gate's and post's gradients need differ only in factors that are fixed within a chunk:
 // e = sum over the chunk of t hh;  ggate = s post e, gpost = sum over the chunks of s gate e.  So the rows add to one
 // accumulator (and to gw's), and gpost's, touched once a chunk, lies in shared memory.
-template <typename T, int V, int IT, int MAXT>
-__global__ void __launch_bounds__(MAXT, BwdRing<T, V, IT, MAXT>::BLOCKS)
+template <typename T, int V, int IT, int MAXT, bool MIS>
+__global__ void __launch_bounds__(MAXT, BwdRing<T, V, IT, MAXT, MIS>::BLOCKS)
 norm_bwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks ch, const NormStrides ld) {
   __shared__ float red[8][64];
   extern __shared__ __align__(16) unsigned char ring[];
-  using P = Part<T, V, IT>;
-  using Rg = BwdRing<T, V, IT, MAXT>;
+  using P = Part<T, V, IT, MIS>;
+  using Rg = BwdRing<T, V, IT, MAXT, MIS>;
   constexpr int S = Rg::S;
   const int group = threadIdx.x / tpr, t = threadIdx.x % tpr, groups = blockDim.x / tpr;
   const int D = a.D, col = t * V * (int)sizeof(T);
@@ -370,7 +434,7 @@ norm_bwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
     auto take = [&](P& v, int k, const void* p, uint32_t stride) {
       if constexpr (S > 0) {
         asm volatile("" ::: "memory");
-        v.template read<Rg>(ring, here, k);
+        v.template read<Rg>(ring, here, k, row_at(p, at.row, stride, col), tpr, t, D);
       } else {
         v.zero();
         if (p != nullptr) v.load((const T*)row_at(p, at.row, stride, 0), tpr, t, D);
@@ -390,7 +454,7 @@ norm_bwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
       g.zero();
       if (a.gate) {
         if constexpr (S > 0)
-          g.template read<Rg>(ring, here, 4);
+          g.template read<Rg>(ring, here, 4, row_at(a.gate, at.gate, ld.d, col), tpr, t, D);
         else
           g.load((const T*)row_at(a.gate, at.gate, ld.d, 0), tpr, t, D);
       }
@@ -466,7 +530,7 @@ norm_bwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
         bool loaded = false;
         if constexpr (S > 0)
           if (alone) {
-            g.template read<Rg>(ring, here, 4);
+            g.template read<Rg>(ring, here, 4, row_at(a.gate, gate, ld.d, col), tpr, t, D);
             loaded = true;
           }
         if (!loaded) g.load((const T*)row_at(a.gate, gate, ld.d, 0), tpr, t, D);
@@ -583,10 +647,10 @@ static NormChunks norm_chunks(const InbNormArgs& a, const NormPlan& p, bool bwd,
 }
 
 // Runs the call, or (elems != NULL) says how many floats of work it needs
-template <typename T, int V, int IT, int MAXT>
+template <typename T, int V, int IT, int MAXT, bool MIS>
 static int norm_launch(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_t* elems, cudaStream_t s) {
-  using F = FwdRing<T, V, IT, MAXT>;
-  using B = BwdRing<T, V, IT, MAXT>;
+  using F = FwdRing<T, V, IT, MAXT, MIS>;
+  using B = BwdRing<T, V, IT, MAXT, MIS>;
   const int per_sm = bwd ? B::BLOCKS : F::BLOCKS;
   const NormChunks ch = norm_chunks(a, p, bwd, per_sm);
   const int blocks = norm_blocks(p, ch.n, per_sm);
@@ -605,37 +669,39 @@ static int norm_launch(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_
   if (smem > 48 * 1024) {
     // the most that any D asks of the kernel: a block has 16 elements of a row to a thread at most
     const cudaError_t e =
-        bwd ? allow_smem<KernelKey<norm_bwd_kernel<T, V, IT, MAXT>>>((const void*)norm_bwd_kernel<T, V, IT, MAXT>,
+        bwd ? allow_smem<KernelKey<norm_bwd_kernel<T, V, IT, MAXT, MIS>>>((const void*)norm_bwd_kernel<T, V, IT, MAXT, MIS>,
                                                                      B::S * B::ROW * MAXT + MAXT * 16 * 4)
-            : allow_smem<KernelKey<norm_fwd_kernel<T, V, IT, MAXT>>>((const void*)norm_fwd_kernel<T, V, IT, MAXT>,
+            : allow_smem<KernelKey<norm_fwd_kernel<T, V, IT, MAXT, MIS>>>((const void*)norm_fwd_kernel<T, V, IT, MAXT, MIS>,
                                                                      F::S * F::ROW * MAXT);
     if (e != cudaSuccess) return -100 - (int)e;
   }
   if (!bwd) {
-    norm_fwd_kernel<T, V, IT, MAXT><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
+    norm_fwd_kernel<T, V, IT, MAXT, MIS><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
     return launch_status();
   }
-  norm_bwd_kernel<T, V, IT, MAXT><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
+  norm_bwd_kernel<T, V, IT, MAXT, MIS><<<blocks, p.block, smem, s>>>(a, p.tpr, ch, ld);
   const dim3 grid((a.D + 31) / 32, 2 + (a.gate != nullptr && ch.cpg > 1 ? ch.n / ch.cpg : 0));
   norm_sum_kernel<T><<<grid, 1024, 0, s>>>(a, blocks, ch);
   return launch_status();
 }
 
-template <typename T, int V>
+template <typename T, int V, bool MIS>
 static int norm_go(const InbNormArgs& a, const NormPlan& p, bool bwd, int64_t* elems, cudaStream_t s) {
-  const bool wide = p.block > 256;
-  if (p.IT * V == 16)
-    return wide ? norm_launch<T, V, 16 / V, 512>(a, p, bwd, elems, s) : norm_launch<T, V, 16 / V, 256>(a, p, bwd, elems, s);
-  return wide ? norm_launch<T, V, 8 / V, 512>(a, p, bwd, elems, s) : norm_launch<T, V, 8 / V, 256>(a, p, bwd, elems, s);
+  // rows of 8 elements a thread are narrow (D <= 256): they never need more than 256 threads
+  if (p.IT * V == 8) return norm_launch<T, V, 8 / V, 256, MIS>(a, p, bwd, elems, s);
+  return p.block > 256 ? norm_launch<T, V, 16 / V, 512, MIS>(a, p, bwd, elems, s)
+                       : norm_launch<T, V, 16 / V, 256, MIS>(a, p, bwd, elems, s);
 }
 
 template <typename T>
 static int norm_type(const InbNormArgs& a, bool bwd, int64_t* elems, cudaStream_t s) {
   const NormPlan p = norm_plan(a, bwd);
-  if (p.V == 16 / (int)sizeof(T)) return norm_go<T, 16 / (int)sizeof(T)>(a, p, bwd, elems, s);
-  if constexpr (sizeof(T) == 2)
-    if (p.V == 2) return norm_go<T, 2>(a, p, bwd, elems, s);
-  return norm_go<T, 1>(a, p, bwd, elems, s);
+  if constexpr (sizeof(T) == 2) {
+    if (p.mis) return norm_go<T, 8, true>(a, p, bwd, elems, s);
+    return p.V == 8 ? norm_go<T, 8, false>(a, p, bwd, elems, s) : norm_go<T, 2, false>(a, p, bwd, elems, s);
+  } else {
+    return p.V == 4 ? norm_go<T, 4, false>(a, p, bwd, elems, s) : norm_go<T, 1, false>(a, p, bwd, elems, s);
+  }
 }
 
 static int norm_run(const InbNormArgs& a, bool bwd, int64_t* elems, void* stream) {
