@@ -4,9 +4,9 @@
 // from DRAM.  A block takes two groups of 16 weight rows (16 rows of Wg and the same of Wu; or 32 rows of Wd), its eight
 // warps take turns along k, and where that leaves SMs idle a cluster of up to 8 blocks shares one k.  A thread copies 16
 // bytes of a weight row at a time (cp.async, through its own places of a ring in shared memory: 96 KB on their way to an
-// SM) and gives them to the m16n8k16 matrix instruction as they are: the sum over k
-// may run in any order, so the 8 consecutive elements a thread holds are simply declared to be the k slots that the
-// instruction expects of it, for weights and activations alike, and nothing is exchanged.  (128-row tcgen05 tiles would
+// SM) and gives them to the m16n8k16 matrix instruction as they are: the sum over k may run in any order, so the 8
+// consecutive elements a thread holds are simply declared to be the k slots that the instruction expects of it, for
+// weights and activations alike, and nothing is exchanged.  (128-row tcgen05 tiles would
 // spend 3/4 of their operand on padding here and gain nothing: the tensor cores idle either way.)  The warps' and the
 // blocks' partial sums meet in shared memory, in a fixed order.
 //

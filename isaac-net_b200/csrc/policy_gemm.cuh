@@ -7,11 +7,11 @@
 // together (CG = 2: each holds half of A's rows and half of B's, so a slice of B crosses L2 once for both).  Warp 0 fills a
 // ring of slices of 64 k with TMA, warp 1 of the first block issues the matrix instructions, sixteen more warps read
 // finished accumulators out and run the epilogue (four to a scheduler: one alone waits on its own instructions most of the
-// time, and a product over few slices is bound by its epilogue).  Tensor memory holds two accumulators of 256 columns, so the epilogue of one tile
-// runs under the products of the next.  Each operand is read as it lies in memory, k or m / n contiguous: the 128-byte
-// swizzle of the shared tiles and the descriptor's major bits cover both, so no operand is ever transposed by a pass of its
-// own.  Where a product has fewer tiles than the GPU has SMs, its k is split and the parts are added by a second launch in
-// a fixed order.
+// time, and a product over few slices is bound by its epilogue).  Tensor memory holds two accumulators of 256 columns, so
+// the epilogue of one tile runs under the products of the next.  Each operand is read as it lies in memory, k or m / n
+// contiguous: the 128-byte swizzle of the shared tiles and the descriptor's major bits cover both, so no operand is ever
+// transposed by a pass of its own.  Where a product has fewer tiles than the GPU has SMs, its k is split and the parts are
+// added by a second launch in a fixed order.
 //
 // Every wait has a time limit (WAIT_NS).  A wait that runs out sets the device status word and ends the block: its copies
 // in flight are waited for, its tensor memory is freed, its results are not to be used.
