@@ -11,8 +11,8 @@
 // 2^20 elements together cannot be off by more than 2^-20 of the largest one, and 2^22 of them (the longest
 // row) do not overflow 64 bits.
 //
-// Rows of up to 128 logits take 8, 16 or 32 lanes of a warp each: the cut-offs are found by taking the largest remaining
-// logit away until the count or the mass is reached.  Longer rows take a block, or a cluster of 2 to 8 blocks when there
+// Rows of up to 384 logits take 8, 16 or 32 lanes of a warp each: the cut-offs are found by bisection, and then by taking
+// the largest remaining logit away until the count or the mass is reached.  Longer rows take a block, or a cluster of 2 to 8 blocks when there
 // are fewer rows than SMs: the row stays in shared memory, a histogram over z finds the bin of the cut-off, and
 // histograms over the float's ordered bits narrow that bin to one value.  Either way the logits are read from memory
 // once, which is the floor; what bounds the kernel is the latency of its passes, not DRAM.
@@ -126,15 +126,20 @@ struct Group {
   }
 };
 
-// Masses of up to 128 elements as two words, q = hi 2^20 + lo with lo < 2^20: either sum fits 32 bits
+// Masses of up to 512 elements as two words, q = hi 2^20 + lo with lo < 2^20: either sum fits 32 bits
 __device__ __forceinline__ long long mass_of(uint32_t hi, uint32_t lo) { return ((long long)hi << 20) + lo; }
 
 // One row: keys, exponents z and masses of its elements, EPL a lane, element j * GW + lane.  cut() zeroes the masses that a
-// filter takes away: by count (top-k) or by mass (top-p).  Bisection over z, on the high words alone, narrows the range that
-// holds the cut-off; then the largest remaining value is taken away until the target is reached.
+// filter takes away: by count (top-k) or by mass (top-p).  Bisection over the z that the row has, on the high words alone,
+// narrows the range that holds the cut-off; then the largest remaining value is taken away until the target is reached.  (A
+// policy before training has logits that hardly differ: from a fixed range the bisection left all of a row's 33 values to
+// the second part, 80 us for 32768 rows against 25.)
 template <int GW, int EPL>
 struct WarpRow {
   using G = Group<GW>;
+  // of the bisection: each costs a sum, and halves the values that are then taken away one by one.  32768 rows, top-p 0.95:
+  // V = 64 31 us with 6, 33 with 5; V = 128 56 with 7, 69 with 5; V = 200 91 with 9, 101 with 12.
+  static constexpr int STEPS = EPL > 4 ? 9 : (EPL == 4 ? 7 : 6);
   uint32_t key[EPL], hi[EPL], lo[EPL];
   float z[EPL];
 
@@ -158,12 +163,15 @@ struct WarpRow {
   // live: whether this group's row is to be cut at all
   template <bool MASS>
   __device__ __forceinline__ void cut(bool live, long long target) {
-    // z >= up lies above the target's value; z >= down holds it, or every element stays
-    float up = 1.f, down = -Z_SPAN, mid = -4.f;
+    // z >= up lies above the target's value; z >= down, the least z of all, holds it, or every element stays
+    uint32_t least = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) least = max(least, has(j) ? __float_as_uint(z[j]) : 0u);     // z <= 0: the bits fall with z
+    float up = 1.f, down = __uint_as_float(G::max_of(least)), mid = fmaxf(-4.f, 0.5f * down);
     const uint32_t want = (uint32_t)(MASS ? target >> 20 : target);
     bool open = true;
 #pragma unroll 1
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
       bool reached;
       if (MASS) {
         uint32_t h = 0;
@@ -1025,12 +1033,16 @@ template <typename T>
 static int sample_type(const InbSampleArgs& a, cudaStream_t s) {
   // lanes of a row: fewer make a row's fixed work cheaper and its steps longer.  131072 rows, top-p 0.95: V = 16 31 us with
   // 8 lanes, 60 with 32; V = 33 74 with 16, 79 with 32; V = 64 110 with 16, 90 with 32.
+  // A warp a row against a block: 32768 rows, top-k 50: V = 200 80 us and 255, V = 384 138 and 187; one row, top-p 0.95:
+  // V = 256 8 and 15.  Beyond, a lane's elements outgrow its registers (V = 512, top-k 50: 249 and 189).
   if (a.V <= 8) return warp_launch<T, 8, 1>(a, s);
   if (a.V <= 16) return warp_launch<T, 8, 2>(a, s);
   if (a.V <= 32) return warp_launch<T, 16, 2>(a, s);
   if (a.V <= 48) return warp_launch<T, 16, 3>(a, s);
   if (a.V <= 64) return warp_launch<T, 32, 2>(a, s);
   if (a.V <= 128) return warp_launch<T, 32, 4>(a, s);
+  if (a.V <= 256) return warp_launch<T, 32, 8>(a, s);
+  if (a.V <= 384) return warp_launch<T, 32, 12>(a, s);
   if (a.V <= 4096) return block_launch<T, 128, true>(a, 1, a.V, s);
   // blocks of a row: enough to give every SM one while a slice keeps 4096 logits, and enough for the row to be resident
   constexpr int CAP = (SMEM_MOST - (int)((sizeof(BlockState<512>) + 15) / 16 * 16)) / (int)sizeof(T) / 16 * 16;

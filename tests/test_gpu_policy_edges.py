@@ -202,3 +202,23 @@ def test_sample_settings_of_wrong_types():
     with pytest.raises(TypeError):
         ops.sample_logits(l, u, top_p=torch.ones(3, device="cuda").half())
     assert int(ops.sample_logits(l, u, top_k=np.int64(2), temperature=np.float32(0.5))[0][0]) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("v", [16, 47, 127, 130, 256, 257, 384, 385])
+def test_sample_logits_of_rows_that_hardly_differ(v, dtype):
+    """Rows whose logits all lie close together, are equal, or leave one another far behind, on both sides of each length
+    at which the sampler changes its form; expectations as in test_sample_logits_filters."""
+    from test_gpu_policy_ops import check_sample
+    g = gen(3 * v)
+    u = torch.rand(6, generator=g, device="cuda")
+    near = rn(g, 6, v) * 1e-2
+    steep = near.clone()
+    steep[:, 0], steep[:, v // 2] = 60.0, 30.0
+    steps = -torch.arange(v, device="cuda").float().expand(6, v) * 1e-6
+    low = rn(g, 6, v) * 40
+    mask = torch.rand(6, v, generator=g, device="cuda") < 0.5
+    for logits in (near, steep, steps, low):
+        for t, k, p, mp in ((1.0, 0, 0.95, 0.0), (1.5, v // 2, 0.6, 0.0), (0.01, 7, 1.0, 0.0), (1.0, v - 1, 0.99, 0.5)):
+            check_sample(logits.to(dtype), u, t, k, p, mp)
+            check_sample(logits.to(dtype), u, t, k, p, mp, mask=mask)
