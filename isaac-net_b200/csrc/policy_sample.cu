@@ -18,6 +18,8 @@
 // once, which is the floor; what bounds the kernel is the latency of its passes, not DRAM.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "policy_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -455,6 +457,7 @@ __device__ __forceinline__ void add_mass(unsigned long long& sum, long long q) {
 template <typename T, int NT, bool RES>
 struct Row {
   static constexpr int BINS = 2 * NT, LIST = 4 * NT, LOG_BINS = NT == 128 ? 8 : 10, W = 16 / (int)sizeof(T);
+  static constexpr int RANKS = NT == 128 ? 1 : 8;      // the most blocks a row takes; loads from all come before their uses
   const InbSampleArgs& a;
   BlockState<NT>& s;
   T* buf;
@@ -516,14 +519,17 @@ struct Row {
     }
     sync();
     Exchange e = s.ex[par];
-    if (ranks > 1)
-      for (int r = 0; r < ranks; ++r)
-        if (r != rank) {
-          const Exchange& o = peer(r)->ex[par];
-          e.umax = max(e.umax, o.umax);
-          e.umin = min(e.umin, o.umin);
-          e.mass += o.mass;
-        }
+    if (ranks > 1) {                          // a lane reads a block's
+      e = peer(lane < ranks ? lane : rank)->ex[par];
+      e.umax = __reduce_max_sync(M32_ALL, e.umax);
+      e.umin = __reduce_min_sync(M32_ALL, e.umin);
+      if (with_mass) {
+        if (lane >= ranks) e.mass = 0;
+#pragma unroll
+        for (int o = RANKS / 2; o > 0; o >>= 1) e.mass += __shfl_xor_sync(M32_ALL, e.mass, o);
+        e.mass = __shfl_sync(M32_ALL, e.mass, 0);
+      }
+    }
     return e;
   }
   __device__ void clear() {
@@ -571,16 +577,23 @@ struct Row {
     sync();                                   // every block's histogram is complete
     uint32_t c[2] = {s.cnt[b], s.cnt[b + 1]};
     long long q[2] = {(long long)s.mass[b], (long long)s.mass[b + 1]};
-    if (ranks > 1)
-      for (int r = 0; r < ranks; ++r)
-        if (r != rank) {
-          const BlockState<NT>* o = peer(r);
+#pragma unroll 1
+    for (int r0 = 1; r0 < ranks; r0 += 4) {       // the others, four at a time
+      uint2 pc[4];
+      ulonglong2 pq[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            c[i] += o->cnt[b + i];
-            q[i] += (long long)o->mass[b + i];
-          }
+      for (int i = 0; i < 4; ++i) {
+        const BlockState<NT>* o = peer(r0 + i < ranks ? (rank + r0 + i) % ranks : rank);
+        pc[i] = *reinterpret_cast<const uint2*>(&o->cnt[b]);
+        pq[i] = *reinterpret_cast<const ulonglong2*>(&o->mass[b]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + i < ranks) {
+          c[0] += pc[i].x, c[1] += pc[i].y;
+          q[0] += (long long)pq[i].x, q[1] += (long long)pq[i].y;
         }
+    }
     uint32_t ci = c[0] + c[1];
     long long qi = q[0] + q[1];
 #pragma unroll
@@ -674,13 +687,17 @@ struct Row {
     n = __reduce_add_sync(M32_ALL, n);
     if (lane == 0) s.wt[wid] = n;
     sync();
-    uint32_t before = 0, total = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const BlockState<NT>* o = peer(r);
-      const uint32_t v = lane < NT / 32 ? o->wt[lane] : 0u;
-      total += __reduce_add_sync(M32_ALL, v);
-      before += __reduce_add_sync(M32_ALL, r < rank || (r == rank && lane < wid) ? v : 0u);
-    }
+    uint32_t before = 0, total = 0, v[RANKS];
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) v[r] = lane < NT / 32 ? peer(r < ranks ? r : rank)->wt[lane] : 0u;
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r)
+      if (r < ranks) {
+        total += v[r];
+        before += r < rank || (r == rank && lane < wid) ? v[r] : 0u;
+      }
+    total = __reduce_add_sync(M32_ALL, total);
+    before = __reduce_add_sync(M32_ALL, before);
     if (total > (uint32_t)LIST) {
       sync();           // the counts have been read
       return 0;
@@ -714,13 +731,15 @@ struct Row {
     ranks = 1;
     return 1;
   }
-  // With the histogram filled: the value tau at which the target is reached, how many hold it, and what lies above it.
-  __device__ bool find(bool by_mass, uint32_t k, double thr, uint32_t& tau, uint32_t& count, uint32_t& cnt_above,
-                       long long& mass_above) {
-    cnt_above = 0;
-    mass_above = 0;
-    uint32_t bin;
-    if (!cross(by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
+  // With the histogram filled (and `crossed`: its bin found): the value tau at which the target is reached, how many hold
+  // it, and what lies above it.
+  __device__ bool find(bool by_mass, uint32_t k, double thr, bool crossed, uint32_t bin, uint32_t& tau, uint32_t& count,
+                       uint32_t& cnt_above, long long& mass_above) {
+    if (!crossed) {
+      cnt_above = 0;
+      mass_above = 0;
+      if (!cross(by_mass, k, thr, cnt_above, mass_above, bin, count)) return false;
+    }
     // the keys of that bin: what its elements span (a short pass over a list), or all that fall there
     uint32_t lo = M32_ALL, hi = 0;
     if (list) {
@@ -739,13 +758,18 @@ struct Row {
       __syncthreads();                        // f_key has been read
       hi = bin > 0 ? bin_floor(bin - 1) - 1 : key_of(m);
     }
+    // the low bits of a 16-bit type's keys are all 0 or all 1 and decide nothing
+    constexpr int LOW = sizeof(T) == 4 ? 0 : (std::is_same<T, bf16>::value ? 16 : 13);
+    const uint32_t least = lo, most = hi;
+    lo >>= LOW;
+    hi >>= LOW;
     while (hi != lo) {
       const int bits = 32 - __clz(hi - lo), shift = max(0, bits - LOG_BINS);
       clear();
       for (int i = threadIdx.x; i < len; i += NT) {
         const float l = at(i);
-        const uint32_t key = key_of(l);
-        if (key >= lo && key <= hi) {
+        const uint32_t full = key_of(l), key = full >> LOW;
+        if (full >= least && full <= most && key >= lo && key <= hi) {
           const long long q = q_of(expf(z(l)));
           if (q > 0) {
             const uint32_t b = (hi - key) >> shift;
@@ -759,13 +783,16 @@ struct Row {
       const uint32_t span = (1u << shift) - 1u;
       lo = hi - lo > span ? hi - span : lo;
     }
-    tau = hi;
+    tau = hi << LOW;
+    if ((tau & 0x80000000u) == 0) tau |= (1u << LOW) - 1u;
     return true;
   }
 };
 
+// What costs here is the latency of the passes between barriers, so 64 registers: with 100, one block an SM less, 64 rows of
+// 131072 (top-k 1000, top-p 0.9) take 48 us, not 34.
 template <typename T, int NT, bool RES>
-__global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int ranks, int slice) {
+__global__ void __launch_bounds__(NT, 1024 / NT) sample_block_kernel(InbSampleArgs a, int ranks, int slice) {
   extern __shared__ __align__(16) unsigned char dyn[];
   BlockState<NT>& s = *reinterpret_cast<BlockState<NT>*>(dyn);
   constexpr int STATE = (sizeof(BlockState<NT>) + 15) / 16 * 16;
@@ -845,9 +872,10 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   // the cut-off (tau, kept): elements above tau stay, and the first `kept` of those equal to it
   uint32_t tau = 0, kept = 0;
   if (select_k || select_p) {
-    uint32_t count, above = 0, bin;
+    uint32_t count, above = 0, bin = 0;
     long long total = 0, mass_above = 0;
     double thr = 0.0;
+    bool crossed = false;
     if (select_k) {
       // the k-th of the threads' largest bounds the k-th of the row from below: what lies above it is few enough, or else
       // the k-th bin of every element is looked for
@@ -863,9 +891,8 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     } else {
       total = R.all_reduce(0, M32_ALL, R.fill(true), true).mass;
       thr = p_threshold(p.top_p, total);
-      if (R.cross(true, 0, thr, above, mass_above, bin, count) && above + count <= (uint32_t)R.LIST &&
-          R.gather(R.bin_floor(bin)) == 2)
-        return;
+      crossed = R.cross(true, 0, thr, above, mass_above, bin, count);
+      if (crossed && above + count <= (uint32_t)R.LIST && R.gather(R.bin_floor(bin)) == 2) return;
     }
     if (R.list && R.len <= 128) {        // few enough for one warp
       if (wid > 0) return;
@@ -891,7 +918,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
       const long long sum = R.fill(true);
       if (select_k) total = R.all_reduce(0, M32_ALL, sum, true).mass;     // stays if fewer than k have a mass
     }
-    if (select_k && R.find(false, (uint32_t)p.k, 0.0, tau, count, above, mass_above)) {
+    if (select_k && R.find(false, (uint32_t)p.k, 0.0, false, 0, tau, count, above, mass_above)) {
       kept = (uint32_t)p.k - above;
       total = mass_above + (long long)kept * q_of(expf(R.z(of_key(tau))));
       if (select_p) R.fill(true);
@@ -899,7 +926,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
     if (select_p) {
       if (select_k) thr = p_threshold(p.top_p, total);
       uint32_t tp;
-      if (R.find(true, 0, thr, tp, count, above, mass_above)) {
+      if (R.find(true, 0, thr, crossed && !R.list, bin, tp, count, above, mass_above)) {
         tau = tp;
         kept = ties_kept(mass_above, q_of(expf(R.z(of_key(tau)))), count, thr);
       }
@@ -938,11 +965,19 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(InbSampleArgs a, int r
   R.sync();
   // every warp: the mass of the row, what comes before its own run, and the ties before it
   long long total = 0, before = 0;
-  uint32_t seen = 0, my_seen = 0;
-  for (int r = 0; r < R.ranks; ++r) {
-    const BlockState<NT>* o = R.peer(r);
-    uint32_t t = lane < nw ? o->wt[lane] : 0u, ti = t;
-    long long v = lane < nw ? o->wm[lane] : 0;
+  uint32_t seen = 0, my_seen = 0, pt[R.RANKS];
+  long long pv[R.RANKS];
+#pragma unroll
+  for (int r = 0; r < R.RANKS; ++r) {
+    const BlockState<NT>* o = R.peer(r < R.ranks ? r : R.rank);
+    pt[r] = lane < nw ? o->wt[lane] : 0u;
+    pv[r] = lane < nw ? o->wm[lane] : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < R.RANKS; ++r) {
+    if (r >= R.ranks) break;
+    uint32_t t = pt[r], ti = t;
+    long long v = pv[r];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t x = __shfl_up_sync(M32_ALL, ti, d);
