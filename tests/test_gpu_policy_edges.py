@@ -11,6 +11,7 @@ ops = importlib.import_module("isaac-net_b200.policy_ops")
 eng_mod = importlib.import_module("isaac-net_b200.engine")
 
 pytestmark = pytest.mark.gpu
+DT = [torch.bfloat16, torch.float16, torch.float32]
 
 
 def gen(seed):
@@ -220,5 +221,25 @@ def test_sample_logits_of_rows_that_hardly_differ(v, dtype):
     mask = torch.rand(6, v, generator=g, device="cuda") < 0.5
     for logits in (near, steep, steps, low):
         for t, k, p, mp in ((1.0, 0, 0.95, 0.0), (1.5, v // 2, 0.6, 0.0), (0.01, 7, 1.0, 0.0), (1.0, v - 1, 0.99, 0.5)):
+            check_sample(logits.to(dtype), u, t, k, p, mp)
+            check_sample(logits.to(dtype), u, t, k, p, mp, mask=mask)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("v", [700, 4100, 20003])
+def test_sample_logits_of_long_rows_that_hardly_differ(v, dtype):
+    """The same for rows that a block or several share: equal logits, two values, infinities of both signs, masks."""
+    from test_gpu_policy_ops import check_sample
+    g = gen(7 * v)
+    u = torch.rand(3, generator=g, device="cuda")
+    near = rn(g, 3, v) * 1e-3
+    holes = near.clone()
+    holes[:, ::7], holes[0, 5] = -math.inf, math.nan
+    high = near.clone()
+    high[1:, 11::v // 3] = math.inf
+    two = (near > 0).float()
+    mask = torch.rand(3, v, generator=g, device="cuda") < 0.5
+    for logits in (near, holes, high, two, two * 0.0 - 3.0):
+        for t, k, p, mp in ((1.0, 0, 0.95, 0.0), (1.5, v // 2, 0.6, 0.0), (0.01, 50, 1.0, 0.3)):
             check_sample(logits.to(dtype), u, t, k, p, mp)
             check_sample(logits.to(dtype), u, t, k, p, mp, mask=mask)
