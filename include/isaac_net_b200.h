@@ -442,12 +442,12 @@ int inb_block_norm_work(const InbNormArgs *args, int64_t *elems);
 /* Gated feed-forward block over N rows: h = act(x wg^T) * (x wu^T), y = h wd^T; x [N, D], wg, wu [F, D], wd [D, F] of
  * dtype bf16 or fp16, rows ld* elements apart; y, dx, dw* are contiguous.  Products accumulate in fp32; h, dg and du
  * are rounded to dtype.  h [N, ldh] is written by the forward call ([2, N, ldh] for up to INB_FFN_ROWS rows without
- * g and u, where h is kept to twice dtype's precision); g, u (both or neither; N rounded up to 128, times
- * ldh, fp32, in an order of the kernels' own) keep the projections for the backward call, which reads all three, takes
- * dy [N, D], uses dg, du [N, ldh] as scratch and writes whichever of dx, (dwg, dwu), dwd are given.  ldh: a multiple of
- * 8, at least F; h, g, u, dg, du, work: 16-byte aligned.  work: inb_gated_ffn_work() bytes, for operands whose rows are
- * not 16-byte aligned and for the parts of products whose sum is split.  status: device word, set to 1 if a
- * wait inside the kernel ran out (the outputs are then invalid), or NULL.
+ * g and u, where h is kept to twice dtype's precision); g, u (both or neither; N rounded up to 128, times F rounded up
+ * to 16, times 3 bytes, in an order of the kernels' own) keep the upper 24 bits of the projections for the backward
+ * call, which reads all three, takes dy [N, D], uses dg, du [N, ldh] as scratch and writes whichever of dx, (dwg, dwu),
+ * dwd are given.  ldh: a multiple of 8, at least F; h, g, u, dg, du, work: 16-byte aligned.  work: inb_gated_ffn_work()
+ * bytes, for operands whose rows are not 16-byte aligned and for the parts of products whose sum is split.  status:
+ * device word, set to 1 if a wait inside the kernel ran out (the outputs are then invalid), or NULL.
  * -2: sizes, dtype or act out of range; -3: a required pointer is NULL or not aligned; -5: work is too small;
  * -6: no tensor map could be made. */
 enum { INB_ACT_SILU = 0, INB_ACT_GELU = 1 };   /* g / (1 + exp(-g)); g (1 + erf(g / sqrt 2)) / 2 */
@@ -458,7 +458,7 @@ typedef struct {
   int64_t N, ldx, ldwg, ldwu, ldwd, ldh, lddy;
   const void *x, *wg, *wu, *wd;
   void *y, *h;
-  float *g, *u;
+  void *g, *u;
   const void *dy;
   void *dg, *du, *dx, *dwg, *dwu, *dwd, *work;
   int64_t work_bytes;

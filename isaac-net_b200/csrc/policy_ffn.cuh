@@ -8,10 +8,11 @@
 //             dWd = dy^T h
 //
 // A tile of the first product holds 128 columns of g and the same 128 of u, so act(g) * u needs no exchange.  g and u are
-// kept for the backward pass in fp32: rounding them to the operand type would put two more roundings into dg and du (the
-// weights' gradients then are 1.4 times as far from the exact ones), and reading them costs 16 bytes an element of h
-// against the 18 D operations the step does for it.  h, dg and du are rounded to the operand type because the next
-// product multiplies them.
+// kept for the backward pass in the upper 24 bits of fp32: what is cut is below 2^-15 of a value, against the operand
+// type's 2^-9 or 2^-12; rounding them to the operand type would put two more roundings into dg and du (the weights' gradients then
+// are 1.4 times as far from the exact ones).  The whole step runs at the GPU's power limit, where bytes cost time whatever
+// bounds a kernel: with all 32 bits it took 2180 us, not 1960 (N = 131072, D = 512, F = 1408, sustained).  h, dg and du are
+// rounded to the operand type because the next product multiplies them.
 #pragma once
 #include <algorithm>
 #include <initializer_list>
@@ -142,11 +143,11 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, const
   }
 }
 
-// h = act(g) u of 128 columns, 32 a warp; g and u kept in blocked fp32 (NULL: not kept)
+// h = act(g) u of 128 columns, 32 a warp; g and u kept as blocked() says (NULL: not kept)
 template <typename T, int CG, int ACT>
 struct EpiGate {
   using State = NoState;
-  float *g, *u;
+  uint4 *g, *u;
   int M, F, groups;
   __device__ void begin(const EpiCtx&, State&) const {}
   __device__ void operator()(const EpiCtx& c, State&, const CUtensorMap* o0, const CUtensorMap*) const {
@@ -175,16 +176,15 @@ struct EpiGate {
     // after the staged tile has gone: its fence would wait for these stores.
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int cg = (n0 >> 2) + 4 * q;
+      const int cg = (n0 >> 4) + q;
+      if (cg >= groups) break;
       const int64_t at = blocked(r, cg, groups);
+      const Kept16 kg = keep16(vg[q]), ku = keep16(vu[q]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (cg + i < groups) {
-          *reinterpret_cast<float4*>(g + at + i * 512) =
-              make_float4(vg[q][4 * i], vg[q][4 * i + 1], vg[q][4 * i + 2], vg[q][4 * i + 3]);
-          *reinterpret_cast<float4*>(u + at + i * 512) =
-              make_float4(vu[q][4 * i], vu[q][4 * i + 1], vu[q][4 * i + 2], vu[q][4 * i + 3]);
-        }
+      for (int i = 0; i < 3; ++i) {
+        g[at + i * 128] = kg.w[i];
+        u[at + i * 128] = ku.w[i];
+      }
     }
   }
 };
@@ -193,19 +193,17 @@ struct EpiGate {
 template <typename T, int CG, int ACT>
 struct EpiDh {
   struct State {
-    float4 g[4], u[4];              // the next 16 columns, on their way while these are worked on
+    Kept16 g, u;                    // the next 16 columns, on their way while these are worked on
   };
-  const float *g, *u;
+  const uint4 *g, *u;
   int M, F, groups;
   __device__ __forceinline__ void fetch(State& s, int r, int col) const {
-    const int64_t at = blocked(r, col >> 2, groups);
+    const int64_t at = blocked(r, col >> 4, groups);
+    const bool in = r < M && (col >> 4) < groups;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s.g[i] = s.u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < M && (col >> 2) + i < groups) {
-        s.g[i] = *reinterpret_cast<const float4*>(g + at + i * 512);
-        s.u[i] = *reinterpret_cast<const float4*>(u + at + i * 512);
-      }
+    for (int i = 0; i < 3; ++i) {
+      s.g.w[i] = in ? g[at + i * 128] : make_uint4(0, 0, 0, 0);
+      s.u.w[i] = in ? u[at + i * 128] : make_uint4(0, 0, 0, 0);
     }
   }
   __device__ void begin(const EpiCtx& c, State& s) const {
@@ -222,11 +220,8 @@ struct EpiDh {
       for (int q = 0; q < 32; q += 16) {
         float v[16], fg[16], fu[16];
         tmem_ld16(acc + b * 32 + q, v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          fg[4 * i] = s.g[i].x, fg[4 * i + 1] = s.g[i].y, fg[4 * i + 2] = s.g[i].z, fg[4 * i + 3] = s.g[i].w;
-          fu[4 * i] = s.u[i].x, fu[4 * i + 1] = s.u[i].y, fu[4 * i + 2] = s.u[i].z, fu[4 * i + 3] = s.u[i].w;
-        }
+        kept16(s.g, fg);
+        kept16(s.u, fu);
         if (b * 32 + q + 16 < COLS) fetch(s, r, n0 + b * 32 + q + 16);
         tmem_ld_wait();
 #pragma unroll
@@ -465,13 +460,13 @@ template <typename T, int CG, int ACT>
 int gate_product(const GemmMaps& m, const InbFfnArgs& a, int kb, cudaStream_t s) {
   const int tm = cdiv(a.N, BM * CG);
   const GemmShape g = {tm, cdiv(a.F, BN / 2), kb, 0, tm, 1, 16 / CG, 1, kb};
-  return gemm_launch<T, CG, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, CG, ACT>{a.g, a.u, (int)a.N, a.F, (int)(a.ldh / 4)}, a.status, s);
+  return gemm_launch<T, CG, MAJOR_K, MAJOR_K>(m, g, EpiGate<T, CG, ACT>{(uint4*)a.g, (uint4*)a.u, (int)a.N, a.F, cdiv(a.F, 16)}, a.status, s);
 }
 template <typename T, int CG, int ACT>
 int dh_product(const GemmMaps& m, const InbFfnArgs& a, int kb, cudaStream_t s) {
   const int tm = cdiv(a.N, BM * CG);
   const GemmShape g = {tm, cdiv(a.F, BN), kb, 0, tm, 0, 16 / CG, 1, kb};
-  return gemm_launch<T, CG, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, CG, ACT>{a.g, a.u, (int)a.N, a.F, (int)(a.ldh / 4)}, a.status, s);
+  return gemm_launch<T, CG, MAJOR_K, MAJOR_MN>(m, g, EpiDh<T, CG, ACT>{(const uint4*)a.g, (const uint4*)a.u, (int)a.N, a.F, cdiv(a.F, 16)}, a.status, s);
 }
 
 template <typename T>

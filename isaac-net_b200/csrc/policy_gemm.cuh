@@ -448,10 +448,41 @@ __device__ __forceinline__ void send_stage(const CUtensorMap* map, T* p, int64_t
   }
   __syncwarp();
 }
-// Blocked fp32 matrices that only these kernels read: 128-row blocks, in them groups of 4 columns, in them the rows: a
-// warp's 32 rows of one group are 512 consecutive bytes.  The place of column group `cg` of row r, groups groups a row:
+// Matrices that only these kernels read keep the upper 24 bits of fp32: 16 columns of a row are three 16-byte pieces.  They lie
+// in 128-row blocks, in them by groups of 16 columns, in them by pieces, in them by rows: a warp's 32 rows of a piece are 512
+// consecutive bytes.  The place (in pieces) of group `cg` of row r, groups groups a row; its further pieces follow 128 on:
 __device__ __forceinline__ int64_t blocked(int r, int cg, int groups) {
-  return (((int64_t)(r >> 7) * groups + cg) * 128 + (r & 127)) * 4;
+  return ((int64_t)(r >> 7) * groups + cg) * (3 * 128) + (r & 127);
+}
+struct Kept16 {
+  uint4 w[3];
+};
+// cut, not rounded: a carry would turn some NaNs into numbers
+__device__ __forceinline__ Kept16 keep16(const float (&v)[16]) {
+  uint32_t o[12];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __float_as_uint(v[4 * i]), b = __float_as_uint(v[4 * i + 1]), c = __float_as_uint(v[4 * i + 2]),
+                   d = __float_as_uint(v[4 * i + 3]);
+    o[3 * i] = __byte_perm(a, b, 0x5321);
+    o[3 * i + 1] = __byte_perm(b, c, 0x6532);
+    o[3 * i + 2] = __byte_perm(c, d, 0x7653);
+  }
+  Kept16 k;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) k.w[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+  return k;
+}
+__device__ __forceinline__ void kept16(const Kept16& k, float (&v)[16]) {
+  const uint32_t o[12] = {k.w[0].x, k.w[0].y, k.w[0].z, k.w[0].w, k.w[1].x, k.w[1].y,
+                          k.w[1].z, k.w[1].w, k.w[2].x, k.w[2].y, k.w[2].z, k.w[2].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[4 * i] = __uint_as_float(o[3 * i] << 8);
+    v[4 * i + 1] = __uint_as_float(__funnelshift_r(o[3 * i], o[3 * i + 1], 16) & 0xFFFFFF00u);
+    v[4 * i + 2] = __uint_as_float(__funnelshift_r(o[3 * i + 1], o[3 * i + 2], 8) & 0xFFFFFF00u);
+    v[4 * i + 3] = __uint_as_float(o[3 * i + 2] & 0xFFFFFF00u);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------- host side

@@ -327,17 +327,17 @@ Tensor ffn_work(InbFfnArgs& a, bool backward, const Tensor& like) {
   a.work = out(w);
   return w;
 }
-// y, and what a backward pass needs: h [n, ldh], and g and u as [2, n up to 128, ldh]
+// y, and what a backward pass needs: h [n, ldh], and g and u as [2, bytes of one]
 std::tuple<Tensor, Tensor, Tensor> ffn_forward(const FfnIn& i, bool keep) {
   const int64_t n = i.x.numel() / i.x.size(-1), ldh = (i.wg.size(0) + 7) / 8 * 8;
   Tensor y = like(i.x), h = at::empty({!keep && n <= INB_FFN_ROWS ? 2 * n : n, ldh}, i.x.options()), gu;
-  if (keep) gu = at::empty({2, (n + 127) / 128 * 128, ldh}, i.x.options().dtype(at::kFloat));
+  if (keep) gu = at::empty({2, (n + 127) / 128 * 128 * ((ldh + 15) / 16 * 48)}, i.x.options().dtype(at::kByte));
   if (n > 0) {
     const On on(i.x);
     const FfnRows r(i);
     InbFfnArgs a = ffn_args(i, r, ldh);
     a.y = out(y), a.h = out(h);
-    if (keep) a.g = (float*)out(gu), a.u = a.g + gu.numel() / 2;
+    if (keep) a.g = out(gu), a.u = (char*)a.g + gu.size(1);
     const Tensor work = ffn_work(a, false, i.x);
     check(api.ffn_fwd(&a, on.stream), "inb_gated_ffn_fwd");
   }
@@ -369,7 +369,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     InbFfnArgs a = ffn_args(i, r, h.size(1));
     const Rows dy = rows_of(grads[0], i.x.size(-1));
     a.dy = dy.p(), a.lddy = dy.ld;
-    a.h = out(h), a.g = (float*)out(gu), a.u = a.g + gu.numel() / 2;
+    a.h = out(h), a.g = out(gu), a.u = (char*)a.g + gu.size(1);
     a.dx = out(o[0]), a.dwg = out(o[1]), a.dwu = out(o[2]), a.dwd = out(o[3]);
     Tensor dh;
     if (need[0] || gate) {
