@@ -243,3 +243,16 @@ def test_sample_logits_of_long_rows_that_hardly_differ(v, dtype):
         for t, k, p, mp in ((1.0, 0, 0.95, 0.0), (1.5, v // 2, 0.6, 0.0), (0.01, 50, 1.0, 0.3)):
             check_sample(logits.to(dtype), u, t, k, p, mp)
             check_sample(logits.to(dtype), u, t, k, p, mp, mask=mask)
+
+
+@pytest.mark.parametrize("v", [1536, 1537, 4096, 4097])
+@pytest.mark.parametrize("n", [2, 400])
+def test_sample_logits_rows_do_not_depend_on_the_batch(n, v):
+    """A row gives the same token and the same log-probability alone, in a few rows and in many, whatever form each takes."""
+    g = gen(n + v)
+    l, u = rn(g, n, v) * 2, torch.rand(n, generator=g, device="cuda")
+    for kw in (dict(top_p=0.9), dict(top_k=300, top_p=0.8, temperature=1.3), dict(top_k=5), dict(min_p=0.01)):
+        tok, lp = ops.sample_logits(l, u, **kw)
+        for i in (0, 1, n // 2, n - 1):
+            one, lp1 = ops.sample_logits(l[i:i + 1], u[i:i + 1], **kw)
+            assert int(one) == int(tok[i]) and float(lp1) == float(lp[i])
