@@ -12,10 +12,10 @@
 // row) do not overflow 64 bits.
 //
 // Rows of up to 384 logits take 8, 16 or 32 lanes of a warp each: the cut-offs are found by bisection, and then by taking
-// the largest remaining logit away until the count or the mass is reached.  Longer rows take a block, or a cluster of 2 to 8 blocks when there
-// are fewer rows than SMs: the row stays in shared memory, a histogram over z finds the bin of the cut-off, and
-// histograms over the float's ordered bits narrow that bin to one value.  Either way the logits are read from memory
-// once, which is the floor; what bounds the kernel is the latency of its passes, not DRAM.
+// the largest remaining logit away until the count or the mass is reached.  Longer rows take a block, or a cluster of 2 to 8
+// blocks when there are fewer rows than SMs: the row stays in shared memory, a histogram over z finds the bin of the
+// cut-off, and histograms over the float's ordered bits narrow that bin to one value.  Either way the logits are read from
+// memory once, which is the floor; what bounds the kernel is the latency of its passes, not DRAM.
 #include <cooperative_groups.h>
 
 #include <type_traits>
