@@ -48,7 +48,9 @@ __device__ __forceinline__ void buffers_free(const EpiCtx& c) {      // all but 
 
 struct NoState {};
 
-// C, or (tiles from m_split on) a second C, rounded
+// C, or (tiles from m_split on) a second C, rounded.  A warp sends its 64 columns as two staged tiles, one a buffer.  The
+// second may follow while the first is read out, but the first waits for both of the tile before: where the matrix ends
+// within the 64 columns only the first buffer was sent, so the last group in flight need not be the other buffer's.
 template <typename T, int CG>
 struct EpiStore {
   using State = NoState;
@@ -58,6 +60,7 @@ struct EpiStore {
   __device__ void begin(const EpiCtx&, State&) const {}
   __device__ void operator()(const EpiCtx& c, State&, const CUtensorMap* o0, const CUtensorMap* o1) const {
     constexpr int COLS = BN / EPI_COLS;
+    static_assert(COLS / 32 == EPI_BUFS, "a staged tile a buffer");
     const bool second = c.tm >= m_split;
     const int r0 = (second ? c.tm - m_split : c.tm) * Gemm<CG>::TM + (c.row & ~31), n0 = c.tn * BN + c.part * COLS;
     const uint32_t acc = c.tmem + c.part * COLS;
@@ -67,7 +70,10 @@ struct EpiStore {
       float v[2][16];
       tmem_ld16(acc + b * 32, v[0]);
       tmem_ld16(acc + b * 32 + 16, v[1]);
-      if (tma) buffers_free<EPI_BUFS - 1>(c);
+      if (tma && b == 0)
+        buffers_free<0>(c);
+      else if (tma)
+        buffers_free<EPI_BUFS - 1>(c);
       tmem_ld_wait();
       stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, 0, v[0]);
       stage16<T>(c.stage_ptr + b * EPI_BUF, c.lane, 16, v[1]);
