@@ -468,6 +468,13 @@ __device__ __forceinline__ void keep_min(Pack<T, W>& a, const Pack<T, W>& v) {
   }
 }
 
+// Elements that a slice of `len` takes in shared memory: it is filled up with -inf to a whole 16-byte access
+template <typename T>
+__host__ __device__ constexpr int padded(int len) {
+  constexpr int W = 16 / (int)sizeof(T);
+  return (len + W - 1) / W * W;
+}
+
 // A 64-bit sum in shared memory by 32-bit atomics, which it has natively: low word, then high word with the carry
 __device__ __forceinline__ void add_mass(unsigned long long& sum, long long q) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&sum);
@@ -862,7 +869,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) sample_block_kernel(InbSampleAr
       for (int e = 0; e < W; ++e) best = fmaxf(best, to_f(most.v[e])), low = fminf(low, to_f(least.v[e]));
     }
     // the rest, and -inf up to a whole access
-    for (int i = i0 + threadIdx.x; i < (len + W - 1) / W * W; i += NT) {
+    for (int i = i0 + threadIdx.x; i < padded<T>(len); i += NT) {
       const T l = i < len && (mp == nullptr || mp[i] != 0) ? lp[i] : none;
       best = fmaxf(best, to_f(l));
       if (to_f(l) > -INFINITY) low = fminf(low, to_f(l));
@@ -1076,7 +1083,7 @@ constexpr int SMEM_MOST = 227 * 1024;
 
 template <typename T, int NT, bool RES>
 static int block_launch(const InbSampleArgs& a, int ranks, int slice, cudaStream_t s) {
-  const size_t smem = (sizeof(BlockState<NT>) + 15) / 16 * 16 + (RES ? (size_t)slice * sizeof(T) : 0);
+  const size_t smem = (sizeof(BlockState<NT>) + 15) / 16 * 16 + (RES ? (size_t)padded<T>(slice) * sizeof(T) : 0);
   auto* k = sample_block_kernel<T, NT, RES>;
   cudaError_t e;
   if (smem > 48 * 1024) {
