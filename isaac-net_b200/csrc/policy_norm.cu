@@ -337,6 +337,7 @@ norm_fwd_kernel(const __grid_constant__ InbNormArgs a, int tpr, const NormChunks
       fetch(slot == 0 ? S - 1 : slot - 1);         // the place read in the last turn
       slot = slot == S - 1 ? 0 : slot + 1;
     } else {
+      x.zero();             // beyond D it holds the last row's output, which a row that is not finite made NaN there too
       x.load((const T*)row_at(a.x, at.row, ld.x, 0), tpr, t, D);
       if (has_h) h.load((const T*)row_at(a.h, at.row, ld.h, 0), tpr, t, D);
       if (a.gate && at.first) g.load((const T*)row_at(a.gate, at.gate, ld.d, 0), tpr, t, D);

@@ -1,6 +1,7 @@
 """The policy operators where a fault of one tile, row or call could reach another.  Tolerances as in the operators' own
 test files."""
 import importlib
+import math
 
 import pytest
 import torch
@@ -47,3 +48,37 @@ def test_sample_logits_rows_that_end_inside_an_access(v, dtype):
     for mask in (None, ends, last):
         for k, p in ((0, 0.9), (200, 0.8), (v - 1, 1.0)):
             check_sample(logits, u, 1.0, k, p, 0.0, mask=mask)
+
+
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("d,dtype", [(5000, torch.float32), (8191, torch.float32), (8192, torch.float32), (6001, torch.bfloat16),
+                                     *((d, t) for d in (1000, 1001) for t in DT)])
+def test_block_norm_bad_rows_stay_alone(d, dtype, post):
+    """Rows with a NaN or an infinity in x or h and a zero row without eps, among more rows than there are workers: every
+    other row's outputs and gradients have the bits of the run without them."""
+    g = gen(d)
+    n, bad = 700, [5, 6, 300, 512]
+    x, h, w, p = rn(g, n, d).to(dtype), rn(g, n, d).to(dtype), rn(g, d).to(dtype), rn(g, d).to(dtype)
+    gy, gn = rn(g, n, d).to(dtype), rn(g, n, d).to(dtype)
+    xb, hb = x.clone(), h.clone()
+    xb[5, 3] = math.nan
+    hb[6, d - 1] = math.inf
+    xb[300], hb[300] = 0.0, 0.0
+    hb[512, 0] = math.nan
+
+    def run(x, h):
+        leaf = [t.clone().requires_grad_(True) for t in (x, h)]
+        y, o = ops.block_norm(leaf[0], w, leaf[1], post_weight=p if post else None, scale=0.5, eps=0.0)
+        alone = ops.block_norm(x, w, eps=0.0)
+        return [y.detach(), o.detach(), *torch.autograd.grad((y, o), leaf, (gy, gn)), alone]
+
+    ok = torch.ones(n, dtype=torch.bool, device="cuda")
+    ok[bad] = False
+    got, want = run(xb, hb), run(x, h)
+    for a, b in zip(got, want):
+        assert bool(b.isfinite().all()) and torch.equal(a[ok], b[ok])
+    assert bool(got[1][[5, 300, 512]].isnan().all()) and bool(got[4][[5, 300]].isnan().all())
+    for i in (0, 5, 300, 301, 699):                 # a row does not depend on its place
+        one = ops.block_norm(xb[i:i + 1], w, hb[i:i + 1], post_weight=p if post else None, scale=0.5, eps=0.0)
+        for a, b in zip(one, got):
+            assert torch.equal(a[0].view(torch.uint8), b[i].view(torch.uint8))
