@@ -109,10 +109,23 @@ CH_SAMPLE = 0x53       # counter-RNG channel of uniforms()
 def uniforms(s0, n, env_id, episode=None, ctr=None, *, stream=0):
     """[E, n] fp32 uniforms in [0, 1) of the engine's counter RNG (inb_rng_draw), keyed like counter_dropout's draws by
     (s0, env_id[e], episode[e], ctr[e], stream): the given random numbers of sample_logits."""
-    ids = [t for t in (env_id, episode, ctr) if t is not None]
-    for t in ids:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int64 and t.shape == env_id.shape):
-            raise ValueError("env_id, episode and ctr must be int64 CUDA tensors of one shape [E]")
+    if not isinstance(env_id, torch.Tensor):
+        raise TypeError(f"env_id must be a tensor, got {type(env_id).__name__}")
+    for name, t in (("env_id", env_id), ("episode", episode), ("ctr", ctr)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor or None, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise B200Unsupported(f"{name} is on {t.device}: the policy operators run on CUDA tensors only")
+        if t.device != env_id.device:
+            raise ValueError(f"{name} is on {t.device}, env_id on {env_id.device}")
+        if t.dtype != torch.int64:
+            raise TypeError(f"{name} is {t.dtype}, expected torch.int64")
+        if t.dim() != 1 or t.shape != env_id.shape:
+            raise ValueError(f"env_id, episode and ctr must have one shape [E], got {name} of {tuple(t.shape)}")
+    if not (0 <= s0 <= 0xFFFFFFFF and 0 <= stream <= 0xFFFFFFFF):
+        raise ValueError("s0 and stream are 32-bit words")
     e = env_id.shape[0]
     if n < 0 or e * n > 0x7FFFFFFF:
         raise B200Unsupported(f"uniforms: {e} x {n} draws are more than one call makes")
