@@ -279,13 +279,17 @@ py::object block_norm(const Tensor& x, const Tensor& weight, const std::optional
 // ------------------------------------------------------------------------------------------------- gated_ffn
 std::mutex status_lock;
 Tensor status_words[64];
-// The device's status word; not made while a graph is captured, whose memory pool it must not lie in
+// The device's status word.  The first call makes it on a stream of its own and waits for that: so it is zero before any
+// stream's kernels see it, and where that call is captured in a graph neither its memory nor its zeroing is part of the graph.
 int32_t* status_word(const Tensor& like) {
   const std::lock_guard<std::mutex> hold(status_lock);
   Tensor& w = status_words[like.get_device() & 63];
   if (!w.defined()) {
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    const c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, like.get_device());
+    const c10::cuda::CUDAStreamGuard on(side);
     w = at::zeros({1}, like.options().dtype(at::kInt));
+    side.synchronize();
   }
   return (int32_t*)out(w);
 }
@@ -295,7 +299,10 @@ int64_t status(int64_t device) {
     const std::lock_guard<std::mutex> hold(status_lock);
     w = status_words[device & 63];
   }
-  return w.defined() ? w.item<int32_t>() : 0;
+  if (!w.defined()) return 0;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  c10::cuda::device_synchronize();         // the operators may run on any stream
+  return w.item<int32_t>();
 }
 
 struct FfnIn {

@@ -68,7 +68,8 @@ def gated_ffn(x, w_gate, w_up, w_down, *, act="silu"):
     and, in the backward pass, the gradients of the two projections are rounded to the inputs' type.  Differentiable in
     every tensor: a call that autograd records keeps the hidden activations and the upper 24 bits of both projections,
     8 bytes for each of the N x F hidden elements.
-    Rows of x and of the weights may be strided; where they are not 16-byte aligned a padded copy is made in the call."""
+    Rows of x and of the weights may be strided; where they are not 16-byte aligned a padded copy is made in the call.
+    Waits inside the kernels have a limit; outputs of a call whose wait ran out are not valid, which status() tells."""
     code = nat.ACTS.get(act)
     if code is None:
         raise ValueError(f"act must be one of {tuple(nat.ACTS)}, got {act!r}")
@@ -141,8 +142,8 @@ def uniforms(s0, n, env_id, episode=None, ctr=None, *, stream=0):
 
 
 def status(device="cuda"):
-    """The device status word of the operators' kernels on `device` (0 = no wait inside a kernel ever ran out); reading it
-    synchronizes."""
+    """The device status word of the operators' kernels on `device` (0 = no wait inside a kernel ever ran out, in eager calls
+    and in replays of graphs alike); reading it waits for all of the device's work."""
     i = torch.device(device).index
     return _ext.status(torch.cuda.current_device() if i is None else i)
 

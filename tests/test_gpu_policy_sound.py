@@ -2,6 +2,9 @@
 test files."""
 import importlib
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ ops = importlib.import_module("isaac-net_b200.policy_ops")
 eng_mod = importlib.import_module("isaac-net_b200.engine")
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 DT = [torch.bfloat16, torch.float16, torch.float32]
 
 
@@ -82,3 +86,52 @@ def test_block_norm_bad_rows_stay_alone(d, dtype, post):
         one = ops.block_norm(xb[i:i + 1], w, hb[i:i + 1], post_weight=p if post else None, scale=0.5, eps=0.0)
         for a, b in zip(one, got):
             assert torch.equal(a[0].view(torch.uint8), b[i].view(torch.uint8))
+
+
+CAPTURED_FIRST = r"""
+import ctypes, importlib, torch
+nat = importlib.import_module("isaac-net_b200._native")
+ops = importlib.import_module("isaac-net_b200.policy_ops")
+seen = []
+
+
+def entry(args, stream):                  # in place of the library's entry point: notes the word, launches nothing
+    seen.append(args.contents.status)
+    return 0
+
+
+entry = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.POINTER(nat.InbFfnArgs), ctypes.c_void_p)(entry)
+names = [*nat.POLICY_EXPORTS, "inb_block_norm_work", "inb_gated_ffn_work"]
+at = {n: ctypes.cast(getattr(nat.lib(), n), ctypes.c_void_p).value for n in names}
+at["inb_gated_ffn_fwd"] = ctypes.cast(entry, ctypes.c_void_p).value
+ops._ext.bind(at, ValueError)
+x, *w = (torch.zeros(s, device="cuda").bfloat16() for s in ((40, 16), (24, 16), (24, 16), (16, 24)))
+a = torch.ones(3, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.gated_ffn(x, *w)
+    b = a + 1
+graph.replay()
+assert b.tolist() == [2.0, 2.0, 2.0] and ops.status() == 0
+del graph
+ops.gated_ffn(x, *w)
+assert seen[0] is not None and seen[0] == seen[1], seen
+"""
+
+
+def test_status_word_where_the_first_call_is_captured():
+    """The first call of a process, made during a capture, passes the word that every later call passes."""
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+
+def test_status_waits_for_every_stream():
+    g = gen(4)
+    x, *w = (rn(g, *s).bfloat16() for s in ((40, 16), (24, 16), (24, 16), (16, 24)))
+    ops.gated_ffn(x, *w)
+    s, done = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(50_000_000)              # some 30 ms
+        done.record()
+    assert ops.status() == 0 and done.query()
