@@ -421,7 +421,8 @@ enum { INB_BF16 = 0, INB_F16 = 1, INB_F32 = 2 };
  * the backward call, which takes the gradients gy, gn of y and n (NULL: zero) and writes those of x, h, w, post and
  * gate.  work: inb_block_norm_work() floats for the backward call's partial column sums (the call looks at the sizes,
  * strides, pointer alignments and which of h, post and gate are given).
- * -2: sizes out of range; -3: a required pointer is NULL; -4: gate_rows does not divide N; -5: work is too small. */
+ * -2: sizes or strides out of range; -3: a required pointer is NULL; -4: gate_rows does not divide N; -5: work is too
+ * small. */
 typedef struct {
   int32_t dtype, D;
   int64_t N, ldx, ldh, gate_rows;

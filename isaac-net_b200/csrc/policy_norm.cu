@@ -616,6 +616,9 @@ static int norm_check(const InbNormArgs* p, bool bwd, bool sizes_only = false) {
   if (a.N == 0) return 0;
   if (a.x == nullptr || a.w == nullptr) return -3;
   if (a.h == nullptr && (a.post != nullptr || a.gate != nullptr)) return -3;
+  // the kernels hold a row's stride in bytes in 32 bits
+  auto far = [](const void* q, int64_t ld) { return q != nullptr && (ld < 0 || ld > INB_MAX_NORM_LD); };
+  if (far(a.x, a.ldx) || far(a.h, a.ldh) || (bwd && (far(a.gy, a.ldgy) || far(a.gn, a.ldgn)))) return -2;
   if (a.gate != nullptr && (a.gate_rows < 1 || a.N % a.gate_rows != 0)) return -4;
   if (sizes_only) return 0;
   if (!bwd && (a.n == nullptr || (a.h != nullptr && a.y == nullptr))) return -3;

@@ -1,9 +1,11 @@
 """Argument checks of the policy operators that need no GPU."""
+import ctypes
 import importlib
 
 import pytest
 import torch
 
+nat = importlib.import_module("isaac-net_b200._native")
 ops = importlib.import_module("isaac-net_b200.policy_ops")
 eng_mod = importlib.import_module("isaac-net_b200.engine")
 
@@ -36,3 +38,17 @@ def test_uniforms_refuses_what_counter_dropout_refuses():
         with pytest.raises(kind, match="env_id|episode|ctr|32-bit|draws"):
             ops.uniforms(*args, **kw)
             pytest.fail(f"{args}, {kw} was not refused")
+
+
+def test_block_norm_entries_refuse_strides_that_32_bits_cannot_hold():
+    """At the C entry points, which callers of other languages reach without the Python layer's checks; what a check lets
+    pass ends at a NULL output (-3) or at the scratch that is too small (-5), not in a launch."""
+    L, most = nat.lib(), nat.MAX_NORM_LD
+    good = dict(dtype=nat.F32, D=8, N=4, ldx=8, x=256, w=256)
+    back = dict(good, h=256, ldh=8, gy=256, ldgy=8, gn=256, ldgn=8, stats=256, gx=256, gw=256, gh=256, work=256)
+    for base, call, passed in ((good, L.inb_block_norm_fwd, -3), (back, L.inb_block_norm_bwd, -5)):
+        for name in [k for k in base if k.startswith("ld")]:
+            for ld, rc in ((0, passed), (8, passed), (most, passed), (most + 1, -2), (1 << 32, -2), ((1 << 32) + 8, -2), (-8, -2)):
+                assert call(ctypes.byref(nat.InbNormArgs(**dict(base, **{name: ld}))), None) == rc, (name, ld)
+    absent = nat.InbNormArgs(**dict(good, ldh=1 << 40, ldgy=-1))          # strides of tensors that are not given
+    assert L.inb_block_norm_fwd(ctypes.byref(absent), None) == -3
