@@ -51,6 +51,7 @@ __device__ __forceinline__ RowParams row_params(const InbSampleArgs& a, int64_t 
   RowParams p;
   const float t = a.temperature_row ? a.temperature_row[row] : a.temperature;
   p.top_p = a.top_p_row ? a.top_p_row[row] : a.top_p;
+  if (p.top_p != p.top_p) p.top_p = 0.f;      // NaN: the first element alone, never a filter that is off
   p.min_p = a.min_p_row ? a.min_p_row[row] : a.min_p;
   p.k = a.top_k_row ? a.top_k_row[row] : a.top_k;
   if (p.k < 0) p.k = 0;
@@ -82,7 +83,7 @@ __device__ __forceinline__ uint32_t ties_kept(long long before, long long q, uin
 }
 __device__ __forceinline__ double p_threshold(float p, long long total) {
   const double t = __dmul_rn((double)p, __ll2double_rn(total));
-  return t > 1.0 ? t : 1.0;          // p <= 0 (or NaN) keeps the first element
+  return t > 1.0 ? t : 1.0;          // p <= 0 keeps the first element
 }
 __device__ __forceinline__ long long draw_at(float u, long long total) {
   const double t = __dmul_rn((double)u, __ll2double_rn(total));

@@ -92,11 +92,12 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     """One token a row: (token int64 [...], logp fp32 [...]) of logits [..., V] (bf16, fp16 or fp32) and uniforms u [...]
     fp32 in [0, 1) (the engine's counter RNG, or any other).
 
-    In this order: divide by temperature (<= 0: take the largest logit), keep the top_k largest (0: all), of those the
+    In this order: divide by temperature (0: take the largest logit), keep the top_k largest (0: all), of those the
     smallest prefix whose mass reaches top_p (>= 1: all), of those the ones of at least min_p times the largest
     probability, then draw by inverse CDF in index order.  Ties go to the lowest index.  logp is the token's
     log-probability after the filters, what a policy gradient needs of the behaviour.  Each setting is a number or a
-    tensor [...] of one per row (fp32; top_k int32).  mask [..., V] or [V] bool, False = not allowed; NaN logits are not
+    tensor [...] of one per row (fp32; top_k int32).  A number out of its range raises ValueError; a row's entry, which only
+    the device sees, counts as the nearest one in range, and NaN as 0.  mask [..., V] or [V] bool, False = not allowed; NaN logits are not
     allowed either.  A row that allows nothing gives token -1 and logp -inf.
 
     The masses are summed in fixed point (2^-40 of the largest), so the token does not depend on how the sum is split;

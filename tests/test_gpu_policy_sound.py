@@ -135,3 +135,28 @@ def test_status_waits_for_every_stream():
         torch.cuda._sleep(50_000_000)              # some 30 ms
         done.record()
     assert ops.status() == 0 and done.query()
+
+
+@pytest.mark.parametrize("v", [5, 40, 130, 700, 3000, 20003])
+def test_sample_logits_row_settings_out_of_range(v):
+    """Per-row settings that are NaN or beyond their range count as 0 or as the nearest in range, in every form of the sampler."""
+    g = gen(v)
+    n = 8
+    l, u = rn(g, n, v), torch.rand(n, generator=g, device="cuda")
+    row = lambda value, dtype=torch.float32: torch.full((n,), value, dtype=dtype, device="cuda")
+    same = [(dict(top_p=row(math.nan)), dict(top_p=0.0)), (dict(top_p=row(-2.0)), dict(top_p=0.0)),
+            (dict(top_p=row(math.nan), top_k=min(v, 50)), dict(top_p=0.0)), (dict(top_p=row(1.5)), dict()),
+            (dict(temperature=row(math.nan)), dict(temperature=0.0)), (dict(temperature=row(-1.0)), dict(temperature=0.0)),
+            (dict(min_p=row(math.nan)), dict()), (dict(min_p=row(-1.0)), dict()), (dict(min_p=row(2.0)), dict(min_p=1.0)),
+            (dict(top_k=row(-3, torch.int32)), dict()), (dict(top_k=row(v + 1, torch.int32)), dict())]
+    for odd, plain in same:
+        got, want = ops.sample_logits(l, u, **odd), ops.sample_logits(l, u, **plain)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), odd
+    first = l.argmax(-1)
+    for kw in (dict(top_p=row(math.nan)), dict(temperature=row(-1.0))):
+        tok, logp = ops.sample_logits(l, u, **kw)
+        assert torch.equal(tok, first) and not bool(logp.any())
+    mixed = row(0.9)
+    mixed[::2] = math.nan                          # among rows that are in range
+    tok, _ = ops.sample_logits(l, u, top_p=mixed)
+    assert torch.equal(tok[::2], first[::2]) and torch.equal(tok[1::2], ops.sample_logits(l, u, top_p=0.9)[0][1::2])
