@@ -142,6 +142,13 @@ bool any_grad(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+// Forward-mode derivatives are not there: a tangent that came in would be lost, which reads as a zero derivative
+void no_tangents(std::initializer_list<std::pair<const Tensor*, const char*>> ts) {
+  for (const auto& [t, name] : ts)
+    if (t != nullptr && t->_fw_grad(/*level=*/0).defined())
+      refuse(name, " carries a tangent: the policy operators have no forward-mode derivatives");
+}
+const Tensor* given(const std::optional<Tensor>& t) { return t ? &*t : nullptr; }
 // A backward pass's results, which cannot be differentiated again: an attempt raises
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -241,6 +248,7 @@ py::object block_norm(const Tensor& x, const Tensor& weight, const std::optional
                       const std::optional<Tensor>& post, const std::optional<Tensor>& gate, double scale, double eps) {
   first(x, "x");
   const int64_t d = width(x, "x");
+  no_tangents({{&x, "x"}, {&weight, "weight"}, {given(h), "h"}, {given(post), "post_weight"}, {given(gate), "gate"}});
   if (d > INB_MAX_NORM_D) refuse("block_norm: D = ", d, " is above ", (int64_t)INB_MAX_NORM_D);
   if (x.numel() / d > INT32_MAX) refuse("block_norm: more than 2^31 - 1 rows");
   const at::ScalarType t = x.scalar_type();
@@ -402,6 +410,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
   VALUE_CHECK(f >= 1 && shaped(wg, f, d) && shaped(wu, f, d) && shaped(wd, d, f), "w_gate and w_up must be [F, ", d,
                     "] and w_down [", d, ", F], got ", wg.sizes(), ", ", wu.sizes(), ", ", wd.sizes());
   if (d > INB_MAX_FFN || f > INB_MAX_FFN || x.numel() / d > INB_MAX_FFN) refuse("gated_ffn: sizes above ", (int64_t)INB_MAX_FFN);
+  no_tangents({{&x, "x"}, {&wg, "w_gate"}, {&wu, "w_up"}, {&wd, "w_down"}});
   if (any_grad({x, wg, wu, wd})) return GatedFfn::apply(x, wg, wu, wd, act);
   return std::get<0>(ffn_forward({x, wg, wu, wd, act}, false));
 }
@@ -447,6 +456,7 @@ Tensor counter_dropout(const Tensor& x, double p, int64_t s0, const Tensor& env_
                        const std::optional<Tensor>& ctr, int64_t stream) {
   first(x, "x");
   VALUE_CHECK(x.dim() >= 1, "x must be [E, ...]");
+  no_tangents({{&x, "x"}});
   VALUE_CHECK(p >= 0.0 && p <= 1.0, "p must be in [0, 1], got ", p);
   VALUE_CHECK(s0 >= 0 && s0 <= UINT32_MAX && stream >= 0 && stream <= UINT32_MAX, "s0 and stream are 32-bit words");
   const int64_t e = x.size(0), n = e > 0 ? x.numel() / e : 0;
@@ -492,6 +502,7 @@ struct Setting {
 py::tuple sample_logits(const Tensor& logits, const Tensor& u, const py::object& temperature, const py::object& top_k,
                         const py::object& top_p, const py::object& min_p, const std::optional<Tensor>& mask) {
   const int code = first(logits, "logits");
+  no_tangents({{&logits, "logits"}});
   const int64_t v = width(logits, "logits"), n = logits.numel() / v;
   const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
   if (v > INB_MAX_SAMPLE_V || n > INB_MAX_SAMPLE_N)

@@ -6,7 +6,7 @@
     token, logp = sample_logits(logits, u, ...)               temperature, top-k, top-p, min-p from given uniforms
     u    = uniforms(s0, n, env_id, episode, ctr)              such uniforms from the engine's counter RNG
 
-The first three are differentiable (torch.autograd, once).  As everywhere in this package there is no CPU path and no
+The first three are differentiable (torch.autograd, once, in reverse mode; a tensor with a tangent is refused).  As everywhere in this package there is no CPU path and no
 fallback: tensors live on one CUDA device, unsupported settings raise B200Unsupported, wrong shapes ValueError and wrong
 types TypeError before anything is launched, and the work is queued on the current stream of the tensors' device.  The
 calls may be captured in a CUDA graph.  The operators have no counterpart in isaac-net, whose policies are its user's.

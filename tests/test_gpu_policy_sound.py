@@ -160,3 +160,23 @@ def test_sample_logits_row_settings_out_of_range(v):
     mixed[::2] = math.nan                          # among rows that are in range
     tok, _ = ops.sample_logits(l, u, top_p=mixed)
     assert torch.equal(tok[::2], first[::2]) and torch.equal(tok[1::2], ops.sample_logits(l, u, top_p=0.9)[0][1::2])
+
+
+def test_forward_mode_is_refused():
+    """A tangent, with and without reverse mode beside it, is refused and not dropped; a dual tensor without one is taken."""
+    import torch.autograd.forward_ad as fwd
+    g = gen(1)
+    x, w = rn(g, 40, 32).bfloat16(), rn(g, 32).bfloat16()
+    ws = [(rn(g, *s) * 0.2).bfloat16() for s in ((48, 32), (48, 32), (32, 48))]
+    env, u = torch.arange(40, device="cuda"), torch.rand(40, generator=g, device="cuda")
+    for grad, leaf in ((True, False), (True, True), (False, False)):
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            dual = lambda t: fwd.make_dual(t.clone().requires_grad_(leaf), torch.ones_like(t))
+            d, dw, d0 = dual(x), dual(w), dual(ws[0])
+            for f in (lambda: ops.block_norm(d, w), lambda: ops.block_norm(x, dw), lambda: ops.block_norm(x, w, d),
+                      lambda: ops.block_norm(x, w, x, post_weight=dw), lambda: ops.block_norm(x, w, x, gate=d),
+                      lambda: ops.gated_ffn(d, *ws), lambda: ops.gated_ffn(x, d0, *ws[1:]),
+                      lambda: ops.counter_dropout(d, 0.5, 1, env), lambda: ops.sample_logits(d, u)):
+                with pytest.raises(eng_mod.B200Unsupported, match="tangent"):
+                    f()
+            assert torch.equal(ops.block_norm(fwd.unpack_dual(d).primal, w).detach(), ops.block_norm(x, w))
