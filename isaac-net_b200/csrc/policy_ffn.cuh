@@ -392,7 +392,9 @@ bool operand_maps(GemmMaps& m, const Operand& a0, const Operand& a1, const Opera
   if (!map_of<T, AMAJ>(&m.a0, a0) || !map_of<T, BMAJ>(&m.b0, b0)) return false;
   m.a1 = m.a0;
   m.b1 = m.b0;
-  return (a1.p == a0.p || map_of<T, AMAJ>(&m.a1, a1)) && (b1.p == b0.p || map_of<T, BMAJ>(&m.b1, b1));
+  // the two weights may be views that start at one address with strides of their own
+  auto equal = [](const Operand& p, const Operand& q) { return p.p == q.p && p.ld == q.ld; };
+  return (equal(a1, a0) || map_of<T, AMAJ>(&m.a1, a1)) && (equal(b1, b0) || map_of<T, BMAJ>(&m.b1, b1));
 }
 
 // A product whose result is stored: C (and, twin, a second C under it, from a1)

@@ -180,3 +180,23 @@ def test_forward_mode_is_refused():
                 with pytest.raises(eng_mod.B200Unsupported, match="tangent"):
                     f()
             assert torch.equal(ops.block_norm(fwd.unpack_dual(d).primal, w).detach(), ops.block_norm(x, w))
+
+
+@pytest.mark.parametrize("n", [4, 40, 300])
+def test_gated_ffn_views_that_share_an_address_or_rows(n):
+    """w_gate and w_up as views of one matrix that start at one address with different strides; x and a gradient whose rows
+    overlap or are all one row.  Bits as on contiguous copies."""
+    g = gen(n)
+    x, dy, wd = rn(g, n, 64).bfloat16(), rn(g, n, 64).bfloat16(), (rn(g, 64, 96) * 0.2).bfloat16()
+    w = (rn(g, 2 * 96, 64) * 0.2).bfloat16()
+
+    def run(x, wg, wu, dy):
+        leaf = [t.detach().requires_grad_(True) for t in (x, wg, wu, wd)]
+        y = ops.gated_ffn(*leaf)
+        return [ops.gated_ffn(x, wg, wu, wd), y.detach(), *torch.autograd.grad(y, leaf, dy)]
+
+    one, over = rn(g, 1, 64).bfloat16().expand(n, 64), torch.as_strided(rn(g, 64 + 8 * n).bfloat16(), (n, 64), (8, 1))
+    for args in ((x, w[::2], w[:96], dy), (x, w[:96], w[::2], dy), (one, w[:96], w[96:], dy), (over, w[:96], w[96:], dy),
+                 (x, w[:96], w[96:], one), (x, w[:96], w[:96], dy)):
+        for a, b in zip(run(*args), run(*(t.contiguous() for t in args))):
+            assert torch.equal(a, b)
