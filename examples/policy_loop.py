@@ -52,13 +52,24 @@ class Policy:
         return (n @ self.head.T).float()
 
 
-def act(policy, net, obs):
-    """The message class of every robot this step: (send [E, R], its log-probability)."""
+def step_key(net):
+    """What this step's dropout is keyed by; copies, because the engine's counters move on in place."""
+    return net.eng.s0, net.eng.env_id, net.eng.episode.clone(), net.clock.clone()
+
+
+def act(policy, net, obs, drop=None):
+    """The message class of every robot this step: (send [E, R], its log-probability).  Drawn from all classes: a filter
+    (top-k, top-p, min-p) would make logp that of another distribution than log_prob's."""
     eng = net.eng
     with torch.no_grad():
-        logits = policy.logits(obs)
+        logits = policy.logits(obs, drop)
         u = ops.uniforms(eng.s0, net.R, eng.env_id, eng.episode, net.clock, stream=STREAM_ACT)
-        return ops.sample_logits(logits, u, top_p=0.98)
+        return ops.sample_logits(logits, u)
+
+
+def log_prob(policy, obs, send, drop=None):
+    """The log-probability of the classes `send`, with its gradient; drop: that of the call of act that drew them."""
+    return torch.log_softmax(policy.logits(obs, drop), -1).gather(-1, send[..., None])[..., 0]
 
 
 def main(envs=64, robots=16, steps=20, lr=0.05, verbose=True):
@@ -72,16 +83,15 @@ def main(envs=64, robots=16, steps=20, lr=0.05, verbose=True):
     pos, log = motion.current(), []
     for step in range(steps):
         obs = net.obs()
-        send, logp = act(policy, net, obs)
-        key = (net.eng.s0, net.eng.env_id, net.eng.episode.clone(), net.clock.clone())
+        key = step_key(net)
+        send, logp = act(policy, net, obs, key)
         net.submit(None, ib.TrafficRequest(send))
         out = net.step(None, pos.cuda())
         pos = motion.advance()
         # one policy gradient step: fresh information, few queued bytes
         reward = -out["aoi_s"] - 1e-6 * out["queue_bytes"]
         adv = (reward - reward.mean()) / (reward.std() + 1e-6)
-        logits = policy.logits(obs, drop=key)
-        loss = -(adv * torch.log_softmax(logits, -1).gather(-1, send[..., None])[..., 0]).mean()
+        loss = -(adv * log_prob(policy, obs, send, key)).mean()
         for p, g in zip(policy.parameters(), torch.autograd.grad(loss, policy.parameters())):
             with torch.no_grad():
                 p -= lr * g

@@ -200,3 +200,25 @@ def test_gated_ffn_views_that_share_an_address_or_rows(n):
                  (x, w[:96], w[96:], one), (x, w[:96], w[:96], dy)):
         for a, b in zip(run(*args), run(*(t.contiguous() for t in args))):
             assert torch.equal(a, b)
+
+
+def test_the_example_differentiates_what_it_sampled_from():
+    """The log-probability that the policy gradient differentiates is the one that the sampler returned for its token.  Both
+    come from the same fp32 logits by fewer than 16 roundings of 2^-24 of the largest number on the way."""
+    from test_gpu_policy_loop import example
+    ex = example()
+    ib, presets = importlib.import_module("isaac-net_b200"), importlib.import_module("isaac-net_b200.presets")
+    wl = presets.workload(1)
+    net = ib.NetModule("L2", 8, 16, "cuda", wl.config(traffic=(), msg_sizes=(200.0, 1500.0, 8192.0)), seed=wl.seed,
+                       isaac=ib.IsaacNetCfg(radio="engine", obs_features=("aoi", "sinr", "queue_len")))
+    policy = ex.Policy(net.obs_dim, classes=4, seed=3)
+    with torch.no_grad():
+        policy.head.mul_(20)                       # probabilities that differ
+    net.reset()
+    obs = rn(gen(5), *net.obs().shape)
+    for drop in (None, ex.step_key(net)):
+        send, logp = ex.act(policy, net, obs, drop)
+        again = ex.log_prob(policy, obs, send, drop)
+        size = 1 + float(policy.logits(obs, drop).detach().abs().max())
+        assert again.requires_grad and float((again - logp).abs().max()) <= 16 * 2.0 ** -24 * size
+        assert float(logp.std()) > 0.1 and len(send.unique()) == 4
