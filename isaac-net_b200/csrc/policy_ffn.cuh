@@ -8,7 +8,7 @@
 //             dWd = dy^T h
 //
 // A tile of the first product holds 128 columns of g and the same 128 of u, so act(g) * u needs no exchange.  g and u are
-// kept for the backward pass in the upper 24 bits of fp32: what is cut is below 2^-15 of a value, against the operand
+// kept for the backward pass in the upper 24 bits of fp32: what is rounded off is below 2^-16 of a value, against the operand
 // type's 2^-9 or 2^-12; rounding them to the operand type would put two more roundings into dg and du (the weights' gradients then
 // are 1.4 times as far from the exact ones).  The whole step runs at the GPU's power limit, where bytes cost time whatever
 // bounds a kernel: with all 32 bits it took 2180 us, not 1960 (N = 131072, D = 512, F = 1408, sustained).  h, dg and du are

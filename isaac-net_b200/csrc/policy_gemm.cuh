@@ -457,13 +457,18 @@ __device__ __forceinline__ int64_t blocked(int r, int cg, int groups) {
 struct Kept16 {
   uint4 w[3];
 };
-// cut, not rounded: a carry would turn some NaNs into numbers
+// The upper 24 bits of a value, rounded: cut, every value would lose on average 2^-16.5 of itself, and sums over rows would
+// keep that.  A NaN is cut, because the carry would turn some of them into numbers; an infinity has no bits to carry.
+__device__ __forceinline__ uint32_t rounded24(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return v == v ? b + 0x80u : b;
+}
 __device__ __forceinline__ Kept16 keep16(const float (&v)[16]) {
   uint32_t o[12];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t a = __float_as_uint(v[4 * i]), b = __float_as_uint(v[4 * i + 1]), c = __float_as_uint(v[4 * i + 2]),
-                   d = __float_as_uint(v[4 * i + 3]);
+    const uint32_t a = rounded24(v[4 * i]), b = rounded24(v[4 * i + 1]), c = rounded24(v[4 * i + 2]),
+                   d = rounded24(v[4 * i + 3]);
     o[3 * i] = __byte_perm(a, b, 0x5321);
     o[3 * i + 1] = __byte_perm(b, c, 0x6532);
     o[3 * i + 2] = __byte_perm(c, d, 0x7653);

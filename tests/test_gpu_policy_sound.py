@@ -222,3 +222,47 @@ def test_the_example_differentiates_what_it_sampled_from():
         size = 1 + float(policy.logits(obs, drop).detach().abs().max())
         assert again.requires_grad and float((again - logp).abs().max()) <= 16 * 2.0 ** -24 * size
         assert float(logp.std()) > 0.1 and len(send.unique()) == 4
+
+
+@pytest.mark.parametrize("dtype,tie", [(torch.float16, 2.0 ** -5), (torch.bfloat16, 2.0 ** -2)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("n", [1, 200])
+def test_gated_ffn_keeps_projections_rounded(n, act, dtype, tie):
+    """The projections kept for the backward pass are rounded to nearest.  g = |u| = 64 + tie + 5 2^-12, exact in fp32, where
+    act(g) = g and act'(g) = 1: dg and du are the projections themselves (dh = 1), and lie 5 2^-12 above the middle of two
+    numbers of the type.  24 bits hold 2^-9 of them: rounded they stay above it, cut they would fall onto it and go down."""
+    x = torch.zeros(n, 8, dtype=dtype, device="cuda")
+    x[0, :3] = torch.tensor([64.0, tie, 5 * 2.0 ** -12])
+    wg = torch.zeros(24, 8, dtype=dtype, device="cuda")
+    wg[:, :3] = 1.0
+    wu, wd = wg.clone(), torch.zeros(8, 24, dtype=dtype, device="cuda")
+    wu[12:] *= -1.0
+    wd[0] = 1.0
+    dy = torch.zeros(n, 8, dtype=dtype, device="cuda")
+    dy[0, 0] = 1.0
+    leaf = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    _, dwg, dwu, dwd = torch.autograd.grad(ops.gated_ffn(*leaf, act=act), leaf, dy)
+    g = x.detach()[0].double().sum()
+    up = g.to(dtype)
+    assert float(up) == 64 + 2 * tie
+    sign = torch.ones(24, 1, dtype=torch.float64, device="cuda")
+    sign[12:] = -1.0
+    row = x.detach()[0].double()
+    assert torch.equal(dwg, (sign * up.double() * row).to(dtype))
+    assert torch.equal(dwu, (up.double() * row).expand(24, 8).to(dtype))
+
+
+def test_gated_ffn_keeps_nan_and_infinity_for_the_backward_pass():
+    """Projections that are NaN (of either sign and any payload) or infinite reach the gradients as such, and only their own
+    rows' dx."""
+    g = gen(6)
+    n, d, f = 70, 64, 80
+    x, dy = rn(g, n, d).bfloat16(), rn(g, n, d).bfloat16()
+    ws = [(rn(g, *s) * 0.2).bfloat16() for s in ((f, d), (f, d), (d, f))]
+    bits = x.view(torch.int16)
+    bits[3, 5], bits[9, 0], bits[20, 1], bits[21, 1] = 0x7FFF, -1, 0x7F80, -0x80        # NaN, -NaN, inf, -inf
+    leaf = [t.detach().requires_grad_(True) for t in (x, *ws)]
+    dx, = torch.autograd.grad(ops.gated_ffn(*leaf), leaf[:1], dy)
+    ok = torch.ones(n, dtype=torch.bool, device="cuda")
+    ok[[3, 9, 20, 21]] = False
+    assert bool(dx[[3, 9]].isnan().all()) and not bool(dx[[20, 21]].isfinite().any()) and bool(dx[ok].isfinite().all())
