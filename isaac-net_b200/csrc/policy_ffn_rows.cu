@@ -84,12 +84,13 @@ struct RowsRing {
   static constexpr int PIECES = 4 + NT * XS;                       // 16-byte pieces of one step in a thread
   static constexpr int S = NT == 4 ? 3 : 4;
   static constexpr int BYTES = S * PIECES * 16 * 32 * ROWS_WARPS;
+  static constexpr int BLOCKS = NT == 4 ? 1 : 2;                   // on an SM: with the partial sums a block of NT = 4 has 132 KB
 };
 
 // NT: groups of 8 rows of x.  GATE: the two groups are g and u of the same columns, out = act(g) u (NT = 1: as hi + lo); else they
 // are 32 columns of the output.  VEC: every row starts on 16 bytes.
 template <typename T, int NT, bool VEC, bool GATE, int ACT>
-__global__ void __launch_bounds__(32 * ROWS_WARPS, 2) ffn_rows_kernel(const RowsArgs a, int ranks) {
+__global__ void __launch_bounds__(32 * ROWS_WARPS, RowsRing<NT, GATE>::BLOCKS) ffn_rows_kernel(const RowsArgs a, int ranks) {
   __shared__ float part[ROWS_WARPS][2][16][8 * NT + 1];
   extern __shared__ __align__(16) unsigned char ring[];
   using Rg = RowsRing<NT, GATE>;
@@ -223,9 +224,10 @@ static int rows_launch(const RowsArgs& a, cudaStream_t s) {
   using Rg = RowsRing<NT, GATE>;
   const int blocks = cdiv(a.M, GATE ? 16 : 32), smem = VEC ? Rg::BYTES : 0;
   auto* k = ffn_rows_kernel<T, NT, VEC, GATE, ACT>;
-  // blocks of one k: enough for two to an SM while a warp keeps the steps of a ring
+  // blocks of one k: enough for what an SM holds while a warp keeps the steps of a ring (planned for two blocks of NT = 4 an
+  // SM, 32 rows at D = 4096, F = 11264 took 110 us, not 94: the second product came in four waves, not two)
   int ranks = 1;
-  while (ranks < 8 && blocks * ranks < 2 * sm_count() && a.K / (2 * ranks * ROWS_WARPS) >= ROWS_K * Rg::S) ranks *= 2;
+  while (ranks < 8 && blocks * ranks < Rg::BLOCKS * sm_count() && a.K / (2 * ranks * ROWS_WARPS) >= ROWS_K * Rg::S) ranks *= 2;
   cudaError_t e = allow_smem<KernelKey<ffn_rows_kernel<T, NT, VEC, GATE, ACT>>>((const void*)k, smem);
   if (e != cudaSuccess) return -100 - (int)e;
   cudaLaunchConfig_t cfg = {};
