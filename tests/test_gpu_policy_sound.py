@@ -220,7 +220,7 @@ def test_the_example_differentiates_what_it_sampled_from():
         send, logp = ex.act(policy, net, obs, drop)
         again = ex.log_prob(policy, obs, send, drop)
         size = 1 + float(policy.logits(obs, drop).detach().abs().max())
-        assert again.requires_grad and float((again - logp).abs().max()) <= 16 * 2.0 ** -24 * size
+        assert again.requires_grad and float((again.detach() - logp).abs().max()) <= 16 * 2.0 ** -24 * size
         assert float(logp.std()) > 0.1 and len(send.unique()) == 4
 
 
@@ -266,3 +266,96 @@ def test_gated_ffn_keeps_nan_and_infinity_for_the_backward_pass():
     ok = torch.ones(n, dtype=torch.bool, device="cuda")
     ok[[3, 9, 20, 21]] = False
     assert bool(dx[[3, 9]].isnan().all()) and not bool(dx[[20, 21]].isfinite().any()) and bool(dx[ok].isfinite().all())
+
+
+def sample_rows(l, u, k, p, t, mask):
+    """sample_logits' definition in torch operations, a row after another of up to millions of logits (k: 0 off; p: 1 off)."""
+    l = torch.where(torch.isnan(l.float()), -math.inf, l.float())
+    if mask is not None:
+        l = torch.where(mask, l, -math.inf)
+    inv = torch.tensor(1.0, device=l.device) / torch.tensor(t, device=l.device)
+    tok, logp = [], []
+    for row, r in zip(l, u):
+        m = row.max()
+        if m == -math.inf:
+            tok.append(-1), logp.append(-math.inf)
+            continue
+        z = torch.where(row == m, 0.0, (row - m) * inv)
+        q = torch.exp(z).double().mul(2.0 ** 40).long()
+        order = torch.sort(row, descending=True, stable=True).indices
+        qs = q[order]
+        if k > 0:
+            qs[k:] = 0
+        if p < 1:
+            before = qs.cumsum(0) - qs
+            keep = before.double() < float(torch.tensor(p)) * qs.sum().double()
+            keep[0] = True
+            qs = torch.where(keep, qs, 0)
+        run = torch.zeros_like(q).scatter_(0, order, qs).cumsum(0)
+        at = min(int(float(r) * float(run[-1])), int(run[-1]) - 1)
+        i = int((run > at).to(torch.uint8).argmax())
+        tok.append(i), logp.append(float(z[i]) - math.log(int(run[-1]) / 2.0 ** 40))
+    return torch.tensor(tok), torch.tensor(logp, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("n,v,dtype", [(3, 1000003, torch.bfloat16), (2, 1000001, torch.float16), (3, 450001, torch.float32),
+                                       (64, 50257, torch.bfloat16), (200, 8193, torch.float16), (37, 20011, torch.float32)])
+def test_sample_logits_long_rows_of_odd_length(n, v, dtype):
+    """Rows beyond what eight blocks keep in shared memory, and batches of an odd vocabulary, whose rows start on every
+    remainder of an access: with and without a mask, in rows of a wider matrix too, one row allowing nothing."""
+    g = gen(v)
+    wide = (rn(g, n, v + 3) * 2).to(dtype)
+    wide[:, 7], wide[0, 11] = math.nan, -math.inf
+    u = torch.rand(n, generator=g, device="cuda")
+    some = torch.rand(n, v, generator=g, device="cuda") < 0.5
+    some[n - 1] = False
+    for l in (wide[:, 3:].contiguous(), wide[:, 1:v + 1]):
+        for mask, k, p, t in ((None, 0, 0.9, 1.0), (some, 0, 0.95, 0.7), (some, 40, 0.9, 1.0), (None, 5000, 0.8, 1.5),
+                              (some, 1, 1.0, 1.0), (some, 0, 1.0, 1.0)):
+            tok, logp = ops.sample_logits(l, u, top_k=k, top_p=p, temperature=t, mask=mask)
+            want, ref = sample_rows(l, u, k, p, t, mask)
+            assert torch.equal(tok.cpu(), want)
+            fin = torch.isfinite(ref)
+            assert torch.equal(torch.isfinite(logp.cpu()), fin)
+            assert bool(((logp.cpu().double() - ref)[fin].abs() <= 2.0 ** -23 * (1 + ref[fin].abs())).all())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("e,n", [(1500, 4095), (257, 20001), (3, 700003)])
+def test_counter_dropout_large_batches_of_odd_rows(e, n, dtype):
+    """Rows that start on every remainder of an access, forward and backward, against the hash in torch's 64-bit integers."""
+    M = 0xFFFFFFFF
+    p, s0 = 0.3, 77
+    env = torch.arange(e, device="cuda") + 5
+
+    def mix(v):
+        v = v ^ (v >> 16)
+        v = (v * 0x21F0AAAD) & M
+        v = v ^ (v >> 15)
+        v = (v * 0x735A2D97) & M
+        return v ^ (v >> 15)
+
+    salt = lambda w: (mix(w & M) + 0x9E3779B9) & M
+    key = torch.full_like(env, s0)
+    for word in (env, 0 * env, torch.full_like(env, 0x44), 0 * env, 0 * env):
+        key = mix(key ^ salt(word))
+    assert int(key[0]) == _host_key(s0, int(env[0]))
+    j = torch.arange((n + 1) // 2, device="cuda") * 0x9E3779B9 & M
+    x, gy = rn(gen(n), e, n).to(dtype).requires_grad_(True), rn(gen(e), e, n).to(dtype)
+    y = ops.counter_dropout(x, p, s0, env)
+    gx, = torch.autograd.grad(y, x, gy)
+    threshold = round(p * 65536)
+    for i in range(0, e, 64):
+        w = mix(mix((key[i:i + 64, None] + j) & M) ^ key[i:i + 64, None])
+        keep = torch.stack((w & 0xFFFF, w >> 16), -1).flatten(1)[:, :n] >= threshold
+        for a, b in ((y, x), (gx, gy)):
+            want = torch.where(keep, b[i:i + 64].detach().float() * (65536 / (65536 - threshold)), 0.0).to(dtype)
+            assert torch.equal(a[i:i + 64].detach(), want)
+
+
+def _host_key(s0, env):
+    mix, salt = eng_mod._mix32, eng_mod._salt
+    k = mix(s0 ^ salt(env))
+    for v in (0, 0x44, 0, 0):
+        k = mix(k ^ salt(v))
+    return k
