@@ -21,8 +21,9 @@ constexpr int DROP_SPAN = 16;     // elements of one thread
 constexpr int DROP_TILE = DROP_THREADS * DROP_SPAN;
 
 // One block per tile of one env's row.  Bound by instruction issue: a word takes 17 operations to hash and 10 to apply to
-// its two elements.  184.5 M bf16 elements take 136 us, their bytes 113 at the measured copy rate.  Tried and slower:
-// several tiles a block with the next one loaded ahead (7 us more), shifts as multiplies on the idle pipe (3 us more).
+// its two elements.  184.5 M bf16 elements take 135 us alone, 141 each in a forward and backward pair, and their bytes 113
+// at the measured copy rate.  Tried and slower: several tiles a block with the next one loaded ahead (7 us more), shifts as
+// multiplies on the idle pipe (3 us more).
 template <typename T, int V>
 __global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(InbDropoutArgs a, uint32_t tiles, float scale) {
   const uint32_t e = blockIdx.x / tiles, tile = blockIdx.x - e * tiles;

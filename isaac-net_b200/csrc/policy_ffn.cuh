@@ -161,6 +161,8 @@ struct EpiGate {
     static_assert(COLS == 32, "one staged tile a warp");
     const int r0 = c.tm * Gemm<CG>::TM + (c.row & ~31), r = r0 + c.lane, n0 = c.tn * (BN / 2) + c.part * COLS;
     if (n0 >= F) return;
+    // Either buffer would do: both are free once buffers_free<0> returns.  Taking them in turn is worth 5 us of 2005 (a training
+    // step, N = 131072, D = 512, F = 1408); waiting for one alone would need a count of the tiles that this warp has sent.
     const int buf = c.tn & 1;
     float vg[2][16], vu[2][16];
 #pragma unroll

@@ -14,7 +14,9 @@
 // in registers, writes one fp32 partial row per block and a second launch adds those in a fixed order: no atomics, so
 // equal inputs give equal bits.
 //
-// Both directions are bound by DRAM: 4 (forward) and 6 (backward) row passes of N x D elements.
+// The forward pass is bound by DRAM, 4 row passes of N x D elements; the backward pass, with 6 of them, by the latency of
+// its instructions: two dependent row sums a row and 8 warps an SM to hide them (N = 131072, D = 512, bf16, a gate for 32
+// rows: 104 us at 5.2 TB/s, and 170 us at 4.7).
 #include <algorithm>
 
 #include "policy_common.cuh"
