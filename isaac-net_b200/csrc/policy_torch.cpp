@@ -294,10 +294,13 @@ int32_t* status_word(const Tensor& like) {
   Tensor& w = status_words[like.get_device() & 63];
   if (!w.defined()) {
     const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
-    const c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, like.get_device());
-    const c10::cuda::CUDAStreamGuard on(side);
+    auto side = [&] { return c10::cuda::getStreamFromPool(false, like.get_device()); };
+    c10::cuda::CUDAStreamGuard on(side());
+    // torch hands out 32 streams in turn: this one may be the one that is captured
+    for (int i = 0; i < 32 && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; ++i)
+      on.reset_stream(side());
     w = at::zeros({1}, like.options().dtype(at::kInt));
-    side.synchronize();
+    on.current_stream().synchronize();
   }
   return (int32_t*)out(w);
 }

@@ -107,8 +107,8 @@ at["inb_gated_ffn_fwd"] = ctypes.cast(entry, ctypes.c_void_p).value
 ops._ext.bind(at, ValueError)
 x, *w = (torch.zeros(s, device="cuda").bfloat16() for s in ((40, 16), (24, 16), (24, 16), (16, 24)))
 a = torch.ones(3, device="cuda")
-graph = torch.cuda.CUDAGraph()
-with torch.cuda.graph(graph):
+graph, streams = torch.cuda.CUDAGraph(), [torch.cuda.Stream() for _ in range(CYCLE)]
+with torch.cuda.graph(graph, stream=streams[0] if streams else None):
     ops.gated_ffn(x, *w)
     b = a + 1
 graph.replay()
@@ -119,9 +119,12 @@ assert seen[0] is not None and seen[0] == seen[1], seen
 """
 
 
-def test_status_word_where_the_first_call_is_captured():
-    """The first call of a process, made during a capture, passes the word that every later call passes."""
-    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=ROOT, capture_output=True, text=True)
+@pytest.mark.parametrize("cycle", [0, 32])
+def test_status_word_where_the_first_call_is_captured(cycle):
+    """The first call of a process, made during a capture, passes the word that every later call passes.  32: torch hands its
+    streams out in turn, and the next would be the one that is captured."""
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.replace("CYCLE", str(cycle))], cwd=ROOT, capture_output=True,
+                       text=True)
     assert r.returncode == 0, r.stderr
 
 
