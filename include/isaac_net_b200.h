@@ -444,7 +444,7 @@ int inb_block_norm_work(const InbNormArgs *args, int64_t *elems);
  * dtype bf16 or fp16, rows ld* elements apart; y, dx, dw* are contiguous.  Products accumulate in fp32; h, dg and du
  * are rounded to dtype.  h [N, ldh] is written by the forward call ([2, N, ldh] for up to INB_FFN_ROWS rows without
  * g and u, where h is kept to twice dtype's precision); g, u (both or neither; N rounded up to 128, times F rounded up
- * to 16, times 3 bytes, in an order of the kernels' own) keep the upper 24 bits of the projections for the backward
+ * to 16, times 3 bytes, in an order of the kernels' own) keep the projections rounded to 24 bits for the backward
  * call, which reads all three, takes dy [N, D], uses dg, du [N, ldh] as scratch and writes whichever of dx, (dwg, dwu),
  * dwd are given.  ldh: a multiple of 8, at least F; h, g, u, dg, du, work: 16-byte aligned.  work: inb_gated_ffn_work()
  * bytes, for operands whose rows are not 16-byte aligned and for the parts of products whose sum is split.  status:
@@ -487,7 +487,8 @@ typedef struct {
 int inb_dropout(const InbDropoutArgs *args, void *cuda_stream);
 
 /* One token a row from logits [N, V] (rows ld apart) and uniforms u [N] in [0, 1): temperature (<= 0: the largest
- * logit), then top-k (0: off), top-p (>= 1: off), min-p (0: off), each for all rows or (the *_row pointers) per row.
+ * logit), then top-k (0: off), top-p (>= 1: off), min-p (0: off), each for all rows or (the *_row pointers) per row.  A
+ * setting beyond its range counts as the nearest in range, NaN as 0.
  * mask (or NULL): bytes, rows ld_mask apart, 0 = not allowed.  NaN logits count as not allowed.  token -1 and logp
  * -inf where nothing is allowed; otherwise logp is the token's log-probability among what the filters keep.
  * -2: sizes out of range; -3: a required pointer is NULL. */

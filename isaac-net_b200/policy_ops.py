@@ -65,9 +65,9 @@ def gated_ffn(x, w_gate, w_up, w_down, *, act="silu"):
 
     x [..., D], w_gate and w_up [F, D], w_down [D, F] (torch.nn.Linear's layout), all bf16 or all fp16; act "silu" or
     "gelu" (the erf form).  Products accumulate in fp32; the hidden activations (but for up to 8 rows without autograd)
-    and, in the backward pass, the gradients of the two projections are rounded to the inputs' type.  Differentiable in
-    every tensor: a call that autograd records keeps the hidden activations and the upper 24 bits of both projections,
-    8 bytes for each of the N x F hidden elements.
+    and, in the backward pass, the gradients of the two projections are rounded to the inputs' type (fp16: infinite above
+    65504).  Differentiable in every tensor: a call that autograd records keeps the hidden activations and both projections
+    rounded to 24 bits, 8 bytes for each of the N x F hidden elements.
     Rows of x and of the weights may be strided; where they are not 16-byte aligned a padded copy is made in the call.
     Waits inside the kernels have a limit; outputs of a call whose wait ran out are not valid, which status() tells."""
     code = nat.ACTS.get(act)
