@@ -362,3 +362,52 @@ def _host_key(s0, env):
     for v in (0, 0x44, 0, 0):
         k = mix(k ^ salt(v))
     return k
+
+
+def big(rows, cols, dtype=torch.bfloat16):
+    """Rows of a small random matrix over and over, 2^31 elements and more."""
+    part = rn(gen(cols), 4099, cols).to(dtype)
+    return part.repeat(-(-rows // 4099), 1)[:rows].contiguous()
+
+
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: their last rows have the bits that the same rows give alone."""
+    n, d = 525000, 4096
+    x, w = big(n, d), rn(gen(1), d).bfloat16()
+    last = slice(n - 40, n)
+    y, o = ops.block_norm(x, w, x, post_weight=w, scale=0.5)
+    a, b = ops.block_norm(x[last], w, x[last], post_weight=w, scale=0.5)
+    assert torch.equal(y[last], a) and torch.equal(o[last], b)
+    del y, o
+    leaf, part = x.requires_grad_(True), x.detach()[last].requires_grad_(True)
+    gx, = torch.autograd.grad(ops.block_norm(leaf, w), leaf, x.detach())
+    px, = torch.autograd.grad(ops.block_norm(part, w), part, part.detach())
+    assert torch.equal(gx[last], px)
+    del gx
+    x = x.detach()
+    env = torch.arange(n, device="cuda")
+    assert torch.equal(ops.counter_dropout(x, 0.5, 1, env)[last], ops.counter_dropout(x[last], 0.5, 1, env[last]))
+    u = torch.rand(n, generator=gen(2), device="cuda")
+    mask = torch.ones(1, 1, dtype=torch.bool, device="cuda").expand(n, d)
+    for v in (d, 33):                            # the short rows lie 4096 apart
+        tok, logp = ops.sample_logits(x[:, :v], u, top_p=0.9, mask=mask[:, :v])
+        t, p = ops.sample_logits(x[last, :v], u[last], top_p=0.9)
+        assert torch.equal(tok[last], t) and torch.equal(logp[last], p)
+
+
+def test_gated_ffn_offsets_beyond_32_bits():
+    """x, y and dx of more than 2^31 elements, and weights' gradients that sum over all rows."""
+    n, d, f = 2100000, 1024, 64
+    x = big(n, d)
+    ws = [(rn(gen(i), *s) * s[1] ** -0.5).bfloat16() for i, s in enumerate(((f, d), (f, d), (d, f)))]
+    last = slice(n - 400, n)
+
+    def run(x):
+        leaf = x.detach().requires_grad_(True)
+        y = ops.gated_ffn(leaf, *ws)
+        return y.detach(), torch.autograd.grad(y, leaf, x)[0]
+
+    # products are split over k by a rule on the sizes; at k = 64 and 128 neither call splits, so the bits are equal
+    for a, b in zip(run(x), run(x[last])):
+        assert torch.equal(a[last], b)
+    assert ops.status() == 0
