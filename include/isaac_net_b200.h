@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define INB_ABI_VERSION 18
+#define INB_ABI_VERSION 19
 #define INB_MAX_C 3       /* cells (more need an ordered interference sum) */
 #define INB_MAX_S 32      /* RBGs per carrier */
 #define INB_MAX_P 32      /* HARQ processes */
@@ -506,6 +506,98 @@ typedef struct {
   float *logp;
 } InbSampleArgs;
 int inb_sample(const InbSampleArgs *args, void *cuda_stream);
+
+/* ------------------------------------------------------------------------------------------------ policy memory
+ * A policy's memory over control steps, for rollouts of S sequences (one a robot) of T steps and one step at a time.
+ * InbSeq: a tensor [S, T, ...] whose sequence s, step t starts at p + s * seq + t * step elements, contiguous from there.
+ * InbReset: bytes, nonzero where a step starts an episode (nothing before it is seen): of sequence s, step t at
+ * p[s / rows * seq + t * step]; p NULL: none. */
+typedef struct {
+  void *p;
+  int64_t seq, step;
+} InbSeq;
+typedef struct {
+  const uint8_t *p;
+  int64_t rows, seq, step;
+} InbReset;
+
+/* Depthwise causal convolution over time: pre[t, c] = bias[c] + sum_j w[c, K - 1 - j] x[t - j, c], y = act(pre)
+ * (INB_ACT_SILU, or -1: none), j = 0 .. K - 1, 2 <= K <= 4.  x, y: [S, T, C]; w [C, K]; bias [C] or NULL.  state [S, K - 1, C]
+ * (sequences state_seq elements apart; NULL: zeros): the inputs before the first step, oldest first; state_out (the same
+ * shape, state_out_seq; NULL: not wanted): the last K - 1 inputs, 0 where an episode began later; with T = 1 it may be
+ * state itself.  Backward: from gy [S, T, C] and gstate_out (contiguous, or NULL: zero) the gradients gx, gstate
+ * (contiguous, or NULL), gw, gbias (or NULL).  work: inb_causal_conv_work() floats of the backward call.
+ * -2: sizes out of range; -3: a required pointer is NULL; -5: work is too small. */
+#define INB_MAX_MEMORY_C (1 << 20) /* channels of inb_causal_conv_* and inb_selective_scan_* */
+#define INB_MAX_MEMORY_S 0x7FFFFFFF /* sequences, steps */
+typedef struct {
+  int32_t dtype, act, C, K;
+  int64_t S, T;
+  InbSeq x, y;
+  const void *w, *bias, *state;
+  void *state_out;
+  int64_t state_seq, state_out_seq;
+  InbReset reset;
+  InbSeq gy, gx;
+  const void *gstate_out;
+  void *gstate, *gw, *gbias;
+  float *work;
+  int64_t work_elems;
+} InbConvArgs;
+int inb_causal_conv_fwd(const InbConvArgs *args, void *cuda_stream);
+int inb_causal_conv_bwd(const InbConvArgs *args, void *cuda_stream);
+int inb_causal_conv_work(const InbConvArgs *args, int64_t *elems);
+
+/* Selective state space scan: delta = log(1 + exp(dt + dt_bias)), h[t, c, n] = exp(delta a[c, n]) h[t - 1, c, n]
+ * + delta x[t, c] b[t, n], y[t, c] = (sum_n h[t, c, n] c[t, n] + d[c] x[t, c]) silu(z[t, c]); 1 <= N <= 64.
+ * x, dt, z, y [S, T, C], b, c [S, T, N] of dtype; a [C, N], d [C], dt_bias [C], the states fp32; d, dt_bias, z NULL: left
+ * out.  state [S, C, N] (state_seq apart; NULL: zeros), state_out (state_out_seq; or NULL): the states before and after;
+ * with T = 1 state_out may be state itself.  kept: what the backward call needs of the forward call,
+ * inb_selective_scan_kept() floats, 16-byte aligned, or NULL.  Backward: from gy and gstate_out (contiguous, or NULL) the
+ * gradients gx, gdt, gz (NULL without z), gb, gc of dtype and ga, gd, gdt_bias, gstate (contiguous; NULL: not wanted)
+ * fp32.  work: inb_selective_scan_work() floats, 16-byte aligned.  Status as above. */
+#define INB_MAX_SCAN_N 64
+typedef struct {
+  int32_t dtype, C, N, reserved;
+  int64_t S, T;
+  InbSeq x, dt, z, b, c, y;
+  const float *a, *d, *dt_bias, *state;
+  float *state_out;
+  int64_t state_seq, state_out_seq;
+  InbReset reset;
+  float *kept;
+  InbSeq gy, gx, gdt, gz, gb, gc;
+  const float *gstate_out;
+  float *gstate, *ga, *gd, *gdt_bias;
+  float *work;
+  int64_t work_elems;
+} InbScanArgs;
+int inb_selective_scan_fwd(const InbScanArgs *args, void *cuda_stream);
+int inb_selective_scan_bwd(const InbScanArgs *args, void *cuda_stream);
+int inb_selective_scan_kept(const InbScanArgs *args, int64_t *elems);
+int inb_selective_scan_work(const InbScanArgs *args, int32_t backward, int64_t *elems);
+
+/* Distillation from a teacher's top logits: over N rows, p = softmax(teacher / tau) over a row's K entries in use, q =
+ * softmax(logits / tau) over its allowed elements, loss = tau^2 sum p (log p - log q); backward: glogits = gloss tau
+ * (q - p).  logits [N, V] of dtype (rows ld apart), teacher [N, K] of dtype teacher_dtype, index [N, K] int64.  An element is
+ * allowed where mask (bytes, rows ld_mask apart, or NULL) is nonzero and its logit is not -inf; an entry is in use where its
+ * index is in [0, V) and allowed and its logit neither -inf nor NaN; entries of one index add up.  A row without an
+ * entry in use has loss 0 and gradient 0.  stats [N, 4]: written by the forward call unless NULL, read by the backward
+ * call.  glogits is contiguous.  -2: sizes out of range; -3: a required pointer is NULL. */
+#define INB_MAX_DISTILL_K 1024
+typedef struct {
+  int32_t dtype, teacher_dtype, V, K;
+  int64_t N, ld, ld_mask;
+  const void *logits, *teacher;
+  const int64_t *index;
+  const uint8_t *mask;
+  float tau;
+  float *loss, *stats;
+  const float *gloss;
+  void *glogits;
+} InbDistillArgs;
+int inb_distill_fwd(const InbDistillArgs *args, void *cuda_stream);
+int inb_distill_bwd(const InbDistillArgs *args, void *cuda_stream);
 
 /* ABI version of the loaded library (INB_ABI_VERSION).  No counterpart in the reference. */
 int inb_abi_version(void);

@@ -13,7 +13,7 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libisaac_net_b200_check.so" if os.environ.get("INB_CHECK") == "1"
                         else "libisaac_net_b200.so")
 TORCH_LIB = "isaac_net_b200_torch.so"       # policy_ops on torch tensors (csrc/policy_torch.cpp)
-ABI_VERSION = 18
+ABI_VERSION = 19
 MAX_ROWS = 128
 NCTR = 64
 BLK_REGIONS = 4        # INB_BLK_REGIONS
@@ -184,8 +184,46 @@ class InbSampleArgs(ctypes.Structure):
 
 POLICY_EXPORTS = {"inb_block_norm_fwd": InbNormArgs, "inb_block_norm_bwd": InbNormArgs, "inb_dropout": InbDropoutArgs,
                   "inb_sample": InbSampleArgs, "inb_gated_ffn_fwd": InbFfnArgs, "inb_gated_ffn_bwd": InbFfnArgs}    # int f(const Args *, void *stream)
+MAX_MEMORY_C, MAX_MEMORY_S, MAX_SCAN_N, MAX_DISTILL_K = 1 << 20, 0x7FFFFFFF, 64, 1024
+
+
+class InbSeq(ctypes.Structure):
+    _fields_ = [("p", P), ("seq", i64), ("step", i64)]
+
+
+class InbReset(ctypes.Structure):
+    _fields_ = [("p", P), ("rows", i64), ("seq", i64), ("step", i64)]
+
+
+class InbConvArgs(ctypes.Structure):
+    _fields_ = ([(n, i32) for n in ("dtype", "act", "C", "K")] + [("S", i64), ("T", i64), ("x", InbSeq), ("y", InbSeq)]
+                + [(n, P) for n in ("w", "bias", "state", "state_out")] + [("state_seq", i64), ("state_out_seq", i64)]
+                + [("reset", InbReset), ("gy", InbSeq), ("gx", InbSeq)]
+                + [(n, P) for n in ("gstate_out", "gstate", "gw", "gbias", "work")] + [("work_elems", i64)])
+
+
+class InbScanArgs(ctypes.Structure):
+    _fields_ = ([(n, i32) for n in ("dtype", "C", "N", "reserved")] + [("S", i64), ("T", i64)]
+                + [(n, InbSeq) for n in ("x", "dt", "z", "b", "c", "y")]
+                + [(n, P) for n in ("a", "d", "dt_bias", "state", "state_out")]
+                + [("state_seq", i64), ("state_out_seq", i64), ("reset", InbReset), ("kept", P)]
+                + [(n, InbSeq) for n in ("gy", "gx", "gdt", "gz", "gb", "gc")]
+                + [(n, P) for n in ("gstate_out", "gstate", "ga", "gd", "gdt_bias", "work")] + [("work_elems", i64)])
+
+
+class InbDistillArgs(ctypes.Structure):
+    _fields_ = ([(n, i32) for n in ("dtype", "teacher_dtype", "V", "K")] + [(n, i64) for n in ("N", "ld", "ld_mask")]
+                + [(n, P) for n in ("logits", "teacher", "index", "mask")] + [("tau", f32)]
+                + [(n, P) for n in ("loss", "stats", "gloss", "glogits")])
+
+
+MEMORY_EXPORTS = {"inb_causal_conv_fwd": InbConvArgs, "inb_causal_conv_bwd": InbConvArgs, "inb_selective_scan_fwd": InbScanArgs,
+                  "inb_selective_scan_bwd": InbScanArgs, "inb_distill_fwd": InbDistillArgs,
+                  "inb_distill_bwd": InbDistillArgs}                                                    # the same
+MEMORY_SIZES = ("inb_causal_conv_work", "inb_selective_scan_kept", "inb_selective_scan_work")
 EXPORTS = ("inb_nr_step", "inb_nr_step_after", "inb_nr_step_noalloc", "inb_nr_reset", "inb_rng_draw", "inb_traffic_step",
-           "inb_store2", "inb_net_obs", "inb_abi_version", "inb_block_norm_work", "inb_gated_ffn_work", *POLICY_EXPORTS)
+           "inb_store2", "inb_net_obs", "inb_abi_version", "inb_block_norm_work", "inb_gated_ffn_work", *POLICY_EXPORTS,
+           *MEMORY_EXPORTS, *MEMORY_SIZES)
 NOALLOC_GAIN_MAX = 1 << 25
 _lib = None
 
@@ -219,13 +257,17 @@ def lib():
     L.inb_traffic_step.argtypes = [ctypes.POINTER(InbTrafficArgs), P]
     L.inb_net_obs.restype = ctypes.c_int
     L.inb_net_obs.argtypes = [ctypes.POINTER(InbObsArgs), P]
-    for name, args in POLICY_EXPORTS.items():
+    for name, args in (*POLICY_EXPORTS.items(), *MEMORY_EXPORTS.items()):
         f = getattr(L, name)
         f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(args), P]
     L.inb_block_norm_work.restype = ctypes.c_int
     L.inb_block_norm_work.argtypes = [ctypes.POINTER(InbNormArgs), ctypes.POINTER(i64)]
     L.inb_gated_ffn_work.restype = ctypes.c_int
     L.inb_gated_ffn_work.argtypes = [ctypes.POINTER(InbFfnArgs), i32, ctypes.POINTER(i64)]
+    L.inb_causal_conv_work.restype = L.inb_selective_scan_kept.restype = L.inb_selective_scan_work.restype = ctypes.c_int
+    L.inb_causal_conv_work.argtypes = [ctypes.POINTER(InbConvArgs), ctypes.POINTER(i64)]
+    L.inb_selective_scan_kept.argtypes = [ctypes.POINTER(InbScanArgs), ctypes.POINTER(i64)]
+    L.inb_selective_scan_work.argtypes = [ctypes.POINTER(InbScanArgs), i32, ctypes.POINTER(i64)]
     _lib = L
     return L
 

@@ -1,0 +1,49 @@
+// selective_scan: what its forward and backward launches share (formulas: policy_scan.cu).
+#pragma once
+#include "policy_seq.cuh"
+
+namespace inb {
+namespace pol {
+
+constexpr int SCAN_STEPS = 8;        // steps a warp stages at once; the backward pass starts from states kept this far apart
+
+// The time axis in parts of `len` steps (a multiple of SCAN_STEPS), so that few sequences still fill the GPU: their states
+// are joined between two passes (scan_part_kernel, scan_join_kernel).
+struct ScanPlan {
+  int64_t parts, len;
+  bool split() const { return parts > 1; }
+};
+// A part costs its decays twice, so the axis is split only below a quarter of the warps that the GPU holds, and into no
+// more parts than fill it.
+inline ScanPlan scan_plan(const InbScanArgs& a, int channels_a_warp) {
+  ScanPlan p;
+  const int64_t warps = a.S * ceil_div(a.C, channels_a_warp), room = (int64_t)sm_count() * 12;
+  int64_t parts = 1;
+  if (warps * 3 <= room) parts = ceil_div(room, warps);
+  if (parts > a.T / 32) parts = a.T / 32;
+  if (parts < 1) parts = 1;
+  p.len = ceil_div(ceil_div(a.T, parts), SCAN_STEPS) * SCAN_STEPS;
+  p.parts = ceil_div(a.T, p.len);
+  return p;
+}
+inline int64_t scan_n4(const InbScanArgs& a) { return (a.N + 3) / 4 * 4; }       // states of a channel in scratch
+inline int64_t scan_chunks(const InbScanArgs& a) { return ceil_div(a.T, SCAN_STEPS); }
+// Forward pass: states a thread (NS) and lanes a channel (LN) for N states
+inline int scan_lanes(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+// floats of the parts' states [S, parts, C, N4] and of their sums of delta [S, parts, C]
+inline int64_t scan_carry_elems(const InbScanArgs& a, const ScanPlan& p) {
+  return p.split() ? a.S * p.parts * a.C * (scan_n4(a) + 1) : 0;
+}
+
+int scan_check(const InbScanArgs& a);
+int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s);
+int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool reverse, cudaStream_t s);
+
+// The reset flags of up to SCAN_STEPS steps from t as bits, the same in every lane; `bytes` is the warp's sequence's
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* bytes, int64_t step, int64_t t, int64_t end, int lane) {
+  if (bytes == nullptr) return 0;
+  return __ballot_sync(0xFFFFFFFFu, lane < SCAN_STEPS && t + lane < end && bytes[(t + lane) * step] != 0);
+}
+
+}  // namespace pol
+}  // namespace inb

@@ -1,0 +1,99 @@
+// What the policy's memory kernels (policy_conv.cu, policy_scan*.cu, policy_distill.cu) share: sequences and resets, the
+// scalar functions, and the column sums that join the blocks' partial gradients.
+#pragma once
+#include <cmath>
+
+#include "policy_common.cuh"
+
+namespace inb {
+namespace pol {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float ex2(float v) {      // 2^v, 2 ulp
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {      // 1 / v, 1 ulp
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * LOG2E)); }
+
+// log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|.  log(1 + u) = 2 atanh(r), r = u / (2 + u) <= 1 / 3, by its series: every
+// term is positive, so small results keep their relative precision, which log of a rounded 1 + u would lose; the first term
+// left out, r^15 / 15, is below 1e-8 of the sum.  s: the derivative, 1 / (1 + e^-v).
+__device__ __forceinline__ float softplus(float v, float& s) {
+  const float u = ex2(-fabsf(v) * LOG2E);
+  const float r = u * rcp(2.f + u), q = r * r;
+  float p = fmaf(q, 1.f / 13, 1.f / 11);
+  p = fmaf(q, p, 1.f / 9);
+  p = fmaf(q, p, 1.f / 7);
+  p = fmaf(q, p, 1.f / 5);
+  p = fmaf(q, p, 1.f / 3);
+  p = fmaf(q, p, 1.f);
+  const float i = rcp(1.f + u);
+  s = v >= 0.f ? i : u * i;
+  return fmaf(2.f * r, p, fmaxf(v, 0.f));
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row(const InbSeq& q, int64_t s, int64_t t) {
+  return (const T*)q.p + s * q.seq + t * q.step;
+}
+template <typename T>
+__device__ __forceinline__ T* row_out(const InbSeq& q, int64_t s, int64_t t) {
+  return (T*)q.p + s * q.seq + t * q.step;
+}
+// The reset bytes of sequence s, or NULL
+__device__ __forceinline__ const uint8_t* resets(const InbReset& r, int64_t s) {
+  return r.p == nullptr ? nullptr : r.p + s / r.rows * r.seq;
+}
+
+inline bool is_aligned(const InbSeq& q, int64_t bytes, int64_t elem) {
+  return q.p == nullptr || (((uint64_t)(uintptr_t)q.p | (uint64_t)(q.seq * elem) | (uint64_t)(q.step * elem)) & (bytes - 1)) == 0;
+}
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------------------------------------------- column sums
+// part [P, M] fp32 -> sums over P: columns [0, first) to out0, [first, second) to out1, the others to out2 (any may be NULL).  A block takes 32
+// columns, its 8 warps rows p, p + 8, ...; the order of the sum does not depend on timing.
+template <typename T>
+__global__ void __launch_bounds__(256) colsum_kernel(const float* part, int64_t P, int64_t M, int64_t first, int64_t second, T* out0,
+                                                     T* out1, T* out2) {
+  const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+  const int w = threadIdx.x >> 5;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < M) {
+    int64_t p = w;
+    for (; p + 24 < P; p += 32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += part[(p + 8 * i) * M + c];
+    }
+    for (; p < P; p += 8) v[0] += part[p * M + c];
+  }
+  __shared__ float sum[8][32];
+  sum[w][threadIdx.x & 31] = (v[0] + v[1]) + (v[2] + v[3]);
+  __syncthreads();
+  if (w != 0 || c >= M) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += sum[i][threadIdx.x];
+  if (c < first) {
+    if (out0 != nullptr) out0[c] = from_f<T>(s);
+  } else if (c < second) {
+    if (out1 != nullptr) out1[c - first] = from_f<T>(s);
+  } else if (out2 != nullptr) {
+    out2[c - second] = from_f<T>(s);
+  }
+}
+template <typename T>
+inline void colsum(const float* part, int64_t P, int64_t M, int64_t first, int64_t second, void* out0, void* out1, void* out2,
+                   cudaStream_t s) {
+  colsum_kernel<T><<<(unsigned)ceil_div(M, 32), 256, 0, s>>>(part, P, M, first, second, (T*)out0, (T*)out1, (T*)out2);
+}
+
+}  // namespace pol
+}  // namespace inb

@@ -5,8 +5,12 @@
     y    = counter_dropout(x, p, s0, env_id, episode, ctr)    dropout keyed by global env id, mask never stored
     token, logp = sample_logits(logits, u, ...)               temperature, top-k, top-p, min-p from given uniforms
     u    = uniforms(s0, n, env_id, episode, ctr)              such uniforms from the engine's counter RNG
+    y, s = causal_conv(x, w, bias, state=, reset=)            a short convolution over a rollout's control steps
+    y, s = selective_scan(x, dt, a, b, c, d=, z=, ...)        a selective state space scan over them: the policy's memory
+    y    = causal_conv_step(x, w, s, bias), selective_scan_step(x, dt, a, b, c, s)     one step, state updated in place
+    loss = distill_loss(logits, teacher, index)               from a teacher's top logits
 
-The first three are differentiable (torch.autograd, once, in reverse mode; a tensor with a tangent is refused).  As everywhere in this package there is no CPU path and no
+All but the sampling and the steps are differentiable (torch.autograd, once, in reverse mode; a tensor with a tangent is refused).  As everywhere in this package there is no CPU path and no
 fallback: tensors live on one CUDA device, unsupported settings raise B200Unsupported, wrong shapes ValueError and wrong
 types TypeError before anything is launched, and the work is queued on the current stream of the tensors' device.  The
 calls may be captured in a CUDA graph.  The operators have no counterpart in isaac-net, whose policies are its user's.
@@ -39,7 +43,9 @@ def _load():
     loader.exec_module(module)
     lib = nat.lib()
     names = [*nat.POLICY_EXPORTS, "inb_block_norm_work", "inb_gated_ffn_work"]
-    module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, B200Unsupported)
+    at = lambda ns: {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ns}
+    module.bind(at(names), B200Unsupported)
+    module.bind_memory(at([*nat.MEMORY_EXPORTS, *nat.MEMORY_SIZES]), B200Unsupported)
     return module
 
 
@@ -142,6 +148,70 @@ def uniforms(s0, n, env_id, episode=None, ctr=None, *, stream=0):
     return out
 
 
+CONV_ACTS = {"silu": nat.ACTS["silu"], None: -1}
+
+
+def _conv_act(act):
+    if act not in CONV_ACTS:
+        raise ValueError(f"act must be one of {tuple(CONV_ACTS)}, got {act!r}")
+    return CONV_ACTS[act]
+
+
+def causal_conv(x, weight, bias=None, *, state=None, reset=None, act="silu"):
+    """A depthwise causal convolution over the control steps of rollouts, and the state that the next rollout begins with.
+
+        y[t] = act(bias + sum_j weight[:, K - 1 - j] * x[t - j]),  j = 0 .. K - 1
+
+    x [..., T, C] (bf16, fp16 or fp32; sums in fp32), weight [C, K] with 2 to 4 taps, bias [C] or None, all of one type; act
+    "silu" or None.  state [..., K - 1, C] or None (zeros): the inputs before the first step, oldest first.  reset [..., T]
+    bool or None: True where a step starts an episode, which sees nothing from before it; leading sizes those of x up to
+    some axis, 1 from there on ([E, 1, T]: one flag for the robots of an env).  Returns (y, state): y in x's order of axes (a
+    rollout buffer that lies step by step is read and answered as it lies), the state after the last step contiguous.
+    Differentiable in x, weight, bias and state, through both results."""
+    return _ext.causal_conv(x, weight, bias, state, reset, _conv_act(act))
+
+
+def causal_conv_step(x, weight, state, bias=None, *, reset=None, act="silu"):
+    """One control step of causal_conv: x [..., C] -> y [..., C]; state [..., K - 1, C] is updated in place and must not
+    overlap x.  reset [...] bool as there, without the steps ([E, 1] for x [E, R, C]).  Not differentiable: refused where
+    autograd would record it."""
+    return _ext.causal_conv_step(x, weight, state, bias, reset, _conv_act(act))
+
+
+def selective_scan(x, dt, a, b, c, *, d=None, z=None, dt_bias=None, state=None, reset=None):
+    """A selective state space scan over the control steps of rollouts, and the state that the next rollout begins with.
+
+        delta = log(1 + exp(dt + dt_bias));  h[t] = exp(delta a) h[t - 1] + (delta x) b[t];  y = (<h[t], c[t]> + d x) silu(z)
+
+    x, dt, z [..., T, C], b, c [..., T, N] of one type (bf16, fp16 or fp32); a [C, N] (negative where the memory is to fade), d
+    and dt_bias [C], state [..., C, N] in fp32; N up to 64; d, z, dt_bias and state may be None.  reset as for causal_conv: h
+    before such a step counts as 0.  Returns (y, state), y in x's order of axes, state contiguous.  The state and all sums are
+    fp32.  Differentiable in every tensor but reset, through both results: a call that autograd records keeps the state at
+    every eighth step (N / 2 bytes for each element of x)."""
+    return _ext.selective_scan(x, dt, a, b, c, d, z, dt_bias, state, reset)
+
+
+def selective_scan_step(x, dt, a, b, c, state, *, d=None, z=None, dt_bias=None, reset=None):
+    """One control step of selective_scan: x, dt, z [..., C], b, c [..., N] -> y [..., C]; state [..., C, N] is updated in
+    place and must not overlap the others.  reset [...] bool without the steps.  Not differentiable: refused where autograd
+    would record it."""
+    return _ext.selective_scan_step(x, dt, a, b, c, state, d, z, dt_bias, reset)
+
+
+def distill_loss(logits, teacher, index, *, temperature=1.0, mask=None):
+    """The divergence of a policy from a teacher's logged top logits, one value a row (fp32 [...]).
+
+        loss = temperature^2 sum_k p_k (log p_k - log q[index_k]),  p = softmax(teacher / temperature) over the K entries,
+        q = softmax(logits / temperature) over the allowed actions
+
+    logits [..., V], teacher [..., K] (K up to 1024) bf16, fp16 or fp32, index [..., K] int64: the actions of the teacher's
+    logits, in any order.  mask [..., V] or [V] bool, False = not allowed; a logit of -inf is not allowed either.  An entry whose index
+    is outside [0, V) (-1: an empty place) or not allowed, or whose teacher logit is -inf or NaN, is left out; entries of one
+    index add up.  A row without entries has loss 0 and gradient 0.  Differentiable in logits (once); the teacher's logits
+    must not require a gradient."""
+    return _ext.distill_loss(logits, teacher, index, temperature, mask)
+
+
 def status(device="cuda"):
     """The device status word of the operators' kernels on `device` (0 = no wait inside a kernel ever ran out, in eager calls
     and in replays of graphs alike); reading it waits for all of the device's work."""
@@ -149,4 +219,5 @@ def status(device="cuda"):
     return _ext.status(torch.cuda.current_device() if i is None else i)
 
 
-__all__ = ["block_norm", "gated_ffn", "counter_dropout", "sample_logits", "uniforms", "status"]
+__all__ = ["block_norm", "gated_ffn", "counter_dropout", "sample_logits", "uniforms", "causal_conv", "causal_conv_step",
+           "selective_scan", "selective_scan_step", "distill_loss", "status"]
