@@ -13,155 +13,174 @@ constexpr int SCAN_WARPS = 4;        // a block's warps work on their own; no ba
 
 // MODE 0: outputs; 1: outputs, and the state before every SCAN_STEPS steps is kept for the backward pass; 2: a part's
 // end state from zero and its sum of delta (-1 where an episode began inside), 3: the same of the reverse recurrence
-// r[t - 1] = exp(delta[t] a) (r[t] + c[t] g[t]), g = gy silu(z)
+// r[t - 1] = exp(delta[t] a) (r[t] + c[t] g[t]), g = gy silu(z), which runs from the part's last step to its first.
+//
+// Bound by the exponentials (one a state and step, 16 a clock and SM) and, next to that, by instruction issue: a quarter of
+// them goes to the FMA pipe (ex2_poly), which evens the two out; all else is packed in pairs of states.  A step's inputs are
+// loaded as the step SCAN_STEPS before is worked on.
 template <typename T, int NS, int LN, int MODE>
-__global__ void __launch_bounds__(SCAN_WARPS * 32) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry, int64_t tasks) {
-  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32;
-  __shared__ alignas(16) float bc[SCAN_WARPS][TC][2][NP];
+__global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry, int64_t tasks) {
+  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 8;
+  constexpr bool BACK = MODE == 3;
+  __shared__ alignas(16) float bc[SCAN_WARPS][2][TC][2][NP];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane % LN;
   const int64_t task = (int64_t)blockIdx.x * SCAN_WARPS + warp;
   if (task >= tasks) return;
   const int64_t tiles = (a.C + CW - 1) / CW, n4 = (a.N + 3) / 4 * 4;
   const int64_t tile = task % tiles, sp = task / tiles, s = sp % a.S, part = sp / a.S;
-  const int64_t ch = tile * CW + lane / LN;
-  const bool on = ch < a.C;
-  const int64_t t0 = part * pl.len, t1 = t0 + pl.len < a.T ? t0 + pl.len : a.T;
-  const uint8_t* rs = resets(a.reset, s);
-  float A[NS], h[NS], dsum = 0.f;
+  const bool on = tile * CW + lane / LN < a.C;
+  const int64_t ch = on ? tile * CW + lane / LN : a.C - 1;      // lanes beyond the last channel read it too and write nothing
+  const int64_t t0 = part * pl.len, t1 = t0 + pl.len < a.T ? t0 + pl.len : a.T, first = BACK ? t1 - 1 : t0;
+  constexpr int DIR = BACK ? -1 : 1;
+  float2 A[NH], h[NH];
+  float dsum = 0.f;
   bool fresh = false;                              // an episode began in this part
-  const float bias = on && a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f;
-  const float d = on && a.d != nullptr ? a.d[ch] : 0.f;
+  const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = MODE < 2 && a.d != nullptr ? a.d[ch] : 0.f;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     const int k = j * NS + n;
-    A[n] = on && k < a.N ? a.a[ch * a.N + k] * LOG2E : 0.f;
-    h[n] = 0.f;
-    if (MODE < 2 && on && k < a.N) {
-      if (part > 0)
-        h[n] = carry[((s * pl.parts + part) * a.C + ch) * n4 + k];
-      else if (a.state != nullptr)
-        h[n] = a.state[s * a.state_seq + ch * a.N + k];
+    float av = 0.f, hv = 0.f;
+    if (k < a.N) {
+      av = a.a[ch * a.N + k] * LOG2E;
+      if (MODE < 2 && part > 0)
+        hv = carry[((s * pl.parts + part) * a.C + ch) * n4 + k];
+      else if (MODE < 2 && a.state != nullptr)
+        hv = a.state[s * a.state_seq + ch * a.N + k];
     }
+    (n & 1 ? A[n / 2].y : A[n / 2].x) = av;
+    (n & 1 ? h[n / 2].y : h[n / 2].x) = hv;
   }
-  // a chunk's inputs, on their way while the one before is worked on
+  const bool gate = a.z.p != nullptr && MODE != 2;
+  const T *px = row<T>(a.x, s, first) + ch, *pd = row<T>(a.dt, s, first) + ch;
+  const T *pz = gate ? row<T>(a.z, s, first) + ch : nullptr, *pg = BACK ? row<T>(a.gy, s, first) + ch : nullptr;
+  T* py = MODE < 2 ? row_out<T>(a.y, s, first) + ch : nullptr;
+  const T *pb = row<T>(a.b, s, first), *pc = row<T>(a.c, s, first);
+  const uint8_t* rs = resets(a.reset, s);
+  if (rs != nullptr) rs += first * a.reset.step;
+  int64_t left = t1 - t0;
   T x[TC], dt[TC], z[TC], g[TC], bcr[BCL];
-  uint32_t rb = 0;
-  const bool gate = a.z.p != nullptr;
-  auto load = [&](int64_t t) {
-#pragma unroll
-    for (int i = 0; i < TC; ++i) {
-      if (on && t + i < t1) {
-        if (MODE != 3) x[i] = row<T>(a.x, s, t + i)[ch];
-        dt[i] = row<T>(a.dt, s, t + i)[ch];
-        if (gate && MODE != 2) z[i] = row<T>(a.z, s, t + i)[ch];
-        if (MODE == 3) g[i] = row<T>(a.gy, s, t + i)[ch];
-      }
-    }
+  auto load = [&](int i) {
+    if (!BACK) x[i] = *px;
+    dt[i] = *pd;
+    if (gate) z[i] = *pz;
+    if (BACK) g[i] = *pg;
+  };
+  auto next = [&] {
+    if (!BACK) px += DIR * a.x.step;
+    pd += DIR * a.dt.step;
+    if (gate) pz += DIR * a.z.step;
+    if (BACK) pg += DIR * a.gy.step;
+  };
+  auto load_bc = [&](int steps) {
 #pragma unroll
     for (int i = 0; i < BCL; ++i) {
       const int k = i * 32 + lane, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
       bcr[i] = from_f<T>(0.f);
-      if (n < a.N && t + tt < t1 && which < 2 && !(MODE == 2 && which == 1) && !(MODE == 3 && which == 0))
-        bcr[i] = row<T>(which ? a.c : a.b, s, t + tt)[n];
+      if (n < a.N && tt < steps && which < 2 && !(MODE == 2 && which == 1) && !(BACK && which == 0))
+        bcr[i] = which ? pc[DIR * tt * a.c.step + n] : pb[DIR * tt * a.b.step + n];
     }
-    rb = reset_bits(rs, a.reset.step, t, t1, lane);
+    pb += DIR * TC * a.b.step;
+    pc += DIR * TC * a.c.step;
   };
-  constexpr bool BACK = MODE == 3;
-  const int64_t chunks = (t1 - t0 + TC - 1) / TC;
-  load(BACK ? t0 + (chunks - 1) * TC : t0);
-  for (int64_t q = 0; q < chunks; ++q) {
-    const int64_t t = t0 + (BACK ? chunks - 1 - q : q) * TC;
-    __syncwarp();
+  auto store_bc = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < BCL; ++i) {
       const int k = i * 32 + lane, which = k / (TC * NP), r = k % (TC * NP);
-      if (which < 2) bc[warp][r / NP][which][r % NP] = to_f(bcr[i]);
+      if (which < 2) bc[warp][buf][r / NP][which][r % NP] = to_f(bcr[i]);
     }
-    __syncwarp();
-    if (MODE == 1 && t > 0 && on) {
-      float* k = a.kept + ((s * ((a.T + TC - 1) / TC - 1) + t / TC - 1) * a.C + ch) * n4;
+  };
 #pragma unroll
-      for (int n = 0; n < NS; n += 4)
-        if (j * NS + n < n4) *reinterpret_cast<float4*>(k + j * NS + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
+  for (int i = 0; i < TC; ++i) {
+    x[i] = dt[i] = z[i] = g[i] = from_f<T>(0.f);
+    if (i < left) load(i);
+    next();
+  }
+  load_bc(left < TC ? (int)left : TC);
+  store_bc(0);
+  uint32_t bits = reset_bits(rs, DIR * a.reset.step, left, lane);
+  float* kept = MODE == 1 ? a.kept + ((s * ((a.T + TC - 1) / TC - 1) + t0 / TC - 1) * a.C + ch) * n4 + j * NS : nullptr;
+  __syncwarp();
+  for (int buf = 0; left > 0; left -= TC, buf ^= 1) {
+    if (MODE == 1) {
+      if (on && (part > 0 || left < t1 - t0)) {
+#pragma unroll
+        for (int n = 0; n < NS; n += 4)
+          if (j * NS + n < n4)
+            *reinterpret_cast<float4*>(kept + n) = make_float4(h[n / 2].x, h[n / 2].y, h[n / 2 + 1].x, h[n / 2 + 1].y);
+      }
+      kept += a.C * n4;
     }
-    float xs[TC], ds[TC], zs[TC], gs[TC];
+    const int steps = left < TC ? (int)left : TC, ahead = left - TC < TC ? (int)(left - TC) : TC;      // now, and of the next chunk
+    if (ahead > 0) load_bc(ahead);
+    uint32_t later = 0;
+    if (rs != nullptr && ahead > 0) {
+      rs += DIR * TC * a.reset.step;
+      later = reset_bits(rs, DIR * a.reset.step, ahead, lane);
+    }
 #pragma unroll
     for (int i = 0; i < TC; ++i) {
-      xs[i] = MODE != 3 && on && t + i < t1 ? to_f(x[i]) : 0.f;
-      ds[i] = on && t + i < t1 ? to_f(dt[i]) : 0.f;
-      zs[i] = MODE != 2 && gate && on && t + i < t1 ? to_f(z[i]) : 0.f;
-      gs[i] = MODE == 3 && on && t + i < t1 ? to_f(g[i]) : 0.f;
-    }
-    const uint32_t bits = rb;
-    if (q + 1 < chunks) load(BACK ? t - TC : t + TC);
-#pragma unroll
-    for (int ii = 0; ii < TC; ++ii) {
-      const int i = BACK ? TC - 1 - ii : ii;
-      if (t + i >= t1) {
-        if (BACK) continue;
-        break;
-      }
+      if (i >= steps) break;
+      const float xv = to_f(x[i]), zv = to_f(z[i]), gv = to_f(g[i]);
       float slope;
-      const float delta = softplus(ds[i] + bias, slope);
-      if (!BACK) {
-        if (bits >> i & 1) {
-          fresh = true;
+      const float delta = softplus(to_f(dt[i]) + bias, slope);
+      if (i < ahead) load(i);
+      next();
+      const bool cut = bits >> i & 1;
+      fresh |= cut;
+      dsum += delta;
+      if (!BACK && cut) {
 #pragma unroll
-          for (int n = 0; n < NS; ++n) h[n] = 0.f;
-        }
-        const float u = delta * xs[i];
-        float y = 0.f;
+        for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
+      }
+      // BACK: u is g, whose c (in place of b) it multiplies
+      const float u = BACK ? (gate ? gv * (zv * sigmoid(zv)) : gv) : delta * xv;
+      const float2 D = both(delta), U = both(u);
+      float2 y = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int n = 0; n < NS; n += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(&bc[warp][i][0][j * NS + n]);
-          const float bb[4] = {b.x, b.y, b.z, b.w};
-          float cc[4] = {};
-          if (MODE < 2) {
-            const float4 c = *reinterpret_cast<const float4*>(&bc[warp][i][1][j * NS + n]);
-            cc[0] = c.x, cc[1] = c.y, cc[2] = c.z, cc[3] = c.w;
-          }
+      for (int n = 0; n < NH; n += 2) {
+        const float4 q = *reinterpret_cast<const float4*>(&bc[warp][buf][i][BACK ? 1 : 0][j * NS + 2 * n]);
+        float4 c = {};
+        if (MODE < 2) c = *reinterpret_cast<const float4*>(&bc[warp][buf][i][1][j * NS + 2 * n]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            h[n + k] = fmaf(ex2(delta * A[n + k]), h[n + k], u * bb[k]);
-            if (MODE < 2) y = fmaf(h[n + k], cc[k], y);
-          }
-        }
-        if (MODE < 2) {
-#pragma unroll
-          for (int o = 1; o < LN; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-          y = fmaf(d, xs[i], y);
-          if (gate) y *= zs[i] * sigmoid(zs[i]);
-          if (on && j == 0) row_out<T>(a.y, s, t + i)[ch] = from_f<T>(y);
-        } else {
-          dsum += delta;
-        }
-      } else {
-        const float gg = gate ? gs[i] * zs[i] * sigmoid(zs[i]) : gs[i];
-        const bool cut = bits >> i & 1;
-        fresh |= cut;
-        dsum += delta;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const float r = fmaf(bc[warp][i][1][j * NS + n], gg, h[n]);
-          h[n] = cut ? 0.f : ex2(delta * A[n]) * r;
+        for (int k = 0; k < 2; ++k) {
+          const float2 v = mul2(D, A[n + k]), b = k ? make_float2(q.z, q.w) : make_float2(q.x, q.y);
+          const float2 e = n + k < POLY ? ex2_poly(v) : make_float2(ex2(v.x), ex2(v.y));
+          if (BACK)
+            h[n + k] = mul2(e, fma2(b, U, h[n + k]));
+          else
+            h[n + k] = fma2(e, h[n + k], mul2(U, b));
+          if (MODE < 2) y = fma2(h[n + k], k ? make_float2(c.z, c.w) : make_float2(c.x, c.y), y);
         }
       }
+      if (BACK && cut) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
+      }
+      if (MODE < 2) {
+        float o = y.x + y.y;
+#pragma unroll
+        for (int m = 1; m < LN; m *= 2) o += __shfl_xor_sync(0xFFFFFFFFu, o, m);
+        o = fmaf(d, xv, o);
+        if (gate) o *= zv * sigmoid(zv);
+        if (on && j == 0) *py = from_f<T>(o);
+        py += a.y.step;
+      }
     }
+    if (ahead > 0) store_bc(buf ^ 1);
+    bits = later;
+    __syncwarp();
   }
   if (!on) return;
-  if (MODE < 2) {
-    if (t1 == a.T && a.state_out != nullptr) {
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
-        if (j * NS + n < a.N) a.state_out[s * a.state_out_seq + ch * a.N + j * NS + n] = h[n];
-    }
-  } else {
-    const int64_t at = (s * pl.parts + part) * a.C + ch;
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-      if (j * NS + n < a.N) carry[at * n4 + j * NS + n] = h[n];
-    if (j == 0) carry[a.S * pl.parts * a.C * n4 + at] = fresh ? -1.f : dsum;
+  for (int n = 0; n < NS; ++n) {
+    const float v = n & 1 ? h[n / 2].y : h[n / 2].x;
+    if (j * NS + n >= a.N) continue;
+    if (MODE >= 2)
+      carry[((s * pl.parts + part) * a.C + ch) * n4 + j * NS + n] = v;
+    else if (t1 == a.T && a.state_out != nullptr)
+      a.state_out[s * a.state_out_seq + ch * a.N + j * NS + n] = v;
   }
+  if (MODE >= 2 && j == 0) carry[a.S * pl.parts * a.C * n4 + (s * pl.parts + part) * a.C + ch] = fresh ? -1.f : dsum;
 }
 
 // The states that the parts begin (reverse: end) with, in place of what they end with from zero.  A thread a state.
@@ -178,54 +197,109 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
   } else if (a.state != nullptr) {
     h = a.state[s * a.state_seq + ch * a.N + n];
   }
-  for (int64_t q = 0; q < pl.parts; ++q) {
-    const int64_t at = (s * pl.parts + (reverse ? pl.parts - 1 - q : q)) * a.C + ch;
-    const float end = carry[at * n4 + n], sum = sums[at];
-    carry[at * n4 + n] = h;
-    h = sum < 0.f ? end : fmaf(ex2(sum * A), h, end);
+  constexpr int U = 16;               // parts whose loads are on their way at once
+  for (int64_t q0 = 0; q0 < pl.parts; q0 += U) {
+    float end[U], sum[U];
+    int64_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t q = q0 + u < pl.parts ? q0 + u : pl.parts - 1;
+      at[u] = (s * pl.parts + (reverse ? pl.parts - 1 - q : q)) * a.C + ch;
+      end[u] = carry[at[u] * n4 + n], sum[u] = sums[at[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (q0 + u >= pl.parts) break;
+      carry[at[u] * n4 + n] = h;
+      h = sum[u] < 0.f ? end[u] : fmaf(ex2(sum[u] * A), h, end[u]);
+    }
   }
 }
 
-// One step: bound by the states' bytes.  V states a thread, moved by one access where they are aligned; `lanes` threads a
-// channel (a power of two up to 16).
-template <typename T, int V>
-__global__ void __launch_bounds__(256) scan_step_kernel(InbScanArgs a, int lanes) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, sc = i / lanes;
-  const int j = (int)(i % lanes);
-  const bool on = sc < a.S * a.C;
-  const int64_t ch = on ? sc % a.C : 0, s = on ? sc / a.C : 0;
-  float y = 0.f;
-  const bool cut = a.state == nullptr || (a.reset.p != nullptr && *resets(a.reset, s) != 0);
-  const float x = to_f(row<T>(a.x, s, 0)[ch]), raw = to_f(row<T>(a.dt, s, 0)[ch]);
-  const T *b = row<T>(a.b, s, 0), *c = row<T>(a.c, s, 0);
-  float slope;
-  const float delta = softplus(raw + (a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f), slope), u = delta * x;
-  if (on) {
-    const float* A = a.a + ch * a.N;
-    const float* old = a.state + s * a.state_seq + ch * a.N;
-    float* out = a.state_out + s * a.state_out_seq + ch * a.N;
-    for (int n = j * V; n < a.N; n += lanes * V) {
+// One step: bound by the states' bytes.  A thread holds V x G states of one channel (V moved by one access; `lanes` threads a
+// channel, a power of two) and walks over sequences, so a, d and dt_bias are read once.  The next sequence's values are on
+// their way while one is worked on.
+constexpr int STEP_THREADS = 256;
+template <typename T, int V, int G>
+__global__ void __launch_bounds__(STEP_THREADS) scan_step_kernel(InbScanArgs a, int lanes, int per, bool vec) {
+  const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
+  const int64_t c0 = (int64_t)blockIdx.x * chans + threadIdx.x / lanes;
+  const bool on = c0 < a.C;
+  const int64_t ch = on ? c0 : a.C - 1;
+  int64_t s = (int64_t)blockIdx.y * per;
+  const int64_t s1 = s + per < a.S ? s + per : a.S;
+  const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = a.d != nullptr ? a.d[ch] : 0.f;
+  const bool gate = a.z.p != nullptr;
+  float A[G][V];
+  int at[G];                     // this thread's states
+#pragma unroll
+  for (int q = 0; q < G; ++q) {
+    at[q] = (q * lanes + j) * V;
+#pragma unroll
+    for (int k = 0; k < V; ++k) A[q][k] = at[q] < a.N ? a.a[ch * a.N + at[q] + k] * LOG2E : 0.f;
+  }
+  struct In {
+    T x, dt, z;
+    Pack<T, V> b[G], c[G];
+    Pack<float, V> h[G];
+    bool cut;
+  };
+  const T *px = row<T>(a.x, s, 0) + ch, *pd = row<T>(a.dt, s, 0) + ch, *pz = gate ? row<T>(a.z, s, 0) + ch : nullptr;
+  const T *pb = row<T>(a.b, s, 0), *pc = row<T>(a.c, s, 0);
+  const float* ph = a.state != nullptr ? a.state + s * a.state_seq + ch * a.N : nullptr;
+  float* po = a.state_out != nullptr ? a.state_out + s * a.state_out_seq + ch * a.N : nullptr;
+  T* py = row_out<T>(a.y, s, 0) + ch;
+  const uint8_t* rs = a.reset.p;
+  const uint32_t rows = a.reset.rows < INB_MAX_MEMORY_S ? (uint32_t)a.reset.rows : INB_MAX_MEMORY_S;
+  auto load = [&](In& i, int64_t at_s) {
+    i.x = *px, i.dt = *pd;
+    if (gate) i.z = *pz;
+    i.cut = rs != nullptr && rs[(uint32_t)at_s / rows * a.reset.seq] != 0;
+#pragma unroll
+    for (int q = 0; q < G; ++q)
+      if (at[q] < a.N) {
+        if (ph != nullptr) i.h[q] = ld<float, V>(ph + at[q]);
+        if (vec) {
+          i.b[q] = ld<T, V>(pb + at[q]), i.c[q] = ld<T, V>(pc + at[q]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) i.b[q].v[k] = pb[at[q] + k], i.c[q].v[k] = pc[at[q] + k];
+        }
+      }
+    px += a.x.seq, pd += a.dt.seq, pb += a.b.seq, pc += a.c.seq;
+    if (gate) pz += a.z.seq;
+    if (ph != nullptr) ph += a.state_seq;
+  };
+  In now, then;
+  load(now, s);
+  for (; s < s1; ++s) {
+    if (s + 1 < s1) load(then, s + 1);
+    const float x = to_f(now.x);
+    float slope, y = 0.f;
+    const float delta = softplus(to_f(now.dt) + bias, slope), u = delta * x;
+#pragma unroll
+    for (int q = 0; q < G; ++q) {
+      if (at[q] >= a.N) continue;
       Pack<float, V> h;
 #pragma unroll
-      for (int k = 0; k < V; ++k) h.v[k] = 0.f;
-      if (!cut) h = ld<float, V>(old + n);
-      const Pack<float, V> w = ld<float, V>(A + n);
-#pragma unroll
       for (int k = 0; k < V; ++k) {
-        h.v[k] = fmaf(ex2(delta * w.v[k] * LOG2E), h.v[k], u * to_f(b[n + k]));
-        y = fmaf(h.v[k], to_f(c[n + k]), y);
+        const float old = ph == nullptr || now.cut ? 0.f : now.h[q].v[k];
+        h.v[k] = fmaf(ex2(delta * A[q][k]), old, u * to_f(now.b[q].v[k]));
+        y = fmaf(h.v[k], to_f(now.c[q].v[k]), y);
       }
-      if (a.state_out != nullptr) st<float, V>(out + n, h);
+      if (po != nullptr && on) st<float, V>(po + at[q], h);
     }
+    for (int o = 1; o < lanes; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
+    y = fmaf(d, x, y);
+    if (gate) {
+      const float z = to_f(now.z);
+      y *= z * sigmoid(z);
+    }
+    if (on && j == 0) *py = from_f<T>(y);
+    py += a.y.seq;
+    if (po != nullptr) po += a.state_out_seq;
+    now = then;
   }
-  for (int o = 1; o < lanes; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-  if (!on || j != 0) return;
-  if (a.d != nullptr) y = fmaf(a.d[ch], x, y);
-  if (a.z.p != nullptr) {
-    const float z = to_f(row<T>(a.z, s, 0)[ch]);
-    y *= z * sigmoid(z);
-  }
-  row_out<T>(a.y, s, 0)[ch] = from_f<T>(y);
 }
 
 int scan_check(const InbScanArgs& a) {
@@ -270,19 +344,29 @@ static int scan_type(const InbScanArgs& a, const ScanPlan& p, float* carry, int 
   if (a.N <= 32) return scan_mode<T, 16, 2>(a, p, carry, mode, s);
   return scan_mode<T, 16, 4>(a, p, carry, mode, s);
 }
+template <typename T, int V, int G>
+static int step_go(const InbScanArgs& a, int lanes, cudaStream_t s) {
+  const int64_t tiles = ceil_div(a.C, STEP_THREADS / lanes);
+  // as many sequences a block as leave eight blocks an SM, no more than 16, and a grid's second axis ends at 65535
+  int64_t per = a.S * tiles / (sm_count() * 8);
+  if (per > 16) per = 16;
+  if (per < ceil_div(a.S, 65535)) per = ceil_div(a.S, 65535);
+  if (per < 1) per = 1;
+  const bool vec = is_aligned(a.b, V * sizeof(T), sizeof(T)) && is_aligned(a.c, V * sizeof(T), sizeof(T));
+  scan_step_kernel<T, V, G><<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per)), STEP_THREADS, 0, s>>>(a, lanes, (int)per, vec);
+  return launch_status();
+}
 template <typename T>
 static int scan_step(const InbScanArgs& a, cudaStream_t s) {
-  const uint64_t m = (uint64_t)(uintptr_t)a.state | (uint64_t)(uintptr_t)a.state_out | (uint64_t)(uintptr_t)a.a |
-                     (uint64_t)(a.state_seq * 4) | (uint64_t)(a.state_out_seq * 4) | (uint64_t)(a.N * 4);
-  const bool vec = (m & 15) == 0;
+  const uint64_t m = (uint64_t)(uintptr_t)a.state | (uint64_t)(uintptr_t)a.state_out | (uint64_t)(a.state_seq * 4) |
+                     (uint64_t)(a.state_out_seq * 4) | (uint64_t)(a.N * 4);
   int lanes = 1;
-  while (lanes < 16 && lanes * 4 < a.N) lanes *= 2;
-  const unsigned blocks = (unsigned)ceil_div(a.S * a.C * lanes, 256);
-  if (vec)
-    scan_step_kernel<T, 4><<<blocks, 256, 0, s>>>(a, lanes);
-  else
-    scan_step_kernel<T, 1><<<blocks, 256, 0, s>>>(a, lanes);
-  return launch_status();
+  if ((m & 15) == 0) {
+    while (lanes < 16 && lanes * 4 < a.N) lanes *= 2;
+    return step_go<T, 4, 1>(a, lanes, s);
+  }
+  while (lanes < 16 && lanes < a.N) lanes *= 2;
+  return a.N <= 16 ? step_go<T, 1, 1>(a, lanes, s) : step_go<T, 1, 4>(a, lanes, s);
 }
 // mode 0: the forward pass; 3: the backward pass's parts
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s) {

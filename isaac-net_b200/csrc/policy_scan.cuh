@@ -17,7 +17,7 @@ struct ScanPlan {
 // more parts than fill it.
 inline ScanPlan scan_plan(const InbScanArgs& a, int channels_a_warp) {
   ScanPlan p;
-  const int64_t warps = a.S * ceil_div(a.C, channels_a_warp), room = (int64_t)sm_count() * 12;
+  const int64_t warps = a.S * ceil_div(a.C, channels_a_warp), room = (int64_t)sm_count() * 16;
   int64_t parts = 1;
   if (warps * 3 <= room) parts = ceil_div(room, warps);
   if (parts > a.T / 32) parts = a.T / 32;
@@ -39,10 +39,10 @@ int scan_check(const InbScanArgs& a);
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s);
 int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool reverse, cudaStream_t s);
 
-// The reset flags of up to SCAN_STEPS steps from t as bits, the same in every lane; `bytes` is the warp's sequence's
-__device__ __forceinline__ uint32_t reset_bits(const uint8_t* bytes, int64_t step, int64_t t, int64_t end, int lane) {
-  if (bytes == nullptr) return 0;
-  return __ballot_sync(0xFFFFFFFFu, lane < SCAN_STEPS && t + lane < end && bytes[(t + lane) * step] != 0);
+// The reset flags of the next `left` (of them up to SCAN_STEPS) steps as bits, the same in every lane; `at`: the first one's
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* at, int64_t step, int64_t left, int lane) {
+  if (at == nullptr) return 0;
+  return __ballot_sync(0xFFFFFFFFu, lane < SCAN_STEPS && lane < left && at[lane * step] != 0);
 }
 
 }  // namespace pol

@@ -22,11 +22,43 @@ __device__ __forceinline__ float rcp(float v) {      // 1 / v, 1 ulp
 }
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * LOG2E)); }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+// 2^v of two values without the special function unit, which makes 16 results a clock and SM and so bounds the scan: v = i + f,
+// f in [-1/2, 1/2], 2^f = 1 + f P(f) with P the Chebyshev interpolation of (2^f - 1) / f of degree 5 (at most 1.2 * 2^-24
+// off, no bias where 2^v is near 1), times 2^i through the exponent's bits.  v is held to [-127, 128]: 0 and infinity there.
+__device__ __forceinline__ float2 ex2_poly(float2 v) {
+  auto hold = [](float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(r) : "f"(x));      // -127
+    asm("min.NaN.f32 %0, %1, 0f43000000;" : "=f"(r) : "f"(r));      // 128
+    return r;
+  };
+  v = make_float2(hold(v.x), hold(v.y));
+  const float2 magic = both(12582912.f + 127.f);      // 1.5 * 2^23: the sum's low bits are i + 127
+  const float2 r = add2(v, magic);
+  const float2 f = add2(v, mul2(add2(r, both(-12582912.f - 127.f)), both(-1.f)));
+  float2 p = fma2(both(0.00015453163359779865f), f, both(0.0013390863314270973f));
+  p = fma2(p, f, both(0.009618083015084267f));
+  p = fma2(p, f, both(0.055503569543361664f));
+  p = fma2(p, f, both(0.24022650718688965f));
+  p = fma2(p, f, both(0.6931471824645996f));
+  p = fma2(p, f, both(1.f));
+  return mul2(p, make_float2(__uint_as_float(__float_as_uint(r.x) << 23), __uint_as_float(__float_as_uint(r.y) << 23)));
+}
+
 // log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|.  log(1 + u) = 2 atanh(r), r = u / (2 + u) <= 1 / 3, by its series: every
 // term is positive, so small results keep their relative precision, which log of a rounded 1 + u would lose; the first term
 // left out, r^15 / 15, is below 1e-8 of the sum.  s: the derivative, 1 / (1 + e^-v).
 __device__ __forceinline__ float softplus(float v, float& s) {
-  const float u = ex2(-fabsf(v) * LOG2E);
+  const float a = -fabsf(v), t = a * LOG2E;
+  const float low = fmaf(a, LOG2E, -t);              // what t's rounding lost, 2^-24 |v|, and would cost u relative
+  const float e = ex2(t), u = fmaf(e, low * LN2, e);
   const float r = u * rcp(2.f + u), q = r * r;
   float p = fmaf(q, 1.f / 13, 1.f / 11);
   p = fmaf(q, p, 1.f / 9);
