@@ -16,91 +16,85 @@ constexpr int SCAN_WARPS = 4;        // a block's warps work on their own; no ba
 // r[t - 1] = exp(delta[t] a) (r[t] + c[t] g[t]), g = gy silu(z), which runs from the part's last step to its first.
 //
 // Bound by the exponentials (one a state and step, 16 a clock and SM) and, next to that, by instruction issue: a quarter of
-// them goes to the FMA pipe (ex2_poly), which evens the two out; all else is packed in pairs of states.  A step's inputs are
-// loaded as the step SCAN_STEPS before is worked on.
+// them goes to the FMA pipe (ex2_poly), which evens the two out; all else is packed in pairs of states.  A chunk of
+// SCAN_STEPS steps is prepared at once (delta, u, the gate), then the next one's loads are sent, then its steps run.
 template <typename T, int NS, int LN, int MODE>
-__global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry, int64_t tasks) {
+__global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry) {
   constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 8;
   constexpr bool BACK = MODE == 3;
-  __shared__ alignas(16) float bc[SCAN_WARPS][2][TC][2][NP];
+  __shared__ alignas(16) float bc[SCAN_WARPS][TC][2][NP];
+  __shared__ float4 stage[SCAN_WARPS][TC][32];       // delta, u, silu(z) (1 without z), d x of this lane's channel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane % LN;
-  const int64_t task = (int64_t)blockIdx.x * SCAN_WARPS + warp;
-  if (task >= tasks) return;
-  const int64_t tiles = (a.C + CW - 1) / CW, n4 = (a.N + 3) / 4 * 4;
-  const int64_t tile = task % tiles, sp = task / tiles, s = sp % a.S, part = sp / a.S;
-  const bool on = tile * CW + lane / LN < a.C;
-  const int64_t ch = on ? tile * CW + lane / LN : a.C - 1;      // lanes beyond the last channel read it too and write nothing
+  const int n4 = (a.N + 3) / 4 * 4;
+  // a block is one sequence's: what depends on it is the same for all its threads
+  const int64_t part = pl.parts > 1 ? blockIdx.x / (uint32_t)a.S : 0, s = blockIdx.x - part * a.S;
+  const int c0 = (blockIdx.y * (blockDim.x >> 5) + warp) * CW + lane / LN;
+  const bool on = c0 < a.C;
+  const int ch = on ? c0 : a.C - 1;                // lanes beyond the last channel read it too and write nothing
   const int64_t t0 = part * pl.len, t1 = t0 + pl.len < a.T ? t0 + pl.len : a.T, first = BACK ? t1 - 1 : t0;
   constexpr int DIR = BACK ? -1 : 1;
   float2 A[NH], h[NH];
   float dsum = 0.f;
   bool fresh = false;                              // an episode began in this part
   const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = MODE < 2 && a.d != nullptr ? a.d[ch] : 0.f;
+  const float* h0 = nullptr;                       // the state before the first step
+  if (MODE < 2) h0 = part > 0 ? carry + ((s * pl.parts + part) * a.C + ch) * n4 : a.state != nullptr ? a.state + s * a.state_seq + ch * a.N : nullptr;
+  const float* pa = a.a + ch * a.N;
+  if (a.N == NP && ((uintptr_t)a.a & 15) == 0 && (part > 0 || (((uintptr_t)a.state | (a.state_seq * 4)) & 15) == 0)) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    const int k = j * NS + n;
-    float av = 0.f, hv = 0.f;
-    if (k < a.N) {
-      av = a.a[ch * a.N + k] * LOG2E;
-      if (MODE < 2 && part > 0)
-        hv = carry[((s * pl.parts + part) * a.C + ch) * n4 + k];
-      else if (MODE < 2 && a.state != nullptr)
-        hv = a.state[s * a.state_seq + ch * a.N + k];
+    for (int n = 0; n < NH; n += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(pa + j * NS + 2 * n);
+      float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (h0 != nullptr) w = *reinterpret_cast<const float4*>(h0 + j * NS + 2 * n);
+      A[n] = mul2(make_float2(v.x, v.y), both(LOG2E)), A[n + 1] = mul2(make_float2(v.z, v.w), both(LOG2E));
+      h[n] = make_float2(w.x, w.y), h[n + 1] = make_float2(w.z, w.w);
     }
-    (n & 1 ? A[n / 2].y : A[n / 2].x) = av;
-    (n & 1 ? h[n / 2].y : h[n / 2].x) = hv;
+  } else {
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const int k = j * NS + n;
+      (n & 1 ? A[n / 2].y : A[n / 2].x) = k < a.N ? pa[k] * LOG2E : 0.f;
+      (n & 1 ? h[n / 2].y : h[n / 2].x) = k < a.N && h0 != nullptr ? h0[k] : 0.f;
+    }
   }
   const bool gate = a.z.p != nullptr && MODE != 2;
-  const T *px = row<T>(a.x, s, first) + ch, *pd = row<T>(a.dt, s, first) + ch;
-  const T *pz = gate ? row<T>(a.z, s, first) + ch : nullptr, *pg = BACK ? row<T>(a.gy, s, first) + ch : nullptr;
+  const T *px = row<T>(BACK ? a.gy : a.x, s, first) + ch, *pd = row<T>(a.dt, s, first) + ch;
+  const T* pz = gate ? row<T>(a.z, s, first) + ch : nullptr;
   T* py = MODE < 2 ? row_out<T>(a.y, s, first) + ch : nullptr;
   const T *pb = row<T>(a.b, s, first), *pc = row<T>(a.c, s, first);
   const uint8_t* rs = resets(a.reset, s);
   if (rs != nullptr) rs += first * a.reset.step;
   int64_t left = t1 - t0;
-  T x[TC], dt[TC], z[TC], g[TC], bcr[BCL];
-  auto load = [&](int i) {
-    if (!BACK) x[i] = *px;
-    dt[i] = *pd;
-    if (gate) z[i] = *pz;
-    if (BACK) g[i] = *pg;
-  };
-  auto next = [&] {
-    if (!BACK) px += DIR * a.x.step;
-    pd += DIR * a.dt.step;
-    if (gate) pz += DIR * a.z.step;
-    if (BACK) pg += DIR * a.gy.step;
-  };
-  auto load_bc = [&](int steps) {
+  uint32_t x[TC], dt[TC], z[TC], bcr[BCL], flag = 0;      // the next chunk's inputs; BACK: x is gy
+  auto load = [&](int steps) {
+#pragma unroll
+    for (int i = 0; i < TC; ++i) {
+      if (i < steps) {
+        x[i] = ld_raw(px);
+        dt[i] = ld_raw(pd);
+        if (gate) z[i] = ld_raw(pz);
+      }
+      px += DIR * (BACK ? a.gy.step : a.x.step);
+      pd += DIR * a.dt.step;
+      if (gate) pz += DIR * a.z.step;
+    }
 #pragma unroll
     for (int i = 0; i < BCL; ++i) {
       const int k = i * 32 + lane, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
-      bcr[i] = from_f<T>(0.f);
+      bcr[i] = 0;
       if (n < a.N && tt < steps && which < 2 && !(MODE == 2 && which == 1) && !(BACK && which == 0))
-        bcr[i] = which ? pc[DIR * tt * a.c.step + n] : pb[DIR * tt * a.b.step + n];
+        bcr[i] = ld_raw(which ? pc + (DIR * tt * a.c.step + n) : pb + (DIR * tt * a.b.step + n));
     }
     pb += DIR * TC * a.b.step;
     pc += DIR * TC * a.c.step;
-  };
-  auto store_bc = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < BCL; ++i) {
-      const int k = i * 32 + lane, which = k / (TC * NP), r = k % (TC * NP);
-      if (which < 2) bc[warp][buf][r / NP][which][r % NP] = to_f(bcr[i]);
-    }
+    flag = reset_flag(rs, DIR * a.reset.step, steps, lane);
+    if (rs != nullptr) rs += DIR * TC * a.reset.step;
   };
 #pragma unroll
-  for (int i = 0; i < TC; ++i) {
-    x[i] = dt[i] = z[i] = g[i] = from_f<T>(0.f);
-    if (i < left) load(i);
-    next();
-  }
-  load_bc(left < TC ? (int)left : TC);
-  store_bc(0);
-  uint32_t bits = reset_bits(rs, DIR * a.reset.step, left, lane);
+  for (int i = 0; i < TC; ++i) x[i] = dt[i] = z[i] = 0;
+  load(left < TC ? (int)left : TC);
   float* kept = MODE == 1 ? a.kept + ((s * ((a.T + TC - 1) / TC - 1) + t0 / TC - 1) * a.C + ch) * n4 + j * NS : nullptr;
-  __syncwarp();
-  for (int buf = 0; left > 0; left -= TC, buf ^= 1) {
+  for (; left > 0; left -= TC) {
     if (MODE == 1) {
       if (on && (part > 0 || left < t1 - t0)) {
 #pragma unroll
@@ -108,39 +102,46 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
           if (j * NS + n < n4)
             *reinterpret_cast<float4*>(kept + n) = make_float4(h[n / 2].x, h[n / 2].y, h[n / 2 + 1].x, h[n / 2 + 1].y);
       }
-      kept += a.C * n4;
+      kept += (int64_t)a.C * n4;
     }
     const int steps = left < TC ? (int)left : TC, ahead = left - TC < TC ? (int)(left - TC) : TC;      // now, and of the next chunk
-    if (ahead > 0) load_bc(ahead);
-    uint32_t later = 0;
-    if (rs != nullptr && ahead > 0) {
-      rs += DIR * TC * a.reset.step;
-      later = reset_bits(rs, DIR * a.reset.step, ahead, lane);
-    }
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < TC; ++i) {
-      if (i >= steps) break;
-      const float xv = to_f(x[i]), zv = to_f(z[i]), gv = to_f(g[i]);
       float slope;
-      const float delta = softplus(to_f(dt[i]) + bias, slope);
-      if (i < ahead) load(i);
-      next();
+      const float xv = raw_f<T>(x[i]), delta = softplus(raw_f<T>(dt[i]) + bias, slope);
+      float o = 1.f;
+      if (gate) {
+        const float zv = raw_f<T>(z[i]);
+        o = zv * sigmoid(zv);
+      }
+      // BACK: u is g, whose c (in place of b) it multiplies
+      stage[warp][i][lane] = make_float4(delta, BACK ? xv * o : delta * xv, o, d * xv);
+    }
+#pragma unroll
+    for (int i = 0; i < BCL; ++i) {
+      const int k = i * 32 + lane, which = k / (TC * NP), r = k % (TC * NP);
+      if (which < 2) bc[warp][r / NP][which][r % NP] = raw_f<T>(bcr[i]);
+    }
+    const uint32_t bits = __ballot_sync(0xFFFFFFFFu, flag != 0);
+    if (ahead > 0) load(ahead);
+    __syncwarp();
+#pragma unroll 2
+    for (int i = 0; i < steps; ++i) {
+      const float4 in = stage[warp][i][lane];
+      const float2 D = both(in.x), U = both(in.y);
       const bool cut = bits >> i & 1;
-      fresh |= cut;
-      dsum += delta;
+      if (MODE >= 2) fresh |= cut, dsum += in.x;
       if (!BACK && cut) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
       }
-      // BACK: u is g, whose c (in place of b) it multiplies
-      const float u = BACK ? (gate ? gv * (zv * sigmoid(zv)) : gv) : delta * xv;
-      const float2 D = both(delta), U = both(u);
       float2 y = make_float2(0.f, 0.f);
 #pragma unroll
       for (int n = 0; n < NH; n += 2) {
-        const float4 q = *reinterpret_cast<const float4*>(&bc[warp][buf][i][BACK ? 1 : 0][j * NS + 2 * n]);
+        const float4 q = *reinterpret_cast<const float4*>(&bc[warp][i][BACK ? 1 : 0][j * NS + 2 * n]);
         float4 c = {};
-        if (MODE < 2) c = *reinterpret_cast<const float4*>(&bc[warp][buf][i][1][j * NS + 2 * n]);
+        if (MODE < 2) c = *reinterpret_cast<const float4*>(&bc[warp][i][1][j * NS + 2 * n]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float2 v = mul2(D, A[n + k]), b = k ? make_float2(q.z, q.w) : make_float2(q.x, q.y);
@@ -160,15 +161,11 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
         float o = y.x + y.y;
 #pragma unroll
         for (int m = 1; m < LN; m *= 2) o += __shfl_xor_sync(0xFFFFFFFFu, o, m);
-        o = fmaf(d, xv, o);
-        if (gate) o *= zv * sigmoid(zv);
+        o = (o + in.w) * in.z;
         if (on && j == 0) *py = from_f<T>(o);
         py += a.y.step;
       }
     }
-    if (ahead > 0) store_bc(buf ^ 1);
-    bits = later;
-    __syncwarp();
   }
   if (!on) return;
 #pragma unroll
@@ -217,88 +214,81 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 }
 
 // One step: bound by the states' bytes.  A thread holds V x G states of one channel (V moved by one access; `lanes` threads a
-// channel, a power of two) and walks over sequences, so a, d and dt_bias are read once.  The next sequence's values are on
-// their way while one is worked on.
-constexpr int STEP_THREADS = 256;
+// channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.
+constexpr int STEP_THREADS = 256, STEP_B = 4;
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(STEP_THREADS) scan_step_kernel(InbScanArgs a, int lanes, int per, bool vec) {
+__global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs a, int lanes, int per, bool vec) {
   const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
-  const int64_t c0 = (int64_t)blockIdx.x * chans + threadIdx.x / lanes;
+  const int c0 = blockIdx.x * chans + threadIdx.x / lanes;
   const bool on = c0 < a.C;
-  const int64_t ch = on ? c0 : a.C - 1;
-  int64_t s = (int64_t)blockIdx.y * per;
-  const int64_t s1 = s + per < a.S ? s + per : a.S;
+  const int ch = on ? c0 : a.C - 1;
+  const int64_t s0 = (int64_t)blockIdx.y * per, s1 = s0 + per < a.S ? s0 + per : a.S;
   const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = a.d != nullptr ? a.d[ch] : 0.f;
   const bool gate = a.z.p != nullptr;
   float A[G][V];
-  int at[G];                     // this thread's states
+  int at[G];                     // this thread's states; those beyond the last one are read as the last ones and not written
 #pragma unroll
   for (int q = 0; q < G; ++q) {
     at[q] = (q * lanes + j) * V;
 #pragma unroll
     for (int k = 0; k < V; ++k) A[q][k] = at[q] < a.N ? a.a[ch * a.N + at[q] + k] * LOG2E : 0.f;
   }
-  struct In {
-    T x, dt, z;
-    Pack<T, V> b[G], c[G];
-    Pack<float, V> h[G];
-    bool cut;
-  };
-  const T *px = row<T>(a.x, s, 0) + ch, *pd = row<T>(a.dt, s, 0) + ch, *pz = gate ? row<T>(a.z, s, 0) + ch : nullptr;
-  const T *pb = row<T>(a.b, s, 0), *pc = row<T>(a.c, s, 0);
-  const float* ph = a.state != nullptr ? a.state + s * a.state_seq + ch * a.N : nullptr;
-  float* po = a.state_out != nullptr ? a.state_out + s * a.state_out_seq + ch * a.N : nullptr;
-  T* py = row_out<T>(a.y, s, 0) + ch;
-  const uint8_t* rs = a.reset.p;
-  const uint32_t rows = a.reset.rows < INB_MAX_MEMORY_S ? (uint32_t)a.reset.rows : INB_MAX_MEMORY_S;
-  auto load = [&](In& i, int64_t at_s) {
-    i.x = *px, i.dt = *pd;
-    if (gate) i.z = *pz;
-    i.cut = rs != nullptr && rs[(uint32_t)at_s / rows * a.reset.seq] != 0;
+  for (int64_t s = s0; s < s1; s += STEP_B) {
+    const int n = s1 - s < STEP_B ? (int)(s1 - s) : STEP_B;
+    uint32_t x[STEP_B], dt[STEP_B], z[STEP_B], cut[STEP_B];
+    Pack<T, V> b[STEP_B][G], c[STEP_B][G];
+    Pack<float, V> h[STEP_B][G];
+    const T *px = row<T>(a.x, s, 0) + ch, *pd = row<T>(a.dt, s, 0) + ch, *pz = gate ? row<T>(a.z, s, 0) + ch : nullptr;
+    const T *pb = row<T>(a.b, s, 0), *pc = row<T>(a.c, s, 0);
+    const float* ph = a.state != nullptr ? a.state + s * a.state_seq + ch * a.N : nullptr;
 #pragma unroll
-    for (int q = 0; q < G; ++q)
-      if (at[q] < a.N) {
-        if (ph != nullptr) i.h[q] = ld<float, V>(ph + at[q]);
+    for (int u = 0; u < STEP_B; ++u) {
+      // the sequences beyond the last one read it again
+      x[u] = ld_raw(px), dt[u] = ld_raw(pd);
+      if (gate) z[u] = ld_raw(pz);
+      cut[u] = a.reset.p != nullptr ? *resets(a.reset, s + (u < n ? u : n - 1)) : 0;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        const int k0 = at[q] < a.N ? at[q] : a.N - V;
+        if (ph != nullptr) h[u][q] = ld<float, V>(ph + k0);
         if (vec) {
-          i.b[q] = ld<T, V>(pb + at[q]), i.c[q] = ld<T, V>(pc + at[q]);
+          b[u][q] = ld<T, V>(pb + k0), c[u][q] = ld<T, V>(pc + k0);
         } else {
 #pragma unroll
-          for (int k = 0; k < V; ++k) i.b[q].v[k] = pb[at[q] + k], i.c[q].v[k] = pc[at[q] + k];
+          for (int k = 0; k < V; ++k) b[u][q].v[k] = pb[k0 + k], c[u][q].v[k] = pc[k0 + k];
         }
       }
-    px += a.x.seq, pd += a.dt.seq, pb += a.b.seq, pc += a.c.seq;
-    if (gate) pz += a.z.seq;
-    if (ph != nullptr) ph += a.state_seq;
-  };
-  In now, then;
-  load(now, s);
-  for (; s < s1; ++s) {
-    if (s + 1 < s1) load(then, s + 1);
-    const float x = to_f(now.x);
-    float slope, y = 0.f;
-    const float delta = softplus(to_f(now.dt) + bias, slope), u = delta * x;
-#pragma unroll
-    for (int q = 0; q < G; ++q) {
-      if (at[q] >= a.N) continue;
-      Pack<float, V> h;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float old = ph == nullptr || now.cut ? 0.f : now.h[q].v[k];
-        h.v[k] = fmaf(ex2(delta * A[q][k]), old, u * to_f(now.b[q].v[k]));
-        y = fmaf(h.v[k], to_f(now.c[q].v[k]), y);
+      if (u + 1 < n) {
+        px += a.x.seq, pd += a.dt.seq, pb += a.b.seq, pc += a.c.seq;
+        if (gate) pz += a.z.seq;
+        if (ph != nullptr) ph += a.state_seq;
       }
-      if (po != nullptr && on) st<float, V>(po + at[q], h);
     }
-    for (int o = 1; o < lanes; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-    y = fmaf(d, x, y);
-    if (gate) {
-      const float z = to_f(now.z);
-      y *= z * sigmoid(z);
+#pragma unroll
+    for (int u = 0; u < STEP_B; ++u) {
+      if (u >= n) break;
+      const float xv = raw_f<T>(x[u]);
+      float slope, y = 0.f;
+      const float delta = softplus(raw_f<T>(dt[u]) + bias, slope), in = delta * xv;
+      const bool none = ph == nullptr || cut[u] != 0;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        Pack<float, V> o;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          o.v[k] = fmaf(ex2(delta * A[q][k]), none ? 0.f : h[u][q].v[k], in * to_f(b[u][q].v[k]));
+          if (at[q] < a.N) y = fmaf(o.v[k], to_f(c[u][q].v[k]), y);
+        }
+        if (a.state_out != nullptr && on && at[q] < a.N) st<float, V>(a.state_out + (s + u) * a.state_out_seq + ch * a.N + at[q], o);
+      }
+      for (int o = 1; o < lanes; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
+      y = fmaf(d, xv, y);
+      if (gate) {
+        const float zv = raw_f<T>(z[u]);
+        y *= zv * sigmoid(zv);
+      }
+      if (on && j == 0) row_out<T>(a.y, s + u, 0)[ch] = from_f<T>(y);
     }
-    if (on && j == 0) *py = from_f<T>(y);
-    py += a.y.seq;
-    if (po != nullptr) po += a.state_out_seq;
-    now = then;
   }
 }
 
@@ -316,8 +306,8 @@ int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool revers
 
 template <typename T, int NS, int LN, int MODE>
 static void scan_go(const InbScanArgs& a, const ScanPlan& p, float* carry, cudaStream_t s) {
-  const int64_t tasks = a.S * p.parts * ceil_div(a.C, 32 / LN);
-  scan_kernel<T, NS, LN, MODE><<<(unsigned)ceil_div(tasks, SCAN_WARPS), SCAN_WARPS * 32, 0, s>>>(a, p, carry, tasks);
+  const int64_t tiles = ceil_div(a.C, 32 / LN), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
+  scan_kernel<T, NS, LN, MODE><<<dim3((unsigned)(a.S * p.parts), (unsigned)ceil_div(tiles, warps)), (unsigned)warps * 32, 0, s>>>(a, p, carry);
 }
 template <typename T, int NS, int LN>
 static int scan_mode(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s) {
@@ -347,9 +337,10 @@ static int scan_type(const InbScanArgs& a, const ScanPlan& p, float* carry, int 
 template <typename T, int V, int G>
 static int step_go(const InbScanArgs& a, int lanes, cudaStream_t s) {
   const int64_t tiles = ceil_div(a.C, STEP_THREADS / lanes);
-  // as many sequences a block as leave eight blocks an SM, no more than 16, and a grid's second axis ends at 65535
-  int64_t per = a.S * tiles / (sm_count() * 8);
-  if (per > 16) per = 16;
+  // as many sequences a block as leave six blocks an SM, no more than 32, and a grid's second axis ends at 65535
+  int64_t per = a.S * tiles / (sm_count() * 6);
+  if (per > 32) per = 32;
+  if (per > STEP_B) per = per / STEP_B * STEP_B;
   if (per < ceil_div(a.S, 65535)) per = ceil_div(a.S, 65535);
   if (per < 1) per = 1;
   const bool vec = is_aligned(a.b, V * sizeof(T), sizeof(T)) && is_aligned(a.c, V * sizeof(T), sizeof(T));

@@ -39,10 +39,9 @@ int scan_check(const InbScanArgs& a);
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s);
 int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool reverse, cudaStream_t s);
 
-// The reset flags of the next `left` (of them up to SCAN_STEPS) steps as bits, the same in every lane; `at`: the first one's
-__device__ __forceinline__ uint32_t reset_bits(const uint8_t* at, int64_t step, int64_t left, int lane) {
-  if (at == nullptr) return 0;
-  return __ballot_sync(0xFFFFFFFFu, lane < SCAN_STEPS && lane < left && at[lane * step] != 0);
+// The reset flag of this lane's step among the next `steps` (lanes beyond: 0); a ballot makes them the same bits in every lane
+__device__ __forceinline__ uint32_t reset_flag(const uint8_t* at, int64_t step, int steps, int lane) {
+  return at != nullptr && lane < steps ? at[lane * step] : 0u;
 }
 
 }  // namespace pol

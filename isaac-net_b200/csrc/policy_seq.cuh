@@ -42,7 +42,7 @@ __device__ __forceinline__ float2 ex2_poly(float2 v) {
   v = make_float2(hold(v.x), hold(v.y));
   const float2 magic = both(12582912.f + 127.f);      // 1.5 * 2^23: the sum's low bits are i + 127
   const float2 r = add2(v, magic);
-  const float2 f = add2(v, mul2(add2(r, both(-12582912.f - 127.f)), both(-1.f)));
+  const float2 f = fma2(add2(r, both(-12582912.f - 127.f)), both(-1.f), v);
   float2 p = fma2(both(0.00015453163359779865f), f, both(0.0013390863314270973f));
   p = fma2(p, f, both(0.009618083015084267f));
   p = fma2(p, f, both(0.055503569543361664f));
@@ -69,6 +69,24 @@ __device__ __forceinline__ float softplus(float v, float& s) {
   const float i = rcp(1.f + u);
   s = v >= 0.f ? i : u * i;
   return fmaf(2.f * r, p, fmaxf(v, 0.f));
+}
+
+// An element as it lies in memory, in a register of its own: loads that stay on their way must not be packed with others
+template <typename T>
+__device__ __forceinline__ uint32_t ld_raw(const T* p) {
+  if constexpr (sizeof(T) == 2)
+    return *reinterpret_cast<const uint16_t*>(p);
+  else
+    return *reinterpret_cast<const uint32_t*>(p);
+}
+template <typename T>
+__device__ __forceinline__ float raw_f(uint32_t v) {
+  if constexpr (IsBf16<T>::value)
+    return __uint_as_float(v << 16);
+  else if constexpr (sizeof(T) == 2)
+    return __half2float(__ushort_as_half((uint16_t)v));
+  else
+    return __uint_as_float(v);
 }
 
 template <typename T>
