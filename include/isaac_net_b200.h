@@ -529,7 +529,7 @@ typedef struct {
  * (contiguous, or NULL), gw, gbias (or NULL).  work: inb_causal_conv_work() floats of the backward call.
  * -2: sizes out of range; -3: a required pointer is NULL; -5: work is too small. */
 #define INB_MAX_MEMORY_C (1 << 20) /* channels of inb_causal_conv_* and inb_selective_scan_* */
-#define INB_MAX_MEMORY_S 0x7FFFFFFF /* sequences, steps */
+#define INB_MAX_MEMORY_S 0x3FFFFFFF /* sequences, steps */
 typedef struct {
   int32_t dtype, act, C, K;
   int64_t S, T;

@@ -184,7 +184,7 @@ class InbSampleArgs(ctypes.Structure):
 
 POLICY_EXPORTS = {"inb_block_norm_fwd": InbNormArgs, "inb_block_norm_bwd": InbNormArgs, "inb_dropout": InbDropoutArgs,
                   "inb_sample": InbSampleArgs, "inb_gated_ffn_fwd": InbFfnArgs, "inb_gated_ffn_bwd": InbFfnArgs}    # int f(const Args *, void *stream)
-MAX_MEMORY_C, MAX_MEMORY_S, MAX_SCAN_N, MAX_DISTILL_K = 1 << 20, 0x7FFFFFFF, 64, 1024
+MAX_MEMORY_C, MAX_MEMORY_S, MAX_SCAN_N, MAX_DISTILL_K = 1 << 20, 0x3FFFFFFF, 64, 1024
 
 
 class InbSeq(ctypes.Structure):

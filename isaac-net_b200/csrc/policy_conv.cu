@@ -12,114 +12,145 @@ namespace inb {
 namespace pol {
 
 constexpr int CONV_U = 4;       // steps whose loads are sent at once, while the steps before are worked on
+constexpr int CONV_FWD_BLOCKS = 6, CONV_STEP_BLOCKS = 6, CONV_BWD_BLOCKS = 4;      // of 128 threads, an SM
 constexpr int CONV_STEP_B = 4;  // sequences whose loads are sent at once by a single step
 
 struct ConvPlan {
   int64_t parts, len, tasks;    // parts of the time axis, their steps; sequences x parts
 };
 
-// V channels of the weights, [K] taps each
+// V neighbouring channels as pairs (V = 1: the first of one pair)
 template <typename T, int V, int K>
 struct Taps {
-  float w[K][V], bias[V];
-  __device__ void load(const InbConvArgs& a, int64_t ch, bool on) {
+  static constexpr int P = Words<T, V>::P;
+  float2 w[K][P], bias[P];
+  __device__ __forceinline__ void load(const InbConvArgs& a, int64_t ch, bool on) {
+    auto get = [&](const void* p, int64_t i) { return on && p != nullptr ? to_f(((const T*)p)[i]) : 0.f; };
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      bias[v] = on && a.bias != nullptr ? to_f(((const T*)a.bias)[ch + v]) : 0.f;
+    for (int i = 0; i < P; ++i) {
+      const int64_t c = ch + 2 * i;
+      bias[i] = make_float2(get(a.bias, c), V > 1 ? get(a.bias, c + 1) : 0.f);
 #pragma unroll
-      for (int k = 0; k < K; ++k) w[k][v] = on ? to_f(((const T*)a.w)[(ch + v) * K + k]) : 0.f;
+      for (int k = 0; k < K; ++k) w[k][i] = make_float2(get(a.w, c * K + k), V > 1 ? get(a.w, (c + 1) * K + k) : 0.f);
     }
   }
 };
 // The last K - 1 inputs; x[j]: j + 1 steps back
 template <typename T, int V, int K>
 struct Window {
-  float x[K - 1][V];
-  __device__ void zero() {
+  static constexpr int P = Words<T, V>::P;
+  float2 x[K - 1][P];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[j][v] = 0.f;
+      for (int i = 0; i < P; ++i) x[j][i] = make_float2(0.f, 0.f);
   }
-  __device__ void push(const Pack<T, V>& p) {
+  __device__ __forceinline__ void push(const float2 (&v)[P]) {
 #pragma unroll
     for (int j = K - 2; j > 0; --j)
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[j][v] = x[j - 1][v];
+      for (int i = 0; i < P; ++i) x[j][i] = x[j - 1][i];
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[0][v] = to_f(p.v[v]);
+    for (int i = 0; i < P; ++i) x[0][i] = v[i];
   }
-  __device__ float pre(const Taps<T, V, K>& t, float now, int v) const {
-    float p = fmaf(now, t.w[K - 1][v], t.bias[v]);
+  __device__ __forceinline__ void push(const T* p) {
+    Words<T, V> q;
+    q.load(p);
+    float2 v[P];
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) p = fmaf(x[j][v], t.w[K - 2 - j][v], p);
+    for (int i = 0; i < P; ++i) v[i] = q.pair(i);
+    push(v);
+  }
+  __device__ __forceinline__ float2 pre(const Taps<T, V, K>& t, float2 now, int i) const {
+    float2 p = fma2(now, t.w[K - 1][i], t.bias[i]);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) p = fma2(x[j][i], t.w[K - 2 - j][i], p);
     return p;
   }
 };
+template <int V>
+__device__ __forceinline__ float2 silu2(float2 p) {
+  return make_float2(p.x * sigmoid(p.x), V > 1 ? p.y * sigmoid(p.y) : 0.f);
+}
+__device__ __forceinline__ float silu_slope(float p) {
+  const float q = sigmoid(p);
+  return q * fmaf(p, 1.f - q, 1.f);
+}
 
 // ---------------------------------------------------------------------------------------------- forward
 // A block is blockDim.x channel vectors x blockDim.y tasks and strides over the tasks, so that weights are read once.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(128, 6) conv_fwd_kernel(InbConvArgs a, ConvPlan pl) {
+__global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvArgs a, ConvPlan pl) {
+  constexpr int P = Words<T, V>::P;
   const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   if (ch >= a.C) return;
   Taps<T, V, K> taps;
   taps.load(a, ch, true);
   for (int64_t task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; task < pl.tasks; task += (int64_t)gridDim.x * blockDim.y) {
     const int64_t part = pl.parts > 1 ? task / a.S : 0, s = task - part * a.S;      // the next task: the same steps of the next sequence
-    const int64_t t0 = part * pl.len, t1 = t0 + pl.len < a.T ? t0 + pl.len : a.T;
+    const int64_t t0 = part * pl.len;
+    const int n = (int)(t0 + pl.len < a.T ? pl.len : a.T - t0);
     const uint8_t* rs = resets(a.reset, s);
+    const uint8_t* pr = rs != nullptr ? rs + t0 * a.reset.step : nullptr;
     const T* px = row<T>(a.x, s, t0) + ch;
     T* py = row_out<T>(a.y, s, t0) + ch;
-    Pack<T, V> x[CONV_U], nx[CONV_U];
-    uint32_t reset[CONV_U], nr[CONV_U];
-    // loads have no condition: the steps beyond the part's end read its last one again
-    auto load = [&](Pack<T, V>(&to)[CONV_U], uint32_t(&flag)[CONV_U], int64_t t) {
+    Words<T, V> x[CONV_U], nx[CONV_U];
+    uint32_t reset[CONV_U] = {}, nr[CONV_U] = {};
+    auto load = [&](Words<T, V>(&to)[CONV_U], uint32_t(&flag)[CONV_U], int left) {
 #pragma unroll
       for (int u = 0; u < CONV_U; ++u) {
-        to[u] = ld<T, V>(px);
-        flag[u] = rs != nullptr ? rs[(t + u < t1 ? t + u : t1 - 1) * a.reset.step] : 0;
-        if (t + u + 1 < t1) px += a.x.step;
+        if (u < left) to[u].load(px);
+        px += a.x.step;
+      }
+      if (rs != nullptr) {
+#pragma unroll
+        for (int u = 0; u < CONV_U; ++u) {
+          if (u < left) flag[u] = *pr;
+          pr += a.reset.step;
+        }
       }
     };
-    load(x, reset, t0);
+    load(x, reset, n);
     Window<T, V, K> win;
     win.zero();
     for (int64_t t = t0 - (K - 1); t < t0; ++t) {
       if (t >= 0) {
         if (rs != nullptr && rs[t * a.reset.step]) win.zero();
-        win.push(ld<T, V>(row<T>(a.x, s, t) + ch));
+        win.push(row<T>(a.x, s, t) + ch);
       } else if (a.state != nullptr) {
-        win.push(ld<T, V>((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch));
+        win.push((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch);
       }
     }
-    for (int64_t t = t0; t < t1; t += CONV_U) {
-      if (t + CONV_U < t1) load(nx, nr, t + CONV_U);
+    for (int left = n; left > 0; left -= CONV_U) {
+      if (left > CONV_U) load(nx, nr, left - CONV_U);
 #pragma unroll
       for (int u = 0; u < CONV_U; ++u) {
-        if (t + u >= t1) break;
+        if (u >= left) break;
         if (reset[u]) win.zero();
-        Pack<T, V> y;
+        Words<T, V> y;
+        float2 now[P];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float p = win.pre(taps, to_f(x[u].v[v]), v);
-          y.v[v] = from_f<T>(a.act == INB_ACT_SILU ? p * sigmoid(p) : p);
+        for (int i = 0; i < P; ++i) {
+          now[i] = x[u].pair(i);
+          const float2 p = win.pre(taps, now[i], i);
+          y.set(i, a.act == INB_ACT_SILU ? silu2<V>(p) : p);
         }
-        win.push(x[u]);
-        st<T, V>(py, y);
+        win.push(now);
+        y.store(py);
         py += a.y.step;
       }
 #pragma unroll
       for (int u = 0; u < CONV_U; ++u) x[u] = nx[u], reset[u] = nr[u];
     }
-    if (t1 == a.T && a.state_out != nullptr) {
+    if (t0 + n == a.T && a.state_out != nullptr) {
       T* out = (T*)a.state_out + s * a.state_out_seq + ch;
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
-        Pack<T, V> p;
+        Words<T, V> p;
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.v[v] = from_f<T>(win.x[j][v]);      // what was read, or 0: exact
-        st<T, V>(out + (K - 2 - j) * a.C, p);
+        for (int i = 0; i < P; ++i) p.set(i, win.x[j][i]);      // what was read, or 0: exact
+        p.store(out + (K - 2 - j) * a.C);
       }
     }
   }
@@ -127,24 +158,27 @@ __global__ void __launch_bounds__(128, 6) conv_fwd_kernel(InbConvArgs a, ConvPla
 
 // One step: bound by the states' bytes, of which a thread has CONV_STEP_B sequences' on their way at once; state_out may be state.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(128, 6) conv_step_kernel(InbConvArgs a) {
+__global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbConvArgs a) {
+  constexpr int P = Words<T, V>::P;
   const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   if (ch >= a.C) return;
   Taps<T, V, K> taps;
   taps.load(a, ch, true);
   const int64_t stride = (int64_t)gridDim.x * blockDim.y;
   for (int64_t s0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; s0 < a.S; s0 += stride * CONV_STEP_B) {
-    Pack<T, V> x[CONV_STEP_B], old[CONV_STEP_B][K - 1];
+    Words<T, V> x[CONV_STEP_B], old[CONV_STEP_B][K - 1];
     uint32_t reset[CONV_STEP_B];
 #pragma unroll
     for (int b = 0; b < CONV_STEP_B; ++b) {
       const int64_t s = s0 + b * stride;
       if (s >= a.S) break;
-      x[b] = ld<T, V>(row<T>(a.x, s, 0) + ch);
+      x[b].load(row<T>(a.x, s, 0) + ch);
       reset[b] = a.reset.p != nullptr ? *resets(a.reset, s) : 0;
+      if (a.state != nullptr) {
+        const T* p = (const T*)a.state + s * a.state_seq + ch;
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j)
-        if (a.state != nullptr) old[b][j] = ld<T, V>((const T*)a.state + s * a.state_seq + j * a.C + ch);
+        for (int j = 0; j < K - 1; ++j) old[b][j].load(p + j * a.C);
+      }
     }
 #pragma unroll
     for (int b = 0; b < CONV_STEP_B; ++b) {
@@ -154,22 +188,22 @@ __global__ void __launch_bounds__(128, 6) conv_step_kernel(InbConvArgs a) {
 #pragma unroll
         for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-          for (int v = 0; v < V; ++v) old[b][j].v[v] = from_f<T>(0.f);
+          for (int i = 0; i < Words<T, V>::N; ++i) old[b][j].w[i] = 0;
       }
-      Pack<T, V> y;
+      Words<T, V> y;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float p = fmaf(to_f(x[b].v[v]), taps.w[K - 1][v], taps.bias[v]);
+      for (int i = 0; i < P; ++i) {
+        float2 p = fma2(x[b].pair(i), taps.w[K - 1][i], taps.bias[i]);
 #pragma unroll
-        for (int j = K - 2; j >= 0; --j) p = fmaf(to_f(old[b][j].v[v]), taps.w[j][v], p);
-        y.v[v] = from_f<T>(a.act == INB_ACT_SILU ? p * sigmoid(p) : p);
+        for (int j = K - 2; j >= 0; --j) p = fma2(old[b][j].pair(i), taps.w[j][i], p);
+        y.set(i, a.act == INB_ACT_SILU ? silu2<V>(p) : p);
       }
-      st<T, V>(row_out<T>(a.y, s, 0) + ch, y);
+      y.store(row_out<T>(a.y, s, 0) + ch);
       if (a.state_out != nullptr) {
         T* out = (T*)a.state_out + s * a.state_out_seq + ch;
 #pragma unroll
-        for (int j = 0; j < K - 2; ++j) st<T, V>(out + j * a.C, old[b][j + 1]);
-        st<T, V>(out + (K - 2) * a.C, x[b]);
+        for (int j = 0; j < K - 2; ++j) old[b][j + 1].store(out + j * a.C);
+        x[b].store(out + (K - 2) * a.C);
       }
     }
   }
@@ -180,130 +214,141 @@ __global__ void __launch_bounds__(128, 6) conv_step_kernel(InbConvArgs a) {
 // beyond its end, for gx alone.  Blocks as in the forward pass, so that gw and gbias stay in registers; one partial row a
 // block, [C K | C], added by a second launch.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(128, 3) conv_bwd_kernel(InbConvArgs a, ConvPlan pl) {
+__global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvArgs a, ConvPlan pl) {
+  constexpr int P = Words<T, V>::P;
   extern __shared__ float smem[];
   const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool on = ch < a.C;
   Taps<T, V, K> taps;
   taps.load(a, ch, on);
-  float gw[K][V], gb[V];
+  const float2 zero = make_float2(0.f, 0.f);
+  float2 gw[K][P], gb[P];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    gb[v] = 0.f;
+  for (int i = 0; i < P; ++i) {
+    gb[i] = zero;
 #pragma unroll
-    for (int k = 0; k < K; ++k) gw[k][v] = 0.f;
+    for (int k = 0; k < K; ++k) gw[k][i] = zero;
   }
   if (on)
     for (int64_t task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; task < pl.tasks; task += (int64_t)gridDim.x * blockDim.y) {
       const int64_t part = pl.parts > 1 ? task / a.S : 0, s = task - part * a.S;
-      const int64_t t0 = part * pl.len, t1 = t0 + pl.len < a.T ? t0 + pl.len : a.T;
-      const int64_t last = t1 + K - 1, end = last < a.T ? last : a.T;
+      const int64_t t0 = part * pl.len;
+      const int n = (int)(t0 + pl.len < a.T ? pl.len : a.T - t0);                 // the part's steps,
+      const int end = (int)(n + K - 1 < a.T - t0 ? n + K - 1 : a.T - t0);         // and with those that reach back into it
       const uint8_t* rs = resets(a.reset, s);
+      const uint8_t* pr = rs != nullptr ? rs + t0 * a.reset.step : nullptr;
       const T *px = row<T>(a.x, s, t0) + ch, *pg = row<T>(a.gy, s, t0) + ch;
-      Pack<T, V> x[CONV_U], nx[CONV_U], gy[CONV_U], ng[CONV_U];
-      uint32_t reset[CONV_U], nr[CONV_U];
-      auto load = [&](Pack<T, V>(&to)[CONV_U], Pack<T, V>(&tg)[CONV_U], uint32_t(&flag)[CONV_U], int64_t t) {
+      Words<T, V> x[CONV_U], nx[CONV_U], gy[CONV_U], ng[CONV_U];
+      uint32_t reset[CONV_U] = {}, nr[CONV_U] = {};
+      auto load = [&](Words<T, V>(&to)[CONV_U], Words<T, V>(&tg)[CONV_U], uint32_t(&flag)[CONV_U], int left) {
 #pragma unroll
         for (int u = 0; u < CONV_U; ++u) {
-          to[u] = ld<T, V>(px);
-          tg[u] = ld<T, V>(pg);
-          flag[u] = rs != nullptr ? rs[(t + u < end ? t + u : end - 1) * a.reset.step] : 0;
-          if (t + u + 1 < end) px += a.x.step, pg += a.gy.step;
+          if (u < left) to[u].load(px), tg[u].load(pg);
+          px += a.x.step, pg += a.gy.step;
+        }
+        if (rs != nullptr) {
+#pragma unroll
+          for (int u = 0; u < CONV_U; ++u) {
+            if (u < left) flag[u] = *pr;
+            pr += a.reset.step;
+          }
         }
       };
-      load(x, gy, reset, t0);
+      load(x, gy, reset, end);
       Window<T, V, K> win;
-      float pend[K - 1][V];
+      float2 pend[K - 1][P];
       int m = K - 1;                        // how many steps before this one are seen
       win.zero();
 #pragma unroll
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) pend[j][v] = 0.f;
-      auto restart = [&] {
-        m = 0;
-        win.zero();
-      };
-      auto push = [&](const Pack<T, V>& p) {
-        win.push(p);
-        m = m < K - 1 ? m + 1 : m;
-      };
+        for (int i = 0; i < P; ++i) pend[j][i] = zero;
+      for (int64_t t = t0 - (K - 1); t < t0; ++t) {
+        if (t >= 0) {
+          if (rs != nullptr && rs[t * a.reset.step]) {
+            m = 0;
+            win.zero();
+          }
+          win.push(row<T>(a.x, s, t) + ch);
+          m = m < K - 1 ? m + 1 : m;
+        } else if (a.state != nullptr) {
+          win.push((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch);
+        }
+      }
       T* pgx = row_out<T>(a.gx, s, t0) + ch;
-      // gx of step t - (K - 1) is complete; before the sequence it is the initial state's
-      auto emit = [&](int64_t t) {
-        const int64_t at = t - (K - 1);
-        Pack<T, V> p;
+      // step i of the part completes gx of step i - (K - 1); before the sequence it is the initial state's
+      auto emit = [&](int i) {
+        Words<T, V> p;
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.v[v] = from_f<T>(pend[K - 2][v]);
-        if (at >= t0) {
-          st<T, V>(pgx, p);
+        for (int q = 0; q < P; ++q) p.set(q, pend[K - 2][q]);
+        const int at = i - (K - 1);
+        if (at >= 0) {
+          p.store(pgx);
           pgx += a.gx.step;
-        } else if (at < 0 && a.gstate != nullptr) {
-          st<T, V>((T*)a.gstate + (s * (K - 1) + at + K - 1) * a.C + ch, p);
+        } else if (t0 == 0 && a.gstate != nullptr) {
+          p.store((T*)a.gstate + (s * (K - 1) + at + K - 1) * a.C + ch);
         }
       };
-      auto shift = [&](const float (&g)[V]) {
+      auto shift = [&](const float2 (&g)[P]) {
 #pragma unroll
         for (int j = K - 2; j > 0; --j)
 #pragma unroll
-          for (int v = 0; v < V; ++v) pend[j][v] = pend[j - 1][v];
+          for (int i = 0; i < P; ++i) pend[j][i] = pend[j - 1][i];
 #pragma unroll
-        for (int v = 0; v < V; ++v) pend[0][v] = taps.w[K - 1][v] * g[v];
+        for (int i = 0; i < P; ++i) pend[0][i] = mul2(taps.w[K - 1][i], g[i]);
       };
-      for (int64_t t = t0 - (K - 1); t < t0; ++t) {
-        if (t >= 0) {
-          if (rs != nullptr && rs[t * a.reset.step]) restart();
-          push(ld<T, V>(row<T>(a.x, s, t) + ch));
-        } else if (a.state != nullptr) {
-          push(ld<T, V>((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch));
-        }
-      }
-      for (int64_t t = t0; t < end; t += CONV_U) {
-        if (t + CONV_U < end) load(nx, ng, nr, t + CONV_U);
+      for (int i0 = 0; i0 < end; i0 += CONV_U) {
+        if (i0 + CONV_U < end) load(nx, ng, nr, end - i0 - CONV_U);
 #pragma unroll
         for (int u = 0; u < CONV_U; ++u) {
-          if (t + u >= end) break;
-          if (reset[u]) restart();
-          const bool mine = t + u < t1;
-          float g[V];
+          if (i0 + u >= end) break;
+          if (reset[u]) {
+            m = 0;
+            win.zero();
+          }
+          float2 g[P], now[P];
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float xv = to_f(x[u].v[v]);
-            g[v] = to_f(gy[u].v[v]);
+          for (int i = 0; i < P; ++i) {
+            now[i] = x[u].pair(i);
+            g[i] = gy[u].pair(i);
             if (a.act == INB_ACT_SILU) {
-              const float p = win.pre(taps, xv, v), q = sigmoid(p);
-              g[v] *= q * fmaf(p, 1.f - q, 1.f);
+              const float2 p = win.pre(taps, now[i], i);
+              g[i] = mul2(g[i], make_float2(silu_slope(p.x), V > 1 ? silu_slope(p.y) : 0.f));
             }
-            if (mine) {
-              gb[v] += g[v];
-              gw[K - 1][v] = fmaf(g[v], xv, gw[K - 1][v]);
+            if (i0 + u < n) {
+              gb[i] = add2(gb[i], g[i]);
+              gw[K - 1][i] = fma2(g[i], now[i], gw[K - 1][i]);
 #pragma unroll
-              for (int j = 0; j < K - 1; ++j) gw[K - 2 - j][v] = fmaf(g[v], win.x[j][v], gw[K - 2 - j][v]);
+              for (int j = 0; j < K - 1; ++j) gw[K - 2 - j][i] = fma2(g[i], win.x[j][i], gw[K - 2 - j][i]);
             }
           }
 #pragma unroll
           for (int j = 0; j < K - 1; ++j)
             if (j < m) {
 #pragma unroll
-              for (int v = 0; v < V; ++v) pend[j][v] = fmaf(taps.w[K - 2 - j][v], g[v], pend[j][v]);
+              for (int i = 0; i < P; ++i) pend[j][i] = fma2(taps.w[K - 2 - j][i], g[i], pend[j][i]);
             }
-          emit(t + u);
+          emit(i0 + u);
           shift(g);
-          push(x[u]);
+          win.push(now);
+          m = m < K - 1 ? m + 1 : m;
         }
 #pragma unroll
         for (int u = 0; u < CONV_U; ++u) x[u] = nx[u], gy[u] = ng[u], reset[u] = nr[u];
       }
-      // steps beyond the sequence: entry i of the final state is the input of step T - (K - 1) + i
-      for (int64_t t = end; t < last; ++t) {
-        const int i = (int)(t - a.T);
-        if (a.gstate_out != nullptr && K - 1 - i <= m) {
-          const Pack<T, V> p = ld<T, V>((const T*)a.gstate_out + (s * (K - 1) + i) * a.C + ch);
+      // steps beyond the sequence: entry e of the final state is the input of step T - (K - 1) + e
+      for (int i = end; i < n + K - 1; ++i) {
+        const int e = (int)(t0 + i - a.T);
+        if (a.gstate_out != nullptr && K - 1 - e <= m) {
+          Words<T, V> p;
+          p.load((const T*)a.gstate_out + (s * (K - 1) + e) * a.C + ch);
 #pragma unroll
-          for (int v = 0; v < V; ++v) pend[K - 2][v] += to_f(p.v[v]);
+          for (int q = 0; q < P; ++q) pend[K - 2][q] = add2(pend[K - 2][q], p.pair(q));
         }
-        emit(t);
-        const float none[V] = {};
+        emit(i);
+        float2 none[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) none[q] = zero;
         shift(none);
       }
     }
@@ -313,8 +358,8 @@ __global__ void __launch_bounds__(128, 3) conv_bwd_kernel(InbConvArgs a, ConvPla
 #pragma unroll
   for (int v = 0; v < V; ++v) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) mine[(threadIdx.x * V + v) * K + k] = gw[k][v];
-    mine[blockDim.x * V * K + threadIdx.x * V + v] = gb[v];
+    for (int k = 0; k < K; ++k) mine[(threadIdx.x * V + v) * K + k] = v & 1 ? gw[k][v / 2].y : gw[k][v / 2].x;
+    mine[blockDim.x * V * K + threadIdx.x * V + v] = v & 1 ? gb[v / 2].y : gb[v / 2].x;
   }
   __syncthreads();
   const int64_t c0 = (int64_t)blockIdx.y * blockDim.x * V;
@@ -370,7 +415,7 @@ static bool conv_aligned(const InbConvArgs& a, int64_t bytes) {
 }
 static int conv_check(const InbConvArgs& a) {
   if (a.dtype < 0 || a.dtype > 2 || (a.act != -1 && a.act != INB_ACT_SILU) || a.C < 1 || a.C > INB_MAX_MEMORY_C || a.K < 2 ||
-      a.K > 4 || a.S < 0 || a.S > INB_MAX_MEMORY_S || a.T < 0 || a.T > INB_MAX_MEMORY_S || (a.reset.p != nullptr && a.reset.rows < 1))
+      a.K > 4 || a.S < 0 || a.S > INB_MAX_MEMORY_S || a.T < 0 || a.T > INB_MAX_MEMORY_S || (a.reset.p != nullptr && (a.reset.rows < 1 || a.reset.rows > INB_MAX_MEMORY_S)))
     return -2;
   return 0;
 }
@@ -378,17 +423,17 @@ static int conv_check(const InbConvArgs& a) {
 template <typename T, int V, int K>
 static int conv_fwd_go(const InbConvArgs& a, cudaStream_t s) {
   if (a.T == 1) {
-    const ConvLaunch l = conv_plan(a, V, 12);      // two rounds: a block's sequences are few
+    const ConvLaunch l = conv_plan(a, V, CONV_STEP_BLOCKS);
     conv_step_kernel<T, V, K><<<l.grid, l.block, 0, s>>>(a);
   } else {
-    const ConvLaunch l = conv_plan(a, V, 6);
+    const ConvLaunch l = conv_plan(a, V, CONV_FWD_BLOCKS);
     conv_fwd_kernel<T, V, K><<<l.grid, l.block, 0, s>>>(a, l.plan);
   }
   return launch_status();
 }
 template <typename T, int V, int K>
 static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
-  const ConvLaunch l = conv_plan(a, V, 3);
+  const ConvLaunch l = conv_plan(a, V, CONV_BWD_BLOCKS);
   conv_bwd_kernel<T, V, K><<<l.grid, l.block, 128 * V * (K + 1) * 4, s>>>(a, l.plan);
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
@@ -428,7 +473,7 @@ extern "C" int inb_causal_conv_work(const InbConvArgs* args, int64_t* elems) {
   *elems = 0;
   if (a.S == 0 || a.T == 0) return 0;
   const bool vec = inb::pol::conv_aligned(a, 4 * inb::pol::elem_size(a.dtype));
-  *elems = (int64_t)inb::pol::conv_plan(a, vec ? 4 : 1, 3).grid.x * a.C * (a.K + 1);
+  *elems = (int64_t)inb::pol::conv_plan(a, vec ? 4 : 1, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
   return 0;
 }
 

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 // channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.
 constexpr int STEP_THREADS = 256, STEP_B = 4;
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs a, int lanes, int per, bool vec) {
+__global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs a, int lanes, int per) {
   const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
   const int c0 = blockIdx.x * chans + threadIdx.x / lanes;
   const bool on = c0 < a.C;
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
   for (int64_t s = s0; s < s1; s += STEP_B) {
     const int n = s1 - s < STEP_B ? (int)(s1 - s) : STEP_B;
     uint32_t x[STEP_B], dt[STEP_B], z[STEP_B], cut[STEP_B];
-    Pack<T, V> b[STEP_B][G], c[STEP_B][G];
+    Words<T, V> b[STEP_B][G], c[STEP_B][G];
     Pack<float, V> h[STEP_B][G];
     const T *px = row<T>(a.x, s, 0) + ch, *pd = row<T>(a.dt, s, 0) + ch, *pz = gate ? row<T>(a.z, s, 0) + ch : nullptr;
     const T *pb = row<T>(a.b, s, 0), *pc = row<T>(a.c, s, 0);
@@ -251,12 +251,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
       for (int q = 0; q < G; ++q) {
         const int k0 = at[q] < a.N ? at[q] : a.N - V;
         if (ph != nullptr) h[u][q] = ld<float, V>(ph + k0);
-        if (vec) {
-          b[u][q] = ld<T, V>(pb + k0), c[u][q] = ld<T, V>(pc + k0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) b[u][q].v[k] = pb[k0 + k], c[u][q].v[k] = pc[k0 + k];
-        }
+        b[u][q].load(pb + k0), c[u][q].load(pc + k0);
       }
       if (u + 1 < n) {
         px += a.x.seq, pd += a.dt.seq, pb += a.b.seq, pc += a.c.seq;
@@ -276,8 +271,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
         Pack<float, V> o;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          o.v[k] = fmaf(ex2(delta * A[q][k]), none ? 0.f : h[u][q].v[k], in * to_f(b[u][q].v[k]));
-          if (at[q] < a.N) y = fmaf(o.v[k], to_f(c[u][q].v[k]), y);
+          const float2 bp = b[u][q].pair(k / 2), cp = c[u][q].pair(k / 2);
+          o.v[k] = fmaf(ex2(delta * A[q][k]), none ? 0.f : h[u][q].v[k], in * (k & 1 ? bp.y : bp.x));
+          if (at[q] < a.N) y = fmaf(o.v[k], k & 1 ? cp.y : cp.x, y);
         }
         if (a.state_out != nullptr && on && at[q] < a.N) st<float, V>(a.state_out + (s + u) * a.state_out_seq + ch * a.N + at[q], o);
       }
@@ -294,7 +290,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
 
 int scan_check(const InbScanArgs& a) {
   if (a.dtype < 0 || a.dtype > 2 || a.C < 1 || a.C > INB_MAX_MEMORY_C || a.N < 1 || a.N > INB_MAX_SCAN_N || a.S < 0 ||
-      a.S > INB_MAX_MEMORY_S || a.T < 0 || a.T > INB_MAX_MEMORY_S || (a.reset.p != nullptr && a.reset.rows < 1))
+      a.S > INB_MAX_MEMORY_S || a.T < 0 || a.T > INB_MAX_MEMORY_S || (a.reset.p != nullptr && (a.reset.rows < 1 || a.reset.rows > INB_MAX_MEMORY_S)))
     return -2;
   if (a.S * (int64_t)a.C > (1ll << 34)) return -2;      // blocks of one launch
   return 0;
@@ -343,8 +339,7 @@ static int step_go(const InbScanArgs& a, int lanes, cudaStream_t s) {
   if (per > STEP_B) per = per / STEP_B * STEP_B;
   if (per < ceil_div(a.S, 65535)) per = ceil_div(a.S, 65535);
   if (per < 1) per = 1;
-  const bool vec = is_aligned(a.b, V * sizeof(T), sizeof(T)) && is_aligned(a.c, V * sizeof(T), sizeof(T));
-  scan_step_kernel<T, V, G><<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per)), STEP_THREADS, 0, s>>>(a, lanes, (int)per, vec);
+  scan_step_kernel<T, V, G><<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per)), STEP_THREADS, 0, s>>>(a, lanes, (int)per);
   return launch_status();
 }
 template <typename T>
@@ -352,7 +347,7 @@ static int scan_step(const InbScanArgs& a, cudaStream_t s) {
   const uint64_t m = (uint64_t)(uintptr_t)a.state | (uint64_t)(uintptr_t)a.state_out | (uint64_t)(a.state_seq * 4) |
                      (uint64_t)(a.state_out_seq * 4) | (uint64_t)(a.N * 4);
   int lanes = 1;
-  if ((m & 15) == 0) {
+  if ((m & 15) == 0 && is_aligned(a.b, 4 * sizeof(T), sizeof(T)) && is_aligned(a.c, 4 * sizeof(T), sizeof(T))) {
     while (lanes < 16 && lanes * 4 < a.N) lanes *= 2;
     return step_go<T, 4, 1>(a, lanes, s);
   }

@@ -89,6 +89,54 @@ __device__ __forceinline__ float raw_f(uint32_t v) {
     return __uint_as_float(v);
 }
 
+// V (1 or 4) neighbouring elements as they lie in memory; their values as pairs (V = 1: the first of one pair)
+template <typename T, int V>
+struct Words {
+  static constexpr int P = V < 2 ? 1 : V / 2, N = V * sizeof(T) / 4 > 0 ? V * sizeof(T) / 4 : 1;
+  uint32_t w[N];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (V == 1) {
+      w[0] = ld_raw(p);
+    } else if constexpr (N == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (V == 1 && sizeof(T) == 2)
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    else if constexpr (V == 1)
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    else if constexpr (N == 2)
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (V == 1)
+      return make_float2(raw_f<T>(w[0]), 0.f);
+    else if constexpr (sizeof(T) == 4)
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (IsBf16<T>::value)
+      return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    else
+      return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  }
+  __device__ __forceinline__ void set(int i, float2 v) {
+    if constexpr (sizeof(T) == 4) {
+      w[V == 1 ? 0 : 2 * i] = __float_as_uint(v.x);
+      if constexpr (V > 1) w[2 * i + 1] = __float_as_uint(v.y);
+    } else {
+      T t[2];
+      down2(v, t[0], t[1]);
+      w[i] = *reinterpret_cast<const uint16_t*>(&t[0]) | (uint32_t)*reinterpret_cast<const uint16_t*>(&t[1]) << 16;
+    }
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ const T* row(const InbSeq& q, int64_t s, int64_t t) {
   return (const T*)q.p + s * q.seq + t * q.step;
@@ -97,9 +145,10 @@ template <typename T>
 __device__ __forceinline__ T* row_out(const InbSeq& q, int64_t s, int64_t t) {
   return (T*)q.p + s * q.seq + t * q.step;
 }
-// The reset bytes of sequence s, or NULL
+// The reset bytes of sequence s, or NULL.  s and rows are below 2^31 (the entry points hold rows to that): a 64-bit division
+// takes five times as long as a step of the convolution.
 __device__ __forceinline__ const uint8_t* resets(const InbReset& r, int64_t s) {
-  return r.p == nullptr ? nullptr : r.p + s / r.rows * r.seq;
+  return r.p == nullptr ? nullptr : r.p + (uint32_t)s / (uint32_t)r.rows * r.seq;
 }
 
 inline bool is_aligned(const InbSeq& q, int64_t bytes, int64_t elem) {
