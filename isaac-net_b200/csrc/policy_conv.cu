@@ -12,8 +12,8 @@ namespace inb {
 namespace pol {
 
 constexpr int CONV_U = 4;       // steps whose loads are sent at once, while the steps before are worked on
-constexpr int CONV_FWD_BLOCKS = 6, CONV_STEP_BLOCKS = 6, CONV_BWD_BLOCKS = 4;      // of 128 threads, an SM
-constexpr int CONV_STEP_B = 4;  // sequences whose loads are sent at once by a single step
+constexpr int CONV_FWD_BLOCKS = 4, CONV_STEP_BLOCKS = 4, CONV_BWD_BLOCKS = 3;      // of 128 threads, an SM
+constexpr int CONV_STEP_B = 2;  // sequences whose loads are sent at once by a single step
 
 struct ConvPlan {
   int64_t parts, len, tasks;    // parts of the time axis, their steps; sequences x parts
@@ -62,6 +62,33 @@ struct Window {
     for (int i = 0; i < P; ++i) v[i] = q.pair(i);
     push(v);
   }
+  // what lies before step t0; returns how many steps back the episode reaches, up to K - 1
+  __device__ __forceinline__ int before(const InbConvArgs& a, int64_t s, int64_t t0, const uint8_t* rs, int64_t ch) {
+    zero();
+    if (t0 == 0) {
+      if (a.state != nullptr) {
+        const T* p = (const T*)a.state + s * a.state_seq + ch;
+        Words<T, V> q[K - 1];
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) q[j].load(p + j * a.C);
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+          for (int i = 0; i < P; ++i) x[K - 2 - j][i] = q[j].pair(i);
+      }
+      return K - 1;
+    }
+    int m = K - 1;                        // parts are longer than K - 1 steps
+    for (int64_t t = t0 - (K - 1); t < t0; ++t) {
+      if (rs != nullptr && rs[t * a.reset.step]) {
+        m = 0;
+        zero();
+      }
+      push(row<T>(a.x, s, t) + ch);
+      m = m < K - 1 ? m + 1 : m;
+    }
+    return m;
+  }
   __device__ __forceinline__ float2 pre(const Taps<T, V, K>& t, float2 now, int i) const {
     float2 p = fma2(now, t.w[K - 1][i], t.bias[i]);
 #pragma unroll
@@ -69,15 +96,6 @@ struct Window {
     return p;
   }
 };
-template <int V>
-__device__ __forceinline__ float2 silu2(float2 p) {
-  return make_float2(p.x * sigmoid(p.x), V > 1 ? p.y * sigmoid(p.y) : 0.f);
-}
-__device__ __forceinline__ float silu_slope(float p) {
-  const float q = sigmoid(p);
-  return q * fmaf(p, 1.f - q, 1.f);
-}
-
 // ---------------------------------------------------------------------------------------------- forward
 // A block is blockDim.x channel vectors x blockDim.y tasks and strides over the tasks, so that weights are read once.
 template <typename T, int V, int K>
@@ -113,15 +131,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
     };
     load(x, reset, n);
     Window<T, V, K> win;
-    win.zero();
-    for (int64_t t = t0 - (K - 1); t < t0; ++t) {
-      if (t >= 0) {
-        if (rs != nullptr && rs[t * a.reset.step]) win.zero();
-        win.push(row<T>(a.x, s, t) + ch);
-      } else if (a.state != nullptr) {
-        win.push((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch);
-      }
-    }
+    win.before(a, s, t0, rs, ch);
     for (int left = n; left > 0; left -= CONV_U) {
       if (left > CONV_U) load(nx, nr, left - CONV_U);
 #pragma unroll
@@ -134,7 +144,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
         for (int i = 0; i < P; ++i) {
           now[i] = x[u].pair(i);
           const float2 p = win.pre(taps, now[i], i);
-          y.set(i, a.act == INB_ACT_SILU ? silu2<V>(p) : p);
+          y.set(i, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
         }
         win.push(now);
         y.store(py);
@@ -196,7 +206,7 @@ __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbCon
         float2 p = fma2(x[b].pair(i), taps.w[K - 1][i], taps.bias[i]);
 #pragma unroll
         for (int j = K - 2; j >= 0; --j) p = fma2(old[b][j].pair(i), taps.w[j][i], p);
-        y.set(i, a.act == INB_ACT_SILU ? silu2<V>(p) : p);
+        y.set(i, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
       }
       y.store(row_out<T>(a.y, s, 0) + ch);
       if (a.state_out != nullptr) {
@@ -257,24 +267,11 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
       load(x, gy, reset, end);
       Window<T, V, K> win;
       float2 pend[K - 1][P];
-      int m = K - 1;                        // how many steps before this one are seen
-      win.zero();
+      int m = win.before(a, s, t0, rs, ch);      // how many steps before this one are seen
 #pragma unroll
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
         for (int i = 0; i < P; ++i) pend[j][i] = zero;
-      for (int64_t t = t0 - (K - 1); t < t0; ++t) {
-        if (t >= 0) {
-          if (rs != nullptr && rs[t * a.reset.step]) {
-            m = 0;
-            win.zero();
-          }
-          win.push(row<T>(a.x, s, t) + ch);
-          m = m < K - 1 ? m + 1 : m;
-        } else if (a.state != nullptr) {
-          win.push((const T*)a.state + s * a.state_seq + (t + K - 1) * a.C + ch);
-        }
-      }
       T* pgx = row_out<T>(a.gx, s, t0) + ch;
       // step i of the part completes gx of step i - (K - 1); before the sequence it is the initial state's
       auto emit = [&](int i) {
@@ -313,7 +310,8 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
             g[i] = gy[u].pair(i);
             if (a.act == INB_ACT_SILU) {
               const float2 p = win.pre(taps, now[i], i);
-              g[i] = mul2(g[i], make_float2(silu_slope(p.x), V > 1 ? silu_slope(p.y) : 0.f));
+              const float2 q = sigmoid2(p, V > 1);
+              g[i] = mul2(g[i], mul2(q, fma2(p, fma2(q, both(-1.f), both(1.f)), both(1.f))));
             }
             if (i0 + u < n) {
               gb[i] = add2(gb[i], g[i]);
@@ -438,18 +436,29 @@ static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
 }
-template <typename T, int V>
-static int conv_go(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  if (a.K == 2) return backward ? conv_bwd_go<T, V, 2>(a, s) : conv_fwd_go<T, V, 2>(a, s);
-  if (a.K == 3) return backward ? conv_bwd_go<T, V, 3>(a, s) : conv_fwd_go<T, V, 3>(a, s);
-  return backward ? conv_bwd_go<T, V, 4>(a, s) : conv_fwd_go<T, V, 4>(a, s);
+// Channels a thread: 16 bytes (forward) or 4 channels (backward, whose sums take the registers), moved by one access, where
+// every row allows it, else one.
+template <typename T>
+static int conv_width(const InbConvArgs& a, bool backward) {
+  const int v = backward ? 4 : 16 / (int)sizeof(T);
+  return conv_aligned(a, v * sizeof(T)) ? v : 1;
 }
-// Four channels a thread, moved by one access, or one: 8 of 16 bits would hold twice the registers for no more bytes in flight.
+template <typename T>
+static int conv_go(const InbConvArgs& a, bool backward, cudaStream_t s) {
+  constexpr int W = 16 / sizeof(T);
+  if (backward) {
+    if (conv_width<T>(a, true) == 4)
+      return a.K == 2 ? conv_bwd_go<T, 4, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 4, 3>(a, s) : conv_bwd_go<T, 4, 4>(a, s);
+    return a.K == 2 ? conv_bwd_go<T, 1, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 1, 3>(a, s) : conv_bwd_go<T, 1, 4>(a, s);
+  }
+  if (conv_width<T>(a, false) == W)
+    return a.K == 2 ? conv_fwd_go<T, W, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, W, 3>(a, s) : conv_fwd_go<T, W, 4>(a, s);
+  return a.K == 2 ? conv_fwd_go<T, 1, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, 1, 3>(a, s) : conv_fwd_go<T, 1, 4>(a, s);
+}
 static int conv_dispatch(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  const bool vec = conv_aligned(a, 4 * elem_size(a.dtype));
-  if (a.dtype == INB_BF16) return vec ? conv_go<bf16, 4>(a, backward, s) : conv_go<bf16, 1>(a, backward, s);
-  if (a.dtype == INB_F16) return vec ? conv_go<f16, 4>(a, backward, s) : conv_go<f16, 1>(a, backward, s);
-  return vec ? conv_go<float, 4>(a, backward, s) : conv_go<float, 1>(a, backward, s);
+  if (a.dtype == INB_BF16) return conv_go<bf16>(a, backward, s);
+  if (a.dtype == INB_F16) return conv_go<f16>(a, backward, s);
+  return conv_go<float>(a, backward, s);
 }
 
 }  // namespace pol
@@ -472,8 +481,8 @@ extern "C" int inb_causal_conv_work(const InbConvArgs* args, int64_t* elems) {
   if (rc != 0) return rc;
   *elems = 0;
   if (a.S == 0 || a.T == 0) return 0;
-  const bool vec = inb::pol::conv_aligned(a, 4 * inb::pol::elem_size(a.dtype));
-  *elems = (int64_t)inb::pol::conv_plan(a, vec ? 4 : 1, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
+  const int v = a.dtype == INB_F32 ? inb::pol::conv_width<float>(a, true) : inb::pol::conv_width<inb::pol::bf16>(a, true);
+  *elems = (int64_t)inb::pol::conv_plan(a, v, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
   return 0;
 }
 

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 
 // One step: bound by the states' bytes.  A thread holds V x G states of one channel (V moved by one access; `lanes` threads a
 // channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.
-constexpr int STEP_THREADS = 256, STEP_B = 4;
+constexpr int STEP_THREADS = 256, STEP_B = 2;
 template <typename T, int V, int G>
 __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs a, int lanes, int per) {
   const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
@@ -233,6 +233,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
 #pragma unroll
     for (int k = 0; k < V; ++k) A[q][k] = at[q] < a.N ? a.a[ch * a.N + at[q] + k] * LOG2E : 0.f;
   }
+  // the reset flag's row, and how many sequences of it have passed
+  const uint8_t* pr = resets(a.reset, s0);
+  uint32_t of = pr != nullptr ? (uint32_t)s0 % (uint32_t)a.reset.rows : 0;
   for (int64_t s = s0; s < s1; s += STEP_B) {
     const int n = s1 - s < STEP_B ? (int)(s1 - s) : STEP_B;
     uint32_t x[STEP_B], dt[STEP_B], z[STEP_B], cut[STEP_B];
@@ -241,12 +244,21 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
     const T *px = row<T>(a.x, s, 0) + ch, *pd = row<T>(a.dt, s, 0) + ch, *pz = gate ? row<T>(a.z, s, 0) + ch : nullptr;
     const T *pb = row<T>(a.b, s, 0), *pc = row<T>(a.c, s, 0);
     const float* ph = a.state != nullptr ? a.state + s * a.state_seq + ch * a.N : nullptr;
+    float* po = a.state_out != nullptr ? a.state_out + s * a.state_out_seq + ch * a.N : nullptr;
+    T* py = row_out<T>(a.y, s, 0) + ch;
 #pragma unroll
     for (int u = 0; u < STEP_B; ++u) {
       // the sequences beyond the last one read it again
       x[u] = ld_raw(px), dt[u] = ld_raw(pd);
       if (gate) z[u] = ld_raw(pz);
-      cut[u] = a.reset.p != nullptr ? *resets(a.reset, s + (u < n ? u : n - 1)) : 0;
+      cut[u] = 0;
+      if (pr != nullptr && u < n) {
+        cut[u] = *pr;
+        if (++of == (uint32_t)a.reset.rows) {
+          of = 0;
+          if (s + u + 1 < a.S) pr += a.reset.seq;
+        }
+      }
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         const int k0 = at[q] < a.N ? at[q] : a.N - V;
@@ -275,7 +287,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
           o.v[k] = fmaf(ex2(delta * A[q][k]), none ? 0.f : h[u][q].v[k], in * (k & 1 ? bp.y : bp.x));
           if (at[q] < a.N) y = fmaf(o.v[k], k & 1 ? cp.y : cp.x, y);
         }
-        if (a.state_out != nullptr && on && at[q] < a.N) st<float, V>(a.state_out + (s + u) * a.state_out_seq + ch * a.N + at[q], o);
+        if (po != nullptr && on && at[q] < a.N) st<float, V>(po + at[q], o);
       }
       for (int o = 1; o < lanes; o *= 2) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
       y = fmaf(d, xv, y);
@@ -283,7 +295,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
         const float zv = raw_f<T>(z[u]);
         y *= zv * sigmoid(zv);
       }
-      if (on && j == 0) row_out<T>(a.y, s + u, 0)[ch] = from_f<T>(y);
+      if (on && j == 0) *py = from_f<T>(y);
+      py += a.y.seq;
+      if (po != nullptr) po += a.state_out_seq;
     }
   }
 }
@@ -348,11 +362,12 @@ static int scan_step(const InbScanArgs& a, cudaStream_t s) {
                      (uint64_t)(a.state_out_seq * 4) | (uint64_t)(a.N * 4);
   int lanes = 1;
   if ((m & 15) == 0 && is_aligned(a.b, 4 * sizeof(T), sizeof(T)) && is_aligned(a.c, 4 * sizeof(T), sizeof(T))) {
-    while (lanes < 16 && lanes * 4 < a.N) lanes *= 2;
-    return step_go<T, 4, 1>(a, lanes, s);
+    // eight states a thread, so that what is a channel's (delta, the gate) is computed by N / 8 threads
+    while (lanes < 8 && lanes * 8 < a.N) lanes *= 2;
+    return a.N <= 4 ? step_go<T, 4, 1>(a, 1, s) : step_go<T, 4, 2>(a, lanes, s);
   }
-  while (lanes < 16 && lanes < a.N) lanes *= 2;
-  return a.N <= 16 ? step_go<T, 1, 1>(a, lanes, s) : step_go<T, 1, 4>(a, lanes, s);
+  while (lanes < 16 && lanes * 4 < a.N) lanes *= 2;
+  return step_go<T, 1, 4>(a, lanes, s);
 }
 // mode 0: the forward pass; 3: the backward pass's parts
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s) {

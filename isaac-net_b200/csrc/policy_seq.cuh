@@ -22,12 +22,19 @@ __device__ __forceinline__ float rcp(float v) {      // 1 / v, 1 ulp
 }
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * LOG2E)); }
 
+// two at once; of the second only if asked for, so that a lone value costs its own special functions alone
+__device__ __forceinline__ float2 sigmoid2(float2 v, bool two = true);
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("add.rn.f32x2 %0, %1, %2;"
       : "=l"(reinterpret_cast<unsigned long long&>(d))
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return d;
+}
+__device__ __forceinline__ float2 sigmoid2(float2 v, bool two) {
+  const float2 t = mul2(v, both(-LOG2E));
+  const float2 d = add2(make_float2(ex2(t.x), two ? ex2(t.y) : 0.f), both(1.f));
+  return make_float2(rcp(d.x), two ? rcp(d.y) : 0.f);
 }
 // 2^v of two values without the special function unit, which makes 16 results a clock and SM and so bounds the scan: v = i + f,
 // f in [-1/2, 1/2], 2^f = 1 + f P(f) with P the Chebyshev interpolation of (2^f - 1) / f of degree 5 (at most 1.2 * 2^-24
@@ -89,7 +96,7 @@ __device__ __forceinline__ float raw_f(uint32_t v) {
     return __uint_as_float(v);
 }
 
-// V (1 or 4) neighbouring elements as they lie in memory; their values as pairs (V = 1: the first of one pair)
+// V (1, 4 or 8; up to 16 bytes) neighbouring elements as they lie in memory; their values as pairs (V = 1: the first of one pair)
 template <typename T, int V>
 struct Words {
   static constexpr int P = V < 2 ? 1 : V / 2, N = V * sizeof(T) / 4 > 0 ? V * sizeof(T) / 4 : 1;
@@ -130,9 +137,13 @@ struct Words {
       w[V == 1 ? 0 : 2 * i] = __float_as_uint(v.x);
       if constexpr (V > 1) w[2 * i + 1] = __float_as_uint(v.y);
     } else {
-      T t[2];
-      down2(v, t[0], t[1]);
-      w[i] = *reinterpret_cast<const uint16_t*>(&t[0]) | (uint32_t)*reinterpret_cast<const uint16_t*>(&t[1]) << 16;
+      if constexpr (IsBf16<T>::value) {
+        const __nv_bfloat162 q = __float22bfloat162_rn(v);
+        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+      } else {
+        const __half2 q = __float22half2_rn(v);
+        w[i] = *reinterpret_cast<const uint32_t*>(&q);
+      }
     }
   }
 };
