@@ -5,9 +5,10 @@
 //   glogits = gloss tau (q - p)
 //
 // Bound by DRAM: the forward call reads the logits once (running maximum and sum, one exponential an element), the
-// backward call reads them again and writes the gradient.  Rows of up to 1024 logits are a warp's, longer ones a block's, and
-// where rows are few a cluster of blocks shares one (forward: joined through distributed shared memory).  Rows may start
-// anywhere: what lies before the first and behind the last 16-byte boundary goes element by element.
+// backward call reads them again and writes the gradient.  Rows of up to 64 logits are 8 lanes', which hold them in registers, of
+// up to 1024 a warp's, longer ones a block's, and where rows are few a cluster of blocks shares one (forward: joined through
+// distributed shared memory).  Rows may start anywhere: what lies before the first and behind the last 16-byte boundary
+// goes element by element.
 #include <cooperative_groups.h>
 
 #include "policy_seq.cuh"
@@ -16,7 +17,8 @@ namespace inb {
 namespace pol {
 namespace cg = cooperative_groups;
 
-constexpr int DIST_THREADS = 256, DIST_WARP_V = 1024, DIST_WARP_K = 128;
+constexpr int DIST_THREADS = 256, DIST_GROUP_V = 64, DIST_GROUP_K = 32, DIST_WARP_V = 1024, DIST_WARP_K = 128;
+constexpr int DIST_U = 4;      // accesses of a thread on their way at once
 
 template <typename T>
 struct RowView {
@@ -24,6 +26,7 @@ struct RowView {
   const T* x;
   const uint8_t* mask;
   int V, head, nvec;         // elements before the first access, accesses
+  RowView() = default;
   __device__ RowView(const InbDistillArgs& a, int64_t r, const T* out) {
     x = (const T*)a.logits + r * a.ld;
     mask = a.mask != nullptr ? a.mask + r * a.ld_mask : nullptr;
@@ -41,66 +44,91 @@ struct RowView {
     lo = r == 0 ? 0 : head + v0 * W;
     hi = r == n - 1 ? V : head + v1 * W;
   }
-  __device__ bool allowed(int i) const { return mask == nullptr || mask[i] != 0; }
-  // an access's elements, -inf where they are not allowed
-  __device__ void load(int v, float (&o)[W]) const {
-    const Pack<T, W> p = ld<T, W>(x + head + v * W);
+  // DIST_U accesses, `stride` apart from v, of those below end: all on their way before the first is used
+  struct Batch {
+    Words<T, W> q[DIST_U];
+    Words<uint8_t, W> m[DIST_U];
+  };
+  __device__ __forceinline__ void load(Batch& b, int v, int stride, int end) const {
 #pragma unroll
-    for (int k = 0; k < W; ++k) o[k] = to_f(p.v[k]);
+    for (int u = 0; u < DIST_U; ++u)
+      if (v + u * stride < end) {
+        b.q[u].load(x + head + (v + u * stride) * W);
+        if (mask != nullptr) b.m[u].load(mask + head + (v + u * stride) * W);
+      }
+  }
+  // an access's elements, -inf where they are not allowed
+  __device__ __forceinline__ void get(const Batch& b, int u, float (&o)[W]) const {
+#pragma unroll
+    for (int k = 0; k < W; k += 2) {
+      const float2 p = b.q[u].pair(k / 2);
+      o[k] = p.x, o[k + 1] = p.y;
+    }
     if (mask != nullptr) {
-      const Pack<uint8_t, W> m = ld<uint8_t, W>(mask + head + v * W);
 #pragma unroll
       for (int k = 0; k < W; ++k)
-        if (m.v[k] == 0) o[k] = -INFINITY;
+        if ((b.m[u].w[k / 4] >> (k % 4 * 8) & 0xFF) == 0) o[k] = -INFINITY;
     }
   }
-  __device__ float load1(int i) const { return allowed(i) ? to_f(x[i]) : -INFINITY; }
+  __device__ float load1(int i) const { return mask == nullptr || mask[i] != 0 ? to_f(x[i]) : -INFINITY; }
 };
 
-// An entry of the teacher's list: its logit, -inf where it is not in use; z: the student's logit there
-template <typename T>
-__device__ __forceinline__ float entry(const InbDistillArgs& a, const RowView<T>& row, int64_t at, int& index, float& z) {
-  const int64_t i = a.index[at];
-  float t = -INFINITY;
-  index = -1;
-  z = 0.f;
-  if (i < 0 || i >= a.V) return t;
-  if (a.teacher_dtype == INB_BF16)
-    t = to_f(((const bf16*)a.teacher)[at]);
-  else if (a.teacher_dtype == INB_F16)
-    t = to_f(((const f16*)a.teacher)[at]);
-  else
-    t = ((const float*)a.teacher)[at];
-  z = row.load1((int)i);
-  if (z == -INFINITY || t != t || t == -INFINITY) return -INFINITY;
-  index = (int)i;
-  return t;
-}
+// An entry of the teacher's list as it lies in memory, and after the student's logit there has been looked at: the teacher's
+// logit, -inf where it is not in use (index then -1); z: the student's logit
+struct Entry {
+  int64_t i;
+  float t, z;
+  int index;
+  __device__ __forceinline__ void fetch(const InbDistillArgs& a, int64_t at) {
+    i = a.index[at];
+    if (a.teacher_dtype == INB_BF16)
+      t = to_f(((const bf16*)a.teacher)[at]);
+    else if (a.teacher_dtype == INB_F16)
+      t = to_f(((const f16*)a.teacher)[at]);
+    else
+      t = ((const float*)a.teacher)[at];
+  }
+  template <typename T>
+  __device__ __forceinline__ void look(const InbDistillArgs& a, const RowView<T>& row) {
+    const bool in = i >= 0 && i < a.V;
+    index = in ? (int)i : -1;
+    z = in ? row.load1(index) : -INFINITY;
+    if (z == -INFINITY || t != t || t == -INFINITY) t = -INFINITY, index = -1;
+  }
+};
 
 // running maximum and sum of exp((v - m) c / log2 e)
 struct Soft {
   float m = -INFINITY, l = 0.f;
-  template <int W>
-  __device__ void add(const float (&v)[W], float c) {
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N], float c) {
     float top = v[0];
 #pragma unroll
-    for (int k = 1; k < W; ++k) top = fmaxf(top, v[k]);
+    for (int k = 1; k < N; ++k) top = fmaxf(top, v[k]);
     if (top > m) {
       l *= ex2((m - top) * c);
       m = top;
     }
     const float at = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
+    if constexpr (N % 2 == 0) {
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < W; ++k) s += ex2((v[k] - at) * c);
-    l += s;
+      for (int k = 0; k < N; k += 2) {
+        const float2 z = mul2(add2(make_float2(v[k], v[k + 1]), both(-at)), both(c));
+        s = add2(s, make_float2(ex2(z.x), ex2(z.y)));
+      }
+      l += s.x + s.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) l += ex2((v[k] - at) * c);
+    }
   }
-  __device__ void join(float om, float ol, float c) {
+  __device__ __forceinline__ void join(float om, float ol, float c) {
     const float top = fmaxf(m, om), at = top == -INFINITY ? 0.f : top;
     l = l * ex2((m - at) * c) + ol * ex2((om - at) * c);
     m = top;
   }
-  __device__ void over_warp(float c) {
+  __device__ __forceinline__ void over_warp(float c) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float om = __shfl_xor_sync(0xFFFFFFFFu, m, o), ol = __shfl_xor_sync(0xFFFFFFFFu, l, o);
@@ -108,41 +136,78 @@ struct Soft {
     }
   }
 };
-__device__ __forceinline__ float warp_max(float v) {
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
 
-// The row's entries by one warp, after m and l are known
-template <typename T>
-__device__ __forceinline__ void finish(const InbDistillArgs& a, const RowView<T>& row, int64_t r, const Soft& s, float c, int lane) {
-  float top = -INFINITY, z;
-  int index;
-  for (int k = lane; k < a.K; k += 32) top = fmaxf(top, entry(a, row, r * a.K + k, index, z));
-  top = warp_max(top);
-  const bool live = top != -INFINITY;
-  float mass = 0.f, sum = 0.f;
-  const float inv = c * LN2;                      // 1 / tau
-  if (live)
-    for (int k = lane; k < a.K; k += 32) {
-      const float t = entry(a, row, r * a.K + k, index, z);
-      if (index < 0) continue;
-      const float e = ex2((t - top) * c);
-      mass += e;
-      sum = fmaf(e, ((t - top) - (z - s.m)) * inv, sum);
+// A row's list by L lanes: some entries a lane in registers, on their way while the row is; those beyond them from memory later.  Every lane of the warp takes part.
+template <typename T, int L>
+struct Entries {
+  static constexpr int HELD = L == 8 ? 4 : 2;
+  Entry e[HELD];
+  __device__ __forceinline__ void fetch(const InbDistillArgs& a, int64_t r, int lane) {
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) {
+      e[q].i = -1, e[q].t = 0.f;
+      if (lane + q * L < a.K) e[q].fetch(a, r * a.K + lane + q * L);
     }
-  mass = warp_sum(mass);
-  sum = warp_sum(sum);
-  if (lane != 0) return;
-  a.loss[r] = live ? a.tau * a.tau * (sum / mass + (logf(s.l) - logf(mass))) : 0.f;
-  if (a.stats != nullptr)
-    *reinterpret_cast<float4*>(a.stats + 4 * r) = live ? make_float4(s.m, 1.f / s.l, top, 1.f / mass) : make_float4(0.f, 0.f, 0.f, 0.f);
-}
+  }
+  __device__ __forceinline__ void look(const InbDistillArgs& a, const RowView<T>& row) {
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) e[q].look(a, row);
+  }
+  // the loss, and what the backward call needs
+  __device__ __forceinline__ void finish(const InbDistillArgs& a, const RowView<T>& row, int64_t r, float m, float l, float c, int lane,
+                                         bool on) const {
+    float top = e[0].t;
+#pragma unroll
+    for (int q = 1; q < HELD; ++q) top = fmaxf(top, e[q].t);
+    for (int k = lane + HELD * L; k < a.K; k += L) {
+      Entry n;
+      n.fetch(a, r * a.K + k);
+      n.look(a, row);
+      top = fmaxf(top, n.t);
+    }
+    top = lanes_max<L>(top);
+    const bool live = top != -INFINITY;
+    float mass = 0.f, sum = 0.f;
+    const float inv = c * LN2;                      // 1 / tau
+    auto add = [&](const Entry& n) {
+      if (n.index < 0) return;
+      const float w = ex2((n.t - top) * c);
+      mass += w;
+      sum = fmaf(w, ((n.t - top) - (n.z - m)) * inv, sum);
+    };
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) add(e[q]);
+    for (int k = lane + HELD * L; k < a.K; k += L) {
+      Entry n;
+      n.fetch(a, r * a.K + k);
+      n.look(a, row);
+      add(n);
+    }
+    mass = lanes_sum<L>(mass);
+    sum = lanes_sum<L>(sum);
+    if (!on || lane != 0) return;
+    a.loss[r] = live ? a.tau * a.tau * (sum / mass + (logf(l) - logf(mass))) : 0.f;
+    if (a.stats != nullptr)
+      *reinterpret_cast<float4*>(a.stats + 4 * r) = live ? make_float4(m, 1.f / l, top, 1.f / mass) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+};
 
+// A row a warp, or (WARP false) a row `parts` blocks
 template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
-  constexpr int TPR = WARP ? 32 : DIST_THREADS;
+__global__ void __launch_bounds__(DIST_THREADS, 5) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
+  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W;
   const int tid = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
   const int part = WARP ? 0 : blockIdx.x % parts;
@@ -151,12 +216,21 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_fwd_kernel(InbDistillArg
   int v0, v1, lo, hi;
   row.part(part, parts, v0, v1, lo, hi);
   Soft s;
-  for (int v = v0 + tid; v < v1; v += TPR) {
-    float x[RowView<T>::W];
-    row.load(v, x);
-    s.add(x, c);
+  Entries<T, 32> list;
+  const bool lists = WARP || (part == 0 && threadIdx.x < 32);
+  if (lists) list.fetch(a, r, lane);
+  for (int v = v0 + tid; v < v1; v += TPR * DIST_U) {
+    typename RowView<T>::Batch b;
+    row.load(b, v, TPR, v1);
+#pragma unroll
+    for (int u = 0; u < DIST_U; ++u) {
+      if (v + u * TPR >= v1) break;
+      float x[W];
+      row.get(b, u, x);
+      s.add(x, c);
+    }
   }
-  const int body = row.head + v0 * row.W, end = row.head + v1 * row.W;
+  const int body = row.head + v0 * W, end = row.head + v1 * W;
   for (int i = lo + tid; i < body; i += TPR) {
     const float x[1] = {row.load1(i)};
     s.add(x, c);
@@ -165,9 +239,10 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_fwd_kernel(InbDistillArg
     const float x[1] = {row.load1(i)};
     s.add(x, c);
   }
+  if (lists) list.look(a, row);
   s.over_warp(c);
   if (WARP) {
-    finish(a, row, r, s, c, lane);
+    list.finish(a, row, r, s.m, s.l, c, lane, true);
     return;
   }
   __shared__ float2 warps[DIST_THREADS / 32];
@@ -182,7 +257,7 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_fwd_kernel(InbDistillArg
   if (parts > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    if (part == 0 && threadIdx.x < 32) {
+    if (lists) {
       s = Soft();
       for (int p = 0; p < parts; ++p) {
         const float2 o = *cluster.map_shared_rank(&block, p);
@@ -191,13 +266,41 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_fwd_kernel(InbDistillArg
     }
     cluster.sync();         // a block's memory lives until it has been read
   }
-  if (part == 0 && threadIdx.x < 32) finish(a, row, r, s, c, lane);
+  if (lists) list.finish(a, row, r, s.m, s.l, c, lane, true);
 }
 
+// What the backward call knows of a row: q = rl exp(z - m), p = rp exp(teacher / tau - top); 0 where no entry is in use, whatever
+// the row's logits are
+struct Grad {
+  float4 stat;
+  float g, gl, c;
+  bool live;
+  __device__ __forceinline__ Grad(const InbDistillArgs& a, int64_t r, float c) : c(c) {
+    stat = *reinterpret_cast<const float4*>(a.stats + 4 * r);
+    live = stat.w != 0.f;
+    g = a.gloss[r] * a.tau, gl = g * stat.y;
+  }
+  __device__ __forceinline__ float value(float v) const { return live && v != -INFINITY ? gl * ex2((v - stat.x) * c) : 0.f; }
+  // an entry of the row's list as (index or -1, p)
+  template <typename T>
+  __device__ __forceinline__ float2 listed(const InbDistillArgs& a, const RowView<T>& row, Entry e) const {
+    e.look(a, row);
+    return make_float2(__int_as_float(live ? e.index : -1), ex2((e.t - stat.z) * c) * stat.w);
+  }
+  // a listed element, from q and the sum of its entries: every entry of an index gives the same value
+  template <typename T>
+  __device__ __forceinline__ float at(const RowView<T>& row, const float2* list, int K, int i) const {
+    float p = 0.f;
+    for (int o = 0; o < K; ++o)
+      if (__float_as_int(list[o].x) == i) p += list[o].y;
+    return g * (stat.y * ex2((row.load1(i) - stat.x) * c) - p);
+  }
+};
+
 template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
+__global__ void __launch_bounds__(DIST_THREADS, 5) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
   constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W;
-  extern __shared__ float2 entries[];            // (index, p) of the row's list
+  extern __shared__ float2 entries[];
   const int tid = threadIdx.x % TPR;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
   const int part = WARP ? 0 : blockIdx.x % parts;
@@ -206,63 +309,128 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_bwd_kernel(InbDistillArg
   const RowView<T> row(a, r, out);
   int v0, v1, lo, hi;
   row.part(part, parts, v0, v1, lo, hi);
-  const float4 stat = *reinterpret_cast<const float4*>(a.stats + 4 * r);
-  const bool live = stat.w != 0.f;                 // a row without an entry in use: 0, whatever its logits are
-  const float g = a.gloss[r] * a.tau, gl = g * stat.y;
+  const Grad g(a, r, c);
   float2* list = entries + (WARP ? threadIdx.x / 32 * a.K : 0);
-  for (int k = tid; k < a.K; k += TPR) {
-    float z;
-    int index;
-    const float t = entry(a, row, r * a.K + k, index, z);
-    list[k] = make_float2(__int_as_float(live ? index : -1), ex2((t - stat.z) * c) * stat.w);
-  }
-  auto value = [&](float v) { return live && v != -INFINITY ? gl * ex2((v - stat.x) * c) : 0.f; };
-  for (int v = v0 + tid; v < v1; v += TPR) {
-    float x[W];
-    Pack<T, W> o;
-    row.load(v, x);
+  Entry first;                                   // the thread's first entry: on its way while the row is
+  if (tid < a.K) first.fetch(a, r * a.K + tid);
+  for (int v = v0 + tid; v < v1; v += TPR * DIST_U) {
+    typename RowView<T>::Batch b;
+    row.load(b, v, TPR, v1);
 #pragma unroll
-    for (int k = 0; k < W; ++k) o.v[k] = from_f<T>(value(x[k]));
-    st<T, W>(out + row.head + v * W, o);
+    for (int u = 0; u < DIST_U; ++u) {
+      if (v + u * TPR >= v1) break;
+      float x[W];
+      row.get(b, u, x);
+      Words<T, W> o;
+#pragma unroll
+      for (int k = 0; k < W; k += 2) o.set(k / 2, make_float2(g.value(x[k]), g.value(x[k + 1])));
+      o.store(out + row.head + (v + u * TPR) * W);
+    }
   }
   const int body = row.head + v0 * W, end = row.head + v1 * W;
-  for (int i = lo + tid; i < body; i += TPR) out[i] = from_f<T>(value(row.load1(i)));
-  for (int i = end + tid; i < hi; i += TPR) out[i] = from_f<T>(value(row.load1(i)));
+  for (int i = lo + tid; i < body; i += TPR) out[i] = from_f<T>(g.value(row.load1(i)));
+  for (int i = end + tid; i < hi; i += TPR) out[i] = from_f<T>(g.value(row.load1(i)));
+  if (tid < a.K) list[tid] = g.listed(a, row, first);
+  for (int k = tid + TPR; k < a.K; k += TPR) {
+    first.fetch(a, r * a.K + k);
+    list[k] = g.listed(a, row, first);
+  }
   if (WARP)
     __syncwarp();
   else
     __syncthreads();
-  // the listed elements again, from q and the sum of their entries: every entry of an index writes the same value
   for (int k = tid; k < a.K; k += TPR) {
     const int i = __float_as_int(list[k].x);
-    if (i < lo || i >= hi) continue;
-    float p = 0.f;
-    for (int o = 0; o < a.K; ++o)
-      if (__float_as_int(list[o].x) == i) p += list[o].y;
-    out[i] = from_f<T>(g * (stat.y * ex2((row.load1(i) - stat.x) * c) - p));
+    if (i >= lo && i < hi) out[i] = from_f<T>(g.at(row, list, a.K, i));
   }
 }
 
+// Short rows: 8 lanes hold one
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(DIST_THREADS) distill_short_kernel(InbDistillArgs a, float c) {
+  constexpr int L = 8, M = DIST_GROUP_V / L;
+  extern __shared__ float2 entries[];
+  const int lane = threadIdx.x % L;
+  const int64_t r0 = (int64_t)blockIdx.x * (DIST_THREADS / L) + threadIdx.x / L;
+  const bool on = r0 < a.N;
+  const int64_t r = on ? r0 : a.N - 1;           // lanes without a row read the last one and write nothing
+  RowView<T> row;
+  row.x = (const T*)a.logits + r * a.ld;
+  row.mask = a.mask != nullptr ? a.mask + r * a.ld_mask : nullptr;
+  uint32_t raw[M], ok[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const int k = i * L + lane;
+    raw[i] = ok[i] = 0;
+    if (k < a.V) {
+      raw[i] = ld_raw(row.x + k);
+      ok[i] = row.mask != nullptr ? row.mask[k] : 1;
+    }
+  }
+  if constexpr (!BACK) {
+    Entries<T, L> list;
+    list.fetch(a, r, lane);
+    float x[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) x[i] = ok[i] ? raw_f<T>(raw[i]) : -INFINITY;
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < M; ++i) m = fmaxf(m, x[i]);
+    m = lanes_max<L>(m);
+    list.look(a, row);
+    const float at = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (i * L < a.V) l += ex2((x[i] - at) * c);
+    l = lanes_sum<L>(l);
+    list.finish(a, row, r, m, l, c, lane, on);
+  } else {
+    T* out = (T*)a.glogits + r * a.V;
+    const Grad g(a, r, c);
+    float2* list = entries + threadIdx.x / L * a.K;
+    for (int k = lane; k < a.K; k += L) {
+      Entry e;
+      e.fetch(a, r * a.K + k);
+      list[k] = g.listed(a, row, e);
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (on && i * L + lane < a.V) out[i * L + lane] = from_f<T>(g.value(ok[i] ? raw_f<T>(raw[i]) : -INFINITY));
+    __syncwarp();
+    for (int k = lane; k < a.K; k += L) {
+      const int i = __float_as_int(list[k].x);
+      if (on && i >= 0) out[i] = from_f<T>(g.at(row, list, a.K, i));
+    }
+  }
+}
+
+// Which form a call takes, by the length of its rows and lists
+enum { DIST_GROUP, DIST_WARP, DIST_BLOCK };
 struct DistPlan {
-  bool warp;
-  int parts;
+  int form, parts, rows;         // blocks that share a row, rows of a block
   unsigned blocks;
 };
 static DistPlan dist_plan(const InbDistillArgs& a) {
-  DistPlan p = {a.V <= DIST_WARP_V && a.K <= DIST_WARP_K, 1, 0};
-  if (p.warp) {
-    p.blocks = (unsigned)ceil_div(a.N, DIST_THREADS / 32);
-  } else {
+  DistPlan p = {DIST_BLOCK, 1, 1, 0};
+  if (a.V <= DIST_GROUP_V && a.K <= DIST_GROUP_K)
+    p.form = DIST_GROUP, p.rows = DIST_THREADS / 8;
+  else if (a.V <= DIST_WARP_V && a.K <= DIST_WARP_K)
+    p.form = DIST_WARP, p.rows = DIST_THREADS / 32;
+  else
     while (p.parts < 8 && a.N * p.parts < sm_count() * 4 && a.V / (2 * p.parts) >= 4096) p.parts *= 2;
-    p.blocks = (unsigned)(a.N * p.parts);
-  }
+  p.blocks = (unsigned)(ceil_div(a.N, p.rows) * p.parts);
   return p;
 }
 template <typename T>
 static int dist_fwd(const InbDistillArgs& a, cudaStream_t s) {
   const DistPlan p = dist_plan(a);
   const float c = LOG2E / a.tau;
-  if (p.warp) {
+  if (p.form == DIST_GROUP) {
+    distill_short_kernel<T, false><<<p.blocks, DIST_THREADS, 0, s>>>(a, c);
+    return launch_status();
+  }
+  if (p.form == DIST_WARP) {
     distill_fwd_kernel<T, true><<<p.blocks, DIST_THREADS, 0, s>>>(a, 1, c);
     return launch_status();
   }
@@ -283,9 +451,10 @@ template <typename T>
 static int dist_bwd(const InbDistillArgs& a, cudaStream_t s) {
   const DistPlan p = dist_plan(a);
   const float c = LOG2E / a.tau;
-  const int rows = p.warp ? DIST_THREADS / 32 : 1;
-  const size_t smem = (size_t)rows * a.K * 8;
-  if (p.warp)
+  const size_t smem = (size_t)p.rows * a.K * 8;      // at most 8 KB
+  if (p.form == DIST_GROUP)
+    distill_short_kernel<T, true><<<p.blocks, DIST_THREADS, smem, s>>>(a, c);
+  else if (p.form == DIST_WARP)
     distill_bwd_kernel<T, true><<<p.blocks, DIST_THREADS, smem, s>>>(a, 1, c);
   else
     distill_bwd_kernel<T, false><<<p.blocks, DIST_THREADS, smem, s>>>(a, p.parts, c);

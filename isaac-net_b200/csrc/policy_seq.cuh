@@ -104,6 +104,8 @@ struct Words {
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (V == 1) {
       w[0] = ld_raw(p);
+    } else if constexpr (N == 1) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else if constexpr (N == 2) {
       const uint2 v = *reinterpret_cast<const uint2*>(p);
       w[0] = v.x, w[1] = v.y;
