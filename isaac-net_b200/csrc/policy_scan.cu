@@ -15,12 +15,13 @@ constexpr int SCAN_WARPS = 4;        // a block's warps work on their own; no ba
 // end state from zero and its sum of delta (-1 where an episode began inside), 3: the same of the reverse recurrence
 // r[t - 1] = exp(delta[t] a) (r[t] + c[t] g[t]), g = gy silu(z), which runs from the part's last step to its first.
 //
-// Bound by the exponentials (one a state and step, 16 a clock and SM) and, next to that, by instruction issue: a quarter of
+// Bound by the exponentials (one a state and step, 16 a clock and SM) and, next to that, by instruction issue: an eighth of
 // them goes to the FMA pipe (ex2_poly), which evens the two out; all else is packed in pairs of states.  A chunk of
 // SCAN_STEPS steps is prepared at once (delta, u, the gate), then the next one's loads are sent, then its steps run.
-template <typename T, int NS, int LN, int MODE>
+// WIDE: the rows of b and c are NS whole, aligned to 16 bytes and moved by that
+template <typename T, int NS, int LN, int MODE, bool WIDE>
 __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry) {
-  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 8;
+  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 16, BCW = 16 / sizeof(T);
   constexpr bool BACK = MODE == 3;
   __shared__ alignas(16) float bc[SCAN_WARPS][TC][2][NP];
   __shared__ float4 stage[SCAN_WARPS][TC][32];       // delta, u, silu(z) (1 without z), d x of this lane's channel
@@ -65,7 +66,8 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
   const uint8_t* rs = resets(a.reset, s);
   if (rs != nullptr) rs += first * a.reset.step;
   int64_t left = t1 - t0;
-  uint32_t x[TC], dt[TC], z[TC], bcr[BCL], flag = 0;      // the next chunk's inputs; BACK: x is gy
+  uint32_t x[TC], dt[TC], z[TC], bcr[WIDE ? 1 : BCL], flag = 0;      // the next chunk's inputs; BACK: x is gy
+  Words<T, BCW> wide[WIDE ? BCL / BCW : 1];
   auto load = [&](int steps) {
 #pragma unroll
     for (int i = 0; i < TC; ++i) {
@@ -78,12 +80,22 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
       pd += DIR * a.dt.step;
       if (gate) pz += DIR * a.z.step;
     }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < BCL / BCW; ++i) {
+        const int k = (i * 32 + lane) * BCW, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
+        // the steps beyond the last one read it again
+        const int tl = tt < steps ? tt : steps - 1;
+        wide[i].load(which ? pc + (DIR * tl * a.c.step + n) : pb + (DIR * tl * a.b.step + n));
+      }
+    } else {
 #pragma unroll
     for (int i = 0; i < BCL; ++i) {
       const int k = i * 32 + lane, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
       bcr[i] = 0;
       if (n < a.N && tt < steps && which < 2 && !(MODE == 2 && which == 1) && !(BACK && which == 0))
         bcr[i] = ld_raw(which ? pc + (DIR * tt * a.c.step + n) : pb + (DIR * tt * a.b.step + n));
+    }
     }
     pb += DIR * TC * a.b.step;
     pc += DIR * TC * a.c.step;
@@ -108,8 +120,7 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < TC; ++i) {
-      float slope;
-      const float xv = raw_f<T>(x[i]), delta = softplus(raw_f<T>(dt[i]) + bias, slope);
+      const float xv = raw_f<T>(x[i]), delta = softplus(raw_f<T>(dt[i]) + bias);
       float o = 1.f;
       if (gate) {
         const float zv = raw_f<T>(z[i]);
@@ -118,10 +129,23 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
       // BACK: u is g, whose c (in place of b) it multiplies
       stage[warp][i][lane] = make_float4(delta, BACK ? xv * o : delta * xv, o, d * xv);
     }
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < BCL; ++i) {
-      const int k = i * 32 + lane, which = k / (TC * NP), r = k % (TC * NP);
-      if (which < 2) bc[warp][r / NP][which][r % NP] = raw_f<T>(bcr[i]);
+      for (int i = 0; i < BCL / BCW; ++i) {
+        const int k = (i * 32 + lane) * BCW, which = k / (TC * NP), r = k % (TC * NP);
+        float4* to = reinterpret_cast<float4*>(&bc[warp][r / NP][which][r % NP]);
+#pragma unroll
+        for (int e = 0; e < BCW / 4; ++e) {
+          const float2 p = wide[i].pair(2 * e), q = wide[i].pair(2 * e + 1);
+          to[e] = make_float4(p.x, p.y, q.x, q.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < BCL; ++i) {
+        const int k = i * 32 + lane, which = k / (TC * NP), r = k % (TC * NP);
+        if (which < 2) bc[warp][r / NP][which][r % NP] = raw_f<T>(bcr[i]);
+      }
     }
     const uint32_t bits = __ballot_sync(0xFFFFFFFFu, flag != 0);
     if (ahead > 0) load(ahead);
@@ -135,6 +159,7 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
       if (!BACK && cut) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
+        keep_branch();
       }
       float2 y = make_float2(0.f, 0.f);
 #pragma unroll
@@ -156,6 +181,7 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
       if (BACK && cut) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
+        keep_branch();
       }
       if (MODE < 2) {
         float o = y.x + y.y;
@@ -168,16 +194,18 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
     }
   }
   if (!on) return;
-#pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    const float v = n & 1 ? h[n / 2].y : h[n / 2].x;
-    if (j * NS + n >= a.N) continue;
-    if (MODE >= 2)
-      carry[((s * pl.parts + part) * a.C + ch) * n4 + j * NS + n] = v;
-    else if (t1 == a.T && a.state_out != nullptr)
-      a.state_out[s * a.state_out_seq + ch * a.N + j * NS + n] = v;
-  }
   if (MODE >= 2 && j == 0) carry[a.S * pl.parts * a.C * n4 + (s * pl.parts + part) * a.C + ch] = fresh ? -1.f : dsum;
+  float* to = MODE >= 2 ? carry + ((s * pl.parts + part) * a.C + ch) * n4
+                        : t1 == a.T && a.state_out != nullptr ? a.state_out + s * a.state_out_seq + ch * a.N : nullptr;
+  if (to == nullptr) return;
+  if (a.N == NP && (MODE >= 2 || (((uintptr_t)a.state_out | (a.state_out_seq * 4)) & 15) == 0)) {
+#pragma unroll
+    for (int n = 0; n < NH; n += 2) *reinterpret_cast<float4*>(to + j * NS + 2 * n) = make_float4(h[n].x, h[n].y, h[n + 1].x, h[n + 1].y);
+  } else {
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+      if (j * NS + n < a.N) to[j * NS + n] = n & 1 ? h[n / 2].y : h[n / 2].x;
+  }
 }
 
 // The states that the parts begin (reverse: end) with, in place of what they end with from zero.  A thread a state.
@@ -275,8 +303,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs 
     for (int u = 0; u < STEP_B; ++u) {
       if (u >= n) break;
       const float xv = raw_f<T>(x[u]);
-      float slope, y = 0.f;
-      const float delta = softplus(raw_f<T>(dt[u]) + bias, slope), in = delta * xv;
+      float y = 0.f;
+      const float delta = softplus(raw_f<T>(dt[u]) + bias), in = delta * xv;
       const bool none = ph == nullptr || cut[u] != 0;
 #pragma unroll
       for (int q = 0; q < G; ++q) {
@@ -317,7 +345,14 @@ int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool revers
 template <typename T, int NS, int LN, int MODE>
 static void scan_go(const InbScanArgs& a, const ScanPlan& p, float* carry, cudaStream_t s) {
   const int64_t tiles = ceil_div(a.C, 32 / LN), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
-  scan_kernel<T, NS, LN, MODE><<<dim3((unsigned)(a.S * p.parts), (unsigned)ceil_div(tiles, warps)), (unsigned)warps * 32, 0, s>>>(a, p, carry);
+  const dim3 grid((unsigned)(a.S * p.parts), (unsigned)ceil_div(tiles, warps));
+  if constexpr (NS == 16 && LN == 1) {
+    if (a.N == 16 && is_aligned(a.b, 16, sizeof(T)) && is_aligned(a.c, 16, sizeof(T))) {
+      scan_kernel<T, NS, LN, MODE, true><<<grid, (unsigned)warps * 32, 0, s>>>(a, p, carry);
+      return;
+    }
+  }
+  scan_kernel<T, NS, LN, MODE, false><<<grid, (unsigned)warps * 32, 0, s>>>(a, p, carry);
 }
 template <typename T, int NS, int LN>
 static int scan_mode(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s) {

@@ -55,12 +55,15 @@ struct Chunk {
 // once a chunk: a lane leaves its parts where its states were, and one lane adds four channels' of a step.  Shared memory
 // (25 KB a warp, of it 20 for states and parts) leaves 8 warps an SM, so a chunk's inputs are loaded a chunk ahead.
 // VEC: rows of x, dt, z, gy and their gradients are moved four channels at a time (aligned, C a multiple of 4)
-template <typename T, int LN, bool VEC>
+// WIDE: b and c have NP states whose rows are aligned to 16 bytes and moved by that
+template <typename T, int LN, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPlan pl, const float* carry, float* part_bc,
                                                           float* part_par) {
   using S = BwdShape<LN>;
   constexpr int TC = S::TC, NP = S::NP, CW = S::CW, G = S::G, BCL = TC * NP / 32, ITEMS = S::ITEMS, SLOTS = S::SLOTS,
-                LINE = S::LINE;
+                LINE = S::LINE, UNROLL = 2, BCW = 16 / sizeof(T);
+  // words of b and c a lane loads: in all, and by 16 bytes
+  constexpr int BCN = 2 * TC * NP / (32 * BCW) > 0 ? 2 * TC * NP / (32 * BCW) : 1;
   extern __shared__ float4 smem4[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int j = lane % LN, gr = lane / LN;
@@ -100,7 +103,8 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
     __device__ float f(int c) const { return VEC ? to_f(v.v[c]) : raw_f<T>(e[c]); }
   };
   Raw rx[ITEMS], rd[ITEMS], rz[ITEMS], rg[ITEMS];
-  uint32_t rb[BCL], rc[BCL], flag = 0, bits;
+  uint32_t rb[WIDE ? 1 : BCL], rc[WIDE ? 1 : BCL], flag = 0, bits;
+  Words<T, BCW> wide[WIDE ? BCN : 1];
   float4 rh[4];
   const int chl = VEC ? (many == 4 ? mine : a.C - 4) : 0;
   auto four = [&](Raw& r, const T* p) {
@@ -123,11 +127,20 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
       if (gate) four(rz[i], pz + tl * a.z.step);
     }
     const T *pb = row<T>(a.b, q.s, q.t), *pc = row<T>(a.c, q.s, q.t);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < BCN; ++i) {
+        const int k = (i * 32 + lane) * BCW, which = k / (TC * NP), tt = k % (TC * NP) / NP, n = k % NP;
+        const int tl = tt < q.steps ? tt : q.steps - 1;
+        wide[i].load(which ? pc + (tl * a.c.step + n) : pb + (tl * a.b.step + n));
+      }
+    } else {
 #pragma unroll
     for (int i = 0; i < BCL; ++i) {
       const int tt = (i * 32 + lane) / NP, n = (i * 32 + lane) % NP;
       const int tl = tt < q.steps ? tt : q.steps - 1, nl = n < a.N ? n : a.N - 1;
       rb[i] = ld_raw(pb + (tl * a.b.step + nl)), rc[i] = ld_raw(pc + (tl * a.c.step + nl));
+    }
     }
     const float* from = q.t > 0 ? a.kept + (q.s * (chunks - 1) + q.t / TC - 1) * a.C * n4
                                 : flat && a.state != nullptr ? a.state + q.s * a.state_seq : zero;
@@ -179,11 +192,24 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
       *(float4*)(sD + o) = make_float4(delta[0], delta[1], delta[2], delta[3]);
       *(float4*)(sG + o) = make_float4(g[0], g[1], g[2], g[3]);
     }
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < BCL; ++i) {
-      const bool in = (i * 32 + lane) % NP < a.N;
-      *reinterpret_cast<float2*>(sB + 2 * (i * 32 + lane)) = both(in ? raw_f<T>(rb[i]) : 0.f);
-      *reinterpret_cast<float2*>(sC + 2 * (i * 32 + lane)) = both(in ? raw_f<T>(rc[i]) : 0.f);
+      for (int i = 0; i < BCN; ++i) {
+        const int k = (i * 32 + lane) * BCW, which = k / (TC * NP);
+        float4* to = (float4*)((which ? sC : sB) + 2 * (k % (TC * NP)));
+#pragma unroll
+        for (int e = 0; e < BCW / 2; ++e) {
+          const float2 p = wide[i].pair(e);
+          to[e] = make_float4(p.x, p.x, p.y, p.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < BCL; ++i) {
+        const bool in = (i * 32 + lane) % NP < a.N;
+        *reinterpret_cast<float2*>(sB + 2 * (i * 32 + lane)) = both(in ? raw_f<T>(rb[i]) : 0.f);
+        *reinterpret_cast<float2*>(sC + 2 * (i * 32 + lane)) = both(in ? raw_f<T>(rc[i]) : 0.f);
+      }
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -213,10 +239,13 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
     }
     __syncthreads();                 // this chunk is staged, and the block has read the parts of the one before
     // forward again: the state before each step
-    for (int i = 0; i < steps; ++i) {
+#pragma unroll UNROLL
+    for (int i = 0; i < TC; ++i) {
+      if (i >= steps) break;
       if (bits >> i & 1) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) h[0][n] = h[1][n] = make_float2(0.f, 0.f);
+        keep_branch();
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p)
@@ -237,7 +266,9 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
           h[p][n] = fma2(make_float2(ex2(v.x), ex2(v.y)), h[p][n], mul2(U[p], B[n]));
         }
     }
-    for (int i = steps - 1; i >= 0; --i) {
+#pragma unroll UNROLL
+    for (int i = TC - 1; i >= 0; --i) {
+      if (i >= steps) continue;
       const float4 D4 = *(const float4*)(sD + i * CW + gr * 4), X4 = *(const float4*)(sX + i * CW + gr * 4),
                    G4 = *(const float4*)(sG + i * CW + gr * 4);
       const float4 *B4 = (const float4*)(sB + (i * NP + j * 4) * 2), B0 = B4[0], B1 = B4[1];
@@ -268,6 +299,7 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(InbScanArgs a, ScanPla
       if (bits >> i & 1) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) r[0][n] = r[1][n] = make_float2(0.f, 0.f);
+        keep_branch();
       }
       // this lane's parts, in place of the states that it alone has read
       float4* to = H + i * SLOTS * LINE + lane;
@@ -436,11 +468,12 @@ static BwdPlan bwd_plan(const InbScanArgs& a) {
   b.par = (int64_t)b.blocks * a.C * (a.N + 2);
   return b;
 }
-template <typename T, int LN, bool VEC>
+template <typename T, int LN, bool VEC, bool WIDE>
 static int bwd_launch(const InbScanArgs& a, const BwdPlan& b, const float* carry, float* bc, float* par, cudaStream_t s) {
-  const cudaError_t e = allow_smem<KernelKey<scan_bwd_kernel<T, LN, VEC>>>((const void*)scan_bwd_kernel<T, LN, VEC>, 227 * 1024);
+  constexpr auto kernel = scan_bwd_kernel<T, LN, VEC, WIDE>;
+  const cudaError_t e = allow_smem<KernelKey<scan_bwd_kernel<T, LN, VEC, WIDE>>>((const void*)kernel, 227 * 1024);
   if (e != cudaSuccess) return -100 - (int)e;
-  scan_bwd_kernel<T, LN, VEC><<<dim3(b.blocks, b.tiles), b.warps * 32, b.smem, s>>>(a, b.plan, carry, b.bc > 0 ? bc : nullptr, par);
+  kernel<<<dim3(b.blocks, b.tiles), b.warps * 32, b.smem, s>>>(a, b.plan, carry, b.bc > 0 ? bc : nullptr, par);
   return 0;
 }
 template <typename T, int LN>
@@ -450,7 +483,11 @@ static int bwd_go(const InbScanArgs& a, const BwdPlan& b, cudaStream_t s) {
   if (rc != 0) return rc;
   bool vec = a.C % 4 == 0;
   for (const InbSeq& q : {a.x, a.dt, a.z, a.gy, a.gx, a.gdt, a.gz}) vec = vec && is_aligned(q, 4 * sizeof(T), sizeof(T));
-  rc = vec ? bwd_launch<T, LN, true>(a, b, carry, bc, par, s) : bwd_launch<T, LN, false>(a, b, carry, bc, par, s);
+  const bool wide = LN >= 4 && vec && a.N == 4 * LN && is_aligned(a.b, 16, sizeof(T)) && is_aligned(a.c, 16, sizeof(T));
+  if (wide)
+    rc = bwd_launch<T, LN, true, LN >= 4>(a, b, carry, bc, par, s);
+  else
+    rc = vec ? bwd_launch<T, LN, true, false>(a, b, carry, bc, par, s) : bwd_launch<T, LN, false, false>(a, b, carry, bc, par, s);
   if (rc != 0) return rc;
   if (b.bc > 0) scan_bc_kernel<T><<<(unsigned)ceil_div(a.S * a.T * 2 * a.N, 256), 256, 0, s>>>(a, bc, b.tiles);
   colsum<float>(par, b.blocks, (int64_t)a.C * (a.N + 2), (int64_t)a.C * a.N, (int64_t)a.C * (a.N + 1), a.ga, a.gd, a.gdt_bias, s);
