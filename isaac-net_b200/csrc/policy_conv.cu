@@ -3,7 +3,7 @@
 //   pre[t] = bias + sum_j w[K - 1 - j] x[t - j],  y = act(pre);     taps before a reset, or before the sequence, are 0
 //   g[t] = gy[t] act'(pre[t]);   gx[t] = sum_j w[K - 1 - j] g[t + j];   gw[K - 1 - j] = sum_t g[t] x[t - j];   gbias = sum_t g[t]
 //
-// Bound by DRAM: 2K operations an element against 2 (forward) or 4 (backward, which recomputes pre) moved elements.  A
+// Bound by DRAM: 2K operations an element against 2 (forward) or 3 (backward, which recomputes pre) moved elements.  A
 // thread holds V neighbouring channels, walks along time and keeps the last K - 1 inputs in registers, so every element is
 // read once; where sequences are few the time axis is split and a part re-reads K - 1 steps at its edge.
 #include "policy_seq.cuh"
@@ -11,8 +11,8 @@
 namespace inb {
 namespace pol {
 
-constexpr int CONV_U = 4;       // steps whose loads are sent at once, while the steps before are worked on
-constexpr int CONV_FWD_BLOCKS = 4, CONV_STEP_BLOCKS = 4, CONV_BWD_BLOCKS = 3;      // of 128 threads, an SM
+constexpr int CONV_R = 8;       // rows of a chunk
+constexpr int CONV_FWD_BLOCKS = 4, CONV_STEP_BLOCKS = 4, CONV_BWD_BLOCKS = 4;      // of 128 threads, an SM
 constexpr int CONV_STEP_B = 2;  // sequences whose loads are sent at once by a single step
 
 struct ConvPlan {
@@ -54,40 +54,11 @@ struct Window {
 #pragma unroll
     for (int i = 0; i < P; ++i) x[0][i] = v[i];
   }
-  __device__ __forceinline__ void push(const T* p) {
-    Words<T, V> q;
-    q.load(p);
+  __device__ __forceinline__ void push(const Words<T, V>& q) {
     float2 v[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) v[i] = q.pair(i);
     push(v);
-  }
-  // what lies before step t0; returns how many steps back the episode reaches, up to K - 1
-  __device__ __forceinline__ int before(const InbConvArgs& a, int64_t s, int64_t t0, const uint8_t* rs, int64_t ch) {
-    zero();
-    if (t0 == 0) {
-      if (a.state != nullptr) {
-        const T* p = (const T*)a.state + s * a.state_seq + ch;
-        Words<T, V> q[K - 1];
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) q[j].load(p + j * a.C);
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-          for (int i = 0; i < P; ++i) x[K - 2 - j][i] = q[j].pair(i);
-      }
-      return K - 1;
-    }
-    int m = K - 1;                        // parts are longer than K - 1 steps
-    for (int64_t t = t0 - (K - 1); t < t0; ++t) {
-      if (rs != nullptr && rs[t * a.reset.step]) {
-        m = 0;
-        zero();
-      }
-      push(row<T>(a.x, s, t) + ch);
-      m = m < K - 1 ? m + 1 : m;
-    }
-    return m;
   }
   __device__ __forceinline__ float2 pre(const Taps<T, V, K>& t, float2 now, int i) const {
     float2 p = fma2(now, t.w[K - 1][i], t.bias[i]);
@@ -96,70 +67,190 @@ struct Window {
     return p;
   }
 };
+// ---------------------------------------------------------------------------------------------- rows on their way
+// A task's rows go by chunks of CONV_R through memory that the thread alone writes and reads (no barrier): while one chunk is
+// worked on, the next one's rows, the next task's among them, are on their way by cp.async; rows of 2 bytes, which cp.async
+// cannot move, by registers.  A task's first chunk also brings the K - 1 rows before it, of the state or of the part before.
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// STREAMS 2: x and gy, whose rows end with those that reach back into the part
+template <typename T, int V, int K, int STREAMS>
+struct Feed {
+  static constexpr int B = V * sizeof(T), ROWS = K - 1 + CONV_R * STREAMS, STAGE = ROWS * 128 * B;
+  // a chunk: sequence s, rows [lo, hi) of its part [t0, t0 + n)
+  struct Chunk {
+    int64_t task, s, t0;
+    int n, to, lo, hi;
+    bool on;
+  };
+  char* base;
+  uint32_t held[B < 4 ? ROWS : 1];
+  uint32_t flag[2];
+  int64_t stride, rounds, round;
+  int chunks, chunk, tx, lane, stage;
+  Chunk next;
+  __device__ __forceinline__ char* slot(int st, int row) const { return base + st * STAGE + row * 128 * B; }
+  __device__ __forceinline__ void put(int row, const T* p) {
+    if constexpr (B < 4)
+      held[row] = ld_raw(p);
+    else if constexpr (B == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(slot(stage, row))), "l"(p) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_at(slot(stage, row))), "l"(p), "n"(B) : "memory");
+  }
+  __device__ __forceinline__ Words<T, V> get(int row) const {      // of the chunk that now() gave
+    Words<T, V> w;
+    if constexpr (B == 2)
+      w.w[0] = *(const uint16_t*)slot(stage ^ 1, row);
+    else
+      w.load((const T*)slot(stage ^ 1, row));
+    return w;
+  }
+  __device__ __forceinline__ void place(const InbConvArgs& a, const ConvPlan& pl, int64_t ch) {
+    next.lo = chunk * CONV_R;
+    if (chunk == 0) {
+      next.on = next.task < pl.tasks;
+      const int64_t part = pl.parts > 1 ? next.task / a.S : 0;      // the next task: the same steps of the next sequence
+      next.s = next.task - part * a.S;
+      next.t0 = part * pl.len;
+      const int64_t left = a.T - next.t0;
+      next.n = (int)(pl.len < left ? pl.len : left);
+      next.to = STREAMS == 1 ? next.n : next.n + K - 1 < left ? next.n + K - 1 : (int)left;
+    }
+    next.hi = next.lo + CONV_R < next.to ? next.lo + CONV_R : next.to;
+  }
+  __device__ __forceinline__ void send(const InbConvArgs& a, int64_t ch) {
+    flag[0] = flag[1] = 0;
+    if (next.on && next.lo < next.hi) {
+      const int count = next.hi - next.lo;
+      if (ch < a.C) rows(a, ch, count);
+      const uint8_t* rs = resets(a.reset, next.s);
+      if (rs != nullptr) {
+        rs += (next.t0 + next.lo) * a.reset.step;
+        const int l = threadIdx.x & 31;           // the lanes of a task read its flags together, those beyond the channels too
+        if (l < CONV_R && l < count) flag[0] = rs[l * a.reset.step];
+        if (tx == 4 && l + 4 < count) flag[1] = rs[(l + 4) * a.reset.step];
+      }
+    }
+    if constexpr (B >= 4) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void rows(const InbConvArgs& a, int64_t ch, int count) {
+    const T* p = row<T>(a.x, next.s, next.t0 + next.lo) + ch;
+    const T* g = STREAMS > 1 ? row<T>(a.gy, next.s, next.t0 + next.lo) + ch : nullptr;
+#pragma unroll
+    for (int i = 0; i < CONV_R; ++i)
+      if (i < count) {
+        put(K - 1 + i, p);
+        p += a.x.step;
+        if (STREAMS > 1) {
+          put(K - 1 + CONV_R + i, g);
+          g += a.gy.step;
+        }
+      }
+    if (chunk == 0 && (next.t0 > 0 || a.state != nullptr)) {
+      const bool state = next.t0 == 0;
+      const T* h = state ? (const T*)a.state + next.s * a.state_seq + ch : row<T>(a.x, next.s, next.t0 - (K - 1)) + ch;
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) {
+        put(j, h);
+        h += state ? a.C : a.x.step;
+      }
+    }
+  }
+  __device__ __forceinline__ void start(const InbConvArgs& a, const ConvPlan& pl, char* smem, int64_t ch) {
+    tx = blockDim.x;
+    const int id = threadIdx.y * tx + threadIdx.x;
+    base = smem + id * B;
+    lane = id & 31;
+    stride = (int64_t)gridDim.x * blockDim.y;
+    rounds = (pl.tasks + stride - 1) / stride;
+    const int64_t rows = pl.parts > 1 && STREAMS > 1 ? pl.len + K - 1 : pl.len;
+    chunks = (int)((rows + CONV_R - 1) / CONV_R);
+    round = chunk = stage = 0;
+    next.task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    place(a, pl, ch);
+    send(a, ch);
+  }
+  __device__ __forceinline__ bool more() const { return round < rounds; }      // the same for every thread of the block
+  // the next chunk, landed; bit i of `cuts`: its row i starts an episode.  The chunk after it is sent for.
+  __device__ __forceinline__ Chunk now(const InbConvArgs& a, const ConvPlan& pl, int64_t ch, uint32_t& cuts) {
+    const Chunk c = next;
+    if constexpr (B < 4) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) *(uint16_t*)slot(stage, i) = (uint16_t)held[i];
+    }
+    const int first = lane & ~((tx < 32 ? tx : 32) - 1);
+    cuts = __ballot_sync(0xFFFFFFFFu, flag[0] != 0) >> first & (tx == 4 ? 0xFu : 0xFFu);
+    if (tx == 4) cuts |= (__ballot_sync(0xFFFFFFFFu, flag[1] != 0) >> first & 0xFu) << 4;
+    stage ^= 1;
+    if (++chunk == chunks) chunk = 0, ++round, next.task += stride;
+    if (round < rounds) {
+      place(a, pl, ch);
+      send(a, ch);
+    } else if constexpr (B >= 4) {
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    if constexpr (B >= 4) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    return c;
+  }
+};
+
 // ---------------------------------------------------------------------------------------------- forward
 // A block is blockDim.x channel vectors x blockDim.y tasks and strides over the tasks, so that weights are read once.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvArgs a, ConvPlan pl) {
   constexpr int P = Words<T, V>::P;
+  extern __shared__ float4 smem4[];
   const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (ch >= a.C) return;
+  Feed<T, V, K, 1> feed;
+  feed.start(a, pl, (char*)smem4, ch);
   Taps<T, V, K> taps;
-  taps.load(a, ch, true);
-  for (int64_t task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; task < pl.tasks; task += (int64_t)gridDim.x * blockDim.y) {
-    const int64_t part = pl.parts > 1 ? task / a.S : 0, s = task - part * a.S;      // the next task: the same steps of the next sequence
-    const int64_t t0 = part * pl.len;
-    const int n = (int)(t0 + pl.len < a.T ? pl.len : a.T - t0);
-    const uint8_t* rs = resets(a.reset, s);
-    const uint8_t* pr = rs != nullptr ? rs + t0 * a.reset.step : nullptr;
-    const T* px = row<T>(a.x, s, t0) + ch;
-    T* py = row_out<T>(a.y, s, t0) + ch;
-    Words<T, V> x[CONV_U], nx[CONV_U];
-    uint32_t reset[CONV_U] = {}, nr[CONV_U] = {};
-    auto load = [&](Words<T, V>(&to)[CONV_U], uint32_t(&flag)[CONV_U], int left) {
+  taps.load(a, ch, ch < a.C);
+  Window<T, V, K> win;
+  T* py = nullptr;
+  while (feed.more()) {
+    uint32_t cuts;
+    const auto q = feed.now(a, pl, ch, cuts);
+    if (!q.on || ch >= a.C) continue;
+    if (q.lo == 0) {
+      win.zero();
+      if (q.t0 > 0 || a.state != nullptr) {
+        const uint8_t* rs = q.t0 > 0 ? resets(a.reset, q.s) : nullptr;
 #pragma unroll
-      for (int u = 0; u < CONV_U; ++u) {
-        if (u < left) to[u].load(px);
-        px += a.x.step;
-      }
-      if (rs != nullptr) {
-#pragma unroll
-        for (int u = 0; u < CONV_U; ++u) {
-          if (u < left) flag[u] = *pr;
-          pr += a.reset.step;
+        for (int j = 0; j < K - 1; ++j) {
+          if (rs != nullptr && rs[(q.t0 - (K - 1) + j) * a.reset.step] != 0) win.zero();
+          win.push(feed.get(j));
         }
       }
-    };
-    load(x, reset, n);
-    Window<T, V, K> win;
-    win.before(a, s, t0, rs, ch);
-    for (int left = n; left > 0; left -= CONV_U) {
-      if (left > CONV_U) load(nx, nr, left - CONV_U);
-#pragma unroll
-      for (int u = 0; u < CONV_U; ++u) {
-        if (u >= left) break;
-        if (reset[u]) win.zero();
-        Words<T, V> y;
-        float2 now[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-          now[i] = x[u].pair(i);
-          const float2 p = win.pre(taps, now[i], i);
-          y.set(i, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
-        }
-        win.push(now);
-        y.store(py);
-        py += a.y.step;
-      }
-#pragma unroll
-      for (int u = 0; u < CONV_U; ++u) x[u] = nx[u], reset[u] = nr[u];
+      py = row_out<T>(a.y, q.s, q.t0) + ch;
     }
-    if (t0 + n == a.T && a.state_out != nullptr) {
-      T* out = (T*)a.state_out + s * a.state_out_seq + ch;
+    const int count = q.hi - q.lo;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const Words<T, V> x = feed.get(K - 1 + i);
+      if (cuts >> i & 1) {
+        win.zero();
+        keep_branch();
+      }
+      float2 now[P];
+      Words<T, V> y;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        now[k] = x.pair(k);
+        const float2 p = win.pre(taps, now[k], k);
+        y.set(k, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
+      }
+      y.store(py);
+      py += a.y.step;
+      win.push(now);
+    }
+    if (q.hi == q.n && q.lo < q.hi && q.t0 + q.n == a.T && a.state_out != nullptr) {
+      T* out = (T*)a.state_out + q.s * a.state_out_seq + ch;
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
         Words<T, V> p;
 #pragma unroll
-        for (int i = 0; i < P; ++i) p.set(i, win.x[j][i]);      // what was read, or 0: exact
+        for (int k = 0; k < P; ++k) p.set(k, win.x[j][k]);      // what was read, or 0: exact
         p.store(out + (K - 2 - j) * a.C);
       }
     }
@@ -220,13 +311,15 @@ __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbCon
 }
 
 // ---------------------------------------------------------------------------------------------- backward
-// pend[j - 1] gathers gx[t - j] while later steps still add to it; step t completes gx[t - (K - 1)].  A part goes K - 1 steps
-// beyond its end, for gx alone.  Blocks as in the forward pass, so that gw and gbias stay in registers; one partial row a
-// block, [C K | C], added by a second launch.
+// pend[j - 1] gathers gx[t - j] while later steps still add to it; step t completes gx[t - (K - 1)].  Where an episode begins
+// the K - 1 before it are complete already: they are stored there, and what is gathered for them afterwards is dropped.  A part
+// goes K - 1 steps beyond its end, for gx alone.  Blocks as in the forward pass, so that gw and gbias stay in registers; one
+// partial row a block, [C K | C], added by a second launch.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvArgs a, ConvPlan pl) {
   constexpr int P = Words<T, V>::P;
-  extern __shared__ float smem[];
+  extern __shared__ float4 smem4[];
+  float* smem = (float*)smem4;
   const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
   const bool on = ch < a.C;
   Taps<T, V, K> taps;
@@ -239,117 +332,126 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
 #pragma unroll
     for (int k = 0; k < K; ++k) gw[k][i] = zero;
   }
-  if (on)
-    for (int64_t task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; task < pl.tasks; task += (int64_t)gridDim.x * blockDim.y) {
-      const int64_t part = pl.parts > 1 ? task / a.S : 0, s = task - part * a.S;
-      const int64_t t0 = part * pl.len;
-      const int n = (int)(t0 + pl.len < a.T ? pl.len : a.T - t0);                 // the part's steps,
-      const int end = (int)(n + K - 1 < a.T - t0 ? n + K - 1 : a.T - t0);         // and with those that reach back into it
-      const uint8_t* rs = resets(a.reset, s);
-      const uint8_t* pr = rs != nullptr ? rs + t0 * a.reset.step : nullptr;
-      const T *px = row<T>(a.x, s, t0) + ch, *pg = row<T>(a.gy, s, t0) + ch;
-      Words<T, V> x[CONV_U], nx[CONV_U], gy[CONV_U], ng[CONV_U];
-      uint32_t reset[CONV_U] = {}, nr[CONV_U] = {};
-      auto load = [&](Words<T, V>(&to)[CONV_U], Words<T, V>(&tg)[CONV_U], uint32_t(&flag)[CONV_U], int left) {
+  Window<T, V, K> win;
+  float2 pend[K - 1][P];
+  int seen = 0;                           // rows since the episode or the part began, up to K - 1
+  T* pgx = nullptr;
+  Feed<T, V, K, 2> feed;
+  feed.start(a, pl, (char*)smem, ch);
+  while (feed.more()) {
+    uint32_t cuts;
+    const auto q = feed.now(a, pl, ch, cuts);
+    if (!q.on || ch >= a.C) continue;
+    // gx of the row `at` (pgx's) is complete; before the sequence it is the initial state's
+    auto store = [&](int at, const float2 (&v)[P]) {
+      Words<T, V> p;
 #pragma unroll
-        for (int u = 0; u < CONV_U; ++u) {
-          if (u < left) to[u].load(px), tg[u].load(pg);
-          px += a.x.step, pg += a.gy.step;
-        }
-        if (rs != nullptr) {
+      for (int k = 0; k < P; ++k) p.set(k, v[k]);
+      if (at >= 0)
+        p.store(row_out<T>(a.gx, q.s, q.t0 + at) + ch);
+      else if (q.t0 == 0 && a.gstate != nullptr)
+        p.store((T*)a.gstate + (q.s * (K - 1) + at + K - 1) * a.C + ch);
+    };
+    // an episode begins at row i: the rows before it are complete, but for those that were when the last one began
+    auto flush = [&](int i) {
 #pragma unroll
-          for (int u = 0; u < CONV_U; ++u) {
-            if (u < left) flag[u] = *pr;
-            pr += a.reset.step;
-          }
-        }
-      };
-      load(x, gy, reset, end);
-      Window<T, V, K> win;
-      float2 pend[K - 1][P];
-      int m = win.before(a, s, t0, rs, ch);      // how many steps before this one are seen
+      for (int j = 0; j < K - 1; ++j)
+        if (j < seen && i - 1 - j < q.n) store(i - 1 - j, pend[j]);
+    };
+    auto clear = [&] {
+      win.zero();
 #pragma unroll
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-        for (int i = 0; i < P; ++i) pend[j][i] = zero;
-      T* pgx = row_out<T>(a.gx, s, t0) + ch;
-      // step i of the part completes gx of step i - (K - 1); before the sequence it is the initial state's
-      auto emit = [&](int i) {
+        for (int k = 0; k < P; ++k) pend[j][k] = zero;
+    };
+    auto shift = [&](const float2 (&g)[P]) {
+#pragma unroll
+      for (int j = K - 2; j > 0; --j)
+#pragma unroll
+        for (int k = 0; k < P; ++k) pend[j][k] = pend[j - 1][k];
+#pragma unroll
+      for (int k = 0; k < P; ++k) pend[0][k] = mul2(taps.w[K - 1][k], g[k]);
+    };
+    if (q.lo == 0) {
+      clear();
+      seen = q.t0 == 0 ? K - 1 : 0;       // what lies before a later part is that part's to store
+      if (q.t0 > 0 || a.state != nullptr) {
+        const uint8_t* rs = q.t0 > 0 ? resets(a.reset, q.s) : nullptr;
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+          if (rs != nullptr && rs[(q.t0 - (K - 1) + j) * a.reset.step] != 0) win.zero();
+          win.push(feed.get(j));
+        }
+      }
+      pgx = row_out<T>(a.gx, q.s, q.t0) + ch;
+    }
+    const int count = q.hi - q.lo;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const Words<T, V> x = feed.get(K - 1 + i), gy = feed.get(K - 1 + CONV_R + i);
+      const int row = q.lo + i;
+      if (cuts >> i & 1) {
+        flush(row);
+        clear();
+        seen = 0;
+        keep_branch();
+      }
+      float2 now[P], g[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        now[k] = x.pair(k);
+        g[k] = gy.pair(k);
+        if (a.act == INB_ACT_SILU) {
+          const float2 p = win.pre(taps, now[k], k), s = sigmoid2(p, V > 1);
+          g[k] = mul2(g[k], mul2(s, fma2(p, fma2(s, both(-1.f), both(1.f)), both(1.f))));
+        }
+      }
+      if (row < q.n) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          gb[k] = add2(gb[k], g[k]);
+          gw[K - 1][k] = fma2(g[k], now[k], gw[K - 1][k]);
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) gw[K - 2 - j][k] = fma2(g[k], win.x[j][k], gw[K - 2 - j][k]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+        for (int k = 0; k < P; ++k) pend[j][k] = fma2(taps.w[K - 2 - j][k], g[k], pend[j][k]);
+      if (row >= K - 1 && seen == K - 1) {
         Words<T, V> p;
 #pragma unroll
-        for (int q = 0; q < P; ++q) p.set(q, pend[K - 2][q]);
-        const int at = i - (K - 1);
-        if (at >= 0) {
-          p.store(pgx);
-          pgx += a.gx.step;
-        } else if (t0 == 0 && a.gstate != nullptr) {
-          p.store((T*)a.gstate + (s * (K - 1) + at + K - 1) * a.C + ch);
-        }
-      };
-      auto shift = [&](const float2 (&g)[P]) {
-#pragma unroll
-        for (int j = K - 2; j > 0; --j)
-#pragma unroll
-          for (int i = 0; i < P; ++i) pend[j][i] = pend[j - 1][i];
-#pragma unroll
-        for (int i = 0; i < P; ++i) pend[0][i] = mul2(taps.w[K - 1][i], g[i]);
-      };
-      for (int i0 = 0; i0 < end; i0 += CONV_U) {
-        if (i0 + CONV_U < end) load(nx, ng, nr, end - i0 - CONV_U);
-#pragma unroll
-        for (int u = 0; u < CONV_U; ++u) {
-          if (i0 + u >= end) break;
-          if (reset[u]) {
-            m = 0;
-            win.zero();
-          }
-          float2 g[P], now[P];
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            now[i] = x[u].pair(i);
-            g[i] = gy[u].pair(i);
-            if (a.act == INB_ACT_SILU) {
-              const float2 p = win.pre(taps, now[i], i);
-              const float2 q = sigmoid2(p, V > 1);
-              g[i] = mul2(g[i], mul2(q, fma2(p, fma2(q, both(-1.f), both(1.f)), both(1.f))));
-            }
-            if (i0 + u < n) {
-              gb[i] = add2(gb[i], g[i]);
-              gw[K - 1][i] = fma2(g[i], now[i], gw[K - 1][i]);
-#pragma unroll
-              for (int j = 0; j < K - 1; ++j) gw[K - 2 - j][i] = fma2(g[i], win.x[j][i], gw[K - 2 - j][i]);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j)
-            if (j < m) {
-#pragma unroll
-              for (int i = 0; i < P; ++i) pend[j][i] = fma2(taps.w[K - 2 - j][i], g[i], pend[j][i]);
-            }
-          emit(i0 + u);
-          shift(g);
-          win.push(now);
-          m = m < K - 1 ? m + 1 : m;
-        }
-#pragma unroll
-        for (int u = 0; u < CONV_U; ++u) x[u] = nx[u], gy[u] = ng[u], reset[u] = nr[u];
+        for (int k = 0; k < P; ++k) p.set(k, pend[K - 2][k]);
+        p.store(pgx);
+      } else if (seen == K - 1) {
+        store(row - (K - 1), pend[K - 2]);
       }
-      // steps beyond the sequence: entry e of the final state is the input of step T - (K - 1) + e
-      for (int i = end; i < n + K - 1; ++i) {
-        const int e = (int)(t0 + i - a.T);
-        if (a.gstate_out != nullptr && K - 1 - e <= m) {
+      if (row >= K - 1) pgx += a.gx.step;
+      shift(g);
+      win.push(now);
+      seen = seen < K - 1 ? seen + 1 : seen;
+    }
+    if (q.hi == q.to && q.lo < q.hi) {
+      // the rows that nothing follows: those of the sequence's end, to which the final state's gradient adds
+      // (its entry e is the input of step T - (K - 1) + e)
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) {
+        const int at = q.to - 1 - j;
+        if (at >= q.n || j >= seen) continue;
+        const int e = (int)(q.t0 + at - a.T) + K - 1;
+        if (a.gstate_out != nullptr && e >= 0) {
           Words<T, V> p;
-          p.load((const T*)a.gstate_out + (s * (K - 1) + e) * a.C + ch);
+          p.load((const T*)a.gstate_out + (q.s * (K - 1) + e) * a.C + ch);
 #pragma unroll
-          for (int q = 0; q < P; ++q) pend[K - 2][q] = add2(pend[K - 2][q], p.pair(q));
+          for (int k = 0; k < P; ++k) pend[j][k] = add2(pend[j][k], p.pair(k));
         }
-        emit(i);
-        float2 none[P];
-#pragma unroll
-        for (int q = 0; q < P; ++q) none[q] = zero;
-        shift(none);
+        store(at, pend[j]);
       }
     }
+  }
+  __syncthreads();                        // the rows' memory holds the block's sums from here on
   // the block's tasks, then one partial row
   const int n = blockDim.x * V * (K + 1);
   float* mine = smem + threadIdx.y * n;
@@ -385,7 +487,7 @@ struct ConvLaunch {
 static ConvLaunch conv_plan(const InbConvArgs& a, int V, int resident) {
   ConvLaunch l;
   const int64_t cv = ceil_div(a.C, V), room = (int64_t)sm_count() * resident;
-  unsigned tx = 1;
+  unsigned tx = 4;                 // the lanes of a task share the reading of its reset flags: CONV_R / 2 of them at least
   while (tx < 128 && tx < cv) tx *= 2;
   l.block = dim3(tx, 128 / tx);
   const int64_t gy = ceil_div(cv, tx);
@@ -425,14 +527,19 @@ static int conv_fwd_go(const InbConvArgs& a, cudaStream_t s) {
     conv_step_kernel<T, V, K><<<l.grid, l.block, 0, s>>>(a);
   } else {
     const ConvLaunch l = conv_plan(a, V, CONV_FWD_BLOCKS);
-    conv_fwd_kernel<T, V, K><<<l.grid, l.block, 0, s>>>(a, l.plan);
+    const cudaError_t e = allow_smem<KernelKey<conv_fwd_kernel<T, V, K>>>((const void*)conv_fwd_kernel<T, V, K>, 2 * Feed<T, V, K, 1>::STAGE);
+    if (e != cudaSuccess) return -100 - (int)e;
+    conv_fwd_kernel<T, V, K><<<l.grid, l.block, 2 * Feed<T, V, K, 1>::STAGE, s>>>(a, l.plan);
   }
   return launch_status();
 }
 template <typename T, int V, int K>
 static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
   const ConvLaunch l = conv_plan(a, V, CONV_BWD_BLOCKS);
-  conv_bwd_kernel<T, V, K><<<l.grid, l.block, 128 * V * (K + 1) * 4, s>>>(a, l.plan);
+  constexpr int rows = 2 * Feed<T, V, K, 2>::STAGE, sums = 128 * V * (K + 1) * 4, smem = rows > sums ? rows : sums;
+  const cudaError_t e = allow_smem<KernelKey<conv_bwd_kernel<T, V, K>>>((const void*)conv_bwd_kernel<T, V, K>, smem);
+  if (e != cudaSuccess) return -100 - (int)e;
+  conv_bwd_kernel<T, V, K><<<l.grid, l.block, smem, s>>>(a, l.plan);
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
 }

@@ -39,9 +39,6 @@ int scan_check(const InbScanArgs& a);
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s);
 int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool reverse, cudaStream_t s);
 
-// In a branch that the whole warp takes or skips, and seldom takes: keeps the compiler from running its moves on every step
-__device__ __forceinline__ void keep_branch() { __syncwarp(); }
-
 // The reset flag of this lane's step among the next `steps` (lanes beyond: 0); a ballot makes them the same bits in every lane
 __device__ __forceinline__ uint32_t reset_flag(const uint8_t* at, int64_t step, int steps, int lane) {
   return at != nullptr && lane < steps ? at[lane * step] : 0u;

@@ -176,6 +176,9 @@ __device__ __forceinline__ const uint8_t* resets(const InbReset& r, int64_t s) {
   return r.p == nullptr ? nullptr : r.p + (uint32_t)s / (uint32_t)r.rows * r.seq;
 }
 
+// In a branch that is seldom taken: keeps the compiler from running its moves on every step
+__device__ __forceinline__ void keep_branch() { __syncwarp(__activemask()); }
+
 inline bool is_aligned(const InbSeq& q, int64_t bytes, int64_t elem) {
   return q.p == nullptr || (((uint64_t)(uintptr_t)q.p | (uint64_t)(q.seq * elem) | (uint64_t)(q.step * elem)) & (bytes - 1)) == 0;
 }
