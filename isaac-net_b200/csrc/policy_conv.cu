@@ -11,7 +11,6 @@
 namespace inb {
 namespace pol {
 
-constexpr int CONV_R = 8;       // rows of a chunk
 constexpr int CONV_FWD_BLOCKS = 4, CONV_STEP_BLOCKS = 4, CONV_BWD_BLOCKS = 4;      // of 128 threads, an SM
 constexpr int CONV_STEP_B = 2;  // sequences whose loads are sent at once by a single step
 
@@ -19,19 +18,61 @@ struct ConvPlan {
   int64_t parts, len, tasks;    // parts of the time axis, their steps; sequences x parts
 };
 
-// V neighbouring channels as pairs (V = 1: the first of one pair)
+// A thread's V channels: neighbours, moved by one access of V sizeof(T) bytes where every row is aligned to that, or (WIDE
+// false) blockDim.x apart, each moved by itself, so that a warp's accesses still lie side by side.
+template <typename T, int V, bool WIDE>
+struct Lanes {
+  int64_t first;
+  int gap, count, x;              // count: those below C
+  __device__ __forceinline__ Lanes(const InbConvArgs& a) : gap(WIDE ? 1 : (int)blockDim.x), x(threadIdx.x) {
+    const int64_t c0 = (int64_t)blockIdx.y * blockDim.x * V;
+    first = WIDE ? c0 + x * V : c0 + x;
+    const int64_t left = a.C - first;
+    count = left <= 0 ? 0 : WIDE ? V : (int)((left + gap - 1) / gap < V ? (left + gap - 1) / gap : V);
+  }
+  __device__ __forceinline__ int64_t at(int v) const { return first + (int64_t)v * gap; }
+  __device__ __forceinline__ int local(int v) const { return WIDE ? x * V + v : v * gap + x; }      // in the block's blockDim.x V channels
+  __device__ __forceinline__ void load(Words<T, V>& w, const T* row) const {
+    if constexpr (WIDE) {
+      w.load(row + first);
+    } else {
+      uint32_t e[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        e[v] = 0;
+        if (v < count) e[v] = ld_raw(row + at(v));
+      }
+      w.join(e);
+    }
+  }
+  __device__ __forceinline__ void store(T* row, const Words<T, V>& w) const {
+    if constexpr (WIDE) {
+      w.store(row + first);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (v < count) {
+          if constexpr (sizeof(T) == 4)
+            reinterpret_cast<uint32_t*>(row)[at(v)] = w.w[v];
+          else
+            reinterpret_cast<uint16_t*>(row)[at(v)] = (uint16_t)(v & 1 ? w.w[v / 2] >> 16 : w.w[v / 2]);
+        }
+    }
+  }
+};
+// The weights of a thread's channels, as pairs
 template <typename T, int V, int K>
 struct Taps {
   static constexpr int P = Words<T, V>::P;
   float2 w[K][P], bias[P];
-  __device__ __forceinline__ void load(const InbConvArgs& a, int64_t ch, bool on) {
-    auto get = [&](const void* p, int64_t i) { return on && p != nullptr ? to_f(((const T*)p)[i]) : 0.f; };
+  template <bool WIDE>
+  __device__ __forceinline__ void load(const InbConvArgs& a, const Lanes<T, V, WIDE>& io) {
+    auto get = [&](const void* p, int v, int64_t of, int64_t k) { return v < io.count && p != nullptr ? to_f(((const T*)p)[io.at(v) * of + k]) : 0.f; };
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const int64_t c = ch + 2 * i;
-      bias[i] = make_float2(get(a.bias, c), V > 1 ? get(a.bias, c + 1) : 0.f);
+      bias[i] = make_float2(get(a.bias, 2 * i, 1, 0), get(a.bias, 2 * i + 1, 1, 0));
 #pragma unroll
-      for (int k = 0; k < K; ++k) w[k][i] = make_float2(get(a.w, c * K + k), V > 1 ? get(a.w, (c + 1) * K + k) : 0.f);
+      for (int k = 0; k < K; ++k) w[k][i] = make_float2(get(a.w, 2 * i, K, k), get(a.w, 2 * i + 1, K, k));
     }
   }
 };
@@ -68,15 +109,18 @@ struct Window {
   }
 };
 // ---------------------------------------------------------------------------------------------- rows on their way
-// A task's rows go by chunks of CONV_R through memory that the thread alone writes and reads (no barrier): while one chunk is
+// A task's rows go by chunks through memory that the thread alone writes and reads (no barrier): while one chunk is
 // worked on, the next one's rows, the next task's among them, are on their way by cp.async; rows of 2 bytes, which cp.async
 // cannot move, by registers.  A task's first chunk also brings the K - 1 rows before it, of the state or of the part before.
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // STREAMS 2: x and gy, whose rows end with those that reach back into the part
-template <typename T, int V, int K, int STREAMS>
+template <typename T, int V, bool WIDE, int K, int STREAMS>
 struct Feed {
-  static constexpr int B = V * sizeof(T), ROWS = K - 1 + CONV_R * STREAMS, STAGE = ROWS * 128 * B;
+  static constexpr bool HELD = !WIDE && sizeof(T) == 2;        // by registers
+  static constexpr int R = HELD ? 4 : 8;                       // rows of a chunk
+  static constexpr int B = V * sizeof(T), ROWS = K - 1 + R * STREAMS, STAGE = ROWS * 128 * B;
+  using Io = Lanes<T, V, WIDE>;
   // a chunk: sequence s, rows [lo, hi) of its part [t0, t0 + n)
   struct Chunk {
     int64_t task, s, t0;
@@ -84,30 +128,35 @@ struct Feed {
     bool on;
   };
   char* base;
-  uint32_t held[B < 4 ? ROWS : 1];
+  uint32_t held[HELD ? ROWS * V : 1];
   uint32_t flag[2];
   int64_t stride, rounds, round;
   int chunks, chunk, tx, lane, stage;
   Chunk next;
   __device__ __forceinline__ char* slot(int st, int row) const { return base + st * STAGE + row * 128 * B; }
-  __device__ __forceinline__ void put(int row, const T* p) {
-    if constexpr (B < 4)
-      held[row] = ld_raw(p);
-    else if constexpr (B == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(slot(stage, row))), "l"(p) : "memory");
-    else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_at(slot(stage, row))), "l"(p), "n"(B) : "memory");
+  __device__ __forceinline__ void put(const Io& io, int row, const T* p) {
+    if constexpr (WIDE && B == 16) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(slot(stage, row))), "l"(p + io.first) : "memory");
+    } else if constexpr (WIDE) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_at(slot(stage, row))), "l"(p + io.first), "n"(B) : "memory");
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (v < io.count) {
+          if constexpr (HELD)
+            held[row * V + v] = ld_raw(p + io.at(v));
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(slot(stage, row)) + 4 * v), "l"(p + io.at(v)) : "memory");
+        }
+    }
   }
   __device__ __forceinline__ Words<T, V> get(int row) const {      // of the chunk that now() gave
     Words<T, V> w;
-    if constexpr (B == 2)
-      w.w[0] = *(const uint16_t*)slot(stage ^ 1, row);
-    else
-      w.load((const T*)slot(stage ^ 1, row));
+    w.load((const T*)slot(stage ^ 1, row));
     return w;
   }
-  __device__ __forceinline__ void place(const InbConvArgs& a, const ConvPlan& pl, int64_t ch) {
-    next.lo = chunk * CONV_R;
+  __device__ __forceinline__ void place(const InbConvArgs& a, const ConvPlan& pl) {
+    next.lo = chunk * R;
     if (chunk == 0) {
       next.on = next.task < pl.tasks;
       const int64_t part = pl.parts > 1 ? next.task / a.S : 0;      // the next task: the same steps of the next sequence
@@ -117,47 +166,47 @@ struct Feed {
       next.n = (int)(pl.len < left ? pl.len : left);
       next.to = STREAMS == 1 ? next.n : next.n + K - 1 < left ? next.n + K - 1 : (int)left;
     }
-    next.hi = next.lo + CONV_R < next.to ? next.lo + CONV_R : next.to;
+    next.hi = next.lo + R < next.to ? next.lo + R : next.to;
   }
-  __device__ __forceinline__ void send(const InbConvArgs& a, int64_t ch) {
+  __device__ __forceinline__ void send(const InbConvArgs& a, const Io& io) {
     flag[0] = flag[1] = 0;
     if (next.on && next.lo < next.hi) {
       const int count = next.hi - next.lo;
-      if (ch < a.C) rows(a, ch, count);
+      if (io.count > 0) rows(a, io, count);
       const uint8_t* rs = resets(a.reset, next.s);
       if (rs != nullptr) {
         rs += (next.t0 + next.lo) * a.reset.step;
         const int l = threadIdx.x & 31;           // the lanes of a task read its flags together, those beyond the channels too
-        if (l < CONV_R && l < count) flag[0] = rs[l * a.reset.step];
+        if (l < R && l < count) flag[0] = rs[l * a.reset.step];
         if (tx == 4 && l + 4 < count) flag[1] = rs[(l + 4) * a.reset.step];
       }
     }
-    if constexpr (B >= 4) asm volatile("cp.async.commit_group;" ::: "memory");
+    if constexpr (!HELD) asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ void rows(const InbConvArgs& a, int64_t ch, int count) {
-    const T* p = row<T>(a.x, next.s, next.t0 + next.lo) + ch;
-    const T* g = STREAMS > 1 ? row<T>(a.gy, next.s, next.t0 + next.lo) + ch : nullptr;
+  __device__ __forceinline__ void rows(const InbConvArgs& a, const Io& io, int count) {
+    const T* p = row<T>(a.x, next.s, next.t0 + next.lo);
+    const T* g = STREAMS > 1 ? row<T>(a.gy, next.s, next.t0 + next.lo) : nullptr;
 #pragma unroll
-    for (int i = 0; i < CONV_R; ++i)
+    for (int i = 0; i < R; ++i)
       if (i < count) {
-        put(K - 1 + i, p);
+        put(io, K - 1 + i, p);
         p += a.x.step;
         if (STREAMS > 1) {
-          put(K - 1 + CONV_R + i, g);
+          put(io, K - 1 + R + i, g);
           g += a.gy.step;
         }
       }
     if (chunk == 0 && (next.t0 > 0 || a.state != nullptr)) {
       const bool state = next.t0 == 0;
-      const T* h = state ? (const T*)a.state + next.s * a.state_seq + ch : row<T>(a.x, next.s, next.t0 - (K - 1)) + ch;
+      const T* h = state ? (const T*)a.state + next.s * a.state_seq : row<T>(a.x, next.s, next.t0 - (K - 1));
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
-        put(j, h);
+        put(io, j, h);
         h += state ? a.C : a.x.step;
       }
     }
   }
-  __device__ __forceinline__ void start(const InbConvArgs& a, const ConvPlan& pl, char* smem, int64_t ch) {
+  __device__ __forceinline__ void start(const InbConvArgs& a, const ConvPlan& pl, char* smem, const Io& io) {
     tx = blockDim.x;
     const int id = threadIdx.y * tx + threadIdx.x;
     base = smem + id * B;
@@ -165,19 +214,23 @@ struct Feed {
     stride = (int64_t)gridDim.x * blockDim.y;
     rounds = (pl.tasks + stride - 1) / stride;
     const int64_t rows = pl.parts > 1 && STREAMS > 1 ? pl.len + K - 1 : pl.len;
-    chunks = (int)((rows + CONV_R - 1) / CONV_R);
+    chunks = (int)((rows + R - 1) / R);
     round = chunk = stage = 0;
     next.task = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    place(a, pl, ch);
-    send(a, ch);
+    place(a, pl);
+    send(a, io);
   }
   __device__ __forceinline__ bool more() const { return round < rounds; }      // the same for every thread of the block
   // the next chunk, landed; bit i of `cuts`: its row i starts an episode.  The chunk after it is sent for.
-  __device__ __forceinline__ Chunk now(const InbConvArgs& a, const ConvPlan& pl, int64_t ch, uint32_t& cuts) {
+  __device__ __forceinline__ Chunk now(const InbConvArgs& a, const ConvPlan& pl, const Io& io, uint32_t& cuts) {
     const Chunk c = next;
-    if constexpr (B < 4) {
+    if constexpr (HELD) {
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) *(uint16_t*)slot(stage, i) = (uint16_t)held[i];
+      for (int i = 0; i < ROWS; ++i) {
+        Words<T, V> w;
+        w.join(reinterpret_cast<const uint32_t(&)[V]>(held[i * V]));
+        w.store((T*)slot(stage, i));
+      }
     }
     const int first = lane & ~((tx < 32 ? tx : 32) - 1);
     cuts = __ballot_sync(0xFFFFFFFFu, flag[0] != 0) >> first & (tx == 4 ? 0xFu : 0xFFu);
@@ -185,33 +238,33 @@ struct Feed {
     stage ^= 1;
     if (++chunk == chunks) chunk = 0, ++round, next.task += stride;
     if (round < rounds) {
-      place(a, pl, ch);
-      send(a, ch);
-    } else if constexpr (B >= 4) {
+      place(a, pl);
+      send(a, io);
+    } else if constexpr (!HELD) {
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    if constexpr (B >= 4) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if constexpr (!HELD) asm volatile("cp.async.wait_group 1;" ::: "memory");
     return c;
   }
 };
 
 // ---------------------------------------------------------------------------------------------- forward
 // A block is blockDim.x channel vectors x blockDim.y tasks and strides over the tasks, so that weights are read once.
-template <typename T, int V, int K>
+template <typename T, int V, bool WIDE, int K>
 __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvArgs a, ConvPlan pl) {
   constexpr int P = Words<T, V>::P;
   extern __shared__ float4 smem4[];
-  const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-  Feed<T, V, K, 1> feed;
-  feed.start(a, pl, (char*)smem4, ch);
+  const Lanes<T, V, WIDE> io(a);
+  Feed<T, V, WIDE, K, 1> feed;
+  feed.start(a, pl, (char*)smem4, io);
   Taps<T, V, K> taps;
-  taps.load(a, ch, ch < a.C);
+  taps.load(a, io);
   Window<T, V, K> win;
   T* py = nullptr;
   while (feed.more()) {
     uint32_t cuts;
-    const auto q = feed.now(a, pl, ch, cuts);
-    if (!q.on || ch >= a.C) continue;
+    const auto q = feed.now(a, pl, io, cuts);
+    if (!q.on || io.count == 0) continue;
     if (q.lo == 0) {
       win.zero();
       if (q.t0 > 0 || a.state != nullptr) {
@@ -222,7 +275,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
           win.push(feed.get(j));
         }
       }
-      py = row_out<T>(a.y, q.s, q.t0) + ch;
+      py = row_out<T>(a.y, q.s, q.t0);
     }
     const int count = q.hi - q.lo;
 #pragma unroll 4
@@ -238,33 +291,33 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
       for (int k = 0; k < P; ++k) {
         now[k] = x.pair(k);
         const float2 p = win.pre(taps, now[k], k);
-        y.set(k, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
+        y.set(k, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p)) : p);
       }
-      y.store(py);
+      io.store(py, y);
       py += a.y.step;
       win.push(now);
     }
     if (q.hi == q.n && q.lo < q.hi && q.t0 + q.n == a.T && a.state_out != nullptr) {
-      T* out = (T*)a.state_out + q.s * a.state_out_seq + ch;
+      T* out = (T*)a.state_out + q.s * a.state_out_seq;
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) {
         Words<T, V> p;
 #pragma unroll
         for (int k = 0; k < P; ++k) p.set(k, win.x[j][k]);      // what was read, or 0: exact
-        p.store(out + (K - 2 - j) * a.C);
+        io.store(out + (K - 2 - j) * a.C, p);
       }
     }
   }
 }
 
 // One step: bound by the states' bytes, of which a thread has CONV_STEP_B sequences' on their way at once; state_out may be state.
-template <typename T, int V, int K>
+template <typename T, int V, bool WIDE, int K>
 __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbConvArgs a) {
   constexpr int P = Words<T, V>::P;
-  const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (ch >= a.C) return;
+  const Lanes<T, V, WIDE> io(a);
+  if (io.count == 0) return;
   Taps<T, V, K> taps;
-  taps.load(a, ch, true);
+  taps.load(a, io);
   const int64_t stride = (int64_t)gridDim.x * blockDim.y;
   for (int64_t s0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; s0 < a.S; s0 += stride * CONV_STEP_B) {
     Words<T, V> x[CONV_STEP_B], old[CONV_STEP_B][K - 1];
@@ -273,12 +326,12 @@ __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbCon
     for (int b = 0; b < CONV_STEP_B; ++b) {
       const int64_t s = s0 + b * stride;
       if (s >= a.S) break;
-      x[b].load(row<T>(a.x, s, 0) + ch);
+      io.load(x[b], row<T>(a.x, s, 0));
       reset[b] = a.reset.p != nullptr ? *resets(a.reset, s) : 0;
       if (a.state != nullptr) {
-        const T* p = (const T*)a.state + s * a.state_seq + ch;
+        const T* p = (const T*)a.state + s * a.state_seq;
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) old[b][j].load(p + j * a.C);
+        for (int j = 0; j < K - 1; ++j) io.load(old[b][j], p + j * a.C);
       }
     }
 #pragma unroll
@@ -297,14 +350,14 @@ __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbCon
         float2 p = fma2(x[b].pair(i), taps.w[K - 1][i], taps.bias[i]);
 #pragma unroll
         for (int j = K - 2; j >= 0; --j) p = fma2(old[b][j].pair(i), taps.w[j][i], p);
-        y.set(i, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p, V > 1)) : p);
+        y.set(i, a.act == INB_ACT_SILU ? mul2(p, sigmoid2(p)) : p);
       }
-      y.store(row_out<T>(a.y, s, 0) + ch);
+      io.store(row_out<T>(a.y, s, 0), y);
       if (a.state_out != nullptr) {
-        T* out = (T*)a.state_out + s * a.state_out_seq + ch;
+        T* out = (T*)a.state_out + s * a.state_out_seq;
 #pragma unroll
-        for (int j = 0; j < K - 2; ++j) old[b][j + 1].store(out + j * a.C);
-        x[b].store(out + (K - 2) * a.C);
+        for (int j = 0; j < K - 2; ++j) io.store(out + j * a.C, old[b][j + 1]);
+        io.store(out + (K - 2) * a.C, x[b]);
       }
     }
   }
@@ -315,15 +368,14 @@ __global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbCon
 // the K - 1 before it are complete already: they are stored there, and what is gathered for them afterwards is dropped.  A part
 // goes K - 1 steps beyond its end, for gx alone.  Blocks as in the forward pass, so that gw and gbias stay in registers; one
 // partial row a block, [C K | C], added by a second launch.
-template <typename T, int V, int K>
+template <typename T, int V, bool WIDE, int K>
 __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvArgs a, ConvPlan pl) {
   constexpr int P = Words<T, V>::P;
   extern __shared__ float4 smem4[];
   float* smem = (float*)smem4;
-  const int64_t ch = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
-  const bool on = ch < a.C;
+  const Lanes<T, V, WIDE> io(a);
   Taps<T, V, K> taps;
-  taps.load(a, ch, on);
+  taps.load(a, io);
   const float2 zero = make_float2(0.f, 0.f);
   float2 gw[K][P], gb[P];
 #pragma unroll
@@ -336,21 +388,21 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
   float2 pend[K - 1][P];
   int seen = 0;                           // rows since the episode or the part began, up to K - 1
   T* pgx = nullptr;
-  Feed<T, V, K, 2> feed;
-  feed.start(a, pl, (char*)smem, ch);
+  Feed<T, V, WIDE, K, 2> feed;
+  feed.start(a, pl, (char*)smem, io);
   while (feed.more()) {
     uint32_t cuts;
-    const auto q = feed.now(a, pl, ch, cuts);
-    if (!q.on || ch >= a.C) continue;
+    const auto q = feed.now(a, pl, io, cuts);
+    if (!q.on || io.count == 0) continue;
     // gx of the row `at` (pgx's) is complete; before the sequence it is the initial state's
     auto store = [&](int at, const float2 (&v)[P]) {
       Words<T, V> p;
 #pragma unroll
       for (int k = 0; k < P; ++k) p.set(k, v[k]);
       if (at >= 0)
-        p.store(row_out<T>(a.gx, q.s, q.t0 + at) + ch);
+        io.store(row_out<T>(a.gx, q.s, q.t0 + at), p);
       else if (q.t0 == 0 && a.gstate != nullptr)
-        p.store((T*)a.gstate + (q.s * (K - 1) + at + K - 1) * a.C + ch);
+        io.store((T*)a.gstate + (q.s * (K - 1) + at + K - 1) * a.C, p);
     };
     // an episode begins at row i: the rows before it are complete, but for those that were when the last one began
     auto flush = [&](int i) {
@@ -384,12 +436,12 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
           win.push(feed.get(j));
         }
       }
-      pgx = row_out<T>(a.gx, q.s, q.t0) + ch;
+      pgx = row_out<T>(a.gx, q.s, q.t0);
     }
     const int count = q.hi - q.lo;
 #pragma unroll 4
     for (int i = 0; i < count; ++i) {
-      const Words<T, V> x = feed.get(K - 1 + i), gy = feed.get(K - 1 + CONV_R + i);
+      const Words<T, V> x = feed.get(K - 1 + i), gy = feed.get(K - 1 + feed.R + i);
       const int row = q.lo + i;
       if (cuts >> i & 1) {
         flush(row);
@@ -403,7 +455,7 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
         now[k] = x.pair(k);
         g[k] = gy.pair(k);
         if (a.act == INB_ACT_SILU) {
-          const float2 p = win.pre(taps, now[k], k), s = sigmoid2(p, V > 1);
+          const float2 p = win.pre(taps, now[k], k), s = sigmoid2(p);
           g[k] = mul2(g[k], mul2(s, fma2(p, fma2(s, both(-1.f), both(1.f)), both(1.f))));
         }
       }
@@ -424,7 +476,7 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
         Words<T, V> p;
 #pragma unroll
         for (int k = 0; k < P; ++k) p.set(k, pend[K - 2][k]);
-        p.store(pgx);
+        io.store(pgx, p);
       } else if (seen == K - 1) {
         store(row - (K - 1), pend[K - 2]);
       }
@@ -443,7 +495,7 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
         const int e = (int)(q.t0 + at - a.T) + K - 1;
         if (a.gstate_out != nullptr && e >= 0) {
           Words<T, V> p;
-          p.load((const T*)a.gstate_out + (q.s * (K - 1) + e) * a.C + ch);
+          io.load(p, (const T*)a.gstate_out + (q.s * (K - 1) + e) * a.C);
 #pragma unroll
           for (int k = 0; k < P; ++k) pend[j][k] = add2(pend[j][k], p.pair(k));
         }
@@ -458,8 +510,8 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
 #pragma unroll
   for (int v = 0; v < V; ++v) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) mine[(threadIdx.x * V + v) * K + k] = v & 1 ? gw[k][v / 2].y : gw[k][v / 2].x;
-    mine[blockDim.x * V * K + threadIdx.x * V + v] = v & 1 ? gb[v / 2].y : gb[v / 2].x;
+    for (int k = 0; k < K; ++k) mine[io.local(v) * K + k] = v & 1 ? gw[k][v / 2].y : gw[k][v / 2].x;
+    mine[blockDim.x * V * K + io.local(v)] = v & 1 ? gb[v / 2].y : gb[v / 2].x;
   }
   __syncthreads();
   const int64_t c0 = (int64_t)blockIdx.y * blockDim.x * V;
@@ -487,8 +539,11 @@ struct ConvLaunch {
 static ConvLaunch conv_plan(const InbConvArgs& a, int V, int resident) {
   ConvLaunch l;
   const int64_t cv = ceil_div(a.C, V), room = (int64_t)sm_count() * resident;
-  unsigned tx = 4;                 // the lanes of a task share the reading of its reset flags: CONV_R / 2 of them at least
-  while (tx < 128 && tx < cv) tx *= 2;
+  // lanes of a task: as few beyond the last channel as may be, the more the better; 4 at least, which share the reading of the
+  // task's reset flags
+  unsigned tx = 128;
+  for (unsigned t = 64; t >= (cv >= 16 ? 16 : 4); t /= 2)
+    if (ceil_div(cv, t) * t < ceil_div(cv, tx) * tx) tx = t;
   l.block = dim3(tx, 128 / tx);
   const int64_t gy = ceil_div(cv, tx);
   int64_t parts = ceil_div(room * l.block.y, a.S * gy);
@@ -520,52 +575,47 @@ static int conv_check(const InbConvArgs& a) {
   return 0;
 }
 
-template <typename T, int V, int K>
+template <typename T, int V, bool WIDE, int K>
 static int conv_fwd_go(const InbConvArgs& a, cudaStream_t s) {
   if (a.T == 1) {
     const ConvLaunch l = conv_plan(a, V, CONV_STEP_BLOCKS);
-    conv_step_kernel<T, V, K><<<l.grid, l.block, 0, s>>>(a);
-  } else {
-    const ConvLaunch l = conv_plan(a, V, CONV_FWD_BLOCKS);
-    const cudaError_t e = allow_smem<KernelKey<conv_fwd_kernel<T, V, K>>>((const void*)conv_fwd_kernel<T, V, K>, 2 * Feed<T, V, K, 1>::STAGE);
-    if (e != cudaSuccess) return -100 - (int)e;
-    conv_fwd_kernel<T, V, K><<<l.grid, l.block, 2 * Feed<T, V, K, 1>::STAGE, s>>>(a, l.plan);
+    conv_step_kernel<T, V, WIDE, K><<<l.grid, l.block, 0, s>>>(a);
+    return launch_status();
   }
+  constexpr auto kernel = conv_fwd_kernel<T, V, WIDE, K>;
+  constexpr int smem = 2 * Feed<T, V, WIDE, K, 1>::STAGE;
+  const cudaError_t e = allow_smem<KernelKey<conv_fwd_kernel<T, V, WIDE, K>>>((const void*)kernel, smem);
+  if (e != cudaSuccess) return -100 - (int)e;
+  const ConvLaunch l = conv_plan(a, V, CONV_FWD_BLOCKS);
+  kernel<<<l.grid, l.block, smem, s>>>(a, l.plan);
   return launch_status();
 }
-template <typename T, int V, int K>
+template <typename T, int V, bool WIDE, int K>
 static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
-  const ConvLaunch l = conv_plan(a, V, CONV_BWD_BLOCKS);
-  constexpr int rows = 2 * Feed<T, V, K, 2>::STAGE, sums = 128 * V * (K + 1) * 4, smem = rows > sums ? rows : sums;
-  const cudaError_t e = allow_smem<KernelKey<conv_bwd_kernel<T, V, K>>>((const void*)conv_bwd_kernel<T, V, K>, smem);
+  constexpr auto kernel = conv_bwd_kernel<T, V, WIDE, K>;
+  constexpr int rows = 2 * Feed<T, V, WIDE, K, 2>::STAGE, sums = 128 * V * (K + 1) * 4, smem = rows > sums ? rows : sums;
+  const cudaError_t e = allow_smem<KernelKey<conv_bwd_kernel<T, V, WIDE, K>>>((const void*)kernel, smem);
   if (e != cudaSuccess) return -100 - (int)e;
-  conv_bwd_kernel<T, V, K><<<l.grid, l.block, smem, s>>>(a, l.plan);
+  const ConvLaunch l = conv_plan(a, V, CONV_BWD_BLOCKS);
+  kernel<<<l.grid, l.block, smem, s>>>(a, l.plan);
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
 }
-// Channels a thread: 16 bytes (forward) or 4 channels (backward, whose sums take the registers), moved by one access, where
-// every row allows it, else one.
-template <typename T>
-static int conv_width(const InbConvArgs& a, bool backward) {
-  const int v = backward ? 4 : 16 / (int)sizeof(T);
-  return conv_aligned(a, v * sizeof(T)) ? v : 1;
+// Channels a thread: 16 bytes forward, 4 channels backward, whose sums take the registers; 4 where rows are not aligned to that
+template <typename T, bool WIDE>
+static int conv_go(const InbConvArgs& a, bool backward, cudaStream_t s) {
+  constexpr int W = WIDE ? 16 / sizeof(T) : 4;
+  if (backward) return a.K == 2 ? conv_bwd_go<T, 4, WIDE, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 4, WIDE, 3>(a, s) : conv_bwd_go<T, 4, WIDE, 4>(a, s);
+  return a.K == 2 ? conv_fwd_go<T, W, WIDE, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, W, WIDE, 3>(a, s) : conv_fwd_go<T, W, WIDE, 4>(a, s);
 }
 template <typename T>
-static int conv_go(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  constexpr int W = 16 / sizeof(T);
-  if (backward) {
-    if (conv_width<T>(a, true) == 4)
-      return a.K == 2 ? conv_bwd_go<T, 4, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 4, 3>(a, s) : conv_bwd_go<T, 4, 4>(a, s);
-    return a.K == 2 ? conv_bwd_go<T, 1, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 1, 3>(a, s) : conv_bwd_go<T, 1, 4>(a, s);
-  }
-  if (conv_width<T>(a, false) == W)
-    return a.K == 2 ? conv_fwd_go<T, W, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, W, 3>(a, s) : conv_fwd_go<T, W, 4>(a, s);
-  return a.K == 2 ? conv_fwd_go<T, 1, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, 1, 3>(a, s) : conv_fwd_go<T, 1, 4>(a, s);
+static int conv_type(const InbConvArgs& a, bool backward, cudaStream_t s) {
+  return conv_aligned(a, backward ? 4 * sizeof(T) : 16) ? conv_go<T, true>(a, backward, s) : conv_go<T, false>(a, backward, s);
 }
 static int conv_dispatch(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  if (a.dtype == INB_BF16) return conv_go<bf16>(a, backward, s);
-  if (a.dtype == INB_F16) return conv_go<f16>(a, backward, s);
-  return conv_go<float>(a, backward, s);
+  if (a.dtype == INB_BF16) return conv_type<bf16>(a, backward, s);
+  if (a.dtype == INB_F16) return conv_type<f16>(a, backward, s);
+  return conv_type<float>(a, backward, s);
 }
 
 }  // namespace pol
@@ -588,8 +638,7 @@ extern "C" int inb_causal_conv_work(const InbConvArgs* args, int64_t* elems) {
   if (rc != 0) return rc;
   *elems = 0;
   if (a.S == 0 || a.T == 0) return 0;
-  const int v = a.dtype == INB_F32 ? inb::pol::conv_width<float>(a, true) : inb::pol::conv_width<inb::pol::bf16>(a, true);
-  *elems = (int64_t)inb::pol::conv_plan(a, v, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
+  *elems = (int64_t)inb::pol::conv_plan(a, 4, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
   return 0;
 }
 

@@ -22,8 +22,6 @@ __device__ __forceinline__ float rcp(float v) {      // 1 / v, 1 ulp
 }
 __device__ __forceinline__ float sigmoid(float v) { return rcp(1.f + ex2(-v * LOG2E)); }
 
-// two at once; of the second only if asked for, so that a lone value costs its own special functions alone
-__device__ __forceinline__ float2 sigmoid2(float2 v, bool two = true);
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("add.rn.f32x2 %0, %1, %2;"
@@ -31,10 +29,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return d;
 }
-__device__ __forceinline__ float2 sigmoid2(float2 v, bool two) {
-  const float2 t = mul2(v, both(-LOG2E));
-  const float2 d = add2(make_float2(ex2(t.x), two ? ex2(t.y) : 0.f), both(1.f));
-  return make_float2(rcp(d.x), two ? rcp(d.y) : 0.f);
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  const float2 t = mul2(v, both(-LOG2E)), d = add2(make_float2(ex2(t.x), ex2(t.y)), both(1.f));
+  return make_float2(rcp(d.x), rcp(d.y));
 }
 // 2^v of two values without the special function unit, which makes 16 results a clock and SM and so bounds the scan: v = i + f,
 // f in [-1/2, 1/2], 2^f = 1 + f P(f) with P the Chebyshev interpolation of (2^f - 1) / f of degree 5 (at most 1.2 * 2^-24
@@ -135,6 +132,10 @@ struct Words {
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else
       *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void join(const uint32_t (&e)[V]) {      // of elements as ld_raw gives them
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = sizeof(T) == 4 || V == 1 ? e[i] : e[(2 * i) % V] | e[(2 * i + 1) % V] << 16;
   }
   __device__ __forceinline__ float2 pair(int i) const {
     if constexpr (V == 1)
