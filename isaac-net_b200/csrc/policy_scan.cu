@@ -150,17 +150,20 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
     const uint32_t bits = __ballot_sync(0xFFFFFFFFu, flag != 0);
     if (ahead > 0) load(ahead);
     __syncwarp();
+    float delta = 0.f;                 // the chunk's sum
 #pragma unroll 2
     for (int i = 0; i < steps; ++i) {
       const float4 in = stage[warp][i][lane];
       const float2 D = both(in.x), U = both(in.y);
       const bool cut = bits >> i & 1;
-      if (MODE >= 2) fresh |= cut, dsum += in.x;
+      if (MODE >= 2) fresh |= cut;
       if (!BACK && cut) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) h[n] = make_float2(0.f, 0.f);
+        delta = 0.f;
         keep_branch();
       }
+      delta += in.x;
       float2 y = make_float2(0.f, 0.f);
 #pragma unroll
       for (int n = 0; n < NH; n += 2) {
@@ -192,6 +195,9 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
         py += a.y.step;
       }
     }
+    dsum += delta;
+#pragma unroll
+    for (int n = POLY; n < NH; ++n) h[n] = unbias(h[n], A[n], both(delta));
   }
   if (!on) return;
   if (MODE >= 2 && j == 0) carry[a.S * pl.parts * a.C * n4 + (s * pl.parts + part) * a.C + ch] = fresh ? -1.f : dsum;
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 // channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.
 constexpr int STEP_THREADS = 256, STEP_B = 2;
 template <typename T, int V, int G>
-__global__ void __launch_bounds__(STEP_THREADS, 3) scan_step_kernel(InbScanArgs a, int lanes, int per) {
+__global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs a, int lanes, int per) {
   const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
   const int c0 = blockIdx.x * chans + threadIdx.x / lanes;
   const bool on = c0 < a.C;

@@ -39,6 +39,16 @@ int scan_check(const InbScanArgs& a);
 int scan_launch(const InbScanArgs& a, const ScanPlan& p, float* carry, int mode, cudaStream_t s);
 int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool reverse, cudaStream_t s);
 
+// ex2.approx is low: measured on a B200, by 0.1 * 2^-24 on average for results 2^-v with v below 2^-9, by 0.3 to 0.45 for v from
+// 2^-8 to 1/4, by 0.6 to 0.85 beyond.  A state that fades slowly multiplies hundreds of such decays, whose random errors average
+// out and whose common one adds up (1.7e-6 of a state after 90 steps of 0.01).  So once a chunk a state is raised by what its
+// decays have lost: `delta`, the chunk's sum, times -a, held to what a state keeps of a chunk.
+__device__ __forceinline__ float2 unbias(float2 h, float2 a, float2 delta) {
+  const float2 t = mul2(mul2(delta, both(-1.f)), a), low = mul2(t, both(78.f)), high = fma2(t, both(-0.4f), both(3.2f));
+  const float2 k = make_float2(fmaxf(0.f, fminf(low.x, high.x)), fmaxf(0.f, fminf(low.y, high.y)));
+  return fma2(h, mul2(k, both(1.f / 16777216)), h);
+}
+
 // The reset flag of this lane's step among the next `steps` (lanes beyond: 0); a ballot makes them the same bits in every lane
 __device__ __forceinline__ uint32_t reset_flag(const uint8_t* at, int64_t step, int steps, int lane) {
   return at != nullptr && lane < steps ? at[lane * step] : 0u;

@@ -248,10 +248,12 @@ __global__ void __launch_bounds__(256, 2) scan_bwd_kernel(InbScanArgs a, ScanPla
         h[n] = fma2(make_float2(ex2(v.x), ex2(v.y)), h[n], mul2(U, B[n]));
       }
     }
+    float2 delta = make_float2(0.f, 0.f);      // the chunk's sum
 #pragma unroll 4
     for (int i = steps - 1; i >= 0; --i) {
       const float2 D = *(const float2*)(sD + i * CW + gr * 2), U = mul2(D, *(const float2*)(sX + i * CW + gr * 2));
       const float2 GG = *(const float2*)(sG + i * CW + gr * 2);
+      delta = add2(delta, D);
       const float4 *B4 = (const float4*)(sB + (i * NP + j * 4) * 2), B0 = B4[0], B1 = B4[1];
       const float4 *C4 = (const float4*)(sC + (i * NP + j * 4) * 2), C0 = C4[0], C1 = C4[1];
       const float2 B[4] = {make_float2(B0.x, B0.y), make_float2(B0.z, B0.w), make_float2(B1.x, B1.y), make_float2(B1.z, B1.w)};
@@ -301,6 +303,8 @@ __global__ void __launch_bounds__(256, 2) scan_bwd_kernel(InbScanArgs a, ScanPla
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) r[n] = unbias(r[n], A[n], delta);
     if (now.oldest() && now.part == 0 && a.gstate != nullptr) {
       float* to = a.gstate + now.s * a.C * a.N + (ch0 * a.N + j * 4);
       if (a.N % 4 == 0 && ((uintptr_t)a.gstate & 15) == 0) {
