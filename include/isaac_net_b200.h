@@ -511,7 +511,7 @@ int inb_sample(const InbSampleArgs *args, void *cuda_stream);
  * A policy's memory over control steps, for rollouts of S sequences (one a robot) of T steps and one step at a time.
  * InbSeq: a tensor [S, T, ...] whose sequence s, step t starts at p + s * seq + t * step elements, contiguous from there.
  * InbReset: bytes, nonzero where a step starts an episode (nothing before it is seen): of sequence s, step t at
- * p[s / rows * seq + t * step]; p NULL: none. */
+ * p[s / rows * seq + t * step], 1 <= rows < 2^30; p NULL: none.  Outputs overlap no input, but for a state where that is said. */
 typedef struct {
   void *p;
   int64_t seq, step;
@@ -555,7 +555,7 @@ int inb_causal_conv_work(const InbConvArgs *args, int64_t *elems);
  * with T = 1 state_out may be state itself.  kept: what the backward call needs of the forward call,
  * inb_selective_scan_kept() floats, 16-byte aligned, or NULL.  Backward: from gy and gstate_out (contiguous, or NULL) the
  * gradients gx, gdt, gz (NULL without z), gb, gc of dtype and ga, gd, gdt_bias, gstate (contiguous; NULL: not wanted)
- * fp32.  work: inb_selective_scan_work() floats, 16-byte aligned.  Status as above. */
+ * fp32.  work: inb_selective_scan_work() floats, 16-byte aligned.  Status as above; -3 also where kept or work is not aligned. */
 #define INB_MAX_SCAN_N 64
 typedef struct {
   int32_t dtype, C, N, reserved;
@@ -582,8 +582,8 @@ int inb_selective_scan_work(const InbScanArgs *args, int32_t backward, int64_t *
  * (q - p).  logits [N, V] of dtype (rows ld apart), teacher [N, K] of dtype teacher_dtype, index [N, K] int64.  An element is
  * allowed where mask (bytes, rows ld_mask apart, or NULL) is nonzero and its logit is not -inf; an entry is in use where its
  * index is in [0, V) and allowed and its logit neither -inf nor NaN; entries of one index add up.  A row without an
- * entry in use has loss 0 and gradient 0.  stats [N, 4]: written by the forward call unless NULL, read by the backward
- * call.  glogits is contiguous.  -2: sizes out of range; -3: a required pointer is NULL. */
+ * entry in use has loss 0 and gradient 0.  stats [N, 4], 16-byte aligned: written by the forward call unless NULL, read by the
+ * backward call.  glogits is contiguous.  -2: sizes out of range; -3: a required pointer is NULL or not aligned. */
 #define INB_MAX_DISTILL_K 1024
 typedef struct {
   int32_t dtype, teacher_dtype, V, K;

@@ -278,13 +278,9 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
       py = row_out<T>(a.y, q.s, q.t0);
     }
     const int count = q.hi - q.lo;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
+    auto step = [&](int i, bool cut) {
       const Words<T, V> x = feed.get(K - 1 + i);
-      if (cuts >> i & 1) {
-        win.zero();
-        keep_branch();
-      }
+      if (cut) win.zero();
       float2 now[P];
       Words<T, V> y;
 #pragma unroll
@@ -296,6 +292,13 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
       io.store(py, y);
       py += a.y.step;
       win.push(now);
+    };
+    if (cuts == 0 && count == feed.R) {      // without a branch between them, rows overlap
+#pragma unroll 4
+      for (int i = 0; i < feed.R; ++i) step(i, false);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < count; ++i) step(i, cuts >> i & 1);
     }
     if (q.hi == q.n && q.lo < q.hi && q.t0 + q.n == a.T && a.state_out != nullptr) {
       T* out = (T*)a.state_out + q.s * a.state_out_seq;
@@ -439,15 +442,14 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
       pgx = row_out<T>(a.gx, q.s, q.t0);
     }
     const int count = q.hi - q.lo;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
+    // MIDDLE: rows of the part, whose gx is stored K - 1 rows later
+    auto step = [&](int i, bool cut, bool middle) {
       const Words<T, V> x = feed.get(K - 1 + i), gy = feed.get(K - 1 + feed.R + i);
       const int row = q.lo + i;
-      if (cuts >> i & 1) {
+      if (cut) {
         flush(row);
         clear();
         seen = 0;
-        keep_branch();
       }
       float2 now[P], g[P];
 #pragma unroll
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
           g[k] = mul2(g[k], mul2(s, fma2(p, fma2(s, both(-1.f), both(1.f)), both(1.f))));
         }
       }
-      if (row < q.n) {
+      if (middle || row < q.n) {
 #pragma unroll
         for (int k = 0; k < P; ++k) {
           gb[k] = add2(gb[k], g[k]);
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
       for (int j = 0; j < K - 1; ++j)
 #pragma unroll
         for (int k = 0; k < P; ++k) pend[j][k] = fma2(taps.w[K - 2 - j][k], g[k], pend[j][k]);
-      if (row >= K - 1 && seen == K - 1) {
+      if (middle || (row >= K - 1 && seen == K - 1)) {
         Words<T, V> p;
 #pragma unroll
         for (int k = 0; k < P; ++k) p.set(k, pend[K - 2][k]);
@@ -480,10 +482,24 @@ __global__ void __launch_bounds__(128, CONV_BWD_BLOCKS) conv_bwd_kernel(InbConvA
       } else if (seen == K - 1) {
         store(row - (K - 1), pend[K - 2]);
       }
-      if (row >= K - 1) pgx += a.gx.step;
+      if (middle || row >= K - 1) pgx += a.gx.step;
       shift(g);
       win.push(now);
-      seen = seen < K - 1 ? seen + 1 : seen;
+      if (!middle) seen = seen < K - 1 ? seen + 1 : seen;
+    };
+    if (cuts == 0 && count == feed.R && q.hi <= q.n && seen == K - 1) {      // without a branch between them, rows overlap
+      if (q.lo == 0) {
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) step(i, false, false);
+#pragma unroll
+        for (int i = K - 1; i < feed.R; ++i) step(i, false, true);
+      } else {
+#pragma unroll 4
+        for (int i = 0; i < feed.R; ++i) step(i, false, true);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < count; ++i) step(i, cuts >> i & 1, false);
     }
     if (q.hi == q.to && q.lo < q.hi) {
       // the rows that nothing follows: those of the sequence's end, to which the final state's gradient adds

@@ -476,7 +476,8 @@ extern "C" int inb_distill_fwd(const InbDistillArgs* args, void* cuda_stream) {
   const int rc = inb::pol::dist_check(a);
   if (rc != 0) return rc;
   if (a.N == 0) return 0;
-  if (a.logits == nullptr || a.teacher == nullptr || a.index == nullptr || a.loss == nullptr) return -3;
+  if (a.logits == nullptr || a.teacher == nullptr || a.index == nullptr || a.loss == nullptr || ((uintptr_t)a.stats & 15) != 0)
+    return -3;
   cudaStream_t s = (cudaStream_t)cuda_stream;
   if (a.dtype == INB_BF16) return inb::pol::dist_fwd<inb::pol::bf16>(a, s);
   if (a.dtype == INB_F16) return inb::pol::dist_fwd<inb::pol::f16>(a, s);
@@ -490,7 +491,7 @@ extern "C" int inb_distill_bwd(const InbDistillArgs* args, void* cuda_stream) {
   if (rc != 0) return rc;
   if (a.N == 0) return 0;
   if (a.logits == nullptr || a.teacher == nullptr || a.index == nullptr || a.stats == nullptr || a.gloss == nullptr ||
-      a.glogits == nullptr)
+      a.glogits == nullptr || ((uintptr_t)a.stats & 15) != 0)
     return -3;
   cudaStream_t s = (cudaStream_t)cuda_stream;
   if (a.dtype == INB_BF16) return inb::pol::dist_bwd<inb::pol::bf16>(a, s);

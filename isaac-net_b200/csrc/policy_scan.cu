@@ -391,7 +391,7 @@ static int step_go(const InbScanArgs& a, int lanes, cudaStream_t s) {
   // as many sequences a block as leave six blocks an SM, no more than 32, and a grid's second axis ends at 65535
   int64_t per = a.S * tiles / (sm_count() * 6);
   if (per > 32) per = 32;
-  if (per > STEP_B) per = per / STEP_B * STEP_B;
+  if (per > 1) per = ceil_div(per, STEP_B) * STEP_B;
   if (per < ceil_div(a.S, 65535)) per = ceil_div(a.S, 65535);
   if (per < 1) per = 1;
   scan_step_kernel<T, V, G><<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per)), STEP_THREADS, 0, s>>>(a, lanes, (int)per);
@@ -438,6 +438,7 @@ extern "C" int inb_selective_scan_fwd(const InbScanArgs* args, void* cuda_stream
   if (a.S == 0 || a.T == 0) return 0;
   if (a.x.p == nullptr || a.dt.p == nullptr || a.b.p == nullptr || a.c.p == nullptr || a.y.p == nullptr || a.a == nullptr) return -3;
   cudaStream_t s = (cudaStream_t)cuda_stream;
+  if (((uintptr_t)a.kept & 15) != 0 || ((uintptr_t)a.work & 15) != 0) return -3;
   if (a.T == 1) {
     if (a.dtype == INB_BF16) return scan_step<bf16>(a, s);
     if (a.dtype == INB_F16) return scan_step<f16>(a, s);

@@ -526,7 +526,8 @@ extern "C" int inb_selective_scan_bwd(const InbScanArgs* args, void* cuda_stream
   if (a.S == 0 || a.T == 0) return 0;
   if (a.x.p == nullptr || a.dt.p == nullptr || a.b.p == nullptr || a.c.p == nullptr || a.a == nullptr || a.gy.p == nullptr ||
       a.gx.p == nullptr || a.gdt.p == nullptr || a.gb.p == nullptr || a.gc.p == nullptr || a.ga == nullptr ||
-      (a.z.p != nullptr && a.gz.p == nullptr) || (a.T > SCAN_STEPS && a.kept == nullptr))
+      (a.z.p != nullptr && a.gz.p == nullptr) || (a.T > SCAN_STEPS && a.kept == nullptr) || ((uintptr_t)a.kept & 15) != 0 ||
+      ((uintptr_t)a.work & 15) != 0)
     return -3;
   if (a.work == nullptr || a.work_elems < need) return -5;
   const BwdPlan b = bwd_plan(a);

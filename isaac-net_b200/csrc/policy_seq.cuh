@@ -186,41 +186,42 @@ inline bool is_aligned(const InbSeq& q, int64_t bytes, int64_t elem) {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------------------------------------- column sums
-// part [P, M] fp32 -> sums over P: columns [0, first) to out0, [first, second) to out1, the others to out2 (any may be NULL).  A block takes 32
-// columns, its 8 warps rows p, p + 8, ...; the order of the sum does not depend on timing.
+// part [P, M] fp32 -> sums over P: columns [0, first) to out0, [first, second) to out1, the others to out2 (any may be NULL).
+// A block takes 32 columns, its 32 warps rows p, p + 32, ...; the order of the sum does not depend on timing.
+constexpr int COLSUM_WARPS = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_kernel(const float* part, int64_t P, int64_t M, int64_t first, int64_t second, T* out0,
-                                                     T* out1, T* out2) {
-  const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-  const int w = threadIdx.x >> 5;
+__global__ void __launch_bounds__(COLSUM_WARPS * 32) colsum_kernel(const float* part, int64_t P, int64_t M, int64_t first, int64_t second,
+                                                                   T* out0, T* out1, T* out2) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < M) {
     int64_t p = w;
-    for (; p + 24 < P; p += 32) {
+    for (; p + 3 * COLSUM_WARPS < P; p += 4 * COLSUM_WARPS) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += part[(p + 8 * i) * M + c];
+      for (int i = 0; i < 4; ++i) v[i] += part[(p + COLSUM_WARPS * i) * M + c];
     }
-    for (; p < P; p += 8) v[0] += part[p * M + c];
+    for (; p < P; p += COLSUM_WARPS) v[0] += part[p * M + c];
   }
-  __shared__ float sum[8][32];
-  sum[w][threadIdx.x & 31] = (v[0] + v[1]) + (v[2] + v[3]);
+  __shared__ float sum[COLSUM_WARPS][33];
+  sum[w][lane] = (v[0] + v[1]) + (v[2] + v[3]);
   __syncthreads();
-  if (w != 0 || c >= M) return;
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += sum[i][threadIdx.x];
-  if (c < first) {
-    if (out0 != nullptr) out0[c] = from_f<T>(s);
-  } else if (c < second) {
-    if (out1 != nullptr) out1[c - first] = from_f<T>(s);
+  // a warp a column: the 32 warps' sums of it
+  const float s = warp_sum(sum[lane][w]);
+  const int64_t to = (int64_t)blockIdx.x * 32 + w;
+  if (lane != 0 || to >= M) return;
+  if (to < first) {
+    if (out0 != nullptr) out0[to] = from_f<T>(s);
+  } else if (to < second) {
+    if (out1 != nullptr) out1[to - first] = from_f<T>(s);
   } else if (out2 != nullptr) {
-    out2[c - second] = from_f<T>(s);
+    out2[to - second] = from_f<T>(s);
   }
 }
 template <typename T>
 inline void colsum(const float* part, int64_t P, int64_t M, int64_t first, int64_t second, void* out0, void* out1, void* out2,
                    cudaStream_t s) {
-  colsum_kernel<T><<<(unsigned)ceil_div(M, 32), 256, 0, s>>>(part, P, M, first, second, (T*)out0, (T*)out1, (T*)out2);
+  colsum_kernel<T><<<(unsigned)ceil_div(M, 32), COLSUM_WARPS * 32, 0, s>>>(part, P, M, first, second, (T*)out0, (T*)out1, (T*)out2);
 }
 
 }  // namespace pol

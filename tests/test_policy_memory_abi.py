@@ -72,17 +72,17 @@ def test_refused_calls_return_their_status():
     for kw, rc in [(dict(dtype=3), -2), (dict(C=0), -2), (dict(N=0), -2), (dict(N=65), -2), (dict(S=-1), -2), (dict(T=-1), -2),
                    (dict(S=1 << 25, C=1 << 10), -2), (dict(reset=nat.InbReset(256, 0, 1, 1)), -2), (dict(x=none), -3),
                    (dict(dt=none), -3), (dict(b=none), -3), (dict(c=none), -3), (dict(y=none), -3), (dict(a=None), -3),
-                   (dict(T=0), 0), (dict(T=4000), -5)]:
+                   (dict(T=0), 0), (dict(T=4000), -5), (dict(kept=264), -3), (dict(work=260), -3)]:
         assert L.inb_selective_scan_fwd(r(scan(**kw)), None) == rc, kw
     back = {k: seq() for k in ("gy", "gx", "gdt", "gb", "gc")}
     for kw, rc in [(dict(gy=none), -3), (dict(gx=none), -3), (dict(gdt=none), -3), (dict(gb=none), -3), (dict(gc=none), -3), ({}, -3),
-                   (dict(ga=256, z=seq()), -3), (dict(ga=256, T=9), -3), (dict(ga=256), -5), (dict(ga=256, T=9, kept=256), -5),
+                   (dict(ga=256, z=seq()), -3), (dict(ga=256, T=9), -3), (dict(ga=256), -5), (dict(ga=256, T=9, kept=256), -5), (dict(ga=256, T=9, kept=264), -3),
                    (dict(S=0), 0)]:
         assert L.inb_selective_scan_bwd(r(scan(**{**back, **kw})), None) == rc, kw
     for kw, rc in [(dict(dtype=3), -2), (dict(teacher_dtype=-1), -2), (dict(V=0), -2), (dict(V=(1 << 22) + 1), -2), (dict(K=0), -2),
                    (dict(K=1025), -2), (dict(N=-1), -2), (dict(tau=0.0), -2), (dict(tau=-1.0), -2), (dict(tau=float("nan")), -2),
                    (dict(tau=float("inf")), -2), (dict(logits=None), -3), (dict(teacher=None), -3), (dict(index=None), -3),
-                   (dict(loss=None), -3), (dict(N=0), 0)]:
+                   (dict(loss=None), -3), (dict(stats=264), -3), (dict(N=0), 0)]:
         assert L.inb_distill_fwd(r(distill(**kw)), None) == rc, kw
     for kw, rc in [(dict(), -3), (dict(stats=256), -3), (dict(stats=256, gloss=256), -3), (dict(N=0), 0)]:
         assert L.inb_distill_bwd(r(distill(**kw)), None) == rc, kw
