@@ -67,6 +67,29 @@ struct Taps {
   float2 w[K][P], bias[P];
   template <bool WIDE>
   __device__ __forceinline__ void load(const InbConvArgs& a, const Lanes<T, V, WIDE>& io) {
+    if constexpr (WIDE) {
+      // the V K weights of neighbouring channels lie together
+      if ((((uintptr_t)a.w | (uintptr_t)a.bias) & (V * sizeof(T) - 1)) == 0) {
+        Words<T, V> q[K], b;
+        if (io.count > 0) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) q[k].load((const T*)a.w + io.first * K + k * V);
+          if (a.bias != nullptr) b.load((const T*)a.bias + io.first);
+        }
+        auto element = [&](int e) {
+          const float2 p = q[e / V].pair(e % V / 2);
+          return e & 1 ? p.y : p.x;
+        };
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          bias[i] = io.count > 0 && a.bias != nullptr ? b.pair(i) : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            w[k][i] = io.count > 0 ? make_float2(element(2 * i * K + k), element((2 * i + 1) * K + k)) : make_float2(0.f, 0.f);
+        }
+        return;
+      }
+    }
     auto get = [&](const void* p, int v, int64_t of, int64_t k) { return v < io.count && p != nullptr ? to_f(((const T*)p)[io.at(v) * of + k]) : 0.f; };
 #pragma unroll
     for (int i = 0; i < P; ++i) {

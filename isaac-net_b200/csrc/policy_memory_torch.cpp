@@ -47,29 +47,32 @@ int64_t one_stride(const Tensor& t, int64_t last) {
   }
   return ld < 0 ? 0 : ld;
 }
-// [..., T, C] as sequences: any stride between sequences and between steps, elements contiguous
-bool is_seq(const Tensor& t) {
-  return t.numel() == 0 || ((t.stride(-1) == 1 || t.size(-1) == 1) && one_stride(t, t.dim() - 2) >= 0);
+// [..., T, C] as sequences (a step: [..., C]): any stride between sequences and between steps, elements contiguous
+bool is_seq(const Tensor& t, bool step) {
+  return t.numel() == 0 || ((t.stride(-1) == 1 || t.size(-1) == 1) && one_stride(t, t.dim() - (step ? 1 : 2)) >= 0);
+}
+InbSeq seq_of(const Tensor& t, void* p, bool step) {
+  return {p, one_stride(t, t.dim() - (step ? 1 : 2)), step ? 0 : t.stride(-2)};
 }
 struct Seq {
   Tensor t;
   InbSeq q = {};
   Seq() = default;
-  explicit Seq(const Tensor& in) {
+  explicit Seq(const Tensor& in, bool step = false) {
     if (!in.defined()) return;
-    t = is_seq(in) ? in : in.contiguous();
-    q = {const_cast<void*>(t.const_data_ptr()), one_stride(t, t.dim() - 2), t.stride(-2)};
+    t = is_seq(in, step) ? in : in.contiguous();
+    q = seq_of(t, const_cast<void*>(t.const_data_ptr()), step);
   }
 };
 // A new tensor of t's shape in t's order of axes, so that a rollout that lies step by step gives one that does
-Tensor like_seq(const Tensor& t) {
+Tensor like_seq(const Tensor& t, bool step = false) {
   if (!t.defined()) return {};
   Tensor o = at::empty_like(t);
-  return is_seq(o) ? o : at::empty(t.sizes(), t.options());
+  return is_seq(o, step) ? o : at::empty(t.sizes(), t.options());
 }
-InbSeq write_seq(const Tensor& t) {
+InbSeq write_seq(const Tensor& t, bool step = false) {
   if (!t.defined()) return {};
-  return {t.mutable_data_ptr(), one_stride(t, t.dim() - 2), t.stride(-2)};
+  return seq_of(t, t.mutable_data_ptr(), step);
 }
 // States [..., A, B]: the inner two axes contiguous, one stride between sequences; a copy where that is not so
 struct States {
@@ -85,30 +88,34 @@ struct States {
                               one_stride(t, t.dim() - 2) >= 0);
   }
 };
-// reset [..., T]: leading sizes those of x up to some axis, 1 from there on (missing ones count as 1)
+// reset [..., T] (a step: [...]): leading sizes those of x up to some axis, 1 from there on (missing ones count as 1); `lead`: x's
+// axes before the steps
+int64_t shared_axes(const Tensor& in, int64_t lead, bool step, int64_t& miss) {
+  miss = lead + (step ? 0 : 1) - in.dim();
+  int64_t axis = lead - 1;
+  while (axis >= 0 && (axis < miss || in.size(axis - miss) == 1)) --axis;
+  return axis;
+}
 struct Resets {
   Tensor t;
   InbReset q = {};
   Resets() = default;
-  Resets(const Tensor& in, const Tensor& x, int64_t lead) {      // lead: x's axes before the steps; in's last axis is the steps
+  Resets(const Tensor& in, const Tensor& x, int64_t lead, bool step) {
     if (!in.defined()) return;
-    const int64_t miss = lead + 1 - in.dim();
-    int64_t rows = 1, axis = lead - 1;
-    while (axis >= 0 && (axis < miss || in.size(axis - miss) == 1)) rows *= x.size(axis--);
+    int64_t miss = 0, rows = 1;
+    const int64_t axis = shared_axes(in, lead, step, miss);
+    for (int64_t i = axis + 1; i < lead; ++i) rows *= x.size(i);
     t = in.numel() == 0 || one_stride(in, axis + 1) >= 0 ? in : in.contiguous();
-    q = {(const uint8_t*)t.const_data_ptr(), rows > 0 ? rows : 1, axis < 0 ? 0 : one_stride(t, axis + 1), t.stride(-1)};
+    q = {(const uint8_t*)t.const_data_ptr(), rows > 0 ? rows : 1, axis < 0 ? 0 : one_stride(t, axis + 1), step ? 0 : t.stride(-1)};
   }
 };
-void check_reset(const Tensor& reset, const Tensor& x, int64_t lead, int64_t steps) {
+void check_reset(const Tensor& reset, const Tensor& x, int64_t lead, int64_t steps, bool step) {
   same(reset, "reset", x, at::kBool);
-  const int64_t miss = lead + 1 - reset.dim();
-  bool fits = miss >= 0 && reset.dim() >= 1 && reset.size(-1) == steps;
-  int64_t axis = lead - 1;
-  if (fits)
-    while (axis >= 0 && (axis < miss || reset.size(axis - miss) == 1)) --axis;
+  int64_t miss = 0, axis = shared_axes(reset, lead, step, miss);
+  bool fits = miss >= 0 && (step || (reset.dim() >= 1 && reset.size(-1) == steps));
   for (; fits && axis >= 0; --axis) fits = axis >= miss && reset.size(axis - miss) == x.size(axis);
-  VALUE_CHECK(fits, "reset of shape ", reset.sizes(), " does not fit x of shape ", x.sizes(), ": its leading sizes, then ones, then the ",
-              steps, " steps");
+  VALUE_CHECK(fits, "reset of shape ", reset.sizes(), " does not fit x of shape ", x.sizes(), ": its leading sizes, then ones",
+              step ? "" : ", then the steps");
 }
 void check_shape(const Tensor& t, const char* name, const Tensor& x, int64_t lead, std::initializer_list<int64_t> inner) {
   std::vector<int64_t> want(x.sizes().begin(), x.sizes().begin() + lead);
@@ -139,16 +146,17 @@ void touched(const Tensor& t) {
 
 // ------------------------------------------------------------------------------------------------- causal_conv
 struct ConvIn {
-  Tensor x, w, bias, state, reset;      // x [..., T, C], reset's last axis the steps
+  Tensor x, w, bias, state, reset;      // x [..., T, C], reset's last axis the steps; a step: without them
   int64_t act;
-  int64_t lead() const { return x.dim() - 2; }
+  bool step = false;
+  int64_t lead() const { return x.dim() - (step ? 1 : 2); }
 };
 InbConvArgs conv_args(const ConvIn& i, const Seq& x, const States& st, const Resets& r) {
   InbConvArgs a = {};
   a.dtype = type_code(i.x.scalar_type());
   a.act = (int32_t)i.act;
   a.C = (int32_t)i.x.size(-1), a.K = (int32_t)i.w.size(1);
-  a.S = sequences(i.x, i.lead()), a.T = i.x.size(-2);
+  a.S = sequences(i.x, i.lead()), a.T = i.step ? 1 : i.x.size(-2);
   a.x = x.q;
   a.w = ptr(i.w), a.bias = ptr(i.bias), a.state = ptr(st.t), a.state_seq = st.seq;
   a.reset = r.q;
@@ -171,7 +179,7 @@ std::pair<Tensor, Tensor> conv_forward(const ConvIn& i) {
   const On on(i.x);
   const Seq x(i.x);
   const States st(i.state);
-  const Resets r(i.reset, i.x, i.lead());
+  const Resets r(i.reset, i.x, i.lead(), false);
   InbConvArgs a = conv_args(i, x, st, r);
   a.y = write_seq(y);
   a.state_out = ::out(out), a.state_out_seq = (int64_t)(a.K - 1) * a.C;
@@ -201,7 +209,7 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     const On on(i.x);
     const Seq x(i.x), gy(grads[0].defined() ? grads[0] : at::zeros_like(i.x));
     const States st(i.state);
-    const Resets r(i.reset, i.x, i.lead());
+    const Resets r(i.reset, i.x, i.lead(), false);
     InbConvArgs a = conv_args(i, x, st, r);
     const Tensor gout = grads[1].defined() ? grads[1].contiguous() : Tensor();
     a.gy = gy.q, a.gx = write_seq(o[0]);
@@ -214,7 +222,7 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     return once(o);
   }
 };
-// Shapes, types and limits; x [..., C] with `steps` 1 (a step) or [..., T, C]
+// Shapes, types and limits; x [..., T, C], a step's [..., C]
 void conv_check(const Tensor& x, const Tensor& w, const Maybe& bias, const Maybe& state, const Maybe& reset, bool step) {
   first(x, "x");
   VALUE_CHECK(x.dim() >= (step ? 1 : 2) && x.size(-1) >= 1, "x must be ", step ? "[..., C]" : "[..., T, C]", " with C >= 1, got shape ",
@@ -233,11 +241,7 @@ void conv_check(const Tensor& x, const Tensor& w, const Maybe& bias, const Maybe
     same(*state, "state", x, x.scalar_type());
     check_shape(*state, "state", x, lead, {w.size(1) - 1, c});
   }
-  if (reset) {
-    Tensor r = *reset;
-    if (step) r = r.unsqueeze(-1);
-    check_reset(r, x, lead, t);
-  }
+  if (reset) check_reset(*reset, x, lead, t, step);
   no_tangents({{&x, "x"}, {&w, "weight"}, {given(bias), "bias"}, {given(state), "state"}});
 }
 py::tuple causal_conv(const Tensor& x, const Tensor& w, const Maybe& bias, const Maybe& state, const Maybe& reset, int64_t act) {
@@ -255,39 +259,41 @@ Tensor causal_conv_step(const Tensor& x, const Tensor& w, const Tensor& state, c
   check_in_place(state, "causal_conv_step");
   no_grad_step({x, w, state, bias.value_or(Tensor())}, "causal_conv_step");
   const at::NoGradGuard no_grad;
-  const ConvIn i = {x.unsqueeze(-2), w.contiguous(), bias ? bias->contiguous() : Tensor(), state,
-                    reset ? reset->unsqueeze(-1) : Tensor(), act};
-  const Tensor y = like_seq(i.x);
+  const ConvIn i = {x, w.contiguous(), bias ? bias->contiguous() : Tensor(), state, reset.value_or(Tensor()), act, true};
+  const Tensor y = like_seq(x, true);
   if (x.numel() > 0) {
     const On on(x);
-    const Seq xs(i.x);
+    const Seq xs(x, true);
     const States st(state);
-    const Resets r(i.reset, i.x, i.lead());
+    const Resets r(i.reset, x, i.lead(), true);
     InbConvArgs a = conv_args(i, xs, st, r);
-    a.y = write_seq(y);
+    a.y = write_seq(y, true);
     a.state_out = out(state), a.state_out_seq = st.seq;
     check(api.conv_fwd(&a, on.stream), "inb_causal_conv_fwd");
     touched(state);
   }
-  return y.squeeze(-2);
+  return y;
 }
 
 // ------------------------------------------------------------------------------------------------- selective_scan
 struct ScanIn {
-  Tensor x, dt, a, b, c, d, z, bias, state, reset;      // x, dt, z [..., T, C], b, c [..., T, N]
-  int64_t lead() const { return x.dim() - 2; }
+  Tensor x, dt, a, b, c, d, z, bias, state, reset;      // x, dt, z [..., T, C], b, c [..., T, N]; a step: without T
+  bool step = false;
+  int64_t lead() const { return x.dim() - (step ? 1 : 2); }
 };
 struct ScanRows {
   Seq x, dt, z, b, c;
   States st;
   Resets r;
-  explicit ScanRows(const ScanIn& i) : x(i.x), dt(i.dt), z(i.z), b(i.b), c(i.c), st(i.state), r(i.reset, i.x, i.lead()) {}
+  explicit ScanRows(const ScanIn& i)
+      : x(i.x, i.step), dt(i.dt, i.step), z(i.z, i.step), b(i.b, i.step), c(i.c, i.step), st(i.state),
+        r(i.reset, i.x, i.lead(), i.step) {}
 };
 InbScanArgs scan_args(const ScanIn& i, const ScanRows& r) {
   InbScanArgs a = {};
   a.dtype = type_code(i.x.scalar_type());
   a.C = (int32_t)i.x.size(-1), a.N = (int32_t)i.a.size(1);
-  a.S = sequences(i.x, i.lead()), a.T = i.x.size(-2);
+  a.S = sequences(i.x, i.lead()), a.T = i.step ? 1 : i.x.size(-2);
   a.x = r.x.q, a.dt = r.dt.q, a.z = r.z.q, a.b = r.b.q, a.c = r.c.q;
   a.a = (const float*)ptr(i.a), a.d = (const float*)ptr(i.d), a.dt_bias = (const float*)ptr(i.bias);
   a.state = (const float*)ptr(r.st.t), a.state_seq = r.st.seq;
@@ -401,11 +407,7 @@ void scan_check(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor
     same(*state, "state", x, at::kFloat);
     check_shape(*state, "state", x, lead, {ch, n});
   }
-  if (reset) {
-    Tensor r = *reset;
-    if (step) r = r.unsqueeze(-1);
-    check_reset(r, x, lead, t);
-  }
+  if (reset) check_reset(*reset, x, lead, t, step);
   no_tangents({{&x, "x"}, {&dt, "dt"}, {&a, "a"}, {&b, "b"}, {&c, "c"}, {given(d), "d"}, {given(z), "z"}, {given(bias), "dt_bias"},
                {given(state), "state"}});
 }
@@ -432,20 +434,19 @@ Tensor selective_scan_step(const Tensor& x, const Tensor& dt, const Tensor& a, c
   check_in_place(state, "selective_scan_step");
   no_grad_step({x, dt, a, b, c, state, d.value_or(Tensor()), z.value_or(Tensor()), bias.value_or(Tensor())}, "selective_scan_step");
   const at::NoGradGuard no_grad;
-  auto up = [](const Tensor& t) { return t.unsqueeze(-2); };
-  const ScanIn i = scan_in(up(x), up(dt), a, up(b), up(c), d, z ? Maybe(up(*z)) : std::nullopt, bias, state,
-                           reset ? Maybe(reset->unsqueeze(-1)) : std::nullopt);
-  const Tensor y = like_seq(i.x);
+  ScanIn i = scan_in(x, dt, a, b, c, d, z, bias, state, reset);
+  i.step = true;
+  const Tensor y = like_seq(x, true);
   if (x.numel() > 0) {
     const On on(x);
     const ScanRows r(i);
     InbScanArgs args = scan_args(i, r);
-    args.y = write_seq(y);
+    args.y = write_seq(y, true);
     args.state_out = (float*)out(state), args.state_out_seq = r.st.seq;
     check(api.scan_fwd(&args, on.stream), "inb_selective_scan_fwd");
     touched(state);
   }
-  return y.squeeze(-2);
+  return y;
 }
 
 // ------------------------------------------------------------------------------------------------- distill_loss
