@@ -9,7 +9,8 @@ Public API (a drop-in for ``isaac_net.make_engine("L2", ...)`` on the uplink pat
     NetModule, IsaacNetCfg, TrafficRequest  (the Isaac-side module on the engine's radio, net_module.py)
     ShardedEngine, shard_invariant  (one batch split over several GPUs in one process, sharded.py)
     policy_ops  (the operators of a policy over NetModule's observations: block_norm, gated_ffn, counter_dropout,
-                 sample_logits, uniforms)
+                 sample_logits, uniforms; a memory over control steps: causal_conv, selective_scan and their steps;
+                 distill_loss)
 """
 import importlib as _importlib
 import importlib.abc as _abc

@@ -10,13 +10,14 @@
     y    = causal_conv_step(x, w, s, bias), selective_scan_step(x, dt, a, b, c, s)     one step, state updated in place
     loss = distill_loss(logits, teacher, index)               from a teacher's top logits
 
-All but the sampling and the steps are differentiable (torch.autograd, once, in reverse mode; a tensor with a tangent is refused).  As everywhere in this package there is no CPU path and no
-fallback: tensors live on one CUDA device, unsupported settings raise B200Unsupported, wrong shapes ValueError and wrong
-types TypeError before anything is launched, and the work is queued on the current stream of the tensors' device.  The
-calls may be captured in a CUDA graph.  The operators have no counterpart in isaac-net, whose policies are its user's.
+All but the sampling and the steps are differentiable (torch.autograd, once, in reverse mode; a tensor with a tangent is
+refused).  As everywhere in this package there is no CPU path and no fallback: tensors live on one CUDA device, unsupported
+settings raise B200Unsupported, wrong shapes ValueError and wrong types TypeError before anything is launched, and the work
+is queued on the current stream of the tensors' device.  The calls may be captured in a CUDA graph.  The operators have no
+counterpart in isaac-net, whose policies are its user's.
 
-The functions are csrc/policy_torch.cpp, on top of the C ABI (inb_block_norm_fwd and the others of
-include/isaac_net_b200.h).
+The functions are csrc/policy_torch.cpp and policy_memory_torch.cpp, on top of the C ABI (inb_block_norm_fwd and the others
+of include/isaac_net_b200.h).
 """
 from __future__ import annotations
 
