@@ -21,14 +21,15 @@ constexpr int SCAN_WARPS = 4;        // a block's warps work on their own; no ba
 // WIDE: the rows of b and c are NS whole, aligned to 16 bytes and moved by that
 template <typename T, int NS, int LN, int MODE, bool WIDE>
 __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry) {
-  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 16, BCW = 16 / sizeof(T);
+  constexpr int NP = NS * LN, CW = 32 / LN, TC = SCAN_STEPS, BCL = (2 * TC * NP + 31) / 32, NH = NS / 2, POLY = NS / 16;
+  constexpr int BCW = 16 / sizeof(T);
   constexpr bool BACK = MODE == 3;
   __shared__ alignas(16) float bc[SCAN_WARPS][TC][2][NP];
   __shared__ float4 stage[SCAN_WARPS][TC][32];       // delta, u, silu(z) (1 without z), d x of this lane's channel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane % LN;
   const int n4 = (a.N + 3) / 4 * 4;
   // a block is one sequence's: what depends on it is the same for all its threads
-  const int64_t part = pl.parts > 1 ? blockIdx.x / (uint32_t)a.S : 0, s = blockIdx.x - part * a.S;
+  const int64_t at = pl.parts > 1 ? blockIdx.x / (uint32_t)a.S : 0, s = blockIdx.x - at * a.S, part = at + BACK;
   const int c0 = (blockIdx.y * (blockDim.x >> 5) + warp) * CW + lane / LN;
   const bool on = c0 < a.C;
   const int ch = on ? c0 : a.C - 1;                // lanes beyond the last channel read it too and write nothing
@@ -90,12 +91,12 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
       }
     } else {
 #pragma unroll
-    for (int i = 0; i < BCL; ++i) {
-      const int k = i * 32 + lane, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
-      bcr[i] = 0;
-      if (n < a.N && tt < steps && which < 2 && !(MODE == 2 && which == 1) && !(BACK && which == 0))
-        bcr[i] = ld_raw(which ? pc + (DIR * tt * a.c.step + n) : pb + (DIR * tt * a.b.step + n));
-    }
+      for (int i = 0; i < BCL; ++i) {
+        const int k = i * 32 + lane, which = k / (TC * NP), q = k % (TC * NP), tt = q / NP, n = q % NP;
+        bcr[i] = 0;
+        if (n < a.N && tt < steps && which < 2 && !(MODE == 2 && which == 1) && !(BACK && which == 0))
+          bcr[i] = ld_raw(which ? pc + (DIR * tt * a.c.step + n) : pb + (DIR * tt * a.b.step + n));
+      }
     }
     pb += DIR * TC * a.b.step;
     pc += DIR * TC * a.c.step;
@@ -214,7 +215,8 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a,
   }
 }
 
-// The states that the parts begin (reverse: end) with, in place of what they end with from zero.  A thread a state.
+// The states that the parts begin (reverse: end) with, in place of what they end with from zero (the last one's, which no
+// launch has written, is read and left unused).  A thread a state.
 __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan pl, float* carry, bool reverse) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.S * a.C * a.N) return;
@@ -351,7 +353,8 @@ int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool revers
 template <typename T, int NS, int LN, int MODE>
 static void scan_go(const InbScanArgs& a, const ScanPlan& p, float* carry, cudaStream_t s) {
   const int64_t tiles = ceil_div(a.C, 32 / LN), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
-  const dim3 grid((unsigned)(a.S * p.parts), (unsigned)ceil_div(tiles, warps));
+  // nothing begins with what the last part (reverse: the first) ends with
+  const dim3 grid((unsigned)(a.S * (MODE < 2 ? p.parts : p.parts - 1)), (unsigned)ceil_div(tiles, warps));
   if constexpr (NS == 16 && LN == 1) {
     if (a.N == 16 && is_aligned(a.b, 16, sizeof(T)) && is_aligned(a.c, 16, sizeof(T))) {
       scan_kernel<T, NS, LN, MODE, true><<<grid, (unsigned)warps * 32, 0, s>>>(a, p, carry);

@@ -60,7 +60,10 @@ __device__ __forceinline__ float2 ex2_poly(float2 v) {
 // log(1 + u) / u of degree 9 (at most 2.1 * 2^-24 off), so that small results keep their relative precision, which log of a
 // rounded 1 + u would lose.
 __device__ __forceinline__ float softplus_u(float v, float& u) {
-  const float a = -fabsf(v), t = a * LOG2E;
+  // a step that is to leave the state as it is has dt of -inf or of the type's lowest value: e^-128 is 0, and a NaN stays one
+  float a;
+  asm("max.NaN.f32 %0, %1, 0fC3000000;" : "=f"(a) : "f"(-fabsf(v)));      // -128
+  const float t = a * LOG2E;
   const float low = fmaf(a, LOG2E, -t);              // what t's rounding lost, 2^-24 |v|, and would cost u relative
   const float e = ex2(t);
   u = fmaf(e, low * LN2, e);

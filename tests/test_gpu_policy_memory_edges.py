@@ -164,6 +164,36 @@ def test_nothing_of_an_ended_episode_is_seen(dtype):
         assert near(a[:, :, cut:], c)
 
 
+@pytest.mark.parametrize("dtype", DT)
+def test_steps_of_no_length_leave_the_state(dtype):
+    """dt of -inf or of the type's lowest value: delta is 0, the state stays as it was to the bit, no gradient is NaN; very large
+    dt forget everything; a NaN is not hidden."""
+    g = gen(12)
+    p, q = scan_args(g, 2, 2, 12, 40, 16, dtype)
+    x, w = p["x"], [3, 4, 9]
+    for low in (-math.inf, torch.finfo(dtype).min):
+        dt = p["dt"].clone()
+        dt[:, :, w] = low
+        leaf = {k: v.detach().clone().requires_grad_(True) for k, v in {**p, "dt": dt, **q}.items()}
+        y, new = ops.selective_scan(**leaf)
+        grads = torch.autograd.grad((y.float().sum() + new.sum()), list(leaf.values()))
+        assert all(bool(v.isfinite().all()) for v in (y, new, *grads))
+        assert bool((grads[1][:, :, w] == 0).all())
+        one = {k: v[:, :, 3] if k in ("x", "dt", "b", "c", "z") else v for k, v in {**p, "dt": dt, **q}.items()}
+        st = q["state"].clone()
+        ops.selective_scan_step(**{**one, "state": st})
+        assert torch.equal(st, q["state"])
+    dt = p["dt"].clone()
+    dt[:, :, 11] = 1e4
+    y, new = ops.selective_scan(**{**p, "dt": dt, "a": p["a"] - 1}, **q)
+    v = dt[:, :, 11].float() + q["dt_bias"]
+    want = (v * x[:, :, 11].float())[..., None] * p["b"][:, :, 11, None].float()
+    assert torch.allclose(new, want, rtol=1e-6, atol=1e-3)
+    dt[0, 0, 5, 7] = math.nan
+    y, new = ops.selective_scan(**{**p, "dt": dt, "a": p["a"] - 1}, **q)
+    assert bool(y[0, 0, 5:, 7].isnan().all()) and bool(new[0, 0, 7].isnan().all()) and int(new.isnan().sum()) == 16
+
+
 def test_layouts_and_strides():
     """Views of wider buffers, rows that start anywhere, expanded inputs and gradients, transposed envs: the values of the
     contiguous call, to the bit where its form is the same."""
