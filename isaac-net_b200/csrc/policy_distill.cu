@@ -4,11 +4,12 @@
 //   p = softmax(teacher / tau) over the entries in use;  loss = tau^2 sum_k p_k (log p_k - log q_k)
 //   glogits = gloss tau (q - p)
 //
-// Bound by DRAM: the forward call reads the logits once (running maximum and sum, one exponential an element), the
-// backward call reads them again and writes the gradient.  Rows of up to 64 logits are 8 lanes', which hold them in registers, of
-// up to 1024 a warp's, longer ones a block's, and where rows are few a cluster of blocks shares one (forward: joined through
-// distributed shared memory).  Rows may start anywhere: what lies before the first and behind the last 16-byte boundary
-// goes element by element.
+// Bound by DRAM where rows are long: the forward call reads the logits once (running maximum and sum, one exponential an
+// element), the backward call reads them again and writes the gradient.  8192 rows of 32001 bf16: 121 us forward (4.3 TB/s),
+// 178 us backward (5.9 TB/s).  Rows of up to 128 logits are 8 lanes', which hold them in registers, of up to 1024 a
+// warp's, longer ones a block's, and where rows are few a cluster of blocks shares one (forward: joined through distributed
+// shared memory; 64 rows of 131072: 11 + 10 us).  Short rows are bound by latency and by their lists.  Rows may start anywhere:
+// what lies before the first and behind the last 16-byte boundary goes element by element.
 #include <cooperative_groups.h>
 
 #include "policy_seq.cuh"
@@ -17,8 +18,18 @@ namespace inb {
 namespace pol {
 namespace cg = cooperative_groups;
 
-constexpr int DIST_THREADS = 256, DIST_GROUP_V = 64, DIST_GROUP_K = 32, DIST_WARP_V = 1024, DIST_WARP_K = 128;
-constexpr int DIST_U = 4;      // accesses of a thread on their way at once
+// Forward + backward, bf16.  8 lanes a row against a warp a row: 262144 rows of 33 with lists of 8 86 us against 301, of 100
+// and 8 121 against 287, of 100 and 64 301 against 397; of 160 and 8 (131072 rows) 111 against 139, but of 256 and 32 212
+// against 152, so they end at 128.
+constexpr int DIST_THREADS = 256, DIST_GROUP_V = 128, DIST_GROUP_K = 64, DIST_WARP_V = 1024, DIST_WARP_K = 128;
+// Accesses of a thread on their way at once, and blocks an SM.  A block a row, 8192 rows of 32001: 316 us with 4 and 5; 335 with 4
+// and 4, 346 with 4 and 6, 324 with 2 and 8 and with 3 and 6, 368 with 8 and 3; 320 with blocks of 128 threads, 342 of 512; 358
+// with resident blocks that send for the next row by cp.async.  A warp a row, 65536 rows of 700: 121 us with 1 and 8; 131 with 1
+// and 6, 133 with 2 and 6, 152 with 4 and 5.
+template <bool WARP>
+struct Depth {
+  static constexpr int U = WARP ? 1 : 4, BLOCKS = WARP ? 8 : 5;
+};
 
 template <typename T>
 struct RowView {
@@ -44,21 +55,24 @@ struct RowView {
     lo = r == 0 ? 0 : head + v0 * W;
     hi = r == n - 1 ? V : head + v1 * W;
   }
-  // DIST_U accesses, `stride` apart from v, of those below end: all on their way before the first is used
+  // U accesses, `stride` apart from v, of those below end: all on their way before the first is used
+  template <int U>
   struct Batch {
-    Words<T, W> q[DIST_U];
-    Words<uint8_t, W> m[DIST_U];
+    Words<T, W> q[U];
+    Words<uint8_t, W> m[U];
   };
-  __device__ __forceinline__ void load(Batch& b, int v, int stride, int end) const {
+  template <int U>
+  __device__ __forceinline__ void load(Batch<U>& b, int v, int stride, int end) const {
 #pragma unroll
-    for (int u = 0; u < DIST_U; ++u)
+    for (int u = 0; u < U; ++u)
       if (v + u * stride < end) {
         b.q[u].load(x + head + (v + u * stride) * W);
         if (mask != nullptr) b.m[u].load(mask + head + (v + u * stride) * W);
       }
   }
   // an access's elements, -inf where they are not allowed
-  __device__ __forceinline__ void get(const Batch& b, int u, float (&o)[W]) const {
+  template <int U>
+  __device__ __forceinline__ void get(const Batch<U>& b, int u, float (&o)[W]) const {
 #pragma unroll
     for (int k = 0; k < W; k += 2) {
       const float2 p = b.q[u].pair(k / 2);
@@ -149,10 +163,34 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// A row's list by L lanes: some entries a lane in registers, on their way while the row is; those beyond them from memory later.  Every lane of the warp takes part.
+// What the backward call knows of a row: q = rl exp(z - m), p = rp exp(teacher / tau - top); 0 where no entry is in use, whatever
+// the row's logits are
+struct Grad {
+  float4 stat;
+  float g, gl, c;
+  bool live;
+  __device__ __forceinline__ Grad(const InbDistillArgs& a, int64_t r, float c) : c(c) {
+    stat = *reinterpret_cast<const float4*>(a.stats + 4 * r);
+    live = stat.w != 0.f;
+    g = a.gloss[r] * a.tau, gl = g * stat.y;
+  }
+  __device__ __forceinline__ float value(float v) const { return live && v != -INFINITY ? gl * ex2((v - stat.x) * c) : 0.f; }
+  // an entry of the row's list as (index or -1, p)
+  template <typename T>
+  __device__ __forceinline__ float2 listed(const InbDistillArgs& a, const RowView<T>& row, Entry e) const {
+    e.look(a, row);
+    return make_float2(__int_as_float(live ? e.index : -1), ex2((e.t - stat.z) * c) * stat.w);
+  }
+  // a listed element, from q and the sum of its entries: every entry of an index gives the same value
+  __device__ __forceinline__ float at(float z, float p) const { return g * (stat.y * ex2((z - stat.x) * c) - p); }
+};
+
+__host__ __device__ inline int list_room(int K) { return (K + 1) / 2 * 2; }      // pairs of a list in shared memory
+// A row's list by L lanes: some entries a lane in registers, on their way while the row is; those beyond them from memory later.
+// Every lane of the warp takes part.
 template <typename T, int L>
 struct Entries {
-  static constexpr int HELD = L == 8 ? 4 : 2;
+  static constexpr int HELD = L == 8 ? 4 : L == 32 ? 2 : 1;
   Entry e[HELD];
   __device__ __forceinline__ void fetch(const InbDistillArgs& a, int64_t r, int lane) {
 #pragma unroll
@@ -165,7 +203,54 @@ struct Entries {
 #pragma unroll
     for (int q = 0; q < HELD; ++q) e[q].look(a, row);
   }
-  // the loss, and what the backward call needs
+  // backward: the list as pairs (index or -1, p), an even number of them
+  __device__ __forceinline__ void write(const InbDistillArgs& a, const RowView<T>& row, int64_t r, const Grad& g, int lane, float2* list) const {
+#pragma unroll
+    for (int q = 0; q < HELD; ++q)
+      if (lane + q * L < a.K) list[lane + q * L] = g.listed(a, row, e[q]);
+    for (int k = lane + HELD * L; k < a.K; k += L) {
+      Entry n;
+      n.fetch(a, r * a.K + k);
+      list[k] = g.listed(a, row, n);
+    }
+    if (lane == 0 && (a.K & 1) != 0) list[a.K] = make_float2(__int_as_float(-1), 0.f);
+  }
+  // and, once all of it is there, the listed elements within [lo, hi) of the gradient's row
+  __device__ __forceinline__ void mark(const InbDistillArgs& a, const RowView<T>& row, const Grad& g, int lane, const float2* list, int lo,
+                                       int hi, T* out) const {
+    if (a.K <= L)
+      mark_by<1>(a, row, g, lane, list, lo, hi, out);
+    else
+      mark_by<HELD>(a, row, g, lane, list, lo, hi, out);
+  }
+  // B elements a lane at a time, each the sum over the list
+  template <int B>
+  __device__ __forceinline__ void mark_by(const InbDistillArgs& a, const RowView<T>& row, const Grad& g, int lane, const float2* list, int lo,
+                                          int hi, T* out) const {
+    for (int k0 = lane; k0 < a.K; k0 += B * L) {
+      int i[B];
+      float z[B], p[B];
+#pragma unroll
+      for (int q = 0; q < B; ++q) {
+        i[q] = k0 + q * L < a.K ? __float_as_int(list[k0 + q * L].x) : -1;
+        if (i[q] < lo || i[q] >= hi) i[q] = -1;
+        z[q] = i[q] >= 0 ? row.load1(i[q]) : 0.f;
+        p[q] = 0.f;
+      }
+      for (int o = 0; o < a.K; o += 2) {
+        const float4 two = *reinterpret_cast<const float4*>(list + o);
+#pragma unroll
+        for (int q = 0; q < B; ++q) {
+          if (__float_as_int(two.x) == i[q]) p[q] += two.y;
+          if (__float_as_int(two.z) == i[q]) p[q] += two.w;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < B; ++q)
+        if (i[q] >= 0) out[i[q]] = from_f<T>(g.at(z[q], p[q]));
+    }
+  }
+  // forward: the loss, and what the backward call needs
   __device__ __forceinline__ void finish(const InbDistillArgs& a, const RowView<T>& row, int64_t r, float m, float l, float c, int lane,
                                          bool on) const {
     float top = e[0].t;
@@ -206,8 +291,8 @@ struct Entries {
 
 // A row a warp, or (WARP false) a row `parts` blocks
 template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS, 5) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
-  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W;
+__global__ void __launch_bounds__(DIST_THREADS, Depth<WARP>::BLOCKS) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
+  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Depth<WARP>::U;
   const int tid = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
   const int part = WARP ? 0 : blockIdx.x % parts;
@@ -219,11 +304,11 @@ __global__ void __launch_bounds__(DIST_THREADS, 5) distill_fwd_kernel(InbDistill
   Entries<T, 32> list;
   const bool lists = WARP || (part == 0 && threadIdx.x < 32);
   if (lists) list.fetch(a, r, lane);
-  for (int v = v0 + tid; v < v1; v += TPR * DIST_U) {
-    typename RowView<T>::Batch b;
+  for (int v = v0 + tid; v < v1; v += TPR * U) {
+    typename RowView<T>::template Batch<U> b;
     row.load(b, v, TPR, v1);
 #pragma unroll
-    for (int u = 0; u < DIST_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (v + u * TPR >= v1) break;
       float x[W];
       row.get(b, u, x);
@@ -269,38 +354,10 @@ __global__ void __launch_bounds__(DIST_THREADS, 5) distill_fwd_kernel(InbDistill
   if (lists) list.finish(a, row, r, s.m, s.l, c, lane, true);
 }
 
-// What the backward call knows of a row: q = rl exp(z - m), p = rp exp(teacher / tau - top); 0 where no entry is in use, whatever
-// the row's logits are
-struct Grad {
-  float4 stat;
-  float g, gl, c;
-  bool live;
-  __device__ __forceinline__ Grad(const InbDistillArgs& a, int64_t r, float c) : c(c) {
-    stat = *reinterpret_cast<const float4*>(a.stats + 4 * r);
-    live = stat.w != 0.f;
-    g = a.gloss[r] * a.tau, gl = g * stat.y;
-  }
-  __device__ __forceinline__ float value(float v) const { return live && v != -INFINITY ? gl * ex2((v - stat.x) * c) : 0.f; }
-  // an entry of the row's list as (index or -1, p)
-  template <typename T>
-  __device__ __forceinline__ float2 listed(const InbDistillArgs& a, const RowView<T>& row, Entry e) const {
-    e.look(a, row);
-    return make_float2(__int_as_float(live ? e.index : -1), ex2((e.t - stat.z) * c) * stat.w);
-  }
-  // a listed element, from q and the sum of its entries: every entry of an index gives the same value
-  template <typename T>
-  __device__ __forceinline__ float at(const RowView<T>& row, const float2* list, int K, int i) const {
-    float p = 0.f;
-    for (int o = 0; o < K; ++o)
-      if (__float_as_int(list[o].x) == i) p += list[o].y;
-    return g * (stat.y * ex2((row.load1(i) - stat.x) * c) - p);
-  }
-};
-
 template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS, 5) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
-  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W;
-  extern __shared__ float2 entries[];
+__global__ void __launch_bounds__(DIST_THREADS, Depth<WARP>::BLOCKS) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
+  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Depth<WARP>::U;
+  extern __shared__ float4 lists[];
   const int tid = threadIdx.x % TPR;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
   const int part = WARP ? 0 : blockIdx.x % parts;
@@ -310,14 +367,14 @@ __global__ void __launch_bounds__(DIST_THREADS, 5) distill_bwd_kernel(InbDistill
   int v0, v1, lo, hi;
   row.part(part, parts, v0, v1, lo, hi);
   const Grad g(a, r, c);
-  float2* list = entries + (WARP ? threadIdx.x / 32 * a.K : 0);
-  Entry first;                                   // the thread's first entry: on its way while the row is
-  if (tid < a.K) first.fetch(a, r * a.K + tid);
-  for (int v = v0 + tid; v < v1; v += TPR * DIST_U) {
-    typename RowView<T>::Batch b;
+  float2* list = (float2*)lists + (WARP ? threadIdx.x / 32 * list_room(a.K) : 0);
+  Entries<T, TPR> entries;
+  entries.fetch(a, r, tid);
+  for (int v = v0 + tid; v < v1; v += TPR * U) {
+    typename RowView<T>::template Batch<U> b;
     row.load(b, v, TPR, v1);
 #pragma unroll
-    for (int u = 0; u < DIST_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (v + u * TPR >= v1) break;
       float x[W];
       row.get(b, u, x);
@@ -330,26 +387,19 @@ __global__ void __launch_bounds__(DIST_THREADS, 5) distill_bwd_kernel(InbDistill
   const int body = row.head + v0 * W, end = row.head + v1 * W;
   for (int i = lo + tid; i < body; i += TPR) out[i] = from_f<T>(g.value(row.load1(i)));
   for (int i = end + tid; i < hi; i += TPR) out[i] = from_f<T>(g.value(row.load1(i)));
-  if (tid < a.K) list[tid] = g.listed(a, row, first);
-  for (int k = tid + TPR; k < a.K; k += TPR) {
-    first.fetch(a, r * a.K + k);
-    list[k] = g.listed(a, row, first);
-  }
+  entries.write(a, row, r, g, tid, list);
   if (WARP)
     __syncwarp();
   else
     __syncthreads();
-  for (int k = tid; k < a.K; k += TPR) {
-    const int i = __float_as_int(list[k].x);
-    if (i >= lo && i < hi) out[i] = from_f<T>(g.at(row, list, a.K, i));
-  }
+  entries.mark(a, row, g, tid, list, lo, hi, out);
 }
 
 // Short rows: 8 lanes hold one
-template <typename T, bool BACK>
+template <typename T, int M, bool BACK>
 __global__ void __launch_bounds__(DIST_THREADS) distill_short_kernel(InbDistillArgs a, float c) {
-  constexpr int L = 8, M = DIST_GROUP_V / L;
-  extern __shared__ float2 entries[];
+  constexpr int L = 8;
+  extern __shared__ float4 lists[];
   const int lane = threadIdx.x % L;
   const int64_t r0 = (int64_t)blockIdx.x * (DIST_THREADS / L) + threadIdx.x / L;
   const bool on = r0 < a.N;
@@ -367,9 +417,9 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_short_kernel(InbDistillA
       ok[i] = row.mask != nullptr ? row.mask[k] : 1;
     }
   }
+  Entries<T, L> entries;
+  entries.fetch(a, r, lane);
   if constexpr (!BACK) {
-    Entries<T, L> list;
-    list.fetch(a, r, lane);
     float x[M];
 #pragma unroll
     for (int i = 0; i < M; ++i) x[i] = ok[i] ? raw_f<T>(raw[i]) : -INFINITY;
@@ -377,31 +427,24 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_short_kernel(InbDistillA
 #pragma unroll
     for (int i = 1; i < M; ++i) m = fmaxf(m, x[i]);
     m = lanes_max<L>(m);
-    list.look(a, row);
+    entries.look(a, row);
     const float at = m == -INFINITY ? 0.f : m;
     float l = 0.f;
 #pragma unroll
     for (int i = 0; i < M; ++i)
       if (i * L < a.V) l += ex2((x[i] - at) * c);
     l = lanes_sum<L>(l);
-    list.finish(a, row, r, m, l, c, lane, on);
+    entries.finish(a, row, r, m, l, c, lane, on);
   } else {
     T* out = (T*)a.glogits + r * a.V;
     const Grad g(a, r, c);
-    float2* list = entries + threadIdx.x / L * a.K;
-    for (int k = lane; k < a.K; k += L) {
-      Entry e;
-      e.fetch(a, r * a.K + k);
-      list[k] = g.listed(a, row, e);
-    }
+    float2* list = (float2*)lists + threadIdx.x / L * list_room(a.K);
+    entries.write(a, row, r, g, lane, list);
 #pragma unroll
     for (int i = 0; i < M; ++i)
       if (on && i * L + lane < a.V) out[i * L + lane] = from_f<T>(g.value(ok[i] ? raw_f<T>(raw[i]) : -INFINITY));
     __syncwarp();
-    for (int k = lane; k < a.K; k += L) {
-      const int i = __float_as_int(list[k].x);
-      if (on && i >= 0) out[i] = from_f<T>(g.at(row, list, a.K, i));
-    }
+    entries.mark(a, row, g, lane, list, 0, on ? a.V : 0, out);
   }
 }
 
@@ -427,7 +470,8 @@ static int dist_fwd(const InbDistillArgs& a, cudaStream_t s) {
   const DistPlan p = dist_plan(a);
   const float c = LOG2E / a.tau;
   if (p.form == DIST_GROUP) {
-    distill_short_kernel<T, false><<<p.blocks, DIST_THREADS, 0, s>>>(a, c);
+    const auto kernel = a.V <= DIST_GROUP_V / 2 ? distill_short_kernel<T, 8, false> : distill_short_kernel<T, 16, false>;
+    kernel<<<p.blocks, DIST_THREADS, 0, s>>>(a, c);
     return launch_status();
   }
   if (p.form == DIST_WARP) {
@@ -451,10 +495,11 @@ template <typename T>
 static int dist_bwd(const InbDistillArgs& a, cudaStream_t s) {
   const DistPlan p = dist_plan(a);
   const float c = LOG2E / a.tau;
-  const size_t smem = (size_t)p.rows * a.K * 8;      // at most 8 KB
-  if (p.form == DIST_GROUP)
-    distill_short_kernel<T, true><<<p.blocks, DIST_THREADS, smem, s>>>(a, c);
-  else if (p.form == DIST_WARP)
+  const size_t smem = (size_t)p.rows * list_room(a.K) * 8;      // at most 16 KB
+  if (p.form == DIST_GROUP) {
+    const auto kernel = a.V <= DIST_GROUP_V / 2 ? distill_short_kernel<T, 8, true> : distill_short_kernel<T, 16, true>;
+    kernel<<<p.blocks, DIST_THREADS, smem, s>>>(a, c);
+  } else if (p.form == DIST_WARP)
     distill_bwd_kernel<T, true><<<p.blocks, DIST_THREADS, smem, s>>>(a, 1, c);
   else
     distill_bwd_kernel<T, false><<<p.blocks, DIST_THREADS, smem, s>>>(a, p.parts, c);

@@ -167,3 +167,16 @@ def test_distill_gradient_against_differences():
             got = float((f(logits + h * way) - f(logits - h * way)) / (2 * h))
         want = float((grad.double() * way.double()).sum())
         assert abs(got - want) < 2.0 ** -9 * tau ** 2 * (1 + float(grad.norm()))
+
+
+@pytest.mark.parametrize("v", [64, 65, 128, 129, 1024, 1025])
+@pytest.mark.parametrize("k", [1, 7, 8, 9, 32, 33, 63, 64, 65, 128, 129, 255, 257])
+def test_lists_of_every_form_with_repeated_entries(v, k):
+    """Where the number of lanes of a row, and of entries that a lane holds, changes; odd lists; the same index many times."""
+    g = gen(1000 * v + k)
+    for dtype in DT:
+        rows = 37
+        logits = (rn(g, rows, v) * 2).to(dtype)
+        index = torch.randint(-1, min(v, 40), (rows, k), generator=g, device="cuda")
+        index[3] = v - 1
+        check(logits, rn(g, rows, k).to(dtype), index, mask=torch.rand(rows, v, generator=g, device="cuda") < 0.8)
