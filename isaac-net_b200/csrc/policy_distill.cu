@@ -6,10 +6,10 @@
 //
 // Bound by DRAM where rows are long: the forward call reads the logits once (running maximum and sum, one exponential an
 // element), the backward call reads them again and writes the gradient.  8192 rows of 32001 bf16: 121 us forward (4.3 TB/s),
-// 178 us backward (5.9 TB/s).  Rows of up to 128 logits are 8 lanes', which hold them in registers, of up to 1024 a
-// warp's, longer ones a block's, and where rows are few a cluster of blocks shares one (forward: joined through distributed
-// shared memory; 64 rows of 131072: 11 + 10 us).  Short rows are bound by latency and by their lists.  Rows may start anywhere:
-// what lies before the first and behind the last 16-byte boundary goes element by element.
+// 178 us backward (5.9 TB/s).  Rows of up to 128 logits are 8 lanes', which hold them in registers, longer ones a warp's, very
+// long ones and few a block's or a cluster of blocks' (forward: joined through distributed shared memory; 64 rows of 131072:
+// 11 + 10 us).  Short rows are bound by latency and by their lists (131072 rows of 33, lists of 8: 21 + 23 us).  Rows may start
+// anywhere: what lies before the first and behind the last 16-byte boundary goes element by element.
 #include <cooperative_groups.h>
 
 #include "policy_seq.cuh"
@@ -18,17 +18,25 @@ namespace inb {
 namespace pol {
 namespace cg = cooperative_groups;
 
-// Forward + backward, bf16.  8 lanes a row against a warp a row: 262144 rows of 33 with lists of 8 86 us against 301, of 100
-// and 8 121 against 287, of 100 and 64 301 against 397; of 160 and 8 (131072 rows) 111 against 139, but of 256 and 32 212
-// against 152, so they end at 128.
-constexpr int DIST_THREADS = 256, DIST_GROUP_V = 128, DIST_GROUP_K = 64, DIST_WARP_V = 1024, DIST_WARP_K = 128;
-// Accesses of a thread on their way at once, and blocks an SM.  A block a row, 8192 rows of 32001: 316 us with 4 and 5; 335 with 4
-// and 4, 346 with 4 and 6, 324 with 2 and 8 and with 3 and 6, 368 with 8 and 3; 320 with blocks of 128 threads, 342 of 512; 358
-// with resident blocks that send for the next row by cp.async.  A warp a row, 65536 rows of 700: 121 us with 1 and 8; 131 with 1
-// and 6, 133 with 2 and 6, 152 with 4 and 5.
-template <bool WARP>
-struct Depth {
-  static constexpr int U = WARP ? 1 : 4, BLOCKS = WARP ? 8 : 5;
+// Which form a call takes, by the length of its rows and lists and by its rows.  Forward + backward, bf16:
+//   GROUP, 8 lanes a row, against a warp a row: 262144 rows of 33 with lists of 8 86 us against 301, of 100 and 8 121 against
+//     287, of 100 and 64 301 against 397; of 160 and 8 (131072 rows) 111 against 139, but of 256 and 32 212 against 152
+//   WARP, one access of a lane on its way, 8 blocks an SM, against DEEP: 65536 rows of 700 121 us against 137, of 1024 166 against
+//     184; but 4096 rows of 1024, fewer than the GPU holds warps, 27 against 21
+//   DEEP, a warp a row, four accesses, 4 blocks an SM, against BLOCK: 32768 rows of 2048 113 us against 301, 16384 of 4000 104
+//     against 182, 8192 of 8192 102 against 121, of 16384 176 against 178, of 32001 334 against 315; 2048 rows of 4000 31 against
+//     35, 1024 rows 27 against 25, 64 rows 39 against 16: a warp's time goes by the row, the blocks' by the rows.
+//     With lists of 512 32768 rows of 2048 867 us against 1411, 64 rows of 400 70 against 35
+//   BLOCK: four accesses, 5 blocks an SM.  8192 rows of 32001: 315 us; 335 with 4 blocks, 346 with 6, 324 with 2 accesses and 8
+//     blocks, 368 with 8 and 3; 320 with blocks of 128 threads, 342 of 512; 358 with resident blocks that send for the next row
+//     by cp.async.  `parts` blocks, a cluster, share a row while all are resident: 64 rows of 131072 29 us with 8, 57 with 1
+enum { DIST_GROUP, DIST_WARP, DIST_DEEP, DIST_BLOCK };
+constexpr int DIST_THREADS = 256, DIST_GROUP_V = 128, DIST_GROUP_K = 64, DIST_WARP_V = 1024, DIST_DEEP_V = 16384, DIST_WARP_K = 512;
+template <int FORM>
+struct Form {
+  static constexpr bool WARP = FORM != DIST_BLOCK;
+  static constexpr int U = FORM == DIST_WARP ? 1 : 4;               // accesses of a thread on their way at once
+  static constexpr int BLOCKS = FORM == DIST_WARP ? 8 : FORM == DIST_DEEP ? 4 : 5;      // an SM
 };
 
 template <typename T>
@@ -289,10 +297,11 @@ struct Entries {
   }
 };
 
-// A row a warp, or (WARP false) a row `parts` blocks
-template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS, Depth<WARP>::BLOCKS) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
-  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Depth<WARP>::U;
+// A row a warp, or (BLOCK) a row `parts` blocks
+template <typename T, int FORM>
+__global__ void __launch_bounds__(DIST_THREADS, Form<FORM>::BLOCKS) distill_fwd_kernel(InbDistillArgs a, int parts, float c) {
+  constexpr bool WARP = Form<FORM>::WARP;
+  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Form<FORM>::U;
   const int tid = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
   const int part = WARP ? 0 : blockIdx.x % parts;
@@ -354,9 +363,10 @@ __global__ void __launch_bounds__(DIST_THREADS, Depth<WARP>::BLOCKS) distill_fwd
   if (lists) list.finish(a, row, r, s.m, s.l, c, lane, true);
 }
 
-template <typename T, bool WARP>
-__global__ void __launch_bounds__(DIST_THREADS, Depth<WARP>::BLOCKS) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
-  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Depth<WARP>::U;
+template <typename T, int FORM>
+__global__ void __launch_bounds__(DIST_THREADS, Form<FORM>::BLOCKS) distill_bwd_kernel(InbDistillArgs a, int parts, float c) {
+  constexpr bool WARP = Form<FORM>::WARP;
+  constexpr int TPR = WARP ? 32 : DIST_THREADS, W = RowView<T>::W, U = Form<FORM>::U;
   extern __shared__ float4 lists[];
   const int tid = threadIdx.x % TPR;
   const int64_t r = WARP ? (int64_t)blockIdx.x * (DIST_THREADS / 32) + threadIdx.x / 32 : blockIdx.x / parts;
@@ -448,20 +458,19 @@ __global__ void __launch_bounds__(DIST_THREADS) distill_short_kernel(InbDistillA
   }
 }
 
-// Which form a call takes, by the length of its rows and lists
-enum { DIST_GROUP, DIST_WARP, DIST_BLOCK };
 struct DistPlan {
   int form, parts, rows;         // blocks that share a row, rows of a block
   unsigned blocks;
 };
 static DistPlan dist_plan(const InbDistillArgs& a) {
   DistPlan p = {DIST_BLOCK, 1, 1, 0};
+  const int64_t row = a.V > 8 * a.K ? a.V : 8 * a.K;      // what a warp's time goes by
   if (a.V <= DIST_GROUP_V && a.K <= DIST_GROUP_K)
     p.form = DIST_GROUP, p.rows = DIST_THREADS / 8;
-  else if (a.V <= DIST_WARP_V && a.K <= DIST_WARP_K)
-    p.form = DIST_WARP, p.rows = DIST_THREADS / 32;
+  else if (a.V <= DIST_DEEP_V && a.K <= DIST_WARP_K && (row <= DIST_WARP_V / 2 || a.N * 2 >= row))
+    p.form = a.V <= DIST_WARP_V && a.N >= sm_count() * 64 ? DIST_WARP : DIST_DEEP, p.rows = DIST_THREADS / 32;
   else
-    while (p.parts < 8 && a.N * p.parts < sm_count() * 4 && a.V / (2 * p.parts) >= 4096) p.parts *= 2;
+    while (p.parts < 8 && a.N * p.parts * 2 <= sm_count() * Form<DIST_BLOCK>::BLOCKS && a.V / (2 * p.parts) >= 4096) p.parts *= 2;
   p.blocks = (unsigned)(ceil_div(a.N, p.rows) * p.parts);
   return p;
 }
@@ -474,8 +483,9 @@ static int dist_fwd(const InbDistillArgs& a, cudaStream_t s) {
     kernel<<<p.blocks, DIST_THREADS, 0, s>>>(a, c);
     return launch_status();
   }
-  if (p.form == DIST_WARP) {
-    distill_fwd_kernel<T, true><<<p.blocks, DIST_THREADS, 0, s>>>(a, 1, c);
+  if (p.form != DIST_BLOCK) {
+    const auto kernel = p.form == DIST_WARP ? distill_fwd_kernel<T, DIST_WARP> : distill_fwd_kernel<T, DIST_DEEP>;
+    kernel<<<p.blocks, DIST_THREADS, 0, s>>>(a, 1, c);
     return launch_status();
   }
   cudaLaunchConfig_t cfg = {};
@@ -488,21 +498,23 @@ static int dist_fwd(const InbDistillArgs& a, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T, false>, a, p.parts, c);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T, DIST_BLOCK>, a, p.parts, c);
   return e == cudaSuccess ? launch_status() : -100 - (int)e;
 }
 template <typename T>
 static int dist_bwd(const InbDistillArgs& a, cudaStream_t s) {
   const DistPlan p = dist_plan(a);
   const float c = LOG2E / a.tau;
-  const size_t smem = (size_t)p.rows * list_room(a.K) * 8;      // at most 16 KB
+  const size_t smem = (size_t)p.rows * list_room(a.K) * 8;      // at most 32 KB
   if (p.form == DIST_GROUP) {
     const auto kernel = a.V <= DIST_GROUP_V / 2 ? distill_short_kernel<T, 8, true> : distill_short_kernel<T, 16, true>;
     kernel<<<p.blocks, DIST_THREADS, smem, s>>>(a, c);
-  } else if (p.form == DIST_WARP)
-    distill_bwd_kernel<T, true><<<p.blocks, DIST_THREADS, smem, s>>>(a, 1, c);
-  else
-    distill_bwd_kernel<T, false><<<p.blocks, DIST_THREADS, smem, s>>>(a, p.parts, c);
+  } else {
+    const auto kernel = p.form == DIST_WARP   ? distill_bwd_kernel<T, DIST_WARP>
+                        : p.form == DIST_DEEP ? distill_bwd_kernel<T, DIST_DEEP>
+                                              : distill_bwd_kernel<T, DIST_BLOCK>;
+    kernel<<<p.blocks, DIST_THREADS, smem, s>>>(a, p.parts, c);
+  }
   return launch_status();
 }
 static int dist_check(const InbDistillArgs& a) {

@@ -180,3 +180,14 @@ def test_lists_of_every_form_with_repeated_entries(v, k):
         index = torch.randint(-1, min(v, 40), (rows, k), generator=g, device="cuda")
         index[3] = v - 1
         check(logits, rn(g, rows, k).to(dtype), index, mask=torch.rand(rows, v, generator=g, device="cuda") < 0.8)
+
+
+@pytest.mark.parametrize("rows,v,k", [(9600, 600, 5), (4800, 1000, 33), (4100, 2049, 9), (8200, 16384, 3), (2100, 400, 512), (1000, 400, 511),
+                                      (740, 9000, 4), (370, 9000, 4)])
+def test_many_rows_of_every_form(rows, v, k):
+    """Where rows are many enough for a warp each, or few enough for several blocks each; rows apart and unaligned."""
+    g = gen(rows)
+    for dtype in (torch.bfloat16, torch.float32):
+        wide = (rn(g, rows, v + 3) * 2).to(dtype)
+        index = torch.randint(0, v, (rows, k), generator=g, device="cuda")
+        check(wide[:, 1:1 + v], rn(g, rows, k).to(dtype), index)
