@@ -640,16 +640,22 @@ static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
 }
-// Channels a thread: 16 bytes forward, 4 channels backward, whose sums take the registers; 4 where rows are not aligned to that
-template <typename T, bool WIDE>
-static int conv_go(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  constexpr int W = WIDE ? 16 / sizeof(T) : 4;
-  if (backward) return a.K == 2 ? conv_bwd_go<T, 4, WIDE, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, 4, WIDE, 3>(a, s) : conv_bwd_go<T, 4, WIDE, 4>(a, s);
-  return a.K == 2 ? conv_fwd_go<T, W, WIDE, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, W, WIDE, 3>(a, s) : conv_fwd_go<T, W, WIDE, 4>(a, s);
+// Channels a thread
+template <typename T, int V, bool WIDE>
+static int conv_taps(const InbConvArgs& a, bool backward, cudaStream_t s) {
+  if (backward) {
+    if constexpr (V <= 4) return a.K == 2 ? conv_bwd_go<T, V, WIDE, 2>(a, s) : a.K == 3 ? conv_bwd_go<T, V, WIDE, 3>(a, s) : conv_bwd_go<T, V, WIDE, 4>(a, s);
+    return -2;
+  }
+  return a.K == 2 ? conv_fwd_go<T, V, WIDE, 2>(a, s) : a.K == 3 ? conv_fwd_go<T, V, WIDE, 3>(a, s) : conv_fwd_go<T, V, WIDE, 4>(a, s);
 }
 template <typename T>
 static int conv_type(const InbConvArgs& a, bool backward, cudaStream_t s) {
-  return conv_aligned(a, backward ? 4 * sizeof(T) : 16) ? conv_go<T, true>(a, backward, s) : conv_go<T, false>(a, backward, s);
+  constexpr int W = 16 / sizeof(T), E = sizeof(T);
+  if (!backward && W > 4 && conv_aligned(a, 16)) return conv_taps<T, W, true>(a, false, s);
+  if (conv_aligned(a, 4 * E)) return conv_taps<T, 4, true>(a, backward, s);
+  if (conv_aligned(a, 2 * E)) return conv_taps<T, 2, true>(a, backward, s);
+  return conv_taps<T, 2, false>(a, backward, s);
 }
 static int conv_dispatch(const InbConvArgs& a, bool backward, cudaStream_t s) {
   if (a.dtype == INB_BF16) return conv_type<bf16>(a, backward, s);
@@ -677,7 +683,11 @@ extern "C" int inb_causal_conv_work(const InbConvArgs* args, int64_t* elems) {
   if (rc != 0) return rc;
   *elems = 0;
   if (a.S == 0 || a.T == 0) return 0;
-  *elems = (int64_t)inb::pol::conv_plan(a, 4, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
+  // the rows' alignment, which decides on the channels a thread, is the launch's to find out
+  for (int v : {2, 4}) {
+    const int64_t n = (int64_t)inb::pol::conv_plan(a, v, inb::pol::CONV_BWD_BLOCKS).grid.x * a.C * (a.K + 1);
+    if (n > *elems) *elems = n;
+  }
   return 0;
 }
 

@@ -108,7 +108,7 @@ __device__ __forceinline__ float raw_f(uint32_t v) {
     return __uint_as_float(v);
 }
 
-// V (1, 4 or 8; up to 16 bytes) neighbouring elements as they lie in memory; their values as pairs (V = 1: the first of one pair)
+// V (1, 2, 4 or 8; up to 16 bytes) neighbouring elements as they lie in memory; their values as pairs (V = 1: the first of one pair)
 template <typename T, int V>
 struct Words {
   static constexpr int P = V < 2 ? 1 : V / 2, N = V * sizeof(T) / 4 > 0 ? V * sizeof(T) / 4 : 1;
@@ -129,7 +129,7 @@ struct Words {
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (V == 1 && sizeof(T) == 2)
       *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
-    else if constexpr (V == 1)
+    else if constexpr (N == 1)
       *reinterpret_cast<uint32_t*>(p) = w[0];
     else if constexpr (N == 2)
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
