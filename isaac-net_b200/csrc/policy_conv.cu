@@ -11,7 +11,12 @@
 namespace inb {
 namespace pol {
 
-constexpr int CONV_FWD_BLOCKS = 4, CONV_STEP_BLOCKS = 4, CONV_BWD_BLOCKS = 4;      // of 128 threads, an SM
+// Blocks of 128 threads, an SM.  80 sequences of 3373 steps of 458 bf16 channels, 2 a thread: forward 199 us with 4, 279 with 6, 330
+// with 8; backward 402 with 4, 421 with 6, 516 with 8.
+constexpr int CONV_FWD_BLOCKS = 4, CONV_BWD_BLOCKS = 4;
+// A single step's: 16880 sequences of 458 channels, 2 a thread by one access, bf16 59 us with 4, 49 with 6, 43 with 8, fp32 78, 53, 63;
+// by two accesses (457 channels) 86, 92, 88 and 78, 91, 87
+constexpr int conv_step_blocks(int V, bool wide) { return V == 2 && wide ? 6 : 4; }
 constexpr int CONV_STEP_B = 2;  // sequences whose loads are sent at once by a single step
 
 struct ConvPlan {
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
 
 // One step: bound by the states' bytes, of which a thread has CONV_STEP_B sequences' on their way at once; state_out may be state.
 template <typename T, int V, bool WIDE, int K>
-__global__ void __launch_bounds__(128, CONV_STEP_BLOCKS) conv_step_kernel(InbConvArgs a) {
+__global__ void __launch_bounds__(128, conv_step_blocks(V, WIDE)) conv_step_kernel(InbConvArgs a) {
   constexpr int P = Words<T, V>::P;
   const Lanes<T, V, WIDE> io(a);
   if (io.count == 0) return;
@@ -617,7 +622,7 @@ static int conv_check(const InbConvArgs& a) {
 template <typename T, int V, bool WIDE, int K>
 static int conv_fwd_go(const InbConvArgs& a, cudaStream_t s) {
   if (a.T == 1) {
-    const ConvLaunch l = conv_plan(a, V, CONV_STEP_BLOCKS);
+    const ConvLaunch l = conv_plan(a, V, conv_step_blocks(V, WIDE));
     conv_step_kernel<T, V, WIDE, K><<<l.grid, l.block, 0, s>>>(a);
     return launch_status();
   }

@@ -9,8 +9,8 @@
 namespace inb {
 namespace pol {
 
-constexpr int SCAN_WARPS = 4;        // a block's warps work on their own; no barrier
-
+// A block's SCAN_WARPS warps work on their own; no barrier.
+//
 // MODE 0: outputs; 1: outputs, and the state before every SCAN_STEPS steps is kept for the backward pass; 2: a part's
 // end state from zero and its sum of delta (-1 where an episode began inside), 3: the same of the reverse recurrence
 // r[t - 1] = exp(delta[t] a) (r[t] + c[t] g[t]), g = gy silu(z), which runs from the part's last step to its first.
@@ -250,15 +250,18 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 }
 
 // One step: bound by the states' bytes.  A thread holds V x G states of one channel (V moved by one access; `lanes` threads a
-// channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.
+// channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.  A block takes
+// `chans` channels (a power of two, a warp's at least) of `runs` sequences at a time (MANY: more than one), next to one another, `per` times.
 constexpr int STEP_THREADS = 256, STEP_B = 2;
-template <typename T, int V, int G>
-__global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs a, int lanes, int per) {
-  const int j = threadIdx.x % lanes, chans = STEP_THREADS / lanes;
-  const int c0 = blockIdx.x * chans + threadIdx.x / lanes;
+template <typename T, int V, int G, bool MANY>
+__global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs a, int lanes, int chans, int per) {
+  const int j = threadIdx.x & (lanes - 1), w = threadIdx.x / lanes;
+  const int c0 = blockIdx.x * chans + (w & (chans - 1));
   const bool on = c0 < a.C;
   const int ch = on ? c0 : a.C - 1;
-  const int64_t s0 = (int64_t)blockIdx.y * per, s1 = s0 + per < a.S ? s0 + per : a.S;
+  const uint32_t runs = MANY ? STEP_THREADS / (lanes * chans) : 1;
+  const int64_t b0 = (int64_t)blockIdx.y * per * runs, s0 = MANY ? b0 + w / chans : b0, s1 = b0 + (int64_t)per * runs < a.S ? b0 + (int64_t)per * runs : a.S;
+  if (s0 >= a.S) return;
   const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = a.d != nullptr ? a.d[ch] : 0.f;
   const bool gate = a.z.p != nullptr;
   float A[G][V];
@@ -272,8 +275,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
   // the reset flag's row, and how many sequences of it have passed
   const uint8_t* pr = resets(a.reset, s0);
   uint32_t of = pr != nullptr ? (uint32_t)s0 % (uint32_t)a.reset.rows : 0;
-  for (int64_t s = s0; s < s1; s += STEP_B) {
-    const int n = s1 - s < STEP_B ? (int)(s1 - s) : STEP_B;
+  for (int64_t s = s0; s < s1; s += STEP_B * runs) {
+    const int n = s1 - s > (STEP_B - 1) * (int64_t)runs ? STEP_B : (int)((s1 - s + runs - 1) / runs);
     uint32_t x[STEP_B], dt[STEP_B], z[STEP_B], cut[STEP_B];
     Words<T, V> b[STEP_B][G], c[STEP_B][G];
     Pack<float, V> h[STEP_B][G];
@@ -290,9 +293,11 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
       cut[u] = 0;
       if (pr != nullptr && u < n) {
         cut[u] = *pr;
-        if (++of == (uint32_t)a.reset.rows) {
-          of = 0;
-          if (s + u + 1 < a.S) pr += a.reset.seq;
+        of += runs;
+        if (of >= (uint32_t)a.reset.rows) {
+          const uint32_t past = MANY ? of / (uint32_t)a.reset.rows : 1;
+          of -= past * (uint32_t)a.reset.rows;
+          if (s + (u + 1) * (int64_t)runs < a.S) pr += past * a.reset.seq;
         }
       }
 #pragma unroll
@@ -302,9 +307,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
         b[u][q].load(pb + k0), c[u][q].load(pc + k0);
       }
       if (u + 1 < n) {
-        px += a.x.seq, pd += a.dt.seq, pb += a.b.seq, pc += a.c.seq;
-        if (gate) pz += a.z.seq;
-        if (ph != nullptr) ph += a.state_seq;
+        px += runs * a.x.seq, pd += runs * a.dt.seq, pb += runs * a.b.seq, pc += runs * a.c.seq;
+        if (gate) pz += runs * a.z.seq;
+        if (ph != nullptr) ph += runs * a.state_seq;
       }
     }
 #pragma unroll
@@ -332,8 +337,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
         y *= zv * sigmoid(zv);
       }
       if (on && j == 0) *py = from_f<T>(y);
-      py += a.y.seq;
-      if (po != nullptr) po += a.state_out_seq;
+      py += runs * a.y.seq;
+      if (po != nullptr) po += runs * a.state_out_seq;
     }
   }
 }
@@ -352,7 +357,7 @@ int scan_join(const InbScanArgs& a, const ScanPlan& p, float* carry, bool revers
 
 template <typename T, int NS, int LN, int MODE>
 static void scan_go(const InbScanArgs& a, const ScanPlan& p, float* carry, cudaStream_t s) {
-  const int64_t tiles = ceil_div(a.C, 32 / LN), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
+  const int64_t tiles = ceil_div(a.C, 32 / LN), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;      // as scan_plan has them
   // nothing begins with what the last part (reverse: the first) ends with
   const dim3 grid((unsigned)(a.S * (MODE < 2 ? p.parts : p.parts - 1)), (unsigned)ceil_div(tiles, warps));
   if constexpr (NS == 16 && LN == 1) {
@@ -390,14 +395,17 @@ static int scan_type(const InbScanArgs& a, const ScanPlan& p, float* carry, int 
 }
 template <typename T, int V, int G>
 static int step_go(const InbScanArgs& a, int lanes, cudaStream_t s) {
-  const int64_t tiles = ceil_div(a.C, STEP_THREADS / lanes);
-  // as many sequences a block as leave six blocks an SM, no more than 32, and a grid's second axis ends at 65535
-  int64_t per = a.S * tiles / (sm_count() * 6);
+  int chans = STEP_THREADS / lanes;
+  while (chans / 2 >= a.C && chans * lanes > 32) chans /= 2;      // a warp is one sequence's
+  const int64_t tiles = ceil_div(a.C, chans), runs = STEP_THREADS / (lanes * chans);
+  // as many times as leave six blocks an SM, no more than 32, and a grid's second axis ends at 65535
+  int64_t per = a.S * tiles / (sm_count() * 6 * runs);
   if (per > 32) per = 32;
   if (per > 1) per = ceil_div(per, STEP_B) * STEP_B;
-  if (per < ceil_div(a.S, 65535)) per = ceil_div(a.S, 65535);
+  if (per < ceil_div(a.S, 65535 * runs)) per = ceil_div(a.S, 65535 * runs);
   if (per < 1) per = 1;
-  scan_step_kernel<T, V, G><<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per)), STEP_THREADS, 0, s>>>(a, lanes, (int)per);
+  const auto kernel = runs > 1 ? scan_step_kernel<T, V, G, true> : scan_step_kernel<T, V, G, false>;
+  kernel<<<dim3((unsigned)tiles, (unsigned)ceil_div(a.S, per * runs)), STEP_THREADS, 0, s>>>(a, lanes, chans, (int)per);
   return launch_status();
 }
 template <typename T>
@@ -447,7 +455,7 @@ extern "C" int inb_selective_scan_fwd(const InbScanArgs* args, void* cuda_stream
     if (a.dtype == INB_F16) return scan_step<f16>(a, s);
     return scan_step<float>(a, s);
   }
-  const ScanPlan p = scan_plan(a, 32 / scan_lanes(a.N));
+  const ScanPlan p = scan_plan(a);
   if (p.split() && (a.work == nullptr || a.work_elems < scan_carry_elems(a, p))) return -5;
   return scan_launch(a, p, a.work, 0, s);
 }

@@ -7,29 +7,35 @@ namespace pol {
 
 constexpr int SCAN_STEPS = 8;        // steps a warp stages at once; the backward pass starts from states kept this far apart
 
+constexpr int SCAN_WARPS = 4;        // a block of the forward pass
+
 // The time axis in parts of `len` steps (a multiple of SCAN_STEPS), so that few sequences still fill the GPU: their states
-// are joined between two passes (scan_part_kernel, scan_join_kernel).
+// are joined between two passes (scan_kernel's modes 2 and 3, scan_join_kernel).
 struct ScanPlan {
   int64_t parts, len;
   bool split() const { return parts > 1; }
 };
-// A part costs its decays twice, so the axis is split only below a quarter of the warps that the GPU holds, and into no
-// more parts than fill it.
-inline ScanPlan scan_plan(const InbScanArgs& a, int channels_a_warp) {
-  ScanPlan p;
-  const int64_t warps = a.S * ceil_div(a.C, channels_a_warp), room = (int64_t)sm_count() * 16;
-  int64_t parts = 1;
-  if (warps * 3 <= room) parts = ceil_div(room, warps);
-  if (parts > a.T / 32) parts = a.T / 32;
-  if (parts < 1) parts = 1;
-  p.len = ceil_div(ceil_div(a.T, parts), SCAN_STEPS) * SCAN_STEPS;
-  p.parts = ceil_div(a.T, p.len);
-  return p;
+// As many parts as end soonest.  One takes `units` blocks, of which the GPU holds `room`, and blocks that find no room wait for a
+// whole round; a step takes as long beside 16 warps an SM as alone (0.4 us).  A split pass goes `twice` / 2 times over the axis, and
+// the join costs as much as 16 steps.
+inline ScanPlan scan_split(int64_t T, int64_t units, int64_t room, int twice) {
+  ScanPlan best = {1, ceil_div(T, SCAN_STEPS) * SCAN_STEPS};
+  int64_t cost = ceil_div(units, room) * T * 2;
+  for (int64_t n = 2; n <= T / 16 && n <= 256 && units * n <= 4 * room; ++n) {
+    const int64_t len = ceil_div(ceil_div(T, n), SCAN_STEPS) * SCAN_STEPS, parts = ceil_div(T, len);
+    const int64_t c = ceil_div(units * parts, room) * len * twice + 32;
+    if (c < cost) cost = c, best = {parts, len};
+  }
+  return best;
 }
 inline int64_t scan_n4(const InbScanArgs& a) { return (a.N + 3) / 4 * 4; }       // states of a channel in scratch
 inline int64_t scan_chunks(const InbScanArgs& a) { return ceil_div(a.T, SCAN_STEPS); }
 // Forward pass: states a thread (NS) and lanes a channel (LN) for N states
 inline int scan_lanes(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
+inline ScanPlan scan_plan(const InbScanArgs& a) {
+  const int64_t tiles = ceil_div(a.C, 32 / scan_lanes(a.N)), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
+  return scan_split(a.T, a.S * ceil_div(tiles, warps), (int64_t)sm_count() * (4 * SCAN_WARPS / warps), 4);
+}
 // floats of the parts' states [S, parts, C, N4] and of their sums of delta [S, parts, C]
 inline int64_t scan_carry_elems(const InbScanArgs& a, const ScanPlan& p) {
   return p.split() ? a.S * p.parts * a.C * (scan_n4(a) + 1) : 0;

@@ -447,7 +447,6 @@ static void bwd_shape(BwdPlan& b, int64_t C) {
 static BwdPlan bwd_plan(const InbScanArgs& a) {
   BwdPlan b;
   b.lanes = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
-  b.plan = scan_plan(a, 64 / b.lanes);
   if (b.lanes == 1) bwd_shape<1>(b, a.C);
   if (b.lanes == 2) bwd_shape<2>(b, a.C);
   if (b.lanes == 4) bwd_shape<4>(b, a.C);
@@ -455,9 +454,10 @@ static BwdPlan bwd_plan(const InbScanArgs& a) {
   if (b.lanes == 16) bwd_shape<16>(b, a.C);
   int64_t fit = 227 * 1024 / (b.smem + 1024);
   if (fit > 16 / b.warps) fit = 16 / b.warps;                      // registers
-  const int64_t tasks = a.S * b.plan.parts;
   int64_t blocks = sm_count() * fit / b.tiles;
   if (blocks < 1) blocks = 1;
+  b.plan = scan_split(a.T, a.S, blocks, 3);
+  const int64_t tasks = a.S * b.plan.parts;
   b.blocks = (int)(blocks < tasks ? blocks : tasks);
   b.carry = (scan_carry_elems(a, b.plan) + 3) / 4 * 4;
   b.bc = b.tiles > 1 ? b.tiles * a.S * a.T * 2 * a.N : 0;
@@ -513,7 +513,7 @@ extern "C" int inb_selective_scan_work(const InbScanArgs* args, int32_t backward
     const BwdPlan b = bwd_plan(a);
     *elems = b.carry + b.bc + b.par;
   } else if (a.T > 1) {
-    *elems = scan_carry_elems(a, scan_plan(a, 32 / scan_lanes(a.N)));
+    *elems = scan_carry_elems(a, scan_plan(a));
   }
   return 0;
 }
