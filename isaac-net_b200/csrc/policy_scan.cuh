@@ -16,14 +16,14 @@ struct ScanPlan {
   bool split() const { return parts > 1; }
 };
 // As many parts as end soonest.  One takes `units` blocks, of which the GPU holds `room`, and blocks that find no room wait for a
-// whole round; a step takes as long beside 16 warps an SM as alone (0.4 us).  A split pass goes `twice` / 2 times over the axis, and
-// the join costs as much as 16 steps.
-inline ScanPlan scan_split(int64_t T, int64_t units, int64_t room, int twice) {
+// whole round; a step takes as long beside 16 warps an SM as alone (0.4 us).  A split pass costs `split` / 4 of one that is
+// not, and the join as much as 16 steps.
+inline ScanPlan scan_split(int64_t T, int64_t units, int64_t room, int split) {
   ScanPlan best = {1, ceil_div(T, SCAN_STEPS) * SCAN_STEPS};
-  int64_t cost = ceil_div(units, room) * T * 2;
+  int64_t cost = ceil_div(units, room) * T * 4;
   for (int64_t n = 2; n <= T / 16 && n <= 256 && units * n <= 4 * room; ++n) {
     const int64_t len = ceil_div(ceil_div(T, n), SCAN_STEPS) * SCAN_STEPS, parts = ceil_div(T, len);
-    const int64_t c = ceil_div(units * parts, room) * len * twice + 32;
+    const int64_t c = ceil_div(units * parts, room) * len * split + 64;
     if (c < cost) cost = c, best = {parts, len};
   }
   return best;
@@ -34,7 +34,7 @@ inline int64_t scan_chunks(const InbScanArgs& a) { return ceil_div(a.T, SCAN_STE
 inline int scan_lanes(int n) { return n <= 16 ? 1 : n <= 32 ? 2 : 4; }
 inline ScanPlan scan_plan(const InbScanArgs& a) {
   const int64_t tiles = ceil_div(a.C, 32 / scan_lanes(a.N)), warps = tiles < SCAN_WARPS ? tiles : SCAN_WARPS;
-  return scan_split(a.T, a.S * ceil_div(tiles, warps), (int64_t)sm_count() * (4 * SCAN_WARPS / warps), 4);
+  return scan_split(a.T, a.S * ceil_div(tiles, warps), (int64_t)sm_count() * (4 * SCAN_WARPS / warps), 8);
 }
 // floats of the parts' states [S, parts, C, N4] and of their sums of delta [S, parts, C]
 inline int64_t scan_carry_elems(const InbScanArgs& a, const ScanPlan& p) {

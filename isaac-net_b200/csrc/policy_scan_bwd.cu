@@ -53,9 +53,11 @@ struct Chunk {
   __device__ bool oldest() const { return t == t0; }
 };
 
-// Bound by instruction issue: of a step's 180 warp instructions for 8 states a thread 60 are packed multiplications and
-// additions and 18 exponentials.  16 warps an SM (128 registers, 12 KB of shared memory a warp) cover their latency: with
-// twice the states a thread, and so half the warps, the same work took 1.7 times as long.  A chunk's inputs are loaded a
+// Bound by instruction issue: some 270 warp instructions for 8 states a thread and step, of which 60 are packed multiplications and
+// additions and 20 exponentials; next to that by the exponentials (160 of a step's 280 issue cycles).  1024 x 32 sequences of
+// 16 steps, 128 channels, N = 16: 1750 us, of a pass of 2265 us (860 GB/s).  16 warps an SM (128 registers, 12 KB of shared
+// memory a warp) cover their latency: with twice the states a thread, and so half the warps, the same work took 1750 to 2050
+// us.  A chunk's inputs are loaded a
 // chunk ahead.  What is summed over lanes: over a channel's LN by shuffles (s1, w, y), over channels (gb, gc) once a chunk
 // through shared memory, where a lane leaves its parts in place of its states.
 // VEC: rows of x, dt, z, gy and their gradients, d and dt_bias are moved four channels at a time (aligned, C a multiple of 4)
@@ -439,7 +441,10 @@ template <int LN>
 static void bwd_shape(BwdPlan& b, int64_t C) {
   using S = BwdShape<LN>;
   const int64_t all = ceil_div(C, S::CW);
-  b.tiles = (int)ceil_div(all, 8);
+  // 8 warps a block; of N = 5 to 8 that leaves shared memory for one block an SM, 7 warps for two (256 sequences of 300 steps of 512
+  // channels, N = 8, forward + backward: 1035 us against 1091).  Of N <= 4 two blocks of 5 are no faster (1789 us against 1717).
+  constexpr int most = LN == 2 ? 7 : 8;
+  b.tiles = (int)ceil_div(all, most);
   b.warps = (int)ceil_div(all, b.tiles);
   if (b.warps < S::LEAST) b.warps = S::LEAST;
   b.smem = (S::BLOCK + b.warps * S::WARP) * 4;
@@ -456,7 +461,7 @@ static BwdPlan bwd_plan(const InbScanArgs& a) {
   if (fit > 16 / b.warps) fit = 16 / b.warps;                      // registers
   int64_t blocks = sm_count() * fit / b.tiles;
   if (blocks < 1) blocks = 1;
-  b.plan = scan_split(a.T, a.S, blocks, 3);
+  b.plan = scan_split(a.T, a.S, blocks, 5);
   const int64_t tasks = a.S * b.plan.parts;
   b.blocks = (int)(blocks < tasks ? blocks : tasks);
   b.carry = (scan_carry_elems(a, b.plan) + 3) / 4 * 4;
