@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
 #pragma unroll 4
       for (int i = 0; i < feed.R; ++i) step(i, false);
     } else {
-#pragma unroll 1
+#pragma unroll 4
       for (int i = 0; i < count; ++i) step(i, cuts >> i & 1);
     }
     if (q.hi == q.n && q.lo < q.hi && q.t0 + q.n == a.T && a.state_out != nullptr) {
