@@ -6,6 +6,8 @@
 // Bound by DRAM: 2K operations an element against 2 (forward) or 3 (backward, which recomputes pre) moved elements.  A
 // thread holds V neighbouring channels, walks along time and keeps the last K - 1 inputs in registers, so every element is
 // read once; where sequences are few the time axis is split and a part re-reads K - 1 steps at its edge.
+// 1024 x 32 sequences of 16 steps, 256 channels, K = 4, bf16, SiLU: forward 121 us (4.4 TB/s), backward 256 us (3.1 TB/s: the 15
+// warps an SM that its 128 registers leave issue 55 % of the time, waiting on their own results).
 #include "policy_seq.cuh"
 
 namespace inb {
@@ -17,7 +19,9 @@ constexpr int CONV_FWD_BLOCKS = 4, CONV_BWD_BLOCKS = 4;
 // A single step's: 16880 sequences of 458 channels, 2 a thread by one access, bf16 59 us with 4, 49 with 6, 43 with 8, fp32 78, 53, 63;
 // by two accesses (457 channels) 86, 92, 88 and 78, 91, 87
 constexpr int conv_step_blocks(int V, bool wide) { return V == 2 && wide ? 6 : 4; }
-constexpr int CONV_STEP_B = 2;  // sequences whose loads are sent at once by a single step
+// Sequences whose loads are sent at once by a single step: more leave the registers (3 and 4 at 2 channels a thread: 49 -> 46 and
+// 51 us bf16, 53 -> 72 and 84 us fp32)
+constexpr int CONV_STEP_B = 2;
 
 struct ConvPlan {
   int64_t parts, len, tasks;    // parts of the time axis, their steps; sequences x parts
@@ -342,6 +346,7 @@ __global__ void __launch_bounds__(128, CONV_FWD_BLOCKS) conv_fwd_kernel(InbConvA
 }
 
 // One step: bound by the states' bytes, of which a thread has CONV_STEP_B sequences' on their way at once; state_out may be state.
+// 131072 sequences of 512 channels, K = 4, bf16: 172 us (6.2 TB/s).
 template <typename T, int V, bool WIDE, int K>
 __global__ void __launch_bounds__(128, conv_step_blocks(V, WIDE)) conv_step_kernel(InbConvArgs a) {
   constexpr int P = Words<T, V>::P;
@@ -645,7 +650,10 @@ static int conv_bwd_go(const InbConvArgs& a, cudaStream_t s) {
   colsum<T>(a.work, l.grid.x, (int64_t)a.C * (K + 1), (int64_t)a.C * K, (int64_t)a.C * (K + 1), a.gw, a.gbias, nullptr, s);
   return launch_status();
 }
-// Channels a thread
+// Channels a thread, by what one access can move: 16 bytes forward; 4 channels backward, whose sums take the registers (8 bytes of
+// bf16, 16 of fp32); where rows are not aligned to that 2; and where not even to 2 channels, 2 by an access each.  80 sequences
+// of 3373 steps, fp16, forward + backward: 464 channels (4 backward) 332 us, 460 (4 both ways) 346, 458 (2) 582, 457 (2 by two) 684
+// (2654 with 4 by four accesses, which leave the registers).
 template <typename T, int V, bool WIDE>
 static int conv_taps(const InbConvArgs& a, bool backward, cudaStream_t s) {
   if (backward) {

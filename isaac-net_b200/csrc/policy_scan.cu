@@ -18,6 +18,8 @@ namespace pol {
 // Bound by the exponentials (one a state and step, 16 a clock and SM) and, next to that, by instruction issue: an eighth of
 // them goes to the FMA pipe (ex2_poly), which evens the two out; all else is packed in pairs of states.  A chunk of
 // SCAN_STEPS steps is prepared at once (delta, u, the gate), then the next one's loads are sent, then its steps run.
+// 179 warp instructions a step (32 channels, 16 states), 137 cycles of the special function unit.  1024 x 32 sequences of 16
+// steps, 128 channels, bf16, with the states kept: 540 us (2.5 TB/s); one of 4096 steps, 2048 channels, in 37 parts: 50 + 9 (join) + 68 us.
 // WIDE: the rows of b and c are NS whole, aligned to 16 bytes and moved by that
 template <typename T, int NS, int LN, int MODE, bool WIDE>
 __global__ void __launch_bounds__(SCAN_WARPS * 32, 4) scan_kernel(InbScanArgs a, ScanPlan pl, float* carry) {
@@ -252,16 +254,20 @@ __global__ void __launch_bounds__(256) scan_join_kernel(InbScanArgs a, ScanPlan 
 // One step: bound by the states' bytes.  A thread holds V x G states of one channel (V moved by one access; `lanes` threads a
 // channel, a power of two) and walks over sequences, STEP_B at a time, whose loads are on their way at once.  A block takes
 // `chans` channels (a power of two, a warp's at least) of `runs` sequences at a time (MANY: more than one), next to one another, `per` times.
+// 131072 sequences of 256 channels, N = 16: 800 us alone (5.7 TB/s).  23168 sequences of 18 channels, N = 4: 18 us with shared blocks, 57 with
+// one sequence a block; as a variable, `runs` cost the large call 30 % in registers, hence MANY.
 constexpr int STEP_THREADS = 256, STEP_B = 2;
 template <typename T, int V, int G, bool MANY>
 __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs a, int lanes, int chans, int per) {
-  const int j = threadIdx.x & (lanes - 1), w = threadIdx.x / lanes;
-  const int c0 = blockIdx.x * chans + (w & (chans - 1));
+  if (!MANY) chans = STEP_THREADS / lanes;
+  const int j = threadIdx.x % lanes, w = threadIdx.x / lanes;
+  const int c0 = blockIdx.x * chans + (MANY ? w & (chans - 1) : w);
   const bool on = c0 < a.C;
   const int ch = on ? c0 : a.C - 1;
   const uint32_t runs = MANY ? STEP_THREADS / (lanes * chans) : 1;
-  const int64_t b0 = (int64_t)blockIdx.y * per * runs, s0 = MANY ? b0 + w / chans : b0, s1 = b0 + (int64_t)per * runs < a.S ? b0 + (int64_t)per * runs : a.S;
-  if (s0 >= a.S) return;
+  const int64_t b0 = (int64_t)blockIdx.y * per * runs, b1 = b0 + (int64_t)per * runs, s0 = MANY ? b0 + w / chans : b0;
+  const int64_t s1 = b1 < a.S ? b1 : a.S;
+  if (MANY && s0 >= a.S) return;
   const float bias = a.dt_bias != nullptr ? a.dt_bias[ch] : 0.f, d = a.d != nullptr ? a.d[ch] : 0.f;
   const bool gate = a.z.p != nullptr;
   float A[G][V];
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
   const uint8_t* pr = resets(a.reset, s0);
   uint32_t of = pr != nullptr ? (uint32_t)s0 % (uint32_t)a.reset.rows : 0;
   for (int64_t s = s0; s < s1; s += STEP_B * runs) {
-    const int n = s1 - s > (STEP_B - 1) * (int64_t)runs ? STEP_B : (int)((s1 - s + runs - 1) / runs);
+    const int n = s1 - s > (STEP_B - 1) * (int64_t)runs ? STEP_B : MANY ? (int)((s1 - s + runs - 1) / runs) : (int)(s1 - s);
     uint32_t x[STEP_B], dt[STEP_B], z[STEP_B], cut[STEP_B];
     Words<T, V> b[STEP_B][G], c[STEP_B][G];
     Pack<float, V> h[STEP_B][G];
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) scan_step_kernel(InbScanArgs 
         of += runs;
         if (of >= (uint32_t)a.reset.rows) {
           const uint32_t past = MANY ? of / (uint32_t)a.reset.rows : 1;
-          of -= past * (uint32_t)a.reset.rows;
+          of = MANY ? of - past * (uint32_t)a.reset.rows : 0;
           if (s + (u + 1) * (int64_t)runs < a.S) pr += past * a.reset.seq;
         }
       }

@@ -190,7 +190,8 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------------------------------------------- column sums
 // part [P, M] fp32 -> sums over P: columns [0, first) to out0, [first, second) to out1, the others to out2 (any may be NULL).
-// A block takes 32 columns, its 32 warps rows p, p + 32, ...; the order of the sum does not depend on timing.
+// A block takes 32 columns, its 32 warps rows p, p + 32, ...; the order of the sum does not depend on timing.  Bound by latency
+// (4 loads of a thread on their way): 592 rows of 1280 columns 5.6 us.
 constexpr int COLSUM_WARPS = 32;
 template <typename T>
 __global__ void __launch_bounds__(COLSUM_WARPS * 32) colsum_kernel(const float* part, int64_t P, int64_t M, int64_t first, int64_t second,

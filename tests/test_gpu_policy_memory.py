@@ -365,3 +365,51 @@ def test_gradients_against_differences():
             got = float((closs({**vals, k: q + h * way}) - closs({**vals, k: q - h * way})) / (2 * h))
         want = float((grads[k].double() * way.double()).sum())
         assert abs(got - want) < 2.0 ** -10 * (1 + float(grads[k].norm())), (k, got, want)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("k", [2, 3, 4])
+@pytest.mark.parametrize("c,off", [(2, 0), (6, 0), (6, 2), (10, 1), (130, 0), (258, 4), (457, 0), (460, 0), (460, 3), (464, 2), (464, 4)])
+def test_causal_conv_of_every_alignment(c, off, k, dtype):
+    """Rows by 16, 8 and 4 bytes and by elements: even and odd widths, views off the boundary, time in parts."""
+    g = gen(10 * c + off)
+    for e, r, t in ((3, 2, 19), (1, 1, 150)):
+        x, w, b, state, flags = conv_case(g, e, r, t, c, k, dtype, resets=0.1)
+        wide = torch.zeros(e, r, t, c + 2 * off, device="cuda", dtype=dtype)
+        wide[..., off:off + c] = x
+        check_conv(g, wide[..., off:off + c], w, b, state, flags, "silu")
+        with torch.no_grad():
+            y, new = ops.causal_conv(x, w, b, state=state, reset=flags)
+            live = state.clone()
+            for i in range(t if t < 20 else 0):
+                at = wide[:, :, i, off:off + c]
+                near(ops.causal_conv_step(at, w, live, b, reset=flags[..., i]), y[:, :, i].double(), y[:, :, i].double().abs() + 16, 60)
+            assert t > 19 or torch.equal(live, new)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("e,r,env", [(1, 1, True), (37, 3, True), (300, 1, False), (1, 500, True), (2500, 16, True)])
+@pytest.mark.parametrize("c,n", [(1, 1), (1, 64), (3, 5), (18, 4), (40, 16), (33, 10), (129, 4)])
+def test_scan_steps_of_few_channels(e, r, env, c, n, dtype):
+    """A block takes several sequences side by side: every one of them, its own flag, and nothing behind the last."""
+    g = gen(e + c + n)
+    v, flags = scan_case(g, e, r, 1, c, n, dtype, resets=0.3, env=env)
+    want, mag = scan_refs(v, flags, torch.zeros(e, r, 1, c, device="cuda"), None)
+    vmax, far = float(want["v"].abs().max()), float(want["far"])
+    lim = 2 * (6 + far * (16 + 3 * vmax)) + 2 * (14 + 3 * vmax) + n + 20 + 3 * float(v["z"].abs().max())
+    room = torch.full((e * r + 7, c, n), 5.0, device="cuda")
+    live = room[:e * r].view(e, r, c, n).copy_(v["state"])
+    at = lambda q: v[q][:, :, 0]
+    o = ops.selective_scan_step(at("x"), at("dt"), v["a"], at("b"), at("c"), live, d=v["d"], z=at("z"), dt_bias=v["dt_bias"], reset=flags[..., 0])
+    near(o.reshape(-1, c), want["y"][:, 0], mag["y"][:, 0], lim, "y")
+    near(live.reshape(-1, c, n), want["new"], mag["new"], lim, "state")
+    assert bool((room[e * r:] == 5.0).all())
+
+
+@pytest.mark.parametrize("e,r,t,ch,n", [(1, 3, 127, 377, 10), (1, 1, 64, 512, 16), (1, 16, 700, 200, 5), (2, 32, 130, 64, 64),
+                                        (5, 16, 90, 300, 8), (1, 1, 33, 1024, 4)])
+def test_selective_scan_where_parts_end_soonest(e, r, t, ch, n):
+    """Forward and backward split in their own numbers of parts, down to parts of 16 steps."""
+    g = gen(t + ch)
+    for resets in (0.0, 0.05):
+        check_scan(g, *scan_case(g, e, r, t, ch, n, torch.bfloat16, resets=resets))
